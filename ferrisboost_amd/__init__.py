@@ -26,9 +26,10 @@ from typing import Any, Mapping
 import numpy as np
 
 from . import _native as N
-from . import frame_rows
+from . import frame_rows, heads
 
-__all__ = ["train", "sketch", "Cuts", "Model", "device_available", "release_cached", "__version__"]
+__all__ = ["train", "sketch", "Cuts", "Model", "device_available", "release_cached", "heads",
+           "__version__"]
 __version__ = "0.1.0"
 
 # Canonical name -> default, as python/ferrisboost/__init__.py:_DEFAULTS.
@@ -660,6 +661,58 @@ class Model:
             elif k == 1 or out.ndim == 1:
                 out = out.reshape((n, 1) + out.shape[1:])
         return out
+
+    def leaf_vocabulary(self, n_trees: int | None = None, *,
+                        iteration_range: tuple[int, int] | None = None,
+                        device: str | None = None) -> heads.Vocabulary:
+        """The vocabulary of the leaf ids that predict(pred_leaf=True) gives for the same
+        trees, for heads.embed(): a column a tree, a token a node. Needs torch. (No
+        reference counterpart.)"""
+        b, e = self._tree_range(n_trees, iteration_range)
+        if b == e:
+            raise ValueError("no trees are selected")
+        L = N.train_lib()
+        dev = _parse_device(device) if device is not None else self._device
+        return heads.Vocabulary([L.fbt_model_tree_len(self._h, t) for t in range(b, e)],
+                                device=f"cuda:{dev}")
+
+    def sample(self, data, uniforms, *, temperature: float = 1.0, top_k: int = 0,
+               top_p: float = 1.0, min_p: float = 0.0, return_log_probs: bool = False,
+               n_trees: int | None = None, iteration_range: tuple[int, int] | None = None,
+               missing: float = float("nan"), base_margin=None, device: str | None = None):
+        """A class for every row, drawn from the model's class distribution with the
+        row's uniform number in [0, 1): heads.sample() on the margins that predict()
+        gives with the same arguments, on host arrays. Classes are int64 (n,), -1 where a
+        row's margins are all NaN; with return_log_probs also the logarithms of their
+        shares of what top_k, top_p and min_p leave, float32 (n,). For multi:softprob,
+        multi:softmax and binary:logistic (classes 0 and 1) models. temperature=0 gives
+        multi:softmax's classes. (No reference counterpart: the reference stops at the
+        probabilities.)"""
+        options = heads.check_options(temperature, top_k, top_p, min_p)
+        if not (self.objective.startswith("multi:") or self.objective == "binary:logistic"):
+            raise ValueError(f"{self.objective} models have no classes to draw")
+        m = self.predict(data, output_margin=True, n_trees=n_trees,
+                         iteration_range=iteration_range, missing=missing,
+                         base_margin=base_margin, device=device)
+        if m.ndim == 1:  # binary:logistic: exp(margin) to 1
+            m = np.stack([np.zeros_like(m), m], axis=1)
+        m = np.ascontiguousarray(m, np.float32)
+        n, k = m.shape
+        u = np.ascontiguousarray(np.asarray(uniforms, dtype=np.float32))
+        if u.shape != (n,):
+            raise ValueError(f"uniforms must have one value for each of {n} rows, got shape "
+                             f"{u.shape}")
+        if not ((u >= 0.0) & (u < 1.0)).all():
+            raise ValueError("uniforms must be in [0, 1)")
+        o = N.SampleOptions()
+        o.temperature, o.top_k, o.top_p, o.min_p = options
+        classes = np.zeros(n, np.int64)
+        log_probs = np.zeros(n, np.float32)
+        dev = _parse_device(device) if device is not None else self._device
+        N.check_hip(N.hip().fbh_sample_classes_host(
+            dev, N.ptr(m), n, k, N.ptr(u), C.byref(o), N.ptr(classes),
+            N.ptr(log_probs) if return_log_probs else None))
+        return (classes, log_probs) if return_log_probs else classes
 
     def get_score(self, importance_type: str = "weight") -> dict[str, float]:
         """Feature importance as XGBoost's Booster.get_score (feature_scores,

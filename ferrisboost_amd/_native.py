@@ -170,6 +170,41 @@ class TrainParams(C.Structure):
     ]
 
 
+class Embed(C.Structure):
+    """fbh_embed: positions and vectors of an embedding."""
+
+    _fields_ = [
+        ("n_rows", C.c_uint64),
+        ("n_columns", C.c_uint32),
+        ("dim", C.c_uint32),
+        ("n_tokens", C.c_uint32),
+        ("id_type", C.c_uint32),
+        ("dtype", C.c_uint32),
+        ("pooled", C.c_uint32),
+        ("ids", P),
+        ("first", P),
+        ("drop", C.c_double),
+        ("seed", C.c_uint64),
+        ("scale", C.c_float),
+        ("reserved", C.c_uint32),
+    ]
+
+
+class SampleOptions(C.Structure):
+    """fbh_sample_options: how classes are drawn."""
+
+    _fields_ = [
+        ("temperatures", P),
+        ("top_ks", P),
+        ("top_ps", P),
+        ("min_ps", P),
+        ("temperature", C.c_float),
+        ("top_k", C.c_int32),
+        ("top_p", C.c_float),
+        ("min_p", C.c_float),
+    ]
+
+
 # fbt_rows_fn: int (*)(void *user, uint64_t begin, uint64_t n, float *out)
 ROWS_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_uint64, C.c_uint64, C.POINTER(C.c_float))
 
@@ -239,6 +274,8 @@ HIP_SYMBOLS = [
     "fbh_shap_set_host_order", "fbh_release_cached", "fbh_shap_model_park",
     "fbh_shap_model_unpark", "fbh_shap_models_drop",
     "fbh_saabas_contribs", "fbh_predict", "fbh_predict_device", "fbh_shap_contribs_noalloc",
+    "fbh_embed_rows", "fbh_embed_grad_bytes", "fbh_embed_grad", "fbh_dropout",
+    "fbh_sample_classes", "fbh_sample_classes_host",
 ]
 TRAIN_SYMBOLS = [
     "fbt_last_error", "fbt_train", "fbt_train_cuts", "fbt_train_rows", "fbt_last_stats",
@@ -362,6 +399,15 @@ def hip() -> C.CDLL:
             getattr(L, name).argtypes = [P, P, C.c_uint64, P, P]
         L.fbh_predict.argtypes = [P, P, C.c_uint64, P, C.c_uint32, P]
         L.fbh_predict_device.argtypes = [P, P, C.c_uint64, P, C.c_uint32, P, C.c_int]
+        L.fbh_embed_rows.argtypes = [C.c_int, P, P, P, P]
+        L.fbh_embed_grad_bytes.argtypes = [P]
+        L.fbh_embed_grad_bytes.restype = C.c_uint64
+        L.fbh_embed_grad.argtypes = [C.c_int, P, P, P, P, C.c_uint64, P]
+        L.fbh_dropout.argtypes = [C.c_int, P, P, C.c_uint64, C.c_uint32, C.c_double, C.c_uint64,
+                                  C.c_uint64, P]
+        L.fbh_sample_classes.argtypes = [C.c_int, P, C.c_uint64, C.c_uint32, C.c_uint32, P, P, P,
+                                         P, P]
+        L.fbh_sample_classes_host.argtypes = [C.c_int, P, C.c_uint64, C.c_uint32, P, P, P, P]
         _hip = L
     return _hip
 

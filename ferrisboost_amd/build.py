@@ -35,7 +35,8 @@ HIP_FLAGS = [
 ]
 
 BACKEND_SRCS = ["fbhip_kernels.hip", "fbhip_ctx.hip", "fbhip_shap.hip",
-                "fbhip_shap_paths.hip", "fbhip_predict.hip", "fbhip_sketch.hip", "fbhip_keep.hip"]
+                "fbhip_shap_paths.hip", "fbhip_predict.hip", "fbhip_sketch.hip", "fbhip_keep.hip",
+                "fbhip_embed.hip", "fbhip_dropout.hip", "fbhip_sample.hip"]
 DRIVER_SRCS = ["fbt_data.cpp", "fbt_train.cpp", "fbt_model.cpp", "fbt_json.cpp", "fbt_api.cpp"]
 
 LIB_HIP = os.path.join(HERE, "libfbhip.so")

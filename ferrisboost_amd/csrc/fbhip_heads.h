@@ -1,0 +1,110 @@
+// fbhip_heads.h -- what the kernels of the heads on a model's outputs share
+// (fbhip_embed.hip, fbhip_dropout.hip, fbhip_sample.hip): cell types, 16-byte
+// pieces, the counter-based generator, errors and the calling device.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <stdexcept>
+#include <string>
+
+#include "../../include/fbhip.h"
+#include "fbhip_internal.h"
+
+namespace fbh {
+
+struct HeadError : std::runtime_error {
+    int code;
+    HeadError(int c, const std::string &m) : std::runtime_error(m), code(c) {}
+};
+
+inline void head_check(hipError_t e, const char *what) {
+    if (e != hipSuccess)
+        throw HeadError(FBH_RUNTIME_ERROR, std::string(what) + ": " + hipGetErrorString(e));
+}
+
+inline void head_input(bool ok, const char *message) {
+    if (!ok) throw HeadError(FBH_INPUT_ERROR, message);
+}
+
+template <class F>
+int head_guard(F &&f) {
+    try {
+        f();
+        return FBH_OK;
+    } catch (const HeadError &e) {
+        set_last_error(e.what());
+        return e.code;
+    } catch (const std::exception &e) {
+        set_last_error(e.what());
+        return FBH_RUNTIME_ERROR;
+    } catch (...) {
+        set_last_error("unknown error");
+        return FBH_RUNTIME_ERROR;
+    }
+}
+
+// The call's device, and the caller's one again afterwards.
+class OnDevice {
+    int before_ = -1;
+
+  public:
+    explicit OnDevice(int device) {
+        int now = 0;
+        head_check(hipGetDevice(&now), "hipGetDevice");
+        if (now == device) return;
+        head_check(hipSetDevice(device), "hipSetDevice");
+        before_ = now;
+    }
+    ~OnDevice() {
+        if (before_ >= 0) (void)hipSetDevice(before_);
+    }
+    OnDevice(const OnDevice &) = delete;
+};
+
+// N cells as they lie in memory, moved together whatever their alignment (global
+// loads and stores of up to 16 bytes need none on this device).
+template <class T, int N>
+struct Piece {
+    T v[N];
+};
+template <class T, int N>
+__device__ __forceinline__ Piece<T, N> load_piece(const T *p) {
+    Piece<T, N> r;
+    __builtin_memcpy(&r, p, sizeof(r));
+    return r;
+}
+template <class T, int N>
+__device__ __forceinline__ void store_piece(T *p, const Piece<T, N> &r) {
+    __builtin_memcpy(p, &r, sizeof(r));
+}
+
+// ---- The counter-based generator: element e takes half of the 64 bits that the
+// SplitMix64 finaliser gives for a seed's key and e / 2, as row sampling takes a
+// row's bits from seed and row. Nothing is stored: whoever knows seed and element
+// has the same bits again.
+constexpr uint64_t DROP_STEP = 0xD6E8FEB86659FD93ull;
+
+__host__ __device__ inline uint64_t drop_mix(uint64_t z) {
+    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+    return z ^ (z >> 31);
+}
+inline uint64_t drop_key(uint64_t seed) { return drop_mix(seed ^ 0x9E3779B97F4A7C15ull); }
+
+__device__ __forceinline__ uint64_t drop_word(uint64_t key, uint64_t pair) {
+    return drop_mix(key ^ (pair * DROP_STEP));
+}
+__device__ __forceinline__ uint32_t drop_bits(uint64_t key, uint64_t e) {
+    const uint64_t w = drop_word(key, e >> 1);
+    return (e & 1) ? (uint32_t)(w >> 32) : (uint32_t)w;
+}
+
+// Elements whose 32 bits are below this are dropped.
+inline uint32_t drop_threshold(double drop) {
+    head_input(drop >= 0.0 && drop < 1.0, "drop must be in [0, 1)");
+    const double t = __builtin_rint(drop * 4294967296.0);
+    return t >= 4294967295.0 ? 4294967295u : (uint32_t)t;
+}
+
+}  // namespace fbh

@@ -1,0 +1,365 @@
+"""Heads on a model's outputs, for programs that go on in torch.
+
+A model answers with leaf ids (predict(pred_leaf=True), FBH_PREDICT_LEAF on the
+device) and class margins, and its rows hold categorical codes. What follows them:
+
+  embed / embed_grad  vectors learned for ids: rows of a table looked up by id, as they
+                      are or summed over a row's columns, and the table's gradient
+  dropout             while they are learned, from (seed, element) alone: no mask
+  sample              classes drawn from margins (Model.sample does it on host arrays)
+
+    model = fb.train({"objective": "multi:softprob", "num_class": 4, ...}, X, label=y)
+    leaves = torch.from_numpy(model.predict(X, pred_leaf=True)).cuda()
+    voc = model.leaf_vocabulary()
+    table = torch.zeros(voc.n_tokens, 64, device="cuda", requires_grad=True)
+    h = fb.heads.embed(table, leaves, voc, pooled=True, drop=0.1, seed=step)
+    h = fb.heads.dropout(h, 0.1, seed=step + 1)
+    classes, log_probs = fb.heads.sample(h @ W, torch.rand(len(h), device="cuda"), top_p=0.9)
+
+Tensors are torch tensors on one gfx950 device; torch must be imported before the
+package's first call, so that both share one HIP runtime. Kernels are hand-written HIP
+behind the C ABI of include/fbhip.h, enqueued on torch's current stream of the tensors'
+device; nothing waits, results are the same in every call, and all of it can be captured
+into a graph. A tensor that is not contiguous is copied first. embed and dropout take
+part in autograd. Bad arguments are ValueErrors, device failures RuntimeErrors.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import functools
+
+import numpy as np
+
+from . import _native as N
+
+__all__ = ["Vocabulary", "embed", "embed_grad", "dropout", "sample"]
+
+_torch = None
+_CELLS: dict = {}
+_IDS: dict = {}
+
+
+def _need_torch():
+    """torch, once it is known to share this package's HIP runtime."""
+    global _torch
+    if _torch is not None:
+        return _torch
+    import torch
+
+    N.hip()
+    with open("/proc/self/maps") as f:
+        runtimes = {line.split()[-1] for line in f if "libamdhip64.so" in line}
+    if len(runtimes) > 1:
+        raise N.BackendError(
+            "torch was imported after the package's first call and has brought a HIP runtime of "
+            "its own; import torch first")
+    _CELLS.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    _IDS.update({torch.int32: 0, torch.int64: 1, torch.float32: 2})
+    _torch = torch
+    return torch
+
+
+def _device_tensor(x, what: str):
+    if not isinstance(x, _torch.Tensor):
+        raise ValueError(f"{what} must be a torch tensor, got {type(x).__name__}")
+    if x.device.type != "cuda":
+        raise ValueError(f"{what} must be on a GPU, it is on {x.device}")
+    return x if x.is_contiguous() else x.contiguous()
+
+
+def _cells(x, what: str) -> int:
+    code = _CELLS.get(x.dtype)
+    if code is None:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16, got {x.dtype}")
+    return code
+
+
+def _beside(x, other, what: str):
+    if x.device != other.device:
+        raise ValueError(f"{what} is on {x.device}, the call's other tensors on {other.device}")
+    return x
+
+
+def _seed(seed) -> int:
+    seed = int(seed)
+    if not 0 <= seed < 1 << 64:
+        raise ValueError(f"seed must be in 0..=2^64 - 1, got {seed}")
+    return seed
+
+
+def _drop(drop) -> float:
+    drop = float(drop)
+    if not 0.0 <= drop < 1.0:
+        raise ValueError(f"drop must be in [0, 1), got {drop}")
+    return drop
+
+
+def _stream(device) -> int:
+    return _torch.cuda.current_stream(device).cuda_stream
+
+
+class Vocabulary:
+    """The table rows of several columns' ids: column t's ids 0 .. sizes[t] - 1 are rows
+    first[t] .. first[t] + sizes[t] - 1 of a table of n_tokens rows (a model's trees:
+    Model.leaf_vocabulary(); categorical columns: their numbers of codes)."""
+
+    def __init__(self, sizes, device="cuda:0"):
+        torch = _need_torch()
+        sizes = np.asarray(sizes)
+        if sizes.ndim != 1 or sizes.size == 0 or sizes.dtype.kind not in "iu":
+            raise ValueError("sizes must be a list of whole numbers, one for each column")
+        if sizes.size > 32768:
+            raise ValueError(f"at most 32768 columns, got {sizes.size}")
+        if (sizes < 0).any():
+            raise ValueError("sizes must not be negative")
+        first = np.concatenate([[0], np.cumsum(sizes, dtype=np.int64)])
+        if not 1 <= first[-1] < 1 << 31:
+            raise ValueError(f"a table has 1 to 2^31 - 1 rows, these columns {first[-1]}")
+        self.sizes = sizes.astype(np.int64)
+        self.n_tokens = int(first[-1])
+        self.n_columns = int(sizes.size)
+        self.first = torch.from_numpy(first.astype(np.int32)).to(device)
+        if self.first.device.type != "cuda":
+            raise ValueError(f"device must be a GPU, got {device!r}")
+
+    def __repr__(self):
+        return (f"Vocabulary({self.n_columns} columns, {self.n_tokens} tokens, "
+                f"{self.first.device})")
+
+
+def _positions(ids, vocabulary, pooled: bool, n_tokens: int, dim: int, cells: int, scale: float,
+               drop: float, seed: int):
+    """The call's fbh_embed, and the leading shape of its vectors."""
+    code = _IDS.get(ids.dtype)
+    if code is None:
+        raise ValueError(f"ids must be int32, int64 or float32, got {ids.dtype}")
+    shape = tuple(ids.shape)
+    if pooled or vocabulary is not None:
+        if not shape:
+            raise ValueError("ids must have a last axis of columns")
+        columns = shape[-1]
+        if vocabulary is not None:
+            if columns != vocabulary.n_columns:
+                raise ValueError(f"ids have {columns} columns, the vocabulary "
+                                 f"{vocabulary.n_columns}")
+            _beside(vocabulary.first, ids, "the vocabulary")
+        n_rows = 1
+        for s in shape[:-1]:
+            n_rows *= s
+    else:
+        n_rows, columns = ids.numel(), 1
+    e = N.Embed()
+    e.n_rows, e.n_columns, e.dim, e.n_tokens = n_rows, columns, dim, n_tokens
+    e.id_type, e.dtype, e.pooled = code, cells, 1 if pooled else 0
+    e.ids = ids.data_ptr()
+    if vocabulary is not None:
+        e.first = vocabulary.first.data_ptr()
+    e.drop, e.seed, e.scale = drop, seed, scale
+    return e, shape[:-1] if pooled else shape
+
+
+def _embed(table, ids, vocabulary, scale, pooled, drop, seed):
+    e, lead = _positions(ids, vocabulary, pooled, table.shape[0], table.shape[1],
+                         _cells(table, "table"), scale, drop, seed)
+    out = table.new_empty(lead + (table.shape[1],))
+    if e.n_columns == 0:
+        return out.zero_()
+    N.check_hip(N.hip().fbh_embed_rows(table.device.index, C.byref(e), table.data_ptr(),
+                                       out.data_ptr(), _stream(table.device)))
+    return out
+
+
+@functools.lru_cache(maxsize=None)
+def _functions():
+    torch = _torch
+
+    class Embed(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, table, ids, vocabulary, scale, pooled, drop, seed):
+            ctx.save_for_backward(ids)
+            ctx.rest = (vocabulary if vocabulary is not None else table.shape[0], scale, pooled,
+                        drop, seed)
+            return _embed(table, ids, vocabulary, scale, pooled, drop, seed)
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, grad):
+            tokens, scale, pooled, drop, seed = ctx.rest
+            return (embed_grad(grad, ctx.saved_tensors[0], tokens, scale=scale, pooled=pooled,
+                               drop=drop, seed=seed),) + (None,) * 6
+
+    class Dropout(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, drop, seed, first):
+            ctx.rest = (drop, seed, first)
+            return _dropout(x, drop, seed, first)
+
+        @staticmethod
+        def backward(ctx, grad):
+            return (dropout(grad, *ctx.rest),) + (None,) * 3
+
+    return Embed, Dropout
+
+
+def embed(table, ids, vocabulary: Vocabulary | None = None, *, scale: float = 1.0,
+          pooled: bool = False, drop: float = 0.0, seed: int = 0):
+    """Rows of `table` (n_tokens, dim) by id, times `scale`: (*ids.shape, dim), or with
+    pooled=True summed over the last axis of ids, in float32 and rounded once.
+
+    ids are int32, int64, or float32 as predict(pred_leaf=True) gives leaf ids. With a
+    vocabulary the last axis of ids are its columns, each with its own part of the table;
+    without, every id is a table row. An id outside its column (-1 for a missing or unseen
+    code, say) gives zeros. drop > 0 leaves out each id of the call with that probability,
+    drawn from `seed` and the id's place in `ids`, and scales the others by 1 / (1 - drop):
+    whole trees, or whole columns, of a row."""
+    torch = _need_torch()
+    table = _device_tensor(table, "table")
+    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+        raise ValueError(f"table must be (tokens, cells), got shape {tuple(table.shape)}")
+    if vocabulary is not None and vocabulary.n_tokens != table.shape[0]:
+        raise ValueError(f"table has {table.shape[0]} rows, the vocabulary "
+                         f"{vocabulary.n_tokens} tokens")
+    ids = _beside(_device_tensor(ids, "ids"), table, "ids")
+    args = (table, ids, vocabulary, float(scale), bool(pooled), _drop(drop), _seed(seed))
+    if table.requires_grad and torch.is_grad_enabled():
+        return _functions()[0].apply(*args)
+    return _embed(*args)
+
+
+def embed_grad(grad, ids, tokens, *, scale: float = 1.0, pooled: bool = False,
+               drop: float = 0.0, seed: int = 0):
+    """The gradient of embed()'s table, (n_tokens, dim) in grad's type: `grad` is the
+    gradient of embed()'s output, `tokens` its vocabulary or, without one, the number of
+    table rows, and the rest embed()'s arguments. Sums are taken in float32 in a fixed
+    order (the positions sorted by token) and rounded once. (embed() calls this in
+    backward(); a captured training step can call it by itself.)"""
+    _need_torch()
+    grad = _device_tensor(grad, "grad")
+    ids = _beside(_device_tensor(ids, "ids"), grad, "ids")
+    vocabulary = tokens if isinstance(tokens, Vocabulary) else None
+    n_tokens = int(tokens if vocabulary is None else vocabulary.n_tokens)
+    if not 1 <= n_tokens < 1 << 31:
+        raise ValueError(f"a table has 1 to 2^31 - 1 rows, got {n_tokens}")
+    if grad.dim() < 1 or grad.shape[-1] < 1:
+        raise ValueError(f"grad must have a last axis of cells, got shape {tuple(grad.shape)}")
+    e, lead = _positions(ids, vocabulary, bool(pooled), n_tokens, grad.shape[-1],
+                         _cells(grad, "grad"), float(scale), _drop(drop), _seed(seed))
+    if tuple(grad.shape[:-1]) != lead:
+        raise ValueError(f"grad has shape {tuple(grad.shape)}, expected {lead} vectors")
+    out = grad.new_empty((n_tokens, grad.shape[-1]))
+    if e.n_columns == 0:
+        return out.zero_()
+    L = N.hip()
+    size = L.fbh_embed_grad_bytes(C.byref(e))
+    work = _torch.empty(size, dtype=_torch.uint8, device=grad.device)
+    N.check_hip(L.fbh_embed_grad(grad.device.index, C.byref(e), grad.data_ptr(), out.data_ptr(),
+                                 work.data_ptr(), size, _stream(grad.device)))
+    return out
+
+
+def _dropout(x, drop, seed, first):
+    out = _torch.empty_like(x)
+    N.check_hip(N.hip().fbh_dropout(x.device.index, x.data_ptr(), out.data_ptr(), x.numel(),
+                                    _cells(x, "x"), drop, seed, first, _stream(x.device)))
+    return out
+
+
+def dropout(x, drop: float, seed: int, first: int = 0):
+    """x / (1 - drop) where an element stays, 0 where it is dropped (with probability
+    `drop`), whatever it holds. An element's fate depends on `seed` and its number alone
+    (counted in row-major order from `first`), so the gradient of a call, which
+    backward() takes, is dropout() of the output's gradient with the same arguments, and
+    nothing is stored for it. Use another seed for another layer or step."""
+    torch = _need_torch()
+    x = _device_tensor(x, "x")
+    _cells(x, "x")
+    first = int(first)
+    if not 0 <= first < 1 << 63:
+        raise ValueError(f"first must be in 0..=2^63 - 1, got {first}")
+    args = (x, _drop(drop), _seed(seed), first)
+    if x.requires_grad and torch.is_grad_enabled():
+        return _functions()[1].apply(*args)
+    return _dropout(*args)
+
+
+def _option(value, what: str, lead, like, dtype, check):
+    """(a number, None) or (0, a tensor of one value a row)."""
+    if isinstance(value, _torch.Tensor) and value.dim() > 0:
+        v = _beside(_device_tensor(value, what), like, what)
+        if tuple(v.shape) != lead:
+            raise ValueError(f"{what} must have shape {lead}, got {tuple(v.shape)}")
+        if v.dtype != dtype:
+            raise ValueError(f"{what} must be {dtype}, got {v.dtype}")
+        return 0, v
+    return check(value), None
+
+
+def check_options(temperature, top_k, top_p, min_p) -> tuple[float, int, float, float]:
+    """The options of sample() as one set of numbers."""
+    return (_temperature(temperature), _top_k(top_k), _share("top_p", top_p),
+            _share("min_p", min_p))
+
+
+def _temperature(v) -> float:
+    v = float(v)
+    if not 0.0 <= v <= float(np.finfo(np.float32).max):
+        raise ValueError(f"temperature must be a finite float32, not negative, got {v}")
+    return v
+
+
+def _top_k(v) -> int:
+    if isinstance(v, bool) or int(v) != v or int(v) < 0:
+        raise ValueError(f"top_k must be a whole number, 0 (all) or more, got {v!r}")
+    return min(int(v), 0x7FFFFFFF)
+
+
+def _share(what: str, v) -> float:
+    v = float(v)
+    if not 0.0 <= v <= 1.0:
+        raise ValueError(f"{what} must be in [0, 1], got {v}")
+    return v
+
+
+def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One class for every row of `logits` (..., classes), from a uniform float32 number
+    in [0, 1) a row: (classes int64, log_probs float32), each of shape (...).
+
+    Weights are exp(logit / temperature). Ordered by falling logit (equal ones by class),
+    the first top_k classes stay (0: all), of those the shortest prefix that holds top_p
+    of their weight, and of those the ones with at least min_p times the largest weight.
+    The class is the first, by number, at which the running share of what stays exceeds
+    the row's uniform number; log_probs is the logarithm of its own share. temperature 0
+    takes the largest logit. Each option is a number, or a tensor of one a row (float32;
+    top_k int32), whose values the device reads: there 0 or less, and NaN, are
+    temperature 0, no top_k, top_p 0 (NaN: 1) and min_p 0.
+
+    Logits of -inf or NaN are masked; a row with no others gets class -1 and -inf. At most
+    262144 classes. Weights are held as whole numbers of 2^-45 of the largest one, so the
+    drawn classes are the same wherever and however often they are drawn."""
+    torch = _need_torch()
+    logits = _device_tensor(logits, "logits")
+    cells = _cells(logits, "logits")
+    if logits.dim() < 1 or not 1 <= logits.shape[-1] <= 262144:
+        raise ValueError(f"logits must be (..., 1 to 262144 classes), got shape "
+                         f"{tuple(logits.shape)}")
+    lead = tuple(logits.shape[:-1])
+    uniforms = _beside(_device_tensor(uniforms, "uniforms"), logits, "uniforms")
+    if uniforms.dtype != torch.float32 or tuple(uniforms.shape) != lead:
+        raise ValueError(f"uniforms must be float32 of shape {lead}, got {uniforms.dtype} of "
+                         f"{tuple(uniforms.shape)}")
+    o = N.SampleOptions()
+    f32 = torch.float32
+    o.temperature, a = _option(temperature, "temperature", lead, logits, f32, _temperature)
+    o.top_k, b = _option(top_k, "top_k", lead, logits, torch.int32, _top_k)
+    o.top_p, c = _option(top_p, "top_p", lead, logits, f32, lambda v: _share("top_p", v))
+    o.min_p, d = _option(min_p, "min_p", lead, logits, f32, lambda v: _share("min_p", v))
+    o.temperatures, o.top_ks, o.top_ps, o.min_ps = (
+        None if t is None else t.data_ptr() for t in (a, b, c, d))
+    classes = logits.new_empty(lead, dtype=torch.int64)
+    log_probs = logits.new_empty(lead, dtype=f32)
+    N.check_hip(N.hip().fbh_sample_classes(
+        logits.device.index, logits.data_ptr(), classes.numel(), logits.shape[-1], cells,
+        uniforms.data_ptr(), C.byref(o), classes.data_ptr(), log_probs.data_ptr(),
+        _stream(logits.device)))
+    return classes, log_probs

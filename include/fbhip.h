@@ -713,6 +713,110 @@ int fbh_predict_device(fbh_shap_model *m, const float *d_rows, uint64_t n_rows,
 int fbh_shap_contribs_noalloc(fbh_shap_model *m, const float *rows, uint64_t n_rows,
                               const float *margin, float *out);
 
+/* ------------------------------------------------ heads on a model's outputs
+ * What a program does with leaf ids, categorical codes and class margins after
+ * the model has given them: vectors learned for the ids, dropout while they are
+ * learned, classes drawn from the margins. No reference counterpart.
+ *
+ * All pointers are device memory of `device` unless a comment says host, tensors
+ * are dense and row-major, and any alignment of their cells' size does. Calls
+ * are enqueued on `stream` (a hipStream_t; NULL: the default stream), do not
+ * wait, allocate nothing and can be captured into a graph; the caller's current
+ * device is the same afterwards. Results are the same in every call. Whatever a
+ * call reads must stay unchanged until the stream has passed it. */
+
+/* Cell types of tables, vectors and logits; types of ids. */
+enum { FBH_F32 = 0, FBH_F16 = 1, FBH_BF16 = 2 };
+enum { FBH_ID_I32 = 0, FBH_ID_I64 = 1, FBH_ID_F32 = 2 };
+
+/* Ids of n_rows rows and n_columns columns (trees, categorical columns), and the
+ * table of n_tokens vectors of dim cells that they stand for. Column t's ids are
+ * 0 .. first[t + 1] - first[t] - 1 and take table rows from first[t] on (first:
+ * n_columns + 1 offsets, at most 32768 columns); with first NULL every column's
+ * ids are the table's rows. FBH_ID_F32 are whole numbers as FBH_PREDICT_LEAF
+ * writes them. A position whose id is anything else (negative, too large, no
+ * whole number) takes and gives nothing; so does one that is dropped: with
+ * drop > 0 each position stays with probability 1 - drop, drawn from seed and
+ * the position's number (row * n_columns + column) as fbh_dropout draws its
+ * elements, and what stays is scaled by 1 / (1 - drop). dim at most 32768. */
+typedef struct {
+    uint64_t n_rows;
+    uint32_t n_columns;
+    uint32_t dim;
+    uint32_t n_tokens;
+    uint32_t id_type;
+    uint32_t dtype;
+    uint32_t pooled;  /* 1: a row's vectors are summed, 0: as they are */
+    const void *ids;
+    const uint32_t *first;
+    double drop;
+    uint64_t seed;
+    float scale;
+    uint32_t reserved;
+} fbh_embed;
+
+/* out[row] = scale * the sum over columns of the positions' table rows, [n_rows]
+ * [dim] (pooled), or out[row][column] = scale * the position's table row,
+ * [n_rows][n_columns][dim] (zeros where there is none). Sums are taken in f32 in
+ * an order that depends on the column alone, and rounded once. A model's margins
+ * are the pooled embedding of its leaf ids in the table of its leaf values. */
+int fbh_embed_rows(int device, const fbh_embed *e, const void *table, void *out, void *stream);
+/* Device bytes of workspace that fbh_embed_grad takes; 0 for a call that it
+ * refuses. */
+uint64_t fbh_embed_grad_bytes(const fbh_embed *e);
+/* The gradient of fbh_embed_rows by its table: table_grad[v] = scale * the sum
+ * over positions of token v of the output's gradient there (grad, laid out as
+ * out), for every v (zeros where there is no position), in the table's type.
+ * Positions are sorted by token and summed in f32 in a fixed order. At most
+ * 2^31 - 1 positions. */
+int fbh_embed_grad(int device, const fbh_embed *e, const void *grad, void *table_grad, void *work,
+                   uint64_t work_bytes, void *stream);
+
+/* out[i] = x[i] / (1 - drop) where element first + i stays, else 0 (whatever x[i]
+ * is), for 0 <= drop < 1. Whether an element stays is a function of seed and its
+ * number alone (SplitMix64's finaliser, as for row sampling; the probability is
+ * rounded to 2^-32), so nothing is stored: the gradient is the same call on the
+ * output's gradient, and a part of a tensor is dropped as in the whole when
+ * first is its first element's number. out may be x. */
+int fbh_dropout(int device, const void *x, void *out, uint64_t n, uint32_t dtype, double drop,
+                uint64_t seed, uint64_t first, void *stream);
+
+/* How classes are drawn: a value for every row, or one of each row's own (device
+ * pointers, n_rows values each; NULL: the one beside it). */
+typedef struct {
+    const float *temperatures;
+    const int32_t *top_ks;
+    const float *top_ps;
+    const float *min_ps;
+    float temperature;
+    int32_t top_k;
+    float top_p;
+    float min_p;
+} fbh_sample_options;
+
+/* One class for each row of logits (class margins) [n_rows][n_classes] and uniform
+ * number in [0, 1). With l the row's largest logit, class c has weight
+ * exp((logit[c] - l) / temperature), rounded to 2^-45, so that sums are exact in
+ * any order. Ordered by falling logit (equal ones by class), the first top_k
+ * classes stay (top_k <= 0: all); of those the shortest prefix that holds top_p
+ * of their weight; of those the ones with at least min_p times the largest
+ * weight. classes[row] is the first class, by number, whose weight and those of
+ * the staying classes before it exceed the row's uniform number times the sum of
+ * all that stay; log_probs[row] (may be NULL) the logarithm of its share of that
+ * sum. temperature <= 0 or NaN takes the largest logit (the lowest class of equal
+ * ones). Logits of minus infinity or NaN are masked; a row with nothing else
+ * gets class -1 and minus infinity. top_p is taken to be in 0 .. 1 (0: the first
+ * class; NaN: 1), min_p too (NaN: 0), the uniform number in 0 .. 1 - 2^-31. At
+ * most 262144 classes. */
+int fbh_sample_classes(int device, const void *logits, uint64_t n_rows, uint32_t n_classes,
+                       uint32_t dtype, const float *uniforms, const fbh_sample_options *options,
+                       int64_t *classes, float *log_probs, void *stream);
+/* The same with logits (f32), uniforms and results in host memory and one set of
+ * options (no pointers in it); returns when the results are there. */
+int fbh_sample_classes_host(int device, const float *logits, uint64_t n_rows, uint32_t n_classes,
+                            const float *uniforms, const fbh_sample_options *options,
+                            int64_t *classes, float *log_probs);
+
 #ifdef __cplusplus
 }
 #endif
