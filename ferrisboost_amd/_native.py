@@ -186,7 +186,7 @@ class Embed(C.Structure):
         ("drop", C.c_double),
         ("seed", C.c_uint64),
         ("scale", C.c_float),
-        ("reserved", C.c_uint32),
+        ("most_ids", C.c_uint32),
     ]
 
 

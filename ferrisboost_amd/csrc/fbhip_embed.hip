@@ -43,18 +43,27 @@ __device__ __forceinline__ uint32_t load_id(const void *ids, uint64_t at) {
     }
 }
 
+// A column's part of the table, inside it whatever `first` says.
+struct Part {
+    uint32_t base, size;
+};
+__device__ __forceinline__ Part part_of(const Positions &P, uint32_t column) {
+    if (!P.first) return {0, P.n_tokens};
+    const uint32_t base = min(P.first[column], P.n_tokens);
+    return {base, min(P.first[column + 1] - base, P.n_tokens - base)};
+}
+
 // The table row of a position, or NO_TOKEN.
+template <bool DROP>
+__device__ __forceinline__ uint32_t token_of(const Positions &P, Part part, uint32_t id,
+                                             uint64_t pos) {
+    bool ok = id < part.size;
+    if (DROP) ok = ok && drop_bits(P.key, pos) >= P.threshold;
+    return ok ? part.base + id : NO_TOKEN;
+}
 template <int ID, bool DROP>
 __device__ __forceinline__ uint32_t token_at(const Positions &P, uint64_t pos, uint32_t column) {
-    const uint32_t id = load_id<ID>(P.ids, pos);
-    uint32_t base = 0, size = P.n_tokens;
-    if (P.first) {
-        base = P.first[column];
-        size = P.first[column + 1] - base;
-    }
-    bool ok = id < size && id < P.n_tokens && base < P.n_tokens - id;
-    if (DROP) ok = ok && drop_bits(P.key, pos) >= P.threshold;
-    return ok ? base + id : NO_TOKEN;
+    return token_of<DROP>(P, part_of(P, column), load_id<ID>(P.ids, pos), pos);
 }
 
 // l / d for l + d below 2^31 and l * d below 2^32 (d > 1: m = ceil(2^32 / d)).
@@ -70,45 +79,49 @@ __device__ __forceinline__ uint32_t divide(uint32_t l, Divisor v) {
 
 // ------------------------------------------------------------------- looked up
 constexpr uint32_t ROW_PIECES = 4;  // pieces of a thread, all requested at once
+constexpr uint32_t ROW_BLOCK = EMB_TPB * ROW_PIECES;
 
 // out[pos] = s * table[token(pos)]: the output in pieces of VEC cells, flat over the
-// workgroups. A vector's last piece starts at dim - VEC, so that no piece is partial;
-// the cells it shares with the piece before are written twice, with the same value.
+// workgroups, whose positions' tokens are found once and kept in LDS. A vector's last
+// piece starts at dim - VEC, so that no piece is partial; the cells it shares with the
+// piece before are written twice, with the same value.
 template <class T, int VEC, int ID, bool DROP>
 __global__ __launch_bounds__(EMB_TPB) void embed_rows_kernel(Positions P, const T *table, T *out,
                                                              uint32_t dim, Divisor pieces,
                                                              Divisor columns, float s) {
+    __shared__ uint32_t toks[ROW_BLOCK + 1];
     const uint64_t block = blockIdx.x + (uint64_t)blockIdx.y * gridDim.x;
-    const uint64_t base = block * (EMB_TPB * ROW_PIECES);
+    const uint64_t base = block * ROW_BLOCK;
     const uint64_t n_pos = P.n_rows * P.n_columns;
     const uint64_t pos0 = base / pieces.d;
     const uint32_t rem0 = (uint32_t)(base - pos0 * pieces.d);
     const uint32_t col0 = (uint32_t)(pos0 % columns.d);
-    uint64_t at[ROW_PIECES];
-    uint32_t tok[ROW_PIECES], cell[ROW_PIECES];
+    const uint32_t n = divide(rem0 + ROW_BLOCK - 1, pieces) + 1;  // positions of the block
+    for (uint32_t q = threadIdx.x; q < n; q += EMB_TPB) {
+        const uint32_t c = col0 + q;
+        toks[q] = pos0 + q < n_pos ? token_at<ID, DROP>(P, pos0 + q,
+                                                        c - divide(c, columns) * columns.d)
+                                   : NO_TOKEN;
+    }
+    __syncthreads();
+    uint32_t q[ROW_PIECES], tok[ROW_PIECES], cell[ROW_PIECES];
+    Piece<T, VEC> p[ROW_PIECES];
 #pragma unroll
     for (uint32_t k = 0; k < ROW_PIECES; k++) {
         const uint32_t l = rem0 + k * EMB_TPB + threadIdx.x;
-        const uint32_t q = divide(l, pieces);
-        at[k] = pos0 + q;
-        cell[k] = min((l - q * pieces.d) * VEC, dim - VEC);
-        const uint32_t c = col0 + q;
-        tok[k] = at[k] < n_pos
-                     ? token_at<ID, DROP>(P, at[k], c - divide(c, columns) * columns.d)
-                     : NO_TOKEN;
-    }
-    Piece<T, VEC> p[ROW_PIECES];
-#pragma unroll
-    for (uint32_t k = 0; k < ROW_PIECES; k++)
+        q[k] = divide(l, pieces);
+        cell[k] = min((l - q[k] * pieces.d) * VEC, dim - VEC);
+        tok[k] = toks[q[k]];
         p[k] = load_piece<T, VEC>(table + (uint64_t)(tok[k] == NO_TOKEN ? 0 : tok[k]) * dim +
                                   cell[k]);
+    }
 #pragma unroll
     for (uint32_t k = 0; k < ROW_PIECES; k++) {
-        if (at[k] >= n_pos) continue;
+        if (pos0 + q[k] >= n_pos) continue;
 #pragma unroll
         for (int i = 0; i < VEC; i++)
             p[k].v[i] = tok[k] == NO_TOKEN ? (T)0.0f : (T)((float)p[k].v[i] * s);
-        store_piece<T, VEC>(out + at[k] * dim + cell[k], p[k]);
+        store_piece<T, VEC>(out + (pos0 + q[k]) * dim + cell[k], p[k]);
     }
 }
 
@@ -122,8 +135,9 @@ __device__ __forceinline__ float tree8(const float *a) {
 
 // A workgroup takes 256 / G rows, G = 2^lg_g lanes a row; the tokens of 2^lg_c columns at
 // a time are found by all threads in turn and kept in LDS, so that an id is decoded (and
-// its bits drawn) once and not by every lane of its row.
-template <class T, int VEC, int ID, bool DROP>
+// its bits drawn) once and not by every lane of its row. BUFFER: what is kept are their
+// rows' byte offsets, and the table is read by buffer loads.
+template <class T, int VEC, int ID, bool DROP, bool BUFFER>
 __global__ __launch_bounds__(EMB_TPB) void embed_sum_kernel(Positions P, const T *table, T *out,
                                                             uint32_t dim, uint32_t n_pieces,
                                                             uint32_t lg_g, uint32_t lg_c,
@@ -134,8 +148,10 @@ __global__ __launch_bounds__(EMB_TPB) void embed_sum_kernel(Positions P, const T
     const uint32_t r = threadIdx.x >> lg_g;
     const uint32_t piece = blockIdx.y * (1u << lg_g) + (threadIdx.x & ((1u << lg_g) - 1));
     const bool live = row0 + r < P.n_rows && piece < n_pieces;
-    const uint32_t cell = min(piece * VEC, dim - VEC);
-    const T *from = table + (live ? cell : 0);
+    const uint32_t cell = live ? min(piece * VEC, dim - VEC) : 0;
+    const uint32_t row_bytes = dim * (uint32_t)sizeof(T), cell_bytes = cell * (uint32_t)sizeof(T);
+    const auto rsrc = buffer_of(table, BUFFER ? P.n_tokens * row_bytes : 0);
+    const T *from = table + cell;
     float a[VEC][8];
 #pragma unroll
     for (int i = 0; i < VEC; i++)
@@ -144,10 +160,11 @@ __global__ __launch_bounds__(EMB_TPB) void embed_sum_kernel(Positions P, const T
     for (uint32_t t0 = 0; t0 < P.n_columns; t0 += cols) {
         for (uint32_t i = threadIdx.x; i < rows << lg_c; i += EMB_TPB) {
             const uint32_t rr = i >> lg_c, t = t0 + (i & (cols - 1));
-            toks[rr * pitch + (i & (cols - 1))] =
-                row0 + rr < P.n_rows && t < P.n_columns
-                    ? token_at<ID, DROP>(P, (row0 + rr) * P.n_columns + t, t)
-                    : NO_TOKEN;
+            uint32_t tok = NO_TOKEN;
+            if (row0 + rr < P.n_rows && t < P.n_columns)
+                tok = token_at<ID, DROP>(P, (row0 + rr) * P.n_columns + t, t);
+            if (BUFFER) tok = tok == NO_TOKEN ? NO_OFFSET : tok * row_bytes;
+            toks[rr * pitch + (i & (cols - 1))] = tok;
         }
         __syncthreads();
         const uint32_t most = min(cols, P.n_columns - t0);
@@ -159,15 +176,25 @@ __global__ __launch_bounds__(EMB_TPB) void embed_sum_kernel(Positions P, const T
                     *reinterpret_cast<const uint4 *>(&toks[r * pitch + c]);
                 *reinterpret_cast<uint4 *>(tok + 4) =
                     *reinterpret_cast<const uint4 *>(&toks[r * pitch + c + 4]);
+                if constexpr (BUFFER) {
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-                    p[j] = load_piece<T, VEC>(from +
-                                              (uint64_t)(tok[j] == NO_TOKEN ? 0 : tok[j]) * dim);
+                    for (int j = 0; j < 8; j++)
+                        p[j] = load_offset<T, VEC>(rsrc, tok[j] + cell_bytes);
 #pragma unroll
-                for (int j = 0; j < 8; j++)
+                    for (int j = 0; j < 8; j++)
 #pragma unroll
-                    for (int i = 0; i < VEC; i++)
-                        a[i][j] += tok[j] == NO_TOKEN ? 0.0f : (float)p[j].v[i];
+                        for (int i = 0; i < VEC; i++) a[i][j] += (float)p[j].v[i];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        p[j] = load_piece<T, VEC>(
+                            from + (uint64_t)(tok[j] == NO_TOKEN ? 0 : tok[j]) * dim);
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+#pragma unroll
+                        for (int i = 0; i < VEC; i++)
+                            a[i][j] += tok[j] == NO_TOKEN ? 0.0f : (float)p[j].v[i];
+                }
             }
         __syncthreads();
     }
@@ -554,6 +581,331 @@ __global__ __launch_bounds__(EMB_TPB) void grad_join_kernel(Runs R, T *table) {
     }
 }
 
+// ---- Many rows of columns with few ids each (a model's trees, categorical columns).
+// Each column's part of the table is summed over chunks of rows: a workgroup sorts a
+// chunk's ids of one column in LDS, sums the runs, and leaves a part of the table (with
+// the counts of its tokens) that the last kernel adds up chunk by chunk. Nothing is
+// sorted through memory, and the gradient rows that all columns of a chunk gather stay in
+// one XCD's L2: workgroups of one chunk have numbers equal modulo the 8 XCDs.
+constexpr uint32_t COL_TPB = 512;
+constexpr uint32_t COL_WAVES = COL_TPB / 64;
+constexpr uint32_t COL_ITEMS = 32;                       // rows of a thread at most
+constexpr uint32_t COL_MOST_ROWS = COL_TPB * COL_ITEMS;  // of a chunk: list entries are 16-bit
+constexpr uint32_t COL_MOST_IDS = 1024;
+constexpr uint32_t COL_NONE = 0xFFFF;
+
+// local[column][row]: the id inside its column, COL_NONE where the position gives
+// nothing; rows up to `padded` are written. 64 x 64 positions through LDS.
+template <int ID, bool DROP>
+__global__ __launch_bounds__(256) void column_ids_kernel(Positions P, uint32_t most_ids,
+                                                         uint64_t padded, uint16_t *local) {
+    __shared__ uint16_t tile[64][66];
+    const uint64_t row0 = (uint64_t)blockIdx.x * 64;
+    const uint32_t col0 = blockIdx.y * 64, lane = threadIdx.x & 63, w = threadIdx.x / 64;
+    const uint32_t column = col0 + lane;
+    uint32_t id[16];
+#pragma unroll
+    for (uint32_t r = 0; r < 16; r++) {
+        const uint64_t row = row0 + w + 4 * r;
+        id[r] = row < P.n_rows && column < P.n_columns
+                    ? load_id<ID>(P.ids, row * P.n_columns + column)
+                    : NO_TOKEN;
+    }
+    Part part{0, 0};
+    if (column < P.n_columns) part = part_of(P, column);
+    part.size = min(part.size, most_ids);
+#pragma unroll
+    for (uint32_t r = 0; r < 16; r++) {
+        const uint32_t tok =
+            token_of<DROP>(P, part, id[r], (row0 + w + 4 * r) * P.n_columns + column);
+        tile[w + 4 * r][lane] = tok != NO_TOKEN ? (uint16_t)id[r] : (uint16_t)COL_NONE;
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (uint32_t c = w; c < 64; c += 4)
+        if (col0 + c < P.n_columns && row0 + lane < padded)
+            local[(col0 + c) * padded + row0 + lane] = tile[lane][c];
+}
+
+struct Columns {
+    const uint16_t *local;
+    const uint32_t *first;   // NULL: one column, from row 0
+    uint64_t n_rows, padded;
+    uint32_t n_columns, n_tokens, most_ids;
+    uint32_t chunk, chunks;  // rows of a chunk (a multiple of 64), chunks
+    uint32_t per_row;        // gradient vectors of a row: 1 (pooled) or the columns
+    uint32_t dim, n_pieces, lg_g;
+    float s;
+    float *parts;            // [chunk][token][dim]
+    uint16_t *counts;        // [chunk][token]: positions in the chunk
+};
+
+// LDS of column_sums_kernel, in byte offsets: the waves' counters and later the ranges'
+// open sums; the ids' first blocks; the rows by id, each id's in blocks of 8.
+struct ColumnLds {
+    uint32_t starts, list, bytes;
+};
+__host__ __device__ inline ColumnLds column_lds(uint32_t most_ids, uint32_t chunk, uint32_t vec) {
+    ColumnLds l{};
+    const uint32_t seen = (COL_WAVES * most_ids * 2 + 15) & ~15u, sums = COL_TPB * vec * 4;
+    l.starts = seen > sums ? seen : sums;
+    l.list = l.starts + (((most_ids + 1) * 2 + 15) & ~15u);
+    l.bytes = l.list + (chunk + 8 * most_ids) * 2;
+    return l;
+}
+
+// BUFFER: the chunk's gradient rows are read by buffer loads, and the entries that fill an
+// id's last block (row `chunk`, behind the buffer) read as zeros.
+template <class T, int VEC, bool BUFFER>
+__global__ __launch_bounds__(COL_TPB) void column_sums_kernel(Columns C, const T *grad,
+                                                              T *table) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    __shared__ uint32_t wave_sum[COL_WAVES];
+    // (chunk group, column, chunk of the group): a group's chunks go to one XCD each
+    const uint32_t per = min(C.chunks, 8u);
+    const uint32_t chunk = blockIdx.x / (C.n_columns * per) * per + blockIdx.x % per;
+    const uint32_t t = blockIdx.x / per % C.n_columns;
+    if (chunk >= C.chunks) return;
+    const ColumnLds L = column_lds(C.most_ids, C.chunk, VEC);
+    uint16_t *seen = reinterpret_cast<uint16_t *>(lds);
+    float *sums = reinterpret_cast<float *>(lds);
+    uint16_t *starts = reinterpret_cast<uint16_t *>(lds + L.starts);
+    uint16_t *list = reinterpret_cast<uint16_t *>(lds + L.list);
+    const uint32_t base = C.first ? min(C.first[t], C.n_tokens) : 0;
+    const uint32_t ids = min(C.most_ids, C.first ? min(C.first[t + 1] - base, C.n_tokens - base)
+                                                 : C.n_tokens);
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x / 64;
+    const uint64_t row0 = (uint64_t)chunk * C.chunk;
+    const uint16_t *from = C.local + t * C.padded + row0;
+
+    // ---- the chunk's rows by id. A wave takes `rounds` times 256 rows, a lane 4 of them
+    // side by side; "before" is by wave, then by round and place in the four, then by
+    // lane: any order that is always the same will do.
+    for (uint32_t i = threadIdx.x; i < COL_WAVES * C.most_ids; i += COL_TPB) seen[i] = 0;
+    const uint32_t fill = C.chunk | C.chunk << 16;
+    for (uint32_t i = threadIdx.x; i < (C.chunk + 8 * C.most_ids) / 8; i += COL_TPB)
+        reinterpret_cast<uint4 *>(list)[i] = make_uint4(fill, fill, fill, fill);
+    __syncthreads();
+    uint32_t key[COL_ITEMS / 2], rank[COL_ITEMS / 2];  // two rows a word
+    const uint32_t rounds = (C.chunk + COL_WAVES * 256 - 1) / (COL_WAVES * 256);
+#pragma unroll
+    for (uint32_t r = 0; r < COL_ITEMS / 4; r++) {
+        const uint32_t at = (w * rounds + r) * 256 + lane * 4;
+        uint2 q = make_uint2(~0u, ~0u);
+        if (r < rounds && at < C.chunk) q = *reinterpret_cast<const uint2 *>(from + at);
+        key[2 * r] = q.x;
+        key[2 * r + 1] = q.y;
+    }
+    const uint32_t bits = 32 - __clz(max(C.most_ids - 1, 1u));
+    uint16_t *mine = seen + w * C.most_ids;
+#pragma unroll
+    for (uint32_t r = 0; r < COL_ITEMS / 4; r++)
+        if (r < rounds)
+#pragma unroll
+            for (uint32_t i = 4 * r; i < 4 * r + 4; i++) {
+                const uint32_t k = (key[i / 2] >> (16 * (i & 1))) & 0xFFFFu;
+                const bool in = k != COL_NONE;
+                uint64_t same = __ballot(in);
+                for (uint32_t b = 0; b < bits; b++) {
+                    const bool one = (k >> b) & 1;
+                    const uint64_t ones = __ballot(one);
+                    same &= one ? ones : ~ones;
+                }
+                const uint32_t below = __popcll(same & ((1ull << lane) - 1));
+                uint32_t before = 0;
+                if (in) before = *(volatile uint16_t *)&mine[k];
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                if (in && below == 0)
+                    *(volatile uint16_t *)&mine[k] = (uint16_t)(before + __popcll(same));
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                const uint32_t at = before + below;
+                rank[i / 2] = i & 1 ? rank[i / 2] | at << 16 : at;
+            }
+    __syncthreads();
+    // starts[id]: the blocks of lower ids, two ids a thread
+    {
+        uint32_t c[2] = {0, 0};
+        for (uint32_t j = 0; j < 2; j++) {
+            const uint32_t id = 2 * threadIdx.x + j;
+            if (id < C.most_ids)
+                for (uint32_t v = 0; v < COL_WAVES; v++) c[j] += seen[v * C.most_ids + id];
+        }
+        const uint32_t b0 = (c[0] + 7) / 8, b1 = (c[1] + 7) / 8;
+        uint32_t x = b0 + b1;
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t y = __shfl_up(x, d);
+            if (lane >= (uint32_t)d) x += y;
+        }
+        if (lane == 63) wave_sum[w] = x;
+        __syncthreads();
+        uint32_t at = x - b0 - b1;
+        for (uint32_t v = 0; v < w; v++) at += wave_sum[v];
+        for (uint32_t j = 0; j < 2; j++) {
+            const uint32_t id = 2 * threadIdx.x + j;
+            if (id < C.most_ids) {
+                starts[id] = (uint16_t)at;
+                if (id < ids) C.counts[(uint64_t)chunk * C.n_tokens + base + id] = (uint16_t)c[j];
+                uint32_t a = 8 * at;
+                for (uint32_t v = 0; v < COL_WAVES; v++) {
+                    const uint32_t n = seen[v * C.most_ids + id];
+                    seen[v * C.most_ids + id] = (uint16_t)a;
+                    a += n;
+                }
+                at += j ? b1 : b0;
+                if (id == C.most_ids - 1) starts[C.most_ids] = (uint16_t)at;
+            }
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < COL_ITEMS; i++) {
+        const uint32_t k = (key[i / 2] >> (16 * (i & 1))) & 0xFFFFu;
+        if (i / 4 < rounds && k != COL_NONE)
+            list[mine[k] + ((rank[i / 2] >> (16 * (i & 1))) & 0xFFFFu)] =
+                (uint16_t)((w * rounds + i / 4) * 256 + lane * 4 + (i & 3));
+    }
+    __syncthreads();
+
+    // ---- sums: the blocks in equal ranges, 2^lg_g lanes a range. Runs inside a range go
+    // to memory; a range leaves the sum of the run that it continues in LDS, and adds
+    // those behind it to the run that starts in it and goes on.
+    const uint32_t g = threadIdx.x >> C.lg_g, glane = threadIdx.x & ((1u << C.lg_g) - 1);
+    const uint32_t groups = COL_TPB >> C.lg_g;
+    const uint32_t piece = (blockIdx.y << C.lg_g) + glane;
+    const bool live = piece < C.n_pieces;
+    const uint32_t cell = live ? min(piece * VEC, C.dim - VEC) : 0;
+    const uint32_t n = starts[C.most_ids];
+    const uint32_t each = (n + groups - 1) / groups;
+    const uint32_t i0 = min(g * each, n), i1 = min(i0 + each, n);
+    const uint64_t pitch = (uint64_t)C.per_row * C.dim;
+    const T *rows = grad + row0 * pitch + (C.per_row > 1 ? (uint64_t)t * C.dim : 0);
+    const uint32_t row_bytes = (uint32_t)(pitch * sizeof(T)),
+                   cell_bytes = cell * (uint32_t)sizeof(T);
+    const auto rsrc = buffer_of(rows, BUFFER ? C.chunk * row_bytes : 0);
+    const bool whole = C.chunks == 1;
+    float a[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; i++) a[i] = 0.0f;
+    const auto write = [&](uint32_t id) {
+        const uint64_t at = (uint64_t)(base + id) * C.dim + cell;
+        if (whole) {
+            Piece<T, VEC> o;
+#pragma unroll
+            for (int i = 0; i < VEC; i++) o.v[i] = (T)(a[i] * C.s);
+            store_piece<T, VEC>(table + at, o);
+        } else {
+            Piece<float, VEC> o;
+#pragma unroll
+            for (int i = 0; i < VEC; i++) o.v[i] = a[i];
+            store_piece<float, VEC>(C.parts + (uint64_t)chunk * C.n_tokens * C.dim + at, o);
+        }
+    };
+    const auto leave = [&] {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) sums[threadIdx.x * VEC + i] = a[i];
+    };
+    uint32_t id = 0, end = 0;
+    bool begun = false;  // the run starts in this range
+    if (live && i0 < i1) {
+        uint32_t lo = 0, hi = C.most_ids;  // the last id whose blocks start at or before i0
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (starts[mid] <= i0) lo = mid;
+            else hi = mid;
+        }
+        id = lo;
+        end = starts[id + 1];
+        begun = starts[id] == i0;
+        for (uint32_t b = i0; b < i1; b++) {
+            const uint4 q = reinterpret_cast<const uint4 *>(list)[b];
+            const uint32_t pair[4] = {q.x, q.y, q.z, q.w};
+            Piece<T, VEC> p[8];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) {
+                const uint32_t row = (pair[j / 2] >> (16 * (j & 1))) & 0xFFFFu;
+                if constexpr (BUFFER) p[j] = load_offset<T, VEC>(rsrc, row * row_bytes + cell_bytes);
+                else p[j] = load_piece<T, VEC>(rows + (row < C.chunk ? row : 0) * pitch + cell);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) {
+                const bool none =
+                    !BUFFER && ((pair[j / 2] >> (16 * (j & 1))) & 0xFFFFu) >= C.chunk;
+#pragma unroll
+                for (int i = 0; i < VEC; i++) a[i] += none ? 0.0f : (float)p[j].v[i];
+            }
+            if (b + 1 == end) {
+                if (begun) write(id);
+                else leave();
+                begun = true;
+#pragma unroll
+                for (int i = 0; i < VEC; i++) a[i] = 0.0f;
+                if (b + 1 < i1) {
+                    do id++, end = starts[id + 1];
+                    while (end == b + 1);
+                } else {
+                    end = 0;  // nothing is open
+                }
+            }
+        }
+        if (end && !begun) {
+            leave();
+            end = 0;
+        }
+    }
+    if (whole && live) {
+        for (uint32_t k = g; k < ids; k += groups)
+            if (starts[k] == starts[k + 1]) {
+                const uint64_t at = (uint64_t)(base + k) * C.dim + cell;
+                Piece<T, VEC> o;
+#pragma unroll
+                for (int i = 0; i < VEC; i++) o.v[i] = (T)0.0f;
+                store_piece<T, VEC>(table + at, o);
+            }
+    }
+    __syncthreads();
+    if (end) {
+        for (uint32_t h = g + 1; h * each < end; h++)
+#pragma unroll
+            for (int i = 0; i < VEC; i++) a[i] += sums[((h << C.lg_g) + glane) * VEC + i];
+        write(id);
+    }
+}
+
+// table[token] = s * the sum of its parts, in chunk order.
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void column_join_kernel(Columns C, T *table) {
+    const uint64_t i = blockIdx.x * 256ull + threadIdx.x;
+    const uint64_t tok = i / C.n_pieces;
+    if (tok >= C.n_tokens) return;
+    const uint32_t cell = min((uint32_t)(i - tok * C.n_pieces) * VEC, C.dim - VEC);
+    const float *part = C.parts + tok * C.dim + cell;
+    float a[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; j++) a[j] = 0.0f;
+    for (uint32_t c0 = 0; c0 < C.chunks; c0 += 8) {
+        bool some[8];
+        Piece<float, VEC> p[8];
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k++)
+            some[k] = c0 + k < C.chunks && C.counts[(uint64_t)(c0 + k) * C.n_tokens + tok] != 0;
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k++)
+            if (some[k])
+                p[k] = load_piece<float, VEC>(part + (uint64_t)(c0 + k) * C.n_tokens * C.dim);
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k++)
+            if (some[k])
+#pragma unroll
+                for (int j = 0; j < VEC; j++) a[j] += p[k].v[j];
+    }
+    Piece<T, VEC> o;
+#pragma unroll
+    for (int j = 0; j < VEC; j++) o.v[j] = (T)(a[j] * C.s);
+    store_piece<T, VEC>(table + tok * C.dim + cell, o);
+}
+
 // ------------------------------------------------------------------- host side
 uint32_t lg_at_least(uint64_t n) {
     uint32_t l = 0;
@@ -573,6 +925,7 @@ void check_embed(const fbh_embed *e) {
                "n_tokens must be in 1..=2147483647");
     head_input(e->ids || e->n_rows == 0, "null argument");
     head_input(e->n_rows <= (1ull << 40) / e->n_columns, "more than 2^40 positions");
+    head_input(e->most_ids <= e->n_tokens, "most_ids is larger than the table");
     (void)drop_threshold(e->drop);
 }
 
@@ -587,6 +940,11 @@ Positions positions_of(const fbh_embed *e) {
 }
 
 float scale_of(const fbh_embed *e) { return (float)((double)e->scale / (1.0 - e->drop)); }
+
+// Whether buffer loads reach rows of row_bytes from p on: their bytes, in words.
+bool in_buffer(const void *p, uint64_t bytes, uint64_t row_bytes) {
+    return bytes <= BUFFER_MOST && row_bytes % 4 == 0 && reinterpret_cast<uintptr_t>(p) % 4 == 0;
+}
 
 // Cells of a piece: the largest power of two up to 16 bytes and the vector's width.
 uint32_t piece_cells(uint32_t dim, uint32_t dtype) {
@@ -604,7 +962,7 @@ void launch_embed(const fbh_embed *e, const void *table, void *out, hipStream_t 
     const float sc = scale_of(e);
     if (!e->pooled) {
         const uint64_t blocks =
-            (P.n_rows * P.n_columns * pieces + EMB_TPB * ROW_PIECES - 1) / (EMB_TPB * ROW_PIECES);
+            (P.n_rows * P.n_columns * pieces + ROW_BLOCK - 1) / ROW_BLOCK;
         const uint32_t bx = (uint32_t)std::min<uint64_t>(blocks, 1u << 22);
         const uint64_t by = (blocks + bx - 1) / bx;
         head_input(by <= 65535, "too many cells");
@@ -623,10 +981,17 @@ void launch_embed(const fbh_embed *e, const void *table, void *out, hipStream_t 
             std::min(std::max(lg_at_least(P.n_columns), 3u), lg_at_least(4096 / rows));
         const uint64_t blocks = (P.n_rows + rows - 1) / rows;
         head_input(blocks < 1u << 24, "too many rows");
-        hipLaunchKernelGGL((embed_sum_kernel<T, VEC, ID, DROP>),
-                           dim3((uint32_t)blocks, (pieces + (1u << lg_g) - 1) >> lg_g),
-                           dim3(EMB_TPB), (size_t)rows * ((1u << lg_c) + 4) * 4, s, P, tab, to,
-                           e->dim, pieces, lg_g, lg_c, sc);
+        const auto go = [&](auto buffer) {
+            hipLaunchKernelGGL((embed_sum_kernel<T, VEC, ID, DROP, decltype(buffer)::value>),
+                               dim3((uint32_t)blocks, (pieces + (1u << lg_g) - 1) >> lg_g),
+                               dim3(EMB_TPB), (size_t)rows * ((1u << lg_c) + 4) * 4, s, P, tab,
+                               to, e->dim, pieces, lg_g, lg_c, sc);
+        };
+        if constexpr (VEC * sizeof(T) >= 4) {
+            if (in_buffer(table, (uint64_t)e->n_tokens * e->dim * sizeof(T), e->dim * sizeof(T)))
+                go(std::true_type{});
+            else go(std::false_type{});
+        } else go(std::false_type{});
     }
     head_check(hipGetLastError(), "embedding");
 }
@@ -661,6 +1026,47 @@ void with_ids(uint32_t id_type, bool drop, F &&f) {
     else go(std::false_type{});
 }
 
+// The chunks of rows that columns of few ids are summed in; 0: they are sorted by token
+// instead. A chunk of a column has 8 positions an id on average at least, so that the
+// parts are written and read for less than the gradient rows take, and a call has 64k
+// positions at least.
+struct ColumnPlan {
+    uint32_t chunk = 0, chunks = 0;
+    uint64_t padded = 0, local = 0, counts = 0, parts = 0, bytes = 0;
+};
+
+ColumnPlan column_plan(const fbh_embed *e) {
+    ColumnPlan c;
+    const uint64_t ids = e->first ? e->most_ids : e->n_tokens;
+    const uint64_t columns = e->first ? e->n_columns : 1;
+    const uint64_t rows = e->first ? e->n_rows : e->n_rows * e->n_columns;
+    if (ids == 0 || ids > COL_MOST_IDS || rows < 8 * ids || rows > 1u << 29 ||
+        rows * columns < 65536 ||
+        (!e->first && e->pooled && e->n_columns > 1))
+        return c;
+    const uint32_t vec = piece_cells(e->dim, e->dtype);
+    const uint64_t blocks = columns * (((e->dim + vec - 1) / vec + 63) / 64);
+    const uint64_t most = rows / (8 * ids);
+    uint64_t chunks = std::max((rows + COL_MOST_ROWS - 1) / COL_MOST_ROWS,
+                               std::min(most, (1023 + blocks) / blocks));
+    if (chunks > 4) {  // the same on every XCD
+        const uint64_t up = (chunks + 7) / 8 * 8;
+        chunks = up <= std::max<uint64_t>(most, 8) ? up : chunks;
+    }
+    c.chunk = (uint32_t)(((rows + chunks - 1) / chunks + 63) / 64 * 64);
+    c.chunks = (uint32_t)((rows + c.chunk - 1) / c.chunk);
+    c.padded = (uint64_t)c.chunks * c.chunk;
+    const auto take = [&](uint64_t bytes) {
+        const uint64_t at = c.bytes;
+        c.bytes = (at + bytes + 255) & ~255ull;
+        return at;
+    };
+    c.local = take(2 * c.padded * columns);
+    c.counts = take(2ull * c.chunks * e->n_tokens);
+    c.parts = take(c.chunks > 1 ? 4ull * c.chunks * e->n_tokens * e->dim : 0);
+    return c;
+}
+
 // The gradient's workspace: two lists of sorted positions, a pass' counts, runs' parts.
 struct GradPlan {
     uint32_t n = 0, passes = 0, bits = 0, blocks = 0, vec = 0, pieces = 0, lg_g = 0, chunk = 0,
@@ -671,7 +1077,6 @@ struct GradPlan {
 GradPlan grad_plan(const fbh_embed *e) {
     GradPlan G;
     const uint64_t n = e->n_rows * e->n_columns;
-    head_input(n <= 0x7FFFFFFFull, "a gradient takes at most 2^31 - 1 positions");
     G.n = (uint32_t)n;
     const uint32_t key_bits = lg_at_least((uint64_t)e->n_tokens + 1);  // n_tokens: nothing
     G.passes = (key_bits + 7) / 8;
@@ -701,7 +1106,72 @@ GradPlan grad_plan(const fbh_embed *e) {
     return G;
 }
 
+uint64_t grad_bytes(const fbh_embed *e) {
+    head_input(e->n_rows * e->n_columns <= 0x7FFFFFFFull,
+               "a gradient takes at most 2^31 - 1 positions");
+    const ColumnPlan c = column_plan(e);
+    return c.chunks ? c.bytes : grad_plan(e).bytes;
+}
+
+void columns_grad(const fbh_embed *e, const ColumnPlan &G, const void *grad, void *table,
+                  void *work, hipStream_t s) {
+    Positions P{e->ids, e->first, e->n_rows, e->n_columns, e->n_tokens, drop_key(e->seed),
+                drop_threshold(e->drop)};
+    if (!e->first) {
+        P.n_rows *= P.n_columns;
+        P.n_columns = 1;
+    }
+    const uint32_t most_ids = e->first ? e->most_ids : e->n_tokens;
+    auto *w = static_cast<uint8_t *>(work);
+    auto *local = reinterpret_cast<uint16_t *>(w + G.local);
+    with_ids(e->id_type, e->drop > 0.0, [&](auto id, auto drop) {
+        hipLaunchKernelGGL((column_ids_kernel<decltype(id)::value, decltype(drop)::value>),
+                           dim3((uint32_t)(G.padded / 64), (P.n_columns + 63) / 64), dim3(256), 0,
+                           s, P, most_ids, G.padded, local);
+    });
+    head_check(hipGetLastError(), "column ids");
+    const uint32_t v = piece_cells(e->dim, e->dtype), pieces = (e->dim + v - 1) / v;
+    const uint32_t lg_g = std::min(lg_at_least(pieces), 6u);
+    const Columns C{local, e->first, P.n_rows, G.padded, P.n_columns, e->n_tokens, most_ids,
+                    G.chunk, G.chunks, e->pooled ? 1 : P.n_columns, e->dim, pieces, lg_g,
+                    scale_of(e), reinterpret_cast<float *>(w + G.parts),
+                    reinterpret_cast<uint16_t *>(w + G.counts)};
+    with_cells(e->dtype, v, [&](auto one, auto vec) {
+        using T = decltype(one);
+        constexpr int VEC = decltype(vec)::value;
+        const uint32_t lds = column_lds(most_ids, G.chunk, VEC).bytes;
+        const uint32_t per = std::min(G.chunks, 8u);
+        const auto go = [&](auto buffer) {
+            const auto kernel = &column_sums_kernel<T, VEC, decltype(buffer)::value>;
+            if (lds > 64 * 1024)
+                head_check(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize,
+                                               128 * 1024),
+                           "column sums");
+            hipLaunchKernelGGL(kernel,
+                               dim3((G.chunks + per - 1) / per * per * P.n_columns,
+                                    (pieces + (1u << lg_g) - 1) >> lg_g),
+                               dim3(COL_TPB), lds, s, C, static_cast<const T *>(grad),
+                               static_cast<T *>(table));
+        };
+        const uint64_t row_bytes = (uint64_t)C.per_row * e->dim * sizeof(T);
+        if constexpr (VEC * sizeof(T) >= 4) {
+            if (row_bytes <= BUFFER_MOST / COL_MOST_ROWS &&
+                in_buffer(grad, G.chunk * row_bytes, e->dim * sizeof(T)))
+                go(std::true_type{});
+            else go(std::false_type{});
+        } else go(std::false_type{});
+        head_check(hipGetLastError(), "column sums");
+        if (G.chunks == 1) return;
+        const uint64_t threads = (uint64_t)e->n_tokens * pieces;
+        hipLaunchKernelGGL((column_join_kernel<T, VEC>), dim3((uint32_t)((threads + 255) / 256)),
+                           dim3(256), 0, s, C, static_cast<T *>(table));
+        head_check(hipGetLastError(), "column sums");
+    });
+}
+
 void embed_grad(const fbh_embed *e, const void *grad, void *table, void *work, hipStream_t s) {
+    if (const ColumnPlan G = column_plan(e); G.chunks) return columns_grad(e, G, grad, table, work, s);
     Positions P{e->ids, e->first, e->n_rows, e->n_columns, e->n_tokens, drop_key(e->seed),
                 drop_threshold(e->drop)};
     if (!e->first) {
@@ -783,7 +1253,7 @@ uint64_t fbh_embed_grad_bytes(const fbh_embed *e) {
     uint64_t bytes = 0;
     (void)head_guard([&] {
         check_embed(e);
-        bytes = grad_plan(e).bytes;
+        bytes = grad_bytes(e);
     });
     return bytes;
 }
@@ -793,7 +1263,7 @@ int fbh_embed_grad(int device, const fbh_embed *e, const void *grad, void *table
     return head_guard([&] {
         check_embed(e);
         head_input(table && (grad || e->n_rows == 0), "null argument");
-        const uint64_t need = grad_plan(e).bytes;
+        const uint64_t need = grad_bytes(e);
         head_input(work_bytes >= need && (work || need == 0), "the workspace is too small");
         const OnDevice on(device);
         embed_grad(e, grad, table, work, static_cast<hipStream_t>(stream));

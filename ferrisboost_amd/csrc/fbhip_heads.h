@@ -79,6 +79,32 @@ __device__ __forceinline__ void store_piece(T *p, const Piece<T, N> &r) {
     __builtin_memcpy(p, &r, sizeof(r));
 }
 
+// Buffer loads: 4-byte aligned pieces at byte offsets of up to 2^31 - 1 from an address
+// that all lanes share. What lies at or behind `bytes` reads as zeros, so a position that
+// gives nothing needs an offset (NO_OFFSET) and no select; and an offset takes one
+// 32-bit operation where an address takes a 64-bit product and sum.
+constexpr uint32_t NO_OFFSET = 0x80000000u;
+constexpr uint64_t BUFFER_MOST = 0x7FF00000ull;  // bytes; cells of a row come on top
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void *p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, bytes, 0x00027000);
+}
+template <class T, int N>
+__device__ __forceinline__ Piece<T, N> load_offset(__amdgpu_buffer_rsrc_t r, uint32_t offset) {
+    Piece<T, N> p;
+    if constexpr (sizeof(p) == 16) {
+        const auto q = __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 0);
+        __builtin_memcpy(&p, &q, 16);
+    } else if constexpr (sizeof(p) == 8) {
+        const auto q = __builtin_amdgcn_raw_buffer_load_b64(r, offset, 0, 0);
+        __builtin_memcpy(&p, &q, 8);
+    } else {
+        static_assert(sizeof(p) == 4, "a piece of whole words");
+        const auto q = __builtin_amdgcn_raw_buffer_load_b32(r, offset, 0, 0);
+        __builtin_memcpy(&p, &q, 4);
+    }
+    return p;
+}
+
 // ---- The counter-based generator: element e takes half of the 64 bits that the
 // SplitMix64 finaliser gives for a seed's key and e / 2, as row sampling takes a
 // row's bits from seed and row. Nothing is stored: whoever knows seed and element

@@ -119,6 +119,7 @@ class Vocabulary:
         self.sizes = sizes.astype(np.int64)
         self.n_tokens = int(first[-1])
         self.n_columns = int(sizes.size)
+        self.most_ids = int(sizes.max())
         self.first = torch.from_numpy(first.astype(np.int32)).to(device)
         if self.first.device.type != "cuda":
             raise ValueError(f"device must be a GPU, got {device!r}")
@@ -154,7 +155,7 @@ def _positions(ids, vocabulary, pooled: bool, n_tokens: int, dim: int, cells: in
     e.id_type, e.dtype, e.pooled = code, cells, 1 if pooled else 0
     e.ids = ids.data_ptr()
     if vocabulary is not None:
-        e.first = vocabulary.first.data_ptr()
+        e.first, e.most_ids = vocabulary.first.data_ptr(), vocabulary.most_ids
     e.drop, e.seed, e.scale = drop, seed, scale
     return e, shape[:-1] if pooled else shape
 

@@ -752,7 +752,8 @@ typedef struct {
     double drop;
     uint64_t seed;
     float scale;
-    uint32_t reserved;
+    uint32_t most_ids;  /* the most ids that one column has by first, or 0: not known
+                           (fbh_embed_grad is then slower for many rows) */
 } fbh_embed;
 
 /* out[row] = scale * the sum over columns of the positions' table rows, [n_rows]

@@ -75,6 +75,9 @@ TABLES = [
     (64, [2] * 9, 8), (333, [50, 3, 1000], 5), (1000, [40] * 33, 16), (70, [5] * 600, 127),
     (4097, [31, 77], 33), (9000, [100, 28], 260), (40, [12] * 7, 1100), (30_000, [17] * 5, 2),
     (1, [10_000], 2048),
+    # columns summed chunk by chunk: one chunk, several, uneven ones, wide vectors
+    (3000, [40] * 33, 64), (20_000, [511, 3, 0, 200], 24), (140_000, [9], 7),
+    (70_001, [31, 1000], 3), (9000, [1024, 5] * 4, 600), (66_000, [2, 1], 1),
 ]
 
 
