@@ -88,7 +88,7 @@ constexpr uint32_t ROW_BLOCK = EMB_TPB * ROW_PIECES;
 template <class T, int VEC, int ID, bool DROP>
 __global__ __launch_bounds__(EMB_TPB) void embed_rows_kernel(Positions P, const T *table, T *out,
                                                              uint32_t dim, Divisor pieces,
-                                                             Divisor columns, float s) {
+                                                             Divisor columns, float s, bool past) {
     __shared__ uint32_t toks[ROW_BLOCK + 1];
     const uint64_t block = blockIdx.x + (uint64_t)blockIdx.y * gridDim.x;
     const uint64_t base = block * ROW_BLOCK;
@@ -121,7 +121,9 @@ __global__ __launch_bounds__(EMB_TPB) void embed_rows_kernel(Positions P, const 
 #pragma unroll
         for (int i = 0; i < VEC; i++)
             p[k].v[i] = tok[k] == NO_TOKEN ? (T)0.0f : (T)((float)p[k].v[i] * s);
-        store_piece<T, VEC>(out + (pos0 + q[k]) * dim + cell[k], p[k]);
+        T *to = out + (pos0 + q[k]) * dim + cell[k];
+        if (past) stream_piece<T, VEC>(to, p[k]);
+        else store_piece<T, VEC>(to, p[k]);
     }
 }
 
@@ -968,7 +970,8 @@ void launch_embed(const fbh_embed *e, const void *table, void *out, hipStream_t 
         head_input(by <= 65535, "too many cells");
         hipLaunchKernelGGL((embed_rows_kernel<T, VEC, ID, DROP>), dim3(bx, (uint32_t)by),
                            dim3(EMB_TPB), 0, s, P, tab, to, e->dim, divisor(pieces),
-                           divisor(P.n_columns), sc);
+                           divisor(P.n_columns), sc,
+                           P.n_rows * P.n_columns * e->dim * sizeof(T) >= STREAM_BYTES);
     } else if (P.n_rows * pieces < 64 * EMB_TPB) {
         const uint32_t lg_g = std::min(lg_at_least(pieces), 5u);
         hipLaunchKernelGGL((embed_sum_few_kernel<T, VEC, ID, DROP>),
