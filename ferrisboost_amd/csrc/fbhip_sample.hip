@@ -20,17 +20,9 @@ namespace fbh {
 namespace {
 
 constexpr uint32_t SAMPLE_MOST = 262144;  // classes: their weights' sum is below 2^63
+constexpr uint32_t NO_BIN = 0xFFFFFFFFu;
 constexpr int WEIGHT_BITS = 45;
 constexpr uint64_t WEIGHT_ONE = 1ull << WEIGHT_BITS;
-
-struct Draw {
-    const float *uniforms;
-    fbh_sample_options o;
-    int64_t *classes;
-    float *log_probs;
-    uint64_t n_rows;
-    uint32_t n_classes;
-};
 
 // A row's options, as whole numbers.
 struct RowOptions {
@@ -38,24 +30,42 @@ struct RowOptions {
     uint32_t k;         // classes that stay by rank
     uint32_t p31;       // top_p * 2^31
     uint64_t least;     // smallest weight that stays by min_p
-    uint32_t u31;       // uniform * 2^31
+    __host__ __device__ bool cuts(uint32_t n) const { return k < n || p31 < 1u << 31; }
+};
+
+__host__ __device__ inline RowOptions whole_options(float t, int32_t k, float p, float m,
+                                                    uint32_t n) {
+    RowOptions r;
+    r.k = t > 0.0f ? (k > 0 && (uint32_t)k < n ? (uint32_t)k : n) : 1;
+    r.inv_t = t > 0.0f ? 1.0 / (double)t : 0.0;
+    r.p31 = p < 1.0f ? (p > 0.0f ? (uint32_t)((double)p * 2147483648.0) : 0) : 1u << 31;
+    r.least = m > 0.0f ? (m < 1.0f ? (uint64_t)ceil((double)m * (double)WEIGHT_ONE) : WEIGHT_ONE)
+                       : 0;
+    return r;
+}
+
+struct Draw {
+    const float *uniforms;
+    fbh_sample_options o;
+    RowOptions all;     // of every row, where none has options of its own
+    bool own;           // some have
+    int64_t *classes;
+    float *log_probs;
+    uint64_t n_rows;
+    uint32_t n_classes;
 };
 
 __device__ __forceinline__ RowOptions row_options(const Draw &D, uint64_t row) {
-    RowOptions r;
-    const float t = D.o.temperatures ? D.o.temperatures[row] : D.o.temperature;
-    const int32_t k = D.o.top_ks ? D.o.top_ks[row] : D.o.top_k;
-    float p = D.o.top_ps ? D.o.top_ps[row] : D.o.top_p;
-    float m = D.o.min_ps ? D.o.min_ps[row] : D.o.min_p;
-    const float u = D.uniforms[row];
-    r.k = t > 0.0f ? (k > 0 ? min((uint32_t)k, D.n_classes) : D.n_classes) : 1;
-    r.inv_t = t > 0.0f ? 1.0 / (double)t : 0.0;
-    p = p < 1.0f ? fmaxf(p, 0.0f) : 1.0f;  // (NaN: 1)
-    r.p31 = (uint32_t)((double)p * 2147483648.0);
-    m = m > 0.0f ? fminf(m, 1.0f) : 0.0f;
-    r.least = (uint64_t)ceil((double)m * (double)WEIGHT_ONE);
-    r.u31 = u > 0.0f ? (uint32_t)fmin((double)u * 2147483648.0, 2147483647.0) : 0;
-    return r;
+    if (!D.own) return D.all;
+    return whole_options(D.o.temperatures ? D.o.temperatures[row] : D.o.temperature,
+                         D.o.top_ks ? D.o.top_ks[row] : D.o.top_k,
+                         D.o.top_ps ? D.o.top_ps[row] : D.o.top_p,
+                         D.o.min_ps ? D.o.min_ps[row] : D.o.min_p, D.n_classes);
+}
+
+// uniform * 2^31
+__device__ __forceinline__ uint32_t uniform31(float u) {
+    return u > 0.0f ? (uint32_t)fmin((double)u * 2147483648.0, 2147483647.0) : 0;
 }
 
 // floor((part * total + add) / 2^31)
@@ -111,20 +121,125 @@ struct RowScale {
 
 __device__ __forceinline__ float masked_nan(float l) { return l == l ? l : -INFINITY; }
 
-// -------------------------------------------------------------- few classes
-constexpr uint32_t GROUP_TPB = 256;
-constexpr uint32_t GROUP_MOST = 64;
+__device__ __forceinline__ void put_class(const Draw &D, uint64_t row, int64_t c, double z,
+                                          uint64_t total) {
+    D.classes[row] = c;
+    if (D.log_probs)
+        D.log_probs[row] =
+            c < 0 ? -INFINITY : (float)(z - log((double)total / (double)WEIGHT_ONE));
+}
 
-__device__ __forceinline__ uint64_t shfl64(uint64_t v, int from, int width) {
+// What stays: classes of larger keys, and the first `ties` classes of this one.
+struct Cut {
+    uint32_t key, ties;
+};
+
+__device__ __forceinline__ uint64_t shfl64(uint64_t v, int from, int width = 64) {
     const uint32_t lo = __shfl((uint32_t)v, from, width);
     const uint32_t hi = __shfl((uint32_t)(v >> 32), from, width);
     return (uint64_t)hi << 32 | lo;
 }
-__device__ __forceinline__ uint64_t shfl64_up(uint64_t v, int by, int width) {
+__device__ __forceinline__ uint64_t shfl64_up(uint64_t v, int by, int width = 64) {
     const uint32_t lo = __shfl_up((uint32_t)v, by, width);
     const uint32_t hi = __shfl_up((uint32_t)(v >> 32), by, width);
     return (uint64_t)hi << 32 | lo;
 }
+__device__ __forceinline__ uint64_t scan64(uint64_t v, uint32_t lane) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint64_t y = shfl64_up(v, d);
+        if (lane >= (uint32_t)d) v += y;
+    }
+    return v;
+}
+__device__ __forceinline__ uint32_t scan32(uint32_t v, uint32_t lane) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t y = __shfl_up(v, d);
+        if (lane >= (uint32_t)d) v += y;
+    }
+    return v;
+}
+
+// -------------------------------------------------------------- a row a thread
+constexpr uint32_t THREAD_MOST = 8;
+
+// Up to 8 classes: a thread a row, whose logits it holds; ranks and the weights before a
+// class from every pair of them. Bound by arithmetic: V exponentials and a logarithm of
+// doubles a row. (500k rows of 4: 17 us with a lane a class, where each row's options and
+// logarithm take a whole wave's instructions.)
+template <class T, int V>
+__global__ __launch_bounds__(256) void sample_thread_kernel(const T *logits, Draw D) {
+    const uint64_t row = blockIdx.x * 256ull + threadIdx.x;
+    if (row >= D.n_rows) return;
+    const Piece<T, V> p = load_piece<T, V>(logits + row * V);
+    const RowOptions O = row_options(D, row);
+    float l[V];
+    float most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        l[i] = masked_nan((float)p.v[i]);
+        most = fmaxf(most, l[i]);
+    }
+    const RowScale S{most, (double)most, O.inv_t};
+    uint64_t w[V];
+#pragma unroll
+    for (int i = 0; i < V; i++)
+        w[i] = l[i] == -INFINITY ? 0
+                                 : (O.inv_t == 0.0 ? (l[i] == most ? WEIGHT_ONE : 0)
+                                                   : S.weight(l[i]));
+    if (O.cuts(V)) {
+        uint32_t rank[V];
+        uint64_t all = 0;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            rank[i] = 0;
+#pragma unroll
+            for (int j = 0; j < V; j++)
+                if (j != i) rank[i] += l[j] > l[i] || (l[j] == l[i] && j < i);
+            if (rank[i] >= O.k) w[i] = 0;
+            all += w[i];
+        }
+        if (O.p31 < 1u << 31) {
+            uint64_t most_w = share(O.p31, all, 0x7FFFFFFFu);
+            if (most_w == 0) most_w = 1;
+            uint64_t stay[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                uint64_t before = 0;
+#pragma unroll
+                for (int j = 0; j < V; j++)
+                    if (j != i && rank[j] < rank[i]) before += w[j];
+                stay[i] = before < most_w ? w[i] : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < V; i++) w[i] = stay[i];
+        }
+    }
+    uint64_t total = 0;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        if (w[i] < O.least) w[i] = 0;
+        total += w[i];
+    }
+    const uint64_t target = share(uniform31(D.uniforms[row]), total, 0);
+    int c = -1;
+    float at = most;
+    uint64_t cum = 0;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        cum += w[i];
+        if (c < 0 && cum > target) {
+            c = i;
+            at = l[i];
+        }
+    }
+    put_class(D, row, c, S.z(at), total);
+}
+
+// -------------------------------------------------------------- a lane a class
+constexpr uint32_t GROUP_TPB = 256;
+constexpr uint32_t GROUP_MOST = 64;
 
 // Up to 64 classes: a lane a class, 64 / G rows a wave. Every lane meets every other
 // class of its row once, which gives its rank and the weight before it in the order.
@@ -142,8 +257,7 @@ __global__ __launch_bounds__(GROUP_TPB) void sample_group_kernel(const T *logits
     for (int d = 1; d < G; d <<= 1) most = fmaxf(most, __shfl_xor(most, d, G));
     const RowScale S{most, (double)most, O.inv_t};
     uint64_t w = l == -INFINITY ? 0 : (O.inv_t == 0.0 ? (l == most ? WEIGHT_ONE : 0) : S.weight(l));
-    const bool ranks = O.k < D.n_classes || O.p31 < 1u << 31;
-    if (__any(ranks)) {
+    if (__any(O.cuts(D.n_classes))) {
         const uint32_t key = logit_key(l);
         uint32_t rank = 0;
         for (int j = 0; j < (int)D.n_classes; j++) {
@@ -169,24 +283,335 @@ __global__ __launch_bounds__(GROUP_TPB) void sample_group_kernel(const T *logits
         if (c >= d) cum += y;
     }
     const uint64_t total = shfl64(cum, G - 1, G);
-    const uint64_t hits = __ballot(cum > share(O.u31, total, 0));
+    const uint64_t hits = __ballot(cum > share(uniform31(D.uniforms[at]), total, 0));
     const int lane0 = (threadIdx.x & 63) - c;
     const uint64_t mine = (hits >> lane0) & (G < 64 ? (1ull << (G & 63)) - 1 : ~0ull);
     if (!in) return;
     if (total == 0) {
-        if (c == 0) {
-            D.classes[row] = -1;
-            if (D.log_probs) D.log_probs[row] = -INFINITY;
-        }
+        if (c == 0) put_class(D, row, -1, 0.0, 0);
     } else if (c == __ffsll((long long)mine) - 1) {
-        D.classes[row] = c;
-        if (D.log_probs)
-            D.log_probs[row] = (float)(S.z(l) - log((double)total / (double)WEIGHT_ONE));
+        put_class(D, row, c, S.z(l), total);
+    }
+}
+
+// -------------------------------------------------------------- a row a wave
+constexpr uint32_t WAVE_BINS = 256;
+constexpr uint32_t WAVE_MOST = 1024;
+
+// Up to 64 R classes: a wave a row, which lies in registers, R classes side by side a
+// lane. The cut's bin is found from a histogram in LDS; the bin's classes (with top-k of at
+// most 64, all up to the cut) then take a lane each. Four waves a workgroup, with nothing
+// in common: LDS operations of one wave complete in order.
+struct WaveShared {
+    uint64_t wt[WAVE_BINS];
+    uint32_t ct[WAVE_BINS];
+    uint32_t keys[64];
+    uint32_t classes[64];
+};
+
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <class T, int R>
+__global__ __launch_bounds__(256) void sample_wave_kernel(const T *logits, Draw D) {
+    __shared__ WaveShared shared[4];
+    WaveShared &sh = shared[threadIdx.x / 64];
+    const uint64_t row = blockIdx.x * 4ull + threadIdx.x / 64;
+    if (row >= D.n_rows) return;
+    const uint32_t lane = threadIdx.x & 63, n = D.n_classes, c0 = lane * R;
+    const T *from = logits + row * n;
+    const RowOptions O = row_options(D, row);
+
+    float l[R];
+    if (c0 + R <= n) {
+        constexpr int N = R * sizeof(T) > 16 ? 16 / sizeof(T) : R;
+#pragma unroll
+        for (int i = 0; i < R; i += N) {
+            const Piece<T, N> p = load_piece<T, N>(from + c0 + i);
+#pragma unroll
+            for (int j = 0; j < N; j++) l[i + j] = masked_nan((float)p.v[j]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < R; i++)
+            l[i] = c0 + i < n ? masked_nan((float)from[c0 + i]) : -INFINITY;
+    }
+    float mine = l[0];
+#pragma unroll
+    for (int i = 1; i < R; i++) mine = fmaxf(mine, l[i]);
+    float most = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+    if (most == -INFINITY || O.k == 1) {
+        const uint64_t has = __ballot(mine == most);
+        if (lane == (uint32_t)__ffsll((long long)has) - 1) {
+            int at = 0;
+#pragma unroll
+            for (int i = R - 1; i >= 0; i--)
+                if (l[i] == most) at = i;
+            put_class(D, row, most == -INFINITY ? -1 : (int64_t)(c0 + at), 0.0, WEIGHT_ONE);
+        }
+        return;
+    }
+    const RowScale S{most, (double)most, O.inv_t};
+    const float per_nat = (float)(O.inv_t * (WAVE_BINS / 32));
+    const auto bin_of = [&](float v) {
+        const float d = v == most ? 0.0f : (most - v) * per_nat;
+        return (uint32_t)fminf(d, (float)(WAVE_BINS - 1));
+    };
+    const uint32_t target31 = uniform31(D.uniforms[row]);
+
+    uint64_t w[R];
+    bool weighed = false;
+    const auto weigh = [&] {
+#pragma unroll
+        for (int i = 0; i < R; i++) w[i] = l[i] == -INFINITY ? 0 : S.weight(l[i]);
+        weighed = true;
+    };
+    // The first bin at which the counts (the weights) reach k (weight); what stands before.
+    const auto find = [&](bool by_count, uint32_t k, uint64_t weight, uint32_t &before_c,
+                          uint64_t &before_w, uint32_t &inside) {
+        uint32_t c[WAVE_BINS / 64];
+        uint64_t v[WAVE_BINS / 64];
+        uint32_t cs = 0;
+        uint64_t vs = 0;
+#pragma unroll
+        for (int b = 0; b < (int)WAVE_BINS / 64; b++) {
+            c[b] = sh.ct[lane * (WAVE_BINS / 64) + b];
+            v[b] = by_count ? 0 : sh.wt[lane * (WAVE_BINS / 64) + b];
+            cs += c[b];
+            vs += v[b];
+        }
+        const uint32_t cc = scan32(cs, lane);
+        const uint64_t vv = by_count ? 0 : scan64(vs, lane);
+        const uint64_t hits = __ballot(by_count ? cc >= k : vv >= weight);
+        if (!hits) return NO_BIN;
+        const int who = __ffsll((long long)hits) - 1;
+        uint32_t bc = cc - cs, bin = 0;
+        uint64_t bv = vv - vs;
+        bool found = false;
+#pragma unroll
+        for (int b = 0; b < (int)WAVE_BINS / 64; b++)
+            if (!found) {
+                inside = c[b];
+                bin = lane * (WAVE_BINS / 64) + b;
+                if (by_count ? bc + c[b] >= k : bv + v[b] >= weight) found = true;
+                else {
+                    bc += c[b];
+                    bv += v[b];
+                }
+            }
+        before_c = __shfl(bc, who);
+        before_w = shfl64(bv, who);
+        inside = __shfl(inside, who);
+        return (uint32_t)__shfl(bin, who);
+    };
+    // Classes with take(i) to lanes, in class order; at most 64 of them.
+    const auto gather = [&](auto &&take) {
+        uint32_t some = 0;
+#pragma unroll
+        for (int i = 0; i < R; i++) some += take(i);
+        uint32_t at = scan32(some, lane) - some;
+#pragma unroll
+        for (int i = 0; i < R; i++)
+            if (take(i)) {
+                sh.keys[at] = logit_key(l[i]);
+                sh.classes[at] = c0 + i;
+                at++;
+            }
+        wave_fence();
+    };
+    // This lane's place among `members` lanes by falling key, equal ones by lane.
+    const auto rank_of = [&](uint32_t key, uint32_t members) {
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < members; j++) {
+            const uint32_t kj = __builtin_amdgcn_readlane(key, j);
+            rank += kj > key || (kj == key && j < lane);
+        }
+        return rank;
+    };
+    // The cut among classes of one bin by bisection of their keys, where they are too many
+    // for a lane each.
+    const auto bisect = [&](uint32_t bin, bool by_count, uint32_t k, uint64_t weight,
+                            uint32_t before_c, uint64_t before_w) {
+        uint32_t lo = 0, hi = 0xFFFFFFFFu;  // the cut's key: the largest with enough at or above
+        while (lo < hi) {
+            const uint32_t mid = lo + (hi - lo) / 2 + 1;
+            uint32_t c = 0;
+            uint64_t v = 0;
+#pragma unroll
+            for (int i = 0; i < R; i++)
+                if (l[i] != -INFINITY && bin_of(l[i]) == bin && logit_key(l[i]) >= mid) {
+                    c++;
+                    if (!by_count) v += w[i];
+                }
+            const bool enough =
+                by_count ? before_c + __shfl(scan32(c, lane), 63) >= k
+                         : before_w + shfl64(scan64(v, lane), 63) >= weight;
+            if (enough) lo = mid;
+            else hi = mid - 1;
+        }
+        uint32_t c = 0;
+        uint64_t v = 0;
+#pragma unroll
+        for (int i = 0; i < R; i++)
+            if (l[i] != -INFINITY && bin_of(l[i]) == bin && logit_key(l[i]) > lo) {
+                c++;
+                if (!by_count) v += w[i];
+            }
+        Cut cut{lo, 0};
+        if (by_count) cut.ties = k - before_c - __shfl(scan32(c, lane), 63);
+        else {
+            const uint64_t one = S.weight(key_logit(lo));
+            const uint64_t left = weight - before_w - shfl64(scan64(v, lane), 63);
+            cut.ties = (uint32_t)((left + one - 1) / one);
+        }
+        return cut;
+    };
+    const auto cut_in = [&](uint32_t bin, uint32_t inside, bool by_count, uint32_t k,
+                            uint64_t weight, uint32_t before_c, uint64_t before_w) {
+        if (inside > 64) return bisect(bin, by_count, k, weight, before_c, before_w);
+        gather([&](int i) { return l[i] != -INFINITY && bin_of(l[i]) == bin; });
+        const uint32_t key = lane < inside ? sh.keys[lane] : 0;
+        const uint32_t rank = rank_of(key, inside);
+        wave_fence();
+        // by rank: the keys, and what they add up to
+        if (lane < inside) sh.keys[rank] = key;
+        wave_fence();
+        const uint32_t sorted = lane < inside ? sh.keys[lane] : 0;
+        const uint64_t v =
+            lane < inside && !by_count ? S.weight(key_logit(sorted)) : 0;
+        const uint64_t upto = by_count ? 0 : before_w + scan64(v, lane);
+        const uint64_t hits = __ballot(
+            lane < inside && (by_count ? before_c + lane + 1 >= k : upto >= weight));
+        const uint32_t who = (uint32_t)__ffsll((long long)hits) - 1;
+        const uint32_t at = __shfl(sorted, who);
+        const uint64_t same = __ballot(lane < inside && sorted == at);
+        wave_fence();
+        return Cut{at, who - ((uint32_t)__ffsll((long long)same) - 1) + 1};
+    };
+    const auto histogram = [&](bool weights) {
+        wave_fence();
+#pragma unroll
+        for (int b = 0; b < (int)WAVE_BINS / 64; b++) {
+            sh.ct[lane + 64 * b] = 0;
+            sh.wt[lane + 64 * b] = 0;
+        }
+        wave_fence();
+#pragma unroll
+        for (int i = 0; i < R; i++)
+            if (l[i] != -INFINITY) {
+                const uint32_t b = bin_of(l[i]);
+                atomicAdd(&sh.ct[b], 1u);
+                if (weights)
+                    atomicAdd(reinterpret_cast<unsigned long long *>(&sh.wt[b]),
+                              (unsigned long long)w[i]);
+            }
+        wave_fence();
+    };
+
+    Cut cut{0, 0};
+    uint64_t tie_w = 0;
+    if (O.cuts(n)) {
+        uint32_t before_c = 0, inside = 0;
+        uint64_t before_w = 0;
+        if (O.k <= 64 && O.k < n) {
+            histogram(false);
+            const uint32_t bin = find(true, O.k, 0, before_c, before_w, inside);
+            const uint32_t members = before_c + inside;
+            if (bin != NO_BIN && members <= 64) {
+                // All that can stay has a lane each, in class order.
+                gather([&](int i) { return l[i] != -INFINITY && bin_of(l[i]) <= bin; });
+                const uint32_t key = lane < members ? sh.keys[lane] : 0;
+                const uint32_t rank = rank_of(key, members);
+                const float v = key_logit(key);
+                uint64_t kept = lane < members && rank < O.k ? S.weight(v) : 0;
+                if (O.p31 < 1u << 31) {
+                    if (lane < members) sh.wt[rank] = kept;
+                    wave_fence();
+                    const uint64_t s = lane < members ? sh.wt[lane] : 0;
+                    const uint64_t upto = scan64(s, lane);
+                    uint64_t weight = share(O.p31, shfl64(upto, 63), 0x7FFFFFFFu);
+                    if (weight == 0) weight = 1;
+                    const uint32_t stay = __popcll(__ballot(lane < members && upto - s < weight));
+                    if (rank >= stay) kept = 0;
+                }
+                if (kept < O.least) kept = 0;
+                const uint64_t cum = scan64(kept, lane);
+                const uint64_t total = shfl64(cum, 63);
+                const uint64_t hits = __ballot(cum > share(target31, total, 0));
+                if (lane == (uint32_t)__ffsll((long long)hits) - 1)
+                    put_class(D, row, sh.classes[lane], S.z(v), total);
+                return;
+            }
+        }
+        weigh();
+        histogram(true);
+        uint32_t k_bin = NO_BIN, k_inside = 0, k_c = 0;
+        uint64_t k_w = 0;
+        if (O.k < n) {
+            k_bin = find(true, O.k, 0, k_c, k_w, k_inside);
+            if (k_bin != NO_BIN) {
+                cut = cut_in(k_bin, k_inside, true, O.k, 0, k_c, 0);
+                tie_w = S.weight(key_logit(cut.key));
+            }
+        }
+        if (O.p31 < 1u << 31) {
+            uint64_t mine_w = 0;
+#pragma unroll
+            for (int i = 0; i < R; i++)
+                if (logit_key(l[i]) > cut.key) mine_w += w[i];
+            const uint64_t all = shfl64(scan64(mine_w, lane), 63) + cut.ties * tie_w;
+            uint64_t weight = share(O.p31, all, 0x7FFFFFFFu);
+            if (weight == 0) weight = 1;
+            const uint32_t bin = find(false, 0, weight, before_c, before_w, inside);
+            cut = cut_in(bin, inside, false, 0, weight, 0, before_w);
+            tie_w = S.weight(key_logit(cut.key));
+        }
+        if (tie_w < O.least) cut.ties = 0;
+    }
+    if (!weighed) weigh();
+
+    // The staying weights in class order.
+    uint32_t ties = 0;
+    uint64_t sum = 0;
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        const uint32_t key = logit_key(l[i]);
+        if (key < cut.key || w[i] < O.least) w[i] = 0;
+        if (key == cut.key) {
+            ties++;
+            w[i] = 0;
+        }
+        sum += w[i];
+    }
+    const uint32_t ties0 = scan32(ties, lane) - ties;  // before this lane
+    const uint32_t kept = ties0 < cut.ties ? min(cut.ties - ties0, ties) : 0;
+    sum += kept * tie_w;
+    const uint64_t cum = scan64(sum, lane);
+    const uint64_t total = shfl64(cum, 63);
+    const uint64_t target = share(target31, total, 0);
+    const uint64_t hits = __ballot(cum > target);
+    if (lane == (uint32_t)__ffsll((long long)hits) - 1) {
+        uint64_t at = cum - sum;
+        uint32_t seen = 0;
+        int c = -1;
+        float v = most;
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            at += logit_key(l[i]) == cut.key ? (seen++ < kept ? tie_w : 0) : w[i];
+            if (c < 0 && at > target) {
+                c = (int)c0 + i;
+                v = l[i];
+            }
+        }
+        put_class(D, row, c, S.z(v), total);
     }
 }
 
 // -------------------------------------------------------------- a row a workgroup
-constexpr uint32_t NO_BIN = 0xFFFFFFFFu;
 constexpr uint32_t MOST_TILES = 64;
 
 template <class T>
@@ -202,16 +627,24 @@ struct KeyDigits<__bf16> {
     static constexpr int last = 16;
 };
 
+// Classes in a list: falling logits first, equal ones by class, as one number falls.
+__device__ __forceinline__ uint64_t entry_of(float l, uint32_t c) {
+    return (uint64_t)logit_key(l) << 32 | (uint32_t)~c;
+}
+__device__ __forceinline__ uint32_t entry_key(uint64_t e) { return (uint32_t)(e >> 32); }
+__device__ __forceinline__ uint32_t entry_class(uint64_t e) { return ~(uint32_t)e; }
+
 template <int TPB>
 struct RowShared {
-    static constexpr uint32_t BINS = TPB == 64 ? 256 : 1024;
-    static constexpr uint32_t LIST = TPB == 64 ? 256 : 2048;
+    static constexpr uint32_t BINS = 1024;
+    static constexpr uint32_t LIST = 2048;
+    static constexpr uint32_t MOST_K = TPB / 2;  // of the classes found by the threads' largest
     uint64_t wt[BINS];
     uint32_t ct[BINS];
-    uint32_t list[LIST];
+    uint64_t list[LIST];
     uint64_t tile_w[MOST_TILES];
     uint32_t tile_ties[MOST_TILES];
-    float wave_most[TPB / 64];
+    float wave_most[TPB / 64], wave_least[TPB / 64];
     uint32_t wave_at[TPB / 64];
     uint64_t wave_w[TPB / 64];
     uint32_t wave_ties[TPB / 64];
@@ -221,11 +654,6 @@ struct RowShared {
     uint64_t target;
     uint64_t total;
     uint32_t tile, ties;
-};
-
-// What stays: classes of larger keys, and the first `ties` classes of this one.
-struct Cut {
-    uint32_t key, ties;
 };
 
 // One row. All threads of the workgroup call every function; a barrier stands between
@@ -238,7 +666,7 @@ struct SampleRow {
     const T *row;
     uint32_t n;
     RowScale S;
-    float per_nat;
+    float per;  // bins of a unit of logits
 
     template <class F>
     __device__ __forceinline__ void each(F &&f) const {
@@ -253,8 +681,10 @@ struct SampleRow {
         }
     }
 
-    // The largest logit and its first class.
-    __device__ __forceinline__ void largest(float &most, uint32_t &at) const {
+    // The largest logit and its first class; the thread's own largest, and the least of
+    // those that are not masked.
+    __device__ __forceinline__ void largest(float &most, uint32_t &at, float &own,
+                                            float &least) const {
         most = -INFINITY;
         at = NO_BIN;
         each([&](uint32_t i, float l) {
@@ -263,34 +693,37 @@ struct SampleRow {
                 at = i;
             }
         });
+        own = most;
+        least = most == -INFINITY ? INFINITY : most;
         for (int d = 1; d < 64; d <<= 1) {
             const float m = __shfl_xor(most, d);
             const uint32_t a = __shfl_xor(at, d);
+            least = fminf(least, __shfl_xor(least, d));
             if (m > most || (m == most && a < at)) {
                 most = m;
                 at = a;
             }
         }
-        if constexpr (TPB > 64) {
-            if ((threadIdx.x & 63) == 0) {
-                sh.wave_most[threadIdx.x / 64] = most;
-                sh.wave_at[threadIdx.x / 64] = at;
-            }
-            __syncthreads();
-            for (int w = 0; w < TPB / 64; w++) {
-                const float m = sh.wave_most[w];
-                const uint32_t a = sh.wave_at[w];
-                if (m > most || (m == most && a < at)) {
-                    most = m;
-                    at = a;
-                }
+        if ((threadIdx.x & 63) == 0) {
+            sh.wave_most[threadIdx.x / 64] = most;
+            sh.wave_least[threadIdx.x / 64] = least;
+            sh.wave_at[threadIdx.x / 64] = at;
+        }
+        __syncthreads();
+        for (int w = 0; w < TPB / 64; w++) {
+            const float m = sh.wave_most[w];
+            const uint32_t a = sh.wave_at[w];
+            least = fminf(least, sh.wave_least[w]);
+            if (m > most || (m == most && a < at)) {
+                most = m;
+                at = a;
             }
         }
     }
 
-    // Bins of (max - l) / T, 32 over all of them: monotone, as each step of it is.
+    // Bins of max - l: monotone, as each step of it is.
     __device__ __forceinline__ uint32_t bin_of(float l) const {
-        const float d = l == S.most ? 0.0f : (S.most - l) * per_nat;
+        const float d = l == S.most ? 0.0f : (S.most - l) * per;
         return (uint32_t)fminf(d, (float)(Shared::BINS - 1));
     }
 
@@ -302,9 +735,31 @@ struct SampleRow {
         }
         __syncthreads();
     }
-    __device__ __forceinline__ void count(uint32_t bin, uint64_t w) {
-        atomicAdd(&sh.ct[bin], 1u);
+    __device__ __forceinline__ void add_weight(uint32_t bin, uint64_t w) {
         atomicAdd(reinterpret_cast<unsigned long long *>(&sh.wt[bin]), (unsigned long long)w);
+    }
+    __device__ __forceinline__ void before(uint32_t ct, uint64_t wt) {
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            sh.before_ct = ct;
+            sh.before_wt = wt;
+        }
+    }
+
+    // The sum of all threads' values, and with `upto` that of the threads up to this one.
+    __device__ __forceinline__ uint64_t sum(uint64_t v, uint64_t *upto = nullptr) {
+        const uint64_t x = scan64(v, threadIdx.x & 63);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 63) sh.wave_w[threadIdx.x / 64] = x;
+        __syncthreads();
+        uint64_t all = 0, mine = x;
+        for (uint32_t w = 0; w < TPB / 64; w++) {
+            const uint64_t y = sh.wave_w[w];
+            all += y;
+            if (w < threadIdx.x / 64) mine += y;
+        }
+        if (upto) *upto = mine;
+        return all;
     }
 
     // The first bin at which the counts reach k (or the weights reach `weight`), and
@@ -320,16 +775,8 @@ struct SampleRow {
                 c += sh.ct[b0 + b];
                 w += sh.wt[b0 + b];
             }
-            uint32_t cc = c;
-            uint64_t ww = w;
-            for (int d = 1; d < 64; d <<= 1) {
-                const uint32_t y = __shfl_up(cc, d);
-                const uint64_t z = shfl64_up(ww, d, 64);
-                if ((int)threadIdx.x >= d) {
-                    cc += y;
-                    ww += z;
-                }
-            }
+            const uint32_t cc = scan32(c, threadIdx.x);
+            const uint64_t ww = scan64(w, threadIdx.x);
             uint32_t bc = sh.before_ct;
             uint64_t bw = sh.before_wt;
             const bool reach = by_count ? bc + cc >= k : bw + ww >= weight;
@@ -352,27 +799,22 @@ struct SampleRow {
         __syncthreads();
     }
 
-    // The cut inside bin `bin` of `inside` classes, with sh.before_* standing before it.
-    __device__ __forceinline__ Cut refine(uint32_t bin, uint32_t inside, bool by_count,
-                                          uint32_t k, uint64_t weight) {
-        const bool listed = inside <= Shared::LIST;
-        if (listed) {
-            if (threadIdx.x == 0) sh.n_list = 0;
-            __syncthreads();
-            each([&](uint32_t, float l) {
-                if (l != -INFINITY && bin_of(l) == bin)
-                    sh.list[atomicAdd(&sh.n_list, 1u)] = logit_key(l);
-            });
-        }
+    // The cut inside bin `bin`, whose classes are in the list (n_list of them, or, with
+    // n_list NO_BIN, are to be read again), with sh.before_* standing before it.
+    __device__ __forceinline__ Cut refine(uint32_t bin, uint32_t n_list, bool by_count, uint32_t k,
+                                          uint64_t weight) {
         uint32_t prefix = 0;
         for (int shift = 24; shift >= KeyDigits<T>::last; shift -= 8) {
             clear(256);
             const auto take = [&](uint32_t key) {
-                if (shift == 24 || key >> (shift + 8) == prefix)
-                    count(255 - ((key >> shift) & 255), S.weight(key_logit(key)));
+                if (shift == 24 || key >> (shift + 8) == prefix) {
+                    const uint32_t b = 255 - ((key >> shift) & 255);
+                    atomicAdd(&sh.ct[b], 1u);
+                    add_weight(b, S.weight(key_logit(key)));
+                }
             };
-            if (listed)
-                for (uint32_t i = threadIdx.x; i < inside; i += TPB) take(sh.list[i]);
+            if (n_list != NO_BIN)
+                for (uint32_t i = threadIdx.x; i < n_list; i += TPB) take(entry_key(sh.list[i]));
             else
                 each([&](uint32_t, float l) {
                     if (l != -INFINITY && bin_of(l) == bin) take(logit_key(l));
@@ -393,151 +835,253 @@ struct SampleRow {
         }
         return cut;
     }
+
+    // The classes that `take`, in the list; how many they are, NO_BIN if too many.
+    template <class F>
+    __device__ __forceinline__ uint32_t gather(F &&take) {
+        __syncthreads();
+        if (threadIdx.x == 0) sh.n_list = 0;
+        __syncthreads();
+        each([&](uint32_t c, float l) {
+            if (l != -INFINITY && take(c, l)) {
+                const uint32_t at = atomicAdd(&sh.n_list, 1u);
+                if (at < Shared::LIST) sh.list[at] = entry_of(l, c);
+            }
+        });
+        __syncthreads();
+        return sh.n_list <= Shared::LIST ? sh.n_list : NO_BIN;
+    }
 };
+
+// The draw among the first k classes, which are all in the list of m. Their order is every
+// entry's rank among the list; sums in it and by class then need only k numbers.
+template <class T, int TPB>
+__device__ __forceinline__ void draw_listed(SampleRow<T, TPB> &R, const Draw &D, uint64_t row,
+                                            const RowOptions &O, uint32_t m) {
+    auto &sh = R.sh;
+    uint64_t *weights = sh.wt;   // by rank
+    uint32_t *classes = sh.ct;
+    for (uint32_t i = threadIdx.x; i < m; i += TPB) {
+        const uint64_t e = sh.list[i];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < m; j++) rank += sh.list[j] > e;
+        if (rank < O.k) {
+            weights[rank] = R.S.weight(key_logit(entry_key(e)));
+            classes[rank] = entry_class(e);
+        }
+    }
+    __syncthreads();
+    const uint32_t i = threadIdx.x, k = min(O.k, m);
+    uint64_t w = i < k ? weights[i] : 0;
+    const uint32_t c = i < k ? classes[i] : 0;
+    if (O.p31 < 1u << 31) {
+        uint64_t upto;
+        const uint64_t all = R.sum(w, &upto);
+        uint64_t weight = share(O.p31, all, 0x7FFFFFFFu);
+        if (weight == 0) weight = 1;
+        if (upto - w >= weight) w = 0;
+    }
+    if (w < O.least) w = 0;
+    const uint64_t total = R.sum(w);  // (its barriers stand before the writes)
+    if (i < k) weights[i] = w;
+    __syncthreads();
+    const uint64_t target = share(uniform31(D.uniforms[row]), total, 0);
+    uint64_t before = 0;
+    if (w)
+        for (uint32_t j = 0; j < k; j++) before += classes[j] < c ? weights[j] : 0;
+    if (w && before <= target && target < before + w) {
+        const float l = (float)R.row[c];
+        put_class(D, row, c, R.S.z(l), total);
+    }
+}
 
 template <class T, int TPB>
 __global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D) {
     __shared__ RowShared<TPB> sh;
     constexpr int N = 16 / sizeof(T);
+    constexpr uint32_t BINS = RowShared<TPB>::BINS;
     const uint64_t r = blockIdx.x;
     const uint32_t n = D.n_classes;
     const RowOptions O = row_options(D, r);
     SampleRow<T, TPB> R{sh, logits + r * n, n, {}, 0.0f};
-    float most;
+    float most, own, least;
     uint32_t most_at;
-    R.largest(most, most_at);
-    if (most == -INFINITY || O.inv_t == 0.0 || O.k == 1) {
-        if (threadIdx.x == 0) {
-            const bool none = most == -INFINITY;
-            D.classes[r] = none ? -1 : (int64_t)most_at;
-            if (D.log_probs) D.log_probs[r] = none ? -INFINITY : 0.0f;
-        }
+    R.largest(most, most_at, own, least);
+    if (most == -INFINITY || O.k == 1) {
+        if (threadIdx.x == 0)
+            put_class(D, r, most == -INFINITY ? -1 : (int64_t)most_at, 0.0, WEIGHT_ONE);
         return;
     }
     R.S = RowScale{most, (double)most, O.inv_t};
-    R.per_nat = (float)(O.inv_t * (RowShared<TPB>::BINS / 32));
 
-    Cut cut{0, 0};
-    uint64_t tie_w = 0;
-    if (O.k < n || O.p31 < 1u << 31) {
-        R.clear(RowShared<TPB>::BINS);
-        R.each([&](uint32_t, float l) {
-            if (l != -INFINITY) R.count(R.bin_of(l), R.S.weight(l));
-        });
-        if (threadIdx.x == 0) {
-            sh.before_ct = 0;
-            sh.before_wt = 0;
-        }
-        // (refine() reuses the bins, so top-p looks for its bin first, among all
-        // classes and, once their weight is known, among the first k.)
-        __syncthreads();
-        uint64_t all = 0;
-        for (uint32_t b = threadIdx.x & 63; b < RowShared<TPB>::BINS; b += 64) all += sh.wt[b];
-        for (int d = 1; d < 64; d <<= 1)
-            all += (uint64_t)__shfl_xor((uint32_t)(all >> 32), d) * 0x100000000ull +
-                   __shfl_xor((uint32_t)all, d);
-        uint32_t k_bin = NO_BIN, k_inside = 0, k_before = 0;
-        uint64_t k_weight = 0;
-        if (O.k < n) {
-            R.find(RowShared<TPB>::BINS, true, O.k, 0);
-            k_bin = sh.bin;
-            if (k_bin != NO_BIN) {
-                k_inside = sh.ct[k_bin];
-                k_before = sh.before_ct;
-                k_weight = sh.before_wt;
+    // Few classes by rank: k of the threads' own largest logits are at or above the k-th of
+    // them, so the first k classes of the row are too. One more pass lists those.
+    if (O.k < n && O.k <= RowShared<TPB>::MOST_K) {
+        R.per = most > least ? (float)BINS / (most - least) : 0.0f;
+        R.clear(BINS);
+        if (own != -INFINITY) atomicAdd(&sh.ct[R.bin_of(own)], 1u);
+        R.before(0, 0);
+        R.find(BINS, true, O.k, 0);
+        const uint32_t bin = sh.bin;
+        if (bin != NO_BIN) {
+            const uint32_t m = R.gather([&](uint32_t, float l) { return R.bin_of(l) <= bin; });
+            if (m != NO_BIN) {
+                draw_listed(R, D, r, O, m);
+                return;
             }
         }
+    }
+    R.per = (float)(O.inv_t * (BINS / 32));  // 32 (max - l) / T over all bins
+
+    // tile sums: TPB pieces of N classes a tile, in class order
+    const uint32_t tiles = (n + TPB * N - 1) / (TPB * N);
+    for (uint32_t t = threadIdx.x; t < MOST_TILES; t += TPB) {
+        sh.tile_w[t] = 0;
+        sh.tile_ties[t] = 0;
+    }
+    // Adds up, tile by tile, what f(class, logit, weight, ties) finds in a piece.
+    const auto sum_tiles = [&](auto &&f) {
+        __syncthreads();
+        for (uint32_t t = 0; t < tiles; t++) {
+            uint64_t w = 0;
+            uint32_t ties = 0;
+            const uint32_t i = (t * TPB + threadIdx.x) * N;
+            if (i + N <= n) {
+                const Piece<T, N> p = load_piece<T, N>(R.row + i);
+#pragma unroll
+                for (int j = 0; j < N; j++) f(i + j, masked_nan((float)p.v[j]), w, ties);
+            } else {
+                for (uint32_t j = i; j < n; j++) f(j, masked_nan((float)R.row[j]), w, ties);
+            }
+            for (int d = 32; d; d >>= 1) {
+                w += (uint64_t)__shfl_xor((uint32_t)(w >> 32), d) * 0x100000000ull +
+                     __shfl_xor((uint32_t)w, d);
+                ties += __shfl_xor(ties, d);
+            }
+            if ((threadIdx.x & 63) == 0) {
+                if (w)
+                    atomicAdd(reinterpret_cast<unsigned long long *>(&sh.tile_w[t]),
+                              (unsigned long long)w);
+                if (ties) atomicAdd(&sh.tile_ties[t], ties);
+            }
+        }
+        __syncthreads();
+    };
+    // A class' part in a sum once the cut is known.
+    Cut cut{0, 0};
+    uint64_t tie_w = 0;
+    const auto staying = [&](float l, uint64_t &w, uint32_t &ties) {
+        const uint32_t key = logit_key(l);
+        if (l == -INFINITY || key < cut.key) return;
+        if (key == cut.key) {
+            ties++;
+            return;
+        }
+        const uint64_t v = R.S.weight(l);
+        if (v >= O.least) w += v;
+    };
+
+    if (O.k < n) {
+        // Many classes by rank: both cuts from one histogram, then digits of the key.
+        const auto histogram = [&] {
+            R.clear(BINS);
+            R.each([&](uint32_t, float l) {
+                if (l != -INFINITY) {
+                    const uint32_t b = R.bin_of(l);
+                    atomicAdd(&sh.ct[b], 1u);
+                    R.add_weight(b, R.S.weight(l));
+                }
+            });
+            R.before(0, 0);
+        };
+        histogram();
+        __syncthreads();
+        uint64_t all = 0;
+        for (uint32_t b = threadIdx.x; b < BINS; b += TPB) all += sh.wt[b];
+        all = R.sum(all);
+        R.find(BINS, true, O.k, 0);
+        const uint32_t k_bin = sh.bin;
         if (k_bin != NO_BIN) {
-            cut = R.refine(k_bin, k_inside, true, O.k, 0);
+            const uint32_t inside = sh.ct[k_bin];
+            const uint32_t m =
+                inside <= RowShared<TPB>::LIST
+                    ? R.gather([&](uint32_t, float l) { return R.bin_of(l) == k_bin; })
+                    : NO_BIN;
+            cut = R.refine(k_bin, m, true, O.k, 0);
             tie_w = R.S.weight(key_logit(cut.key));
             all = sh.before_wt + cut.ties * tie_w;
         }
         if (O.p31 < 1u << 31) {
             uint64_t weight = share(O.p31, all, 0x7FFFFFFFu);
             if (weight == 0) weight = 1;
-            // The bins again, unless they still stand.
-            if (k_bin != NO_BIN) {
-                if (weight > k_weight) {  // in the bin of the k-th class
-                    __syncthreads();
-                    if (threadIdx.x == 0) {
-                        sh.before_ct = k_before;
-                        sh.before_wt = k_weight;
-                    }
-                    cut = R.refine(k_bin, k_inside, false, 0, weight);
-                } else {
-                    R.clear(RowShared<TPB>::BINS);
-                    R.each([&](uint32_t, float l) {
-                        if (l != -INFINITY) R.count(R.bin_of(l), R.S.weight(l));
-                    });
-                    if (threadIdx.x == 0) {
-                        sh.before_ct = 0;
-                        sh.before_wt = 0;
-                    }
-                    R.find(RowShared<TPB>::BINS, false, 0, weight);
-                    const uint32_t bin = sh.bin, inside = sh.ct[bin];
-                    cut = R.refine(bin, inside, false, 0, weight);
-                }
-            } else {
-                __syncthreads();
-                if (threadIdx.x == 0) {
-                    sh.before_ct = 0;
-                    sh.before_wt = 0;
-                }
-                R.find(RowShared<TPB>::BINS, false, 0, weight);
-                const uint32_t bin = sh.bin, inside = sh.ct[bin];
-                cut = R.refine(bin, inside, false, 0, weight);
-            }
+            if (k_bin != NO_BIN) histogram();  // (refine() has used the bins)
+            else R.before(0, 0);
+            R.find(BINS, false, 0, weight);
+            const uint32_t bin = sh.bin, inside = sh.ct[bin];
+            const uint32_t m =
+                inside <= RowShared<TPB>::LIST
+                    ? R.gather([&](uint32_t, float l) { return R.bin_of(l) == bin; })
+                    : NO_BIN;
+            cut = R.refine(bin, m, false, 0, weight);
             tie_w = R.S.weight(key_logit(cut.key));
         }
         if (tie_w < O.least) cut.ties = 0;
-    }
-
-    // The staying weight, tile by tile of TPB pieces (in class order).
-    const auto piece_sums = [&](uint32_t i, uint64_t &w, uint32_t &ties) {
-        w = 0;
-        ties = 0;
-        const auto one = [&](float l) {
-            const uint32_t key = logit_key(l);
-            if (l == -INFINITY || key < cut.key) return;
-            if (key == cut.key) {
-                ties++;
-                return;
+        sum_tiles([&](uint32_t, float l, uint64_t &w, uint32_t &t) { staying(l, w, t); });
+    } else if (O.p31 < 1u << 31) {
+        // By weight alone: a histogram finds the cut's bin; one pass then sums the bins
+        // before it and lists its own classes, whose digits find the cut.
+        R.clear(BINS);
+        R.each([&](uint32_t, float l) {
+            if (l != -INFINITY) R.add_weight(R.bin_of(l), R.S.weight(l));
+        });
+        R.before(0, 0);
+        __syncthreads();
+        uint64_t all = 0;
+        for (uint32_t b = threadIdx.x; b < BINS; b += TPB) all += sh.wt[b];
+        all = R.sum(all);
+        uint64_t weight = share(O.p31, all, 0x7FFFFFFFu);
+        if (weight == 0) weight = 1;
+        R.find(BINS, false, 0, weight);
+        const uint32_t bin = sh.bin;
+        if (threadIdx.x == 0) sh.n_list = 0;
+        sum_tiles([&](uint32_t c, float l, uint64_t &w, uint32_t &) {
+            if (l == -INFINITY) return;
+            const uint32_t b = R.bin_of(l);
+            if (b < bin) {
+                const uint64_t v = R.S.weight(l);
+                if (v >= O.least) w += v;
+            } else if (b == bin) {
+                const uint32_t at = atomicAdd(&sh.n_list, 1u);
+                if (at < RowShared<TPB>::LIST) sh.list[at] = entry_of(l, c);
             }
-            const uint64_t v = R.S.weight(l);
-            if (v >= O.least) w += v;
-        };
-        if (i + N <= n) {
-            const Piece<T, N> p = load_piece<T, N>(R.row + i);
-#pragma unroll
-            for (int j = 0; j < N; j++) one(masked_nan((float)p.v[j]));
-        } else {
-            for (uint32_t j = i; j < n; j++) one(masked_nan((float)R.row[j]));
-        }
-    };
-    __syncthreads();
-    for (uint32_t t = threadIdx.x; t < MOST_TILES; t += TPB) {
-        sh.tile_w[t] = 0;
-        sh.tile_ties[t] = 0;
-    }
-    __syncthreads();
-    const uint32_t tiles = (n + TPB * N - 1) / (TPB * N);
-    for (uint32_t t = 0; t < tiles; t++) {
-        uint64_t w;
-        uint32_t ties;
-        piece_sums((t * TPB + threadIdx.x) * N, w, ties);
-        for (int d = 32; d; d >>= 1) {
-            w += (uint64_t)__shfl_xor((uint32_t)(w >> 32), d) * 0x100000000ull +
-                 __shfl_xor((uint32_t)w, d);
-            ties += __shfl_xor(ties, d);
-        }
-        if ((threadIdx.x & 63) == 0) {
+        });
+        const uint32_t m = sh.n_list <= RowShared<TPB>::LIST ? sh.n_list : NO_BIN;
+        cut = R.refine(bin, m, false, 0, weight);
+        tie_w = R.S.weight(key_logit(cut.key));
+        if (tie_w < O.least) cut.ties = 0;
+        const auto one = [&](uint32_t c, float l) {
+            uint64_t w = 0;
+            uint32_t ties = 0;
+            staying(l, w, ties);
+            const uint32_t t = c / (TPB * N);
             if (w)
                 atomicAdd(reinterpret_cast<unsigned long long *>(&sh.tile_w[t]),
                           (unsigned long long)w);
             if (ties) atomicAdd(&sh.tile_ties[t], ties);
+        };
+        if (m != NO_BIN) {
+            for (uint32_t i = threadIdx.x; i < m; i += TPB)
+                one(entry_class(sh.list[i]), key_logit(entry_key(sh.list[i])));
+        } else {
+            R.each([&](uint32_t c, float l) {
+                if (l != -INFINITY && R.bin_of(l) == bin) one(c, l);
+            });
         }
+        __syncthreads();
+    } else {
+        sum_tiles([&](uint32_t, float l, uint64_t &w, uint32_t &t) { staying(l, w, t); });
     }
-    __syncthreads();
+
     if (threadIdx.x == 0) {
         uint64_t total = 0;
         uint32_t left = cut.ties;
@@ -546,7 +1090,7 @@ __global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D
             left -= k;
             total += sh.tile_w[t] + k * tie_w;
         }
-        const uint64_t target = share(O.u31, total, 0);
+        const uint64_t target = share(uniform31(D.uniforms[r]), total, 0);
         uint64_t before = 0;
         left = cut.ties;
         uint32_t t = 0;
@@ -564,20 +1108,12 @@ __global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D
     }
     __syncthreads();
     // The tile that holds the target: its pieces' sums in order, then the piece.
-    const uint32_t i0 = (sh.tile * TPB + threadIdx.x) * N;
-    uint64_t w;
-    uint32_t ties;
-    piece_sums(i0, w, ties);
-    uint64_t cw = w;
-    uint32_t ct = ties;
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t y = shfl64_up(cw, d, 64);
-        const uint32_t z = __shfl_up(ct, d);
-        if ((threadIdx.x & 63) >= (uint32_t)d) {
-            cw += y;
-            ct += z;
-        }
-    }
+    const uint32_t i0 = (sh.tile * TPB + threadIdx.x) * N, i1 = min(i0 + N, n);
+    uint64_t w = 0;
+    uint32_t ties = 0;
+    for (uint32_t j = i0; j < i1; j++) staying(masked_nan((float)R.row[j]), w, ties);
+    uint64_t cw = scan64(w, threadIdx.x & 63);
+    uint32_t ct = scan32(ties, threadIdx.x & 63);
     if ((threadIdx.x & 63) == 63) {
         sh.wave_w[threadIdx.x / 64] = cw;
         sh.wave_ties[threadIdx.x / 64] = ct;
@@ -591,22 +1127,15 @@ __global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D
     uint64_t before = cw - w + min(ct - ties, sh.ties) * tie_w;
     if (before <= sh.target && sh.target < behind) {
         uint32_t seen = ct - ties;
-        for (uint32_t j = i0; j < min(i0 + N, n); j++) {
+        for (uint32_t j = i0; j < i1; j++) {
             const float l = masked_nan((float)R.row[j]);
-            const uint32_t key = logit_key(l);
-            if (l == -INFINITY || key < cut.key) continue;
-            uint64_t v;
-            if (key == cut.key) v = seen++ < sh.ties ? tie_w : 0;
-            else {
-                v = R.S.weight(l);
-                if (v < O.least) v = 0;
-            }
+            uint64_t v = 0;
+            uint32_t tie = 0;
+            staying(l, v, tie);
+            if (tie) v = seen++ < sh.ties ? tie_w : 0;
             before += v;
             if (before > sh.target) {
-                D.classes[r] = j;
-                if (D.log_probs)
-                    D.log_probs[r] =
-                        (float)(R.S.z(l) - log((double)sh.total / (double)WEIGHT_ONE));
+                put_class(D, r, j, R.S.z(l), sh.total);
                 break;
             }
         }
@@ -616,24 +1145,38 @@ __global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D
 template <class T>
 void launch_sample(const void *logits, const Draw &D, hipStream_t s) {
     const auto *l = static_cast<const T *>(logits);
-    if (D.n_classes <= GROUP_MOST) {
-        uint32_t g = 2;
-        while (g < D.n_classes) g *= 2;
-        const uint64_t blocks = (D.n_rows + GROUP_TPB / g - 1) / (GROUP_TPB / g);
+    const uint64_t n = D.n_rows;
+    const uint32_t v = D.n_classes;
+    if (v <= THREAD_MOST) {
+        head_input(n <= 1ull << 31, "too many rows");
+        const dim3 grid((uint32_t)((n + 255) / 256)), tpb(256);
+        if (v == 1) hipLaunchKernelGGL((sample_thread_kernel<T, 1>), grid, tpb, 0, s, l, D);
+        else if (v == 2) hipLaunchKernelGGL((sample_thread_kernel<T, 2>), grid, tpb, 0, s, l, D);
+        else if (v == 3) hipLaunchKernelGGL((sample_thread_kernel<T, 3>), grid, tpb, 0, s, l, D);
+        else if (v == 4) hipLaunchKernelGGL((sample_thread_kernel<T, 4>), grid, tpb, 0, s, l, D);
+        else if (v == 5) hipLaunchKernelGGL((sample_thread_kernel<T, 5>), grid, tpb, 0, s, l, D);
+        else if (v == 6) hipLaunchKernelGGL((sample_thread_kernel<T, 6>), grid, tpb, 0, s, l, D);
+        else if (v == 7) hipLaunchKernelGGL((sample_thread_kernel<T, 7>), grid, tpb, 0, s, l, D);
+        else hipLaunchKernelGGL((sample_thread_kernel<T, 8>), grid, tpb, 0, s, l, D);
+    } else if (v <= GROUP_MOST) {
+        const uint32_t g = v <= 16 ? 16 : v <= 32 ? 32 : 64;
+        const uint64_t blocks = (n + GROUP_TPB / g - 1) / (GROUP_TPB / g);
         head_input(blocks < 1u << 24, "too many rows");
         const dim3 grid((uint32_t)blocks), tpb(GROUP_TPB);
-        if (g == 2) hipLaunchKernelGGL((sample_group_kernel<T, 2>), grid, tpb, 0, s, l, D);
-        else if (g == 4) hipLaunchKernelGGL((sample_group_kernel<T, 4>), grid, tpb, 0, s, l, D);
-        else if (g == 8) hipLaunchKernelGGL((sample_group_kernel<T, 8>), grid, tpb, 0, s, l, D);
-        else if (g == 16) hipLaunchKernelGGL((sample_group_kernel<T, 16>), grid, tpb, 0, s, l, D);
+        if (g == 16) hipLaunchKernelGGL((sample_group_kernel<T, 16>), grid, tpb, 0, s, l, D);
         else if (g == 32) hipLaunchKernelGGL((sample_group_kernel<T, 32>), grid, tpb, 0, s, l, D);
         else hipLaunchKernelGGL((sample_group_kernel<T, 64>), grid, tpb, 0, s, l, D);
+    } else if (v <= WAVE_MOST) {
+        head_input(n < 1u << 25, "too many rows");
+        const dim3 grid((uint32_t)((n + 3) / 4)), tpb(256);
+        if (v <= 128) hipLaunchKernelGGL((sample_wave_kernel<T, 2>), grid, tpb, 0, s, l, D);
+        else if (v <= 256) hipLaunchKernelGGL((sample_wave_kernel<T, 4>), grid, tpb, 0, s, l, D);
+        else if (v <= 512) hipLaunchKernelGGL((sample_wave_kernel<T, 8>), grid, tpb, 0, s, l, D);
+        else hipLaunchKernelGGL((sample_wave_kernel<T, 16>), grid, tpb, 0, s, l, D);
     } else {
-        head_input(D.n_rows < 1u << 22, "too many rows");
-        const dim3 grid((uint32_t)D.n_rows);
-        if (D.n_classes <= 2048)
-            hipLaunchKernelGGL((sample_row_kernel<T, 64>), grid, dim3(64), 0, s, l, D);
-        else if (D.n_classes <= 16384)
+        head_input(n < 1u << 22, "too many rows");
+        const dim3 grid((uint32_t)n);
+        if (v <= 16384)
             hipLaunchKernelGGL((sample_row_kernel<T, 256>), grid, dim3(256), 0, s, l, D);
         else hipLaunchKernelGGL((sample_row_kernel<T, 1024>), grid, dim3(1024), 0, s, l, D);
     }
@@ -644,6 +1187,13 @@ void sample(const void *logits, uint32_t dtype, const Draw &D, hipStream_t s) {
     if (dtype == FBH_F32) launch_sample<float>(logits, D, s);
     else if (dtype == FBH_F16) launch_sample<_Float16>(logits, D, s);
     else launch_sample<__bf16>(logits, D, s);
+}
+
+Draw draw_of(const float *uniforms, const fbh_sample_options *o, int64_t *classes,
+             float *log_probs, uint64_t n_rows, uint32_t n_classes) {
+    return {uniforms, *o, whole_options(o->temperature, o->top_k, o->top_p, o->min_p, n_classes),
+            o->temperatures || o->top_ks || o->top_ps || o->min_ps, classes, log_probs, n_rows,
+            n_classes};
 }
 
 void check_sample(const void *logits, uint64_t n_rows, uint32_t n_classes, const float *uniforms,
@@ -668,7 +1218,8 @@ int fbh_sample_classes(int device, const void *logits, uint64_t n_rows, uint32_t
         head_input(dtype <= FBH_BF16, "unknown cell type");
         if (n_rows == 0) return;
         const OnDevice on(device);
-        sample(logits, dtype, Draw{uniforms, *options, classes, log_probs, n_rows, n_classes},
+        sample(logits, dtype,
+               draw_of(uniforms, options, classes, log_probs, n_rows, n_classes),
                static_cast<hipStream_t>(stream));
     });
 }
@@ -704,7 +1255,7 @@ int fbh_sample_classes_host(int device, const float *logits, uint64_t n_rows, ui
                    "logit upload");
         head_check(hipMemcpyAsync(d_u, uniforms, 4 * n_rows, hipMemcpyHostToDevice, s),
                    "uniform upload");
-        sample(block, FBH_F32, Draw{d_u, *options, d_c, d_p, n_rows, n_classes}, s);
+        sample(block, FBH_F32, draw_of(d_u, options, d_c, d_p, n_rows, n_classes), s);
         head_check(hipMemcpyAsync(classes, d_c, 8 * n_rows, hipMemcpyDeviceToHost, s),
                    "class download");
         if (log_probs)

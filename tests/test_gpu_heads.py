@@ -278,9 +278,11 @@ def _check_sample(heads, x, u, t, k, p, m):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("n, v", [(1, 1), (300, 2), (200, 3), (130, 4), (77, 7), (50, 33),
-                                  (40, 64), (40, 65), (30, 500), (9, 2048), (7, 2049),
-                                  (3, 16_384), (3, 16_385), (2, 131_071)])
+@pytest.mark.parametrize("n, v", [(1, 1), (300, 2), (200, 3), (130, 4), (300, 5), (64, 6), (77, 7),
+                                  (257, 8), (40, 9), (33, 16), (20, 17), (50, 33), (40, 64),
+                                  (40, 65), (9, 128), (9, 129), (13, 256), (10, 400), (30, 500),
+                                  (11, 1000), (6, 1024), (6, 1025), (9, 2048), (7, 2049),
+                                  (3, 16_384), (3, 16_385), (2, 131_071), (1, 262_144)])
 def test_sample(heads, n, v, dtype):
     rng = np.random.default_rng([n, v])
     x = rng.normal(size=(n, v)) * 3
@@ -304,7 +306,7 @@ def test_sample(heads, n, v, dtype):
         _check_sample(heads, x, u, t, k, p, m)
 
 
-@pytest.mark.parametrize("v", [4, 40, 300, 3000, 20_000])
+@pytest.mark.parametrize("v", [4, 8, 40, 90, 300, 1000, 3000, 20_000])
 def test_sample_options_of_each_row(heads, v):
     rng = np.random.default_rng(v)
     n = 64 if v <= 3000 else 12
@@ -317,13 +319,14 @@ def test_sample_options_of_each_row(heads, v):
     _check_sample(heads, x, u, t, k, p, m)
 
 
-@pytest.mark.parametrize("v", [48, 700, 5000, 40_000])
+@pytest.mark.parametrize("v", [8, 48, 120, 700, 5000, 40_000])
 def test_sample_of_ties_and_far_logits(heads, v):
     """Cuts that fall among equal logits, and among ones beyond the range of weights."""
     rng = np.random.default_rng(v)
     n = 24
     x = rng.integers(0, 3, (n, v)).astype(np.float32)
     x[: n // 2, 5:] -= rng.choice([0.0, 50.0, 1e9], (n // 2, v - 5)).astype(np.float32)
+    x[n // 2, 3:] = -1e30  # all but three far below
     u = torch.from_numpy(rng.random(n).astype(np.float32)).cuda()
     for dtype in ("f32", "bf16"):
         d = torch.from_numpy(x).to(TYPES[dtype]).cuda()
