@@ -401,6 +401,140 @@ __global__ __launch_bounds__(SORT_TPB) void sort_scatter_kernel(Positions P, Sor
     }
 }
 
+// ---- Up to 64k positions. Every workgroup owns a range of tokens, goes through all
+// positions and places its own: how many have lower tokens is counted on the way, so one
+// launch does what a radix pass takes three for. It also writes the zeros of its range's
+// tokens that have no position, so the table needs no pass of its own.
+constexpr uint32_t FEW_MOST = 65536;           // positions
+constexpr uint32_t FEW_TPB = 512;
+constexpr uint32_t FEW_WAVES = FEW_TPB / 64;
+constexpr uint32_t FEW_RANGE = 1024;           // tokens of a workgroup at most
+constexpr uint32_t FEW_STEP = 4 * 64;          // positions that a wave takes at a time
+
+template <int ID, bool DROP>
+__global__ __launch_bounds__(256) void few_tokens_kernel(Positions P, uint32_t n, uint32_t padded,
+                                                         uint32_t *tokens) {
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= padded) return;
+    uint32_t tok = NO_TOKEN;
+    if (i < n) tok = token_at<ID, DROP>(P, i, P.n_columns > 1 ? i % P.n_columns : 0);
+    tokens[i] = tok;
+}
+
+struct Few {
+    const uint32_t *tokens;  // of all positions, padded to FEW_WAVES * steps * FEW_STEP
+    uint32_t n, steps;       // positions; steps of a wave
+    uint32_t n_tokens, range, per_row;
+    uint32_t *keys, *vals;   // by token
+};
+
+template <class T, int VEC>
+__global__ __launch_bounds__(FEW_TPB) void few_sort_kernel(Few F, T *table, uint32_t dim,
+                                                           uint32_t n_pieces) {
+    extern __shared__ uint32_t seen[];  // [wave][token]: counts, then places
+    __shared__ uint32_t wave_sum[FEW_WAVES], lower[FEW_WAVES];
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x / 64;
+    const uint32_t t0 = blockIdx.x * F.range, range = min(F.range, F.n_tokens - t0);
+    for (uint32_t i = threadIdx.x; i < FEW_WAVES * F.range; i += FEW_TPB) seen[i] = 0;
+    __syncthreads();
+    const uint4 *from = reinterpret_cast<const uint4 *>(F.tokens) + w * F.steps * 64 + lane;
+    uint32_t *mine = seen + w * F.range;
+    uint32_t below_range = 0;
+#pragma unroll 4
+    for (uint32_t k = 0; k < F.steps; k++) {
+        const uint4 q = from[k * 64];
+        const uint32_t tok[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+            below_range += tok[j] < t0;
+            if (tok[j] - t0 < range) atomicAdd(&mine[tok[j] - t0], 1u);
+        }
+    }
+    for (int d = 32; d; d >>= 1) below_range += __shfl_xor(below_range, d);
+    if (lane == 0) lower[w] = below_range;
+    __syncthreads();
+    // places: by token, then by wave. Two tokens a thread.
+    uint32_t c[2] = {0, 0};
+    for (uint32_t j = 0; j < 2; j++)
+        if (2 * threadIdx.x + j < range)
+            for (uint32_t v = 0; v < FEW_WAVES; v++) c[j] += seen[v * F.range + 2 * threadIdx.x + j];
+    uint32_t x = c[0] + c[1];
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t y = __shfl_up(x, d);
+        if (lane >= (uint32_t)d) x += y;
+    }
+    if (lane == 63) wave_sum[w] = x;
+    __syncthreads();
+    uint32_t at = x - c[0] - c[1], end = 0;
+    for (uint32_t v = 0; v < FEW_WAVES; v++) {
+        at += lower[v] + (v < w ? wave_sum[v] : 0);
+        end += lower[v] + wave_sum[v];
+    }
+    for (uint32_t j = 0; j < 2; j++)
+        if (2 * threadIdx.x + j < range) {
+            uint32_t a = at;
+            for (uint32_t v = 0; v < FEW_WAVES; v++) {
+                uint32_t *p = &seen[v * F.range + 2 * threadIdx.x + j];
+                const uint32_t m = *p;
+                *p = a;
+                a += m;
+            }
+            at += c[j];
+        }
+    __syncthreads();
+    // Every wave places its positions: the lanes of one token after the other.
+    for (uint32_t k0 = 0; k0 < F.steps; k0 += 4) {
+        uint4 q[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) q[i] = from[min(k0 + i, F.steps - 1) * 64];
+#pragma unroll
+        for (uint32_t i = 0; i < 16; i++) {
+            const uint32_t tok = i % 4 == 0   ? q[i / 4].x
+                                 : i % 4 == 1 ? q[i / 4].y
+                                 : i % 4 == 2 ? q[i / 4].z
+                                              : q[i / 4].w;
+            const bool in = k0 + i / 4 < F.steps && tok - t0 < range;
+            uint64_t left = __ballot(in);
+            while (left) {
+                const uint32_t one = __builtin_amdgcn_readlane(tok, __ffsll((long long)left) - 1);
+                const uint64_t same = __ballot(in && tok == one);
+                volatile uint32_t *count = &mine[one - t0];
+                const uint32_t place = *count;
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                if (lane == 0) *count = place + __popcll(same);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                if (in && tok == one) {
+                    const uint32_t to = place + __popcll(same & ((1ull << lane) - 1));
+                    const uint32_t pos = ((w * F.steps + k0 + i / 4) * 64 + lane) * 4 + i % 4;
+                    F.keys[to] = one;
+                    F.vals[to] = F.per_row > 1 ? pos / F.per_row : pos;
+                }
+                left &= ~same;
+            }
+        }
+    }
+    // the positions that give nothing, behind all others
+    if (blockIdx.x == gridDim.x - 1)
+        for (uint32_t i = end + threadIdx.x; i < F.n; i += FEW_TPB) F.keys[i] = F.n_tokens;
+    __syncthreads();
+    // seen[last wave][token] is now the place behind the token's last position, and the
+    // token before it ends where it starts
+    uint32_t first_place = 0;
+    for (uint32_t v = 0; v < FEW_WAVES; v++) first_place += lower[v];
+    const uint32_t *ends = seen + (FEW_WAVES - 1) * F.range;
+    for (uint32_t i = threadIdx.x; i < range * n_pieces; i += FEW_TPB) {
+        const uint32_t tok = i / n_pieces;
+        if ((tok ? ends[tok - 1] : first_place) != ends[tok]) continue;
+        const uint32_t cell = min((i - tok * n_pieces) * VEC, dim - VEC);
+        Piece<T, VEC> o;
+#pragma unroll
+        for (int j = 0; j < VEC; j++) o.v[j] = (T)0.0f;
+        store_piece<T, VEC>(table + (uint64_t)(t0 + tok) * dim + cell, o);
+    }
+}
+
 // 16-byte pieces of zeros, and the rest in bytes.
 __global__ __launch_bounds__(256) void zero_kernel(uint8_t *p, uint64_t bytes) {
     const uint64_t head = min(bytes, (uint64_t)(-(intptr_t)p & 15));
@@ -482,11 +616,12 @@ __global__ __launch_bounds__(EMB_TPB) void grad_runs_kernel(Runs R, const T *gra
 constexpr uint32_t JOIN_SHORT = 16;  // parts that one chunk's lanes join by themselves
 
 // Joins the parts of the runs that start in a chunk and go on behind it.
+constexpr uint32_t JOIN_TPB = 1024;
 template <class T, int VEC>
-__global__ __launch_bounds__(EMB_TPB) void grad_join_kernel(Runs R, T *table) {
-    __shared__ uint32_t longs[EMB_TPB], n_longs;
-    __shared__ float sums[EMB_TPB * VEC];
-    const uint32_t lanes = 1u << R.lg_g, groups = EMB_TPB >> R.lg_g;
+__global__ __launch_bounds__(JOIN_TPB) void grad_join_kernel(Runs R, T *table) {
+    __shared__ uint32_t longs[JOIN_TPB], n_longs;
+    __shared__ float sums[JOIN_TPB * VEC];
+    const uint32_t lanes = 1u << R.lg_g, groups = JOIN_TPB >> R.lg_g;
     const uint32_t g = threadIdx.x >> R.lg_g, lane = threadIdx.x & (lanes - 1);
     const uint32_t piece = (blockIdx.y << R.lg_g) + lane;
     const bool live = piece < R.n_pieces;
@@ -1074,6 +1209,7 @@ ColumnPlan column_plan(const fbh_embed *e) {
 struct GradPlan {
     uint32_t n = 0, passes = 0, bits = 0, blocks = 0, vec = 0, pieces = 0, lg_g = 0, chunk = 0,
              chunks = 0;
+    uint32_t range = 0, steps = 0, padded = 0;  // few positions: of a workgroup, of a wave
     uint64_t keys[2], vals[2], counts = 0, totals = 0, parts = 0, bytes = 0;
 };
 
@@ -1099,6 +1235,17 @@ GradPlan grad_plan(const fbh_embed *e) {
         G.bytes = (at + bytes + 255) & ~255ull;
         return at;
     };
+    if (n <= FEW_MOST && e->n_tokens <= FEW_RANGE * 1024) {
+        // a workgroup a CU, or more where the tokens are many
+        G.range = std::min((e->n_tokens + 255) / 256, FEW_RANGE);
+        G.steps = (G.n + FEW_WAVES * FEW_STEP - 1) / (FEW_WAVES * FEW_STEP);
+        G.padded = G.steps * FEW_WAVES * FEW_STEP;
+        G.keys[1] = take(4ull * G.padded);  // the tokens
+        G.keys[0] = take(4 * n);
+        G.vals[0] = take(4 * n);
+        G.parts = take(8ull * G.chunks * e->dim);
+        return G;
+    }
     for (int i = 0; i < 2; i++) {
         G.keys[i] = take(4 * n);
         G.vals[i] = take(4 * n);
@@ -1181,17 +1328,37 @@ void embed_grad(const fbh_embed *e, const void *grad, void *table, void *work, h
         P.n_rows *= P.n_columns;
         P.n_columns = 1;
     }
-    const uint64_t bytes =
-        (uint64_t)e->n_tokens * e->dim * (e->dtype == FBH_F32 ? 4 : 2);
-    hipLaunchKernelGGL(zero_kernel, dim3((uint32_t)std::min<uint64_t>((bytes + 4095) / 4096, 4096)),
-                       dim3(256), 0, s, static_cast<uint8_t *>(table), bytes);
-    head_check(hipGetLastError(), "table gradient");
     const GradPlan G = grad_plan(e);
-    if (G.n == 0) return;
     auto *w = static_cast<uint8_t *>(work);
     const auto list = [&](uint64_t at) { return reinterpret_cast<uint32_t *>(w + at); };
+    const bool few = G.n && G.range;
+    if (few) {
+        with_ids(e->id_type, e->drop > 0.0, [&](auto id, auto drop) {
+            hipLaunchKernelGGL((few_tokens_kernel<decltype(id)::value, decltype(drop)::value>),
+                               dim3(G.padded / 256), dim3(256), 0, s, P, G.n, G.padded,
+                               list(G.keys[1]));
+        });
+        head_check(hipGetLastError(), "tokens");
+        const Few F{list(G.keys[1]), G.n, G.steps, e->n_tokens, G.range,
+                    e->pooled ? e->n_columns : 1, list(G.keys[0]), list(G.vals[0])};
+        with_cells(e->dtype, G.vec, [&](auto one, auto vec) {
+            using T = decltype(one);
+            hipLaunchKernelGGL((few_sort_kernel<T, decltype(vec)::value>),
+                               dim3((e->n_tokens + G.range - 1) / G.range), dim3(FEW_TPB),
+                               FEW_WAVES * G.range * 4, s, F, static_cast<T *>(table), e->dim,
+                               G.pieces);
+        });
+        head_check(hipGetLastError(), "token sort");
+    } else {
+        const uint64_t bytes = (uint64_t)e->n_tokens * e->dim * (e->dtype == FBH_F32 ? 4 : 2);
+        hipLaunchKernelGGL(zero_kernel,
+                           dim3((uint32_t)std::min<uint64_t>((bytes + 4095) / 4096, 4096)),
+                           dim3(256), 0, s, static_cast<uint8_t *>(table), bytes);
+        head_check(hipGetLastError(), "table gradient");
+        if (G.n == 0) return;
+    }
     uint32_t *counts = list(G.counts), *totals = list(G.totals);
-    for (uint32_t pass = 0; pass < G.passes; pass++) {
+    for (uint32_t pass = 0; pass < (few ? 0 : G.passes); pass++) {
         const uint32_t to = pass & 1;
         const SortFrom S{list(G.keys[1 - to]), list(G.vals[1 - to]), G.n, pass * G.bits, G.bits,
                          e->pooled ? e->n_columns : 1};
@@ -1212,19 +1379,19 @@ void embed_grad(const fbh_embed *e, const void *grad, void *table, void *work, h
         else go(Int<FBH_ID_I32>{}, std::false_type{}, std::false_type{});
         head_check(hipGetLastError(), "token sort");
     }
-    const uint32_t at = (G.passes - 1) & 1;
+    const uint32_t at = few ? 0 : (G.passes - 1) & 1;
     const Runs R{list(G.keys[at]), list(G.vals[at]), G.n, G.chunk, e->n_tokens, e->dim, G.pieces,
                  G.lg_g, scale_of(e), reinterpret_cast<float *>(w + G.parts)};
     with_cells(e->dtype, G.vec, [&](auto one, auto vec) {
         using T = decltype(one);
         constexpr int VEC = decltype(vec)::value;
-        const uint32_t groups = EMB_TPB >> G.lg_g;
-        const dim3 grid((G.chunks + groups - 1) / groups,
-                        (G.pieces + (1u << G.lg_g) - 1) >> G.lg_g);
-        hipLaunchKernelGGL((grad_runs_kernel<T, VEC>), grid, dim3(EMB_TPB), 0, s, R,
-                           static_cast<const T *>(grad), static_cast<T *>(table));
-        hipLaunchKernelGGL((grad_join_kernel<T, VEC>), grid, dim3(EMB_TPB), 0, s, R,
+        const uint32_t groups = EMB_TPB >> G.lg_g, join = JOIN_TPB >> G.lg_g;
+        const uint32_t y = (G.pieces + (1u << G.lg_g) - 1) >> G.lg_g;
+        hipLaunchKernelGGL((grad_runs_kernel<T, VEC>), dim3((G.chunks + groups - 1) / groups, y),
+                           dim3(EMB_TPB), 0, s, R, static_cast<const T *>(grad),
                            static_cast<T *>(table));
+        hipLaunchKernelGGL((grad_join_kernel<T, VEC>), dim3((G.chunks + join - 1) / join, y),
+                           dim3(JOIN_TPB), 0, s, R, static_cast<T *>(table));
     });
     head_check(hipGetLastError(), "table gradient");
 }

@@ -26,8 +26,8 @@ part in autograd. Bad arguments are ValueErrors, device failures RuntimeErrors.
 
 from __future__ import annotations
 
-import ctypes as C
 import functools
+import struct
 
 import numpy as np
 
@@ -36,13 +36,19 @@ from . import _native as N
 __all__ = ["Vocabulary", "embed", "embed_grad", "dropout", "sample"]
 
 _torch = None
+_L = None
 _CELLS: dict = {}
 _IDS: dict = {}
+_raw_stream = None
+# fbh_embed and fbh_sample_options (include/fbhip.h), packed in one call: a small
+# operation's time is its host time.
+_EMBED = struct.Struct("QIIIIIIPPdQfI")
+_OPTIONS = struct.Struct("PPPPfiff")
 
 
 def _need_torch():
     """torch, once it is known to share this package's HIP runtime."""
-    global _torch
+    global _torch, _L, _raw_stream
     if _torch is not None:
         return _torch
     import torch
@@ -56,6 +62,9 @@ def _need_torch():
             "its own; import torch first")
     _CELLS.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
     _IDS.update({torch.int32: 0, torch.int64: 1, torch.float32: 2})
+    # the current stream's handle, as torch.cuda.current_stream() wraps it
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+    _L = N.hip()
     _torch = torch
     return torch
 
@@ -63,7 +72,7 @@ def _need_torch():
 def _device_tensor(x, what: str):
     if not isinstance(x, _torch.Tensor):
         raise ValueError(f"{what} must be a torch tensor, got {type(x).__name__}")
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise ValueError(f"{what} must be on a GPU, it is on {x.device}")
     return x if x.is_contiguous() else x.contiguous()
 
@@ -95,10 +104,6 @@ def _drop(drop) -> float:
     return drop
 
 
-def _stream(device) -> int:
-    return _torch.cuda.current_stream(device).cuda_stream
-
-
 class Vocabulary:
     """The table rows of several columns' ids: column t's ids 0 .. sizes[t] - 1 are rows
     first[t] .. first[t] + sizes[t] - 1 of a table of n_tokens rows (a model's trees:
@@ -123,6 +128,7 @@ class Vocabulary:
         self.first = torch.from_numpy(first.astype(np.int32)).to(device)
         if self.first.device.type != "cuda":
             raise ValueError(f"device must be a GPU, got {device!r}")
+        self.address = self.first.data_ptr()
 
     def __repr__(self):
         return (f"Vocabulary({self.n_columns} columns, {self.n_tokens} tokens, "
@@ -131,7 +137,7 @@ class Vocabulary:
 
 def _positions(ids, vocabulary, pooled: bool, n_tokens: int, dim: int, cells: int, scale: float,
                drop: float, seed: int):
-    """The call's fbh_embed, and the leading shape of its vectors."""
+    """The call's fbh_embed (None without columns), and the leading shape of its vectors."""
     code = _IDS.get(ids.dtype)
     if code is None:
         raise ValueError(f"ids must be int32, int64 or float32, got {ids.dtype}")
@@ -150,13 +156,10 @@ def _positions(ids, vocabulary, pooled: bool, n_tokens: int, dim: int, cells: in
             n_rows *= s
     else:
         n_rows, columns = ids.numel(), 1
-    e = N.Embed()
-    e.n_rows, e.n_columns, e.dim, e.n_tokens = n_rows, columns, dim, n_tokens
-    e.id_type, e.dtype, e.pooled = code, cells, 1 if pooled else 0
-    e.ids = ids.data_ptr()
-    if vocabulary is not None:
-        e.first, e.most_ids = vocabulary.first.data_ptr(), vocabulary.most_ids
-    e.drop, e.seed, e.scale = drop, seed, scale
+    first, most = (0, 0) if vocabulary is None else (vocabulary.address, vocabulary.most_ids)
+    # (a call without columns or positions launches nothing)
+    e = _EMBED.pack(n_rows, columns, dim, n_tokens, code, cells, pooled, ids.data_ptr(), first,
+                    drop, seed, scale, most) if columns else None
     return e, shape[:-1] if pooled else shape
 
 
@@ -164,10 +167,12 @@ def _embed(table, ids, vocabulary, scale, pooled, drop, seed):
     e, lead = _positions(ids, vocabulary, pooled, table.shape[0], table.shape[1],
                          _cells(table, "table"), scale, drop, seed)
     out = table.new_empty(lead + (table.shape[1],))
-    if e.n_columns == 0:
+    if e is None:
         return out.zero_()
-    N.check_hip(N.hip().fbh_embed_rows(table.device.index, C.byref(e), table.data_ptr(),
-                                       out.data_ptr(), _stream(table.device)))
+    dev = table.get_device()
+    rc = _L.fbh_embed_rows(dev, e, table.data_ptr(), out.data_ptr(), _raw_stream(dev))
+    if rc:
+        N.check_hip(rc)
     return out
 
 
@@ -249,20 +254,25 @@ def embed_grad(grad, ids, tokens, *, scale: float = 1.0, pooled: bool = False,
     if tuple(grad.shape[:-1]) != lead:
         raise ValueError(f"grad has shape {tuple(grad.shape)}, expected {lead} vectors")
     out = grad.new_empty((n_tokens, grad.shape[-1]))
-    if e.n_columns == 0:
+    if e is None:
         return out.zero_()
-    L = N.hip()
-    size = L.fbh_embed_grad_bytes(C.byref(e))
-    work = _torch.empty(size, dtype=_torch.uint8, device=grad.device)
-    N.check_hip(L.fbh_embed_grad(grad.device.index, C.byref(e), grad.data_ptr(), out.data_ptr(),
-                                 work.data_ptr(), size, _stream(grad.device)))
+    dev = grad.get_device()
+    size = _L.fbh_embed_grad_bytes(e)
+    work = grad.new_empty(size, dtype=_torch.uint8)
+    rc = _L.fbh_embed_grad(dev, e, grad.data_ptr(), out.data_ptr(), work.data_ptr(), size,
+                           _raw_stream(dev))
+    if rc:
+        N.check_hip(rc)
     return out
 
 
 def _dropout(x, drop, seed, first):
     out = _torch.empty_like(x)
-    N.check_hip(N.hip().fbh_dropout(x.device.index, x.data_ptr(), out.data_ptr(), x.numel(),
-                                    _cells(x, "x"), drop, seed, first, _stream(x.device)))
+    dev = x.get_device()
+    rc = _L.fbh_dropout(dev, x.data_ptr(), out.data_ptr(), x.numel(), _cells(x, "x"), drop, seed,
+                        first, _raw_stream(dev))
+    if rc:
+        N.check_hip(rc)
     return out
 
 
@@ -284,16 +294,21 @@ def dropout(x, drop: float, seed: int, first: int = 0):
     return _dropout(*args)
 
 
-def _option(value, what: str, lead, like, dtype, check):
-    """(a number, None) or (0, a tensor of one value a row)."""
-    if isinstance(value, _torch.Tensor) and value.dim() > 0:
-        v = _beside(_device_tensor(value, what), like, what)
-        if tuple(v.shape) != lead:
-            raise ValueError(f"{what} must have shape {lead}, got {tuple(v.shape)}")
-        if v.dtype != dtype:
-            raise ValueError(f"{what} must be {dtype}, got {v.dtype}")
-        return 0, v
-    return check(value), None
+def _option(value, what: str, lead, like, dtype):
+    """The tensor of one value a row that `value` is, or None."""
+    if not isinstance(value, _torch.Tensor) or value.dim() == 0:
+        return None
+    v = _beside(_device_tensor(value, what), like, what)
+    if tuple(v.shape) != lead:
+        raise ValueError(f"{what} must have shape {lead}, got {tuple(v.shape)}")
+    if v.dtype != dtype:
+        raise ValueError(f"{what} must be {dtype}, got {v.dtype}")
+    return v
+
+
+@functools.lru_cache(maxsize=256, typed=True)
+def _packed_numbers(temperature, top_k, top_p, min_p) -> bytes:
+    return _OPTIONS.pack(0, 0, 0, 0, *check_options(temperature, top_k, top_p, min_p))
 
 
 def check_options(temperature, top_k, top_p, min_p) -> tuple[float, int, float, float]:
@@ -349,18 +364,22 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if uniforms.dtype != torch.float32 or tuple(uniforms.shape) != lead:
         raise ValueError(f"uniforms must be float32 of shape {lead}, got {uniforms.dtype} of "
                          f"{tuple(uniforms.shape)}")
-    o = N.SampleOptions()
     f32 = torch.float32
-    o.temperature, a = _option(temperature, "temperature", lead, logits, f32, _temperature)
-    o.top_k, b = _option(top_k, "top_k", lead, logits, torch.int32, _top_k)
-    o.top_p, c = _option(top_p, "top_p", lead, logits, f32, lambda v: _share("top_p", v))
-    o.min_p, d = _option(min_p, "min_p", lead, logits, f32, lambda v: _share("min_p", v))
-    o.temperatures, o.top_ks, o.top_ps, o.min_ps = (
-        None if t is None else t.data_ptr() for t in (a, b, c, d))
+    given = (temperature, top_k, top_p, min_p)
+    if all(type(v) is float or type(v) is int for v in given):
+        o = _packed_numbers(*given)
+    else:
+        rows = [_option(v, w, lead, logits, torch.int32 if w == "top_k" else f32)
+                for v, w in zip(given, ("temperature", "top_k", "top_p", "min_p"))]
+        numbers = check_options(*(off if r is not None else v
+                                  for v, r, off in zip(given, rows, (1.0, 0, 1.0, 0.0))))
+        o = _OPTIONS.pack(*(0 if r is None else r.data_ptr() for r in rows), *numbers)
     classes = logits.new_empty(lead, dtype=torch.int64)
     log_probs = logits.new_empty(lead, dtype=f32)
-    N.check_hip(N.hip().fbh_sample_classes(
-        logits.device.index, logits.data_ptr(), classes.numel(), logits.shape[-1], cells,
-        uniforms.data_ptr(), C.byref(o), classes.data_ptr(), log_probs.data_ptr(),
-        _stream(logits.device)))
+    dev = logits.get_device()
+    rc = _L.fbh_sample_classes(dev, logits.data_ptr(), classes.numel(), logits.shape[-1], cells,
+                               uniforms.data_ptr(), o, classes.data_ptr(), log_probs.data_ptr(),
+                               _raw_stream(dev))
+    if rc:
+        N.check_hip(rc)
     return classes, log_probs

@@ -75,6 +75,7 @@ TABLES = [
     (64, [2] * 9, 8), (333, [50, 3, 1000], 5), (1000, [40] * 33, 16), (70, [5] * 600, 127),
     (4097, [31, 77], 33), (9000, [100, 28], 260), (40, [12] * 7, 1100), (30_000, [17] * 5, 2),
     (1, [10_000], 2048),
+    (900, [1500] * 80, 20),  # many positions, sorted through memory
     # columns summed chunk by chunk: one chunk, several, uneven ones, wide vectors
     (3000, [40] * 33, 64), (20_000, [511, 3, 0, 200], 24), (140_000, [9], 7),
     (70_001, [31, 1000], 3), (9000, [1024, 5] * 4, 600), (66_000, [2, 1], 1),
@@ -112,7 +113,9 @@ def test_embed_and_its_gradient(heads, case, dtype):
 @pytest.mark.parametrize("n, v, dim, skew", [
     (1, 1, 1, False), (7, 3, 4, False), (4096, 50_000, 32, True), (32_768, 300, 1024, True),
     (100_000, 5, 24, False), (20_000, 70_000, 7, True), (300_000, 260, 3, True),
-    (65_537, 16_777_217, 1, False)])
+    (65_537, 16_777_217, 1, False), (70_000, 3000, 20, True), (200_000, 100_000, 5, False),
+    (66_000, 70_000, 260, True), (5000, 600_000, 3, False), (65_536, 1_048_576, 2, True),
+    (65_536, 1_048_577, 2, True)])
 def test_one_vocabulary(heads, n, v, dim, skew):
     """Flat ids without a vocabulary: one to four radix passes, runs over many chunks."""
     rng = np.random.default_rng(n + v)
