@@ -260,8 +260,7 @@ __global__ void embed_sum_few_kernel(Positions P, const T *table, T *out, uint32
 // one chunk goes to the table, the parts of longer runs are joined in chunk order. All
 // orders are fixed, so the gradient is the same in every call.
 constexpr uint32_t SORT_TPB = 256;
-constexpr uint32_t SORT_ROUNDS = 16;
-constexpr uint32_t SORT_ITEMS = SORT_TPB * SORT_ROUNDS;
+constexpr uint32_t SORT_ROUNDS = 16;  // of a thread's positions; 1 where they are few
 constexpr uint32_t SORT_WAVES = SORT_TPB / 64;
 
 // What a pass sorts: positions decoded from the ids (pass 0), or the pass before's output.
@@ -280,21 +279,46 @@ __device__ __forceinline__ uint32_t sort_key(const Positions &P, const SortFrom 
 }
 
 // counts[digit * blocks + block]
-template <int ID, bool DROP, bool FIRST>
+template <int ID, bool DROP, bool FIRST, uint32_t ROUNDS>
 __global__ __launch_bounds__(SORT_TPB) void sort_count_kernel(Positions P, SortFrom S,
                                                               uint32_t *counts) {
     __shared__ uint32_t c[256];
     c[threadIdx.x] = 0;
     __syncthreads();
-    const uint32_t base = blockIdx.x * SORT_ITEMS, mask = (1u << S.bits) - 1;
+    const uint32_t base = blockIdx.x * (SORT_TPB * ROUNDS), mask = (1u << S.bits) - 1;
 #pragma unroll 4
-    for (uint32_t r = 0; r < SORT_ROUNDS; r++) {
+    for (uint32_t r = 0; r < ROUNDS; r++) {
         const uint32_t i = base + r * SORT_TPB + threadIdx.x;
         if (i < S.n)
             atomicAdd(&c[(sort_key<ID, DROP, FIRST>(P, S, i) >> S.shift) & mask], 1u);
     }
     __syncthreads();
     if (threadIdx.x <= mask) counts[(uint64_t)threadIdx.x * gridDim.x + blockIdx.x] = c[threadIdx.x];
+}
+
+// The lanes that are `in` with this lane's digit.
+__device__ __forceinline__ uint64_t same_digit(bool in, uint32_t digit, uint32_t bits) {
+    uint64_t same = __ballot(in);
+    for (uint32_t b = 0; b < bits; b++) {
+        const bool one = (digit >> b) & 1;
+        const uint64_t ones = __ballot(one);
+        same &= one ? ones : ~ones;
+    }
+    return same;
+}
+// Takes places from a counter that only this wave uses: what it held, plus the number of
+// lower lanes in `same`.
+__device__ __forceinline__ uint32_t take_places(uint32_t *counter, bool in, uint64_t same) {
+    const uint32_t below = __popcll(same & ((1ull << (threadIdx.x & 63)) - 1));
+    volatile uint32_t *c = counter;
+    uint32_t before = 0;
+    if (in) before = *c;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (in && below == 0) *c = before + __popcll(same);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    return before + below;
 }
 
 // A digit's counts to the positions before them in its own part; its total.
@@ -327,7 +351,7 @@ __global__ __launch_bounds__(SORT_TPB) void sort_scan_kernel(uint32_t *counts, u
 // Items of equal digits keep their order: a wave's 16 rounds are one after the other, a
 // lane's place in its round is the number of lower lanes with its digit, and the waves'
 // counts are summed up in wave order.
-template <int ID, bool DROP, bool FIRST>
+template <int ID, bool DROP, bool FIRST, uint32_t ROUNDS>
 __global__ __launch_bounds__(SORT_TPB) void sort_scatter_kernel(Positions P, SortFrom S,
                                                                 const uint32_t *counts,
                                                                 const uint32_t *totals,
@@ -352,34 +376,19 @@ __global__ __launch_bounds__(SORT_TPB) void sort_scatter_kernel(Positions P, Sor
             base[threadIdx.x] =
                 add + x - v + counts[(uint64_t)threadIdx.x * gridDim.x + blockIdx.x];
     }
-    const uint32_t first = blockIdx.x * SORT_ITEMS + w * (SORT_ROUNDS * 64) + lane;
-    uint32_t key[SORT_ROUNDS], rank[SORT_ROUNDS];
+    const uint32_t first = (blockIdx.x * SORT_WAVES + w) * (ROUNDS * 64) + lane;
+    uint32_t key[ROUNDS], rank[ROUNDS];
 #pragma unroll
-    for (uint32_t r = 0; r < SORT_ROUNDS; r++) {
+    for (uint32_t r = 0; r < ROUNDS; r++) {
         const uint32_t i = first + r * 64;
         key[r] = i < S.n ? sort_key<ID, DROP, FIRST>(P, S, i) : 0;
     }
     // (a wave's LDS operations complete in order, and only it touches its counters)
 #pragma unroll
-    for (uint32_t r = 0; r < SORT_ROUNDS; r++) {
+    for (uint32_t r = 0; r < ROUNDS; r++) {
         const bool in = first + r * 64 < S.n;
         const uint32_t digit = (key[r] >> S.shift) & mask;
-        uint64_t same = __ballot(in);
-        for (uint32_t b = 0; b < S.bits; b++) {
-            const bool one = (digit >> b) & 1;
-            const uint64_t ones = __ballot(one);
-            same &= one ? ones : ~ones;
-        }
-        const uint32_t below = __popcll(same & ((1ull << lane) - 1));
-        volatile uint32_t *count = &seen[w][digit];
-        uint32_t before = 0;
-        if (in) before = *count;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        if (in && below == 0) *count = before + __popcll(same);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        rank[r] = before + below;
+        rank[r] = take_places(&seen[w][digit], in, same_digit(in, digit, S.bits));
     }
     __syncthreads();
     if (threadIdx.x <= mask) {
@@ -392,7 +401,7 @@ __global__ __launch_bounds__(SORT_TPB) void sort_scatter_kernel(Positions P, Sor
     }
     __syncthreads();
 #pragma unroll
-    for (uint32_t r = 0; r < SORT_ROUNDS; r++) {
+    for (uint32_t r = 0; r < ROUNDS; r++) {
         const uint32_t i = first + r * 64;
         if (i >= S.n) continue;
         const uint32_t at = seen[w][(key[r] >> S.shift) & mask] + rank[r];
@@ -401,80 +410,76 @@ __global__ __launch_bounds__(SORT_TPB) void sort_scatter_kernel(Positions P, Sor
     }
 }
 
-// ---- Up to 64k positions. Every workgroup owns a range of tokens, goes through all
-// positions and places its own: how many have lower tokens is counted on the way, so one
-// launch does what a radix pass takes three for. It also writes the zeros of its range's
-// tokens that have no position, so the table needs no pass of its own.
-constexpr uint32_t FEW_MOST = 65536;           // positions
+// ---- Up to 64k positions: one radix pass, of the tokens' high bits and with one position a
+// thread so that its launches are short, parts them into buckets; then each bucket is
+// sorted in a workgroup, which also writes the zeros of the bucket's tokens that have no
+// position, so the table needs no pass of its own. (32768 positions, 50000 tokens of 2 KB:
+// two passes of 16 positions a thread and a pass of zeros took 75 us; workgroups that each
+// look for their own tokens among all positions 39; workgroups that count all positions
+// and place 1024 of them, instead of the pass' three launches, 39 alone.)
+constexpr uint32_t FEW_MOST = 65536;     // positions
 constexpr uint32_t FEW_TPB = 512;
 constexpr uint32_t FEW_WAVES = FEW_TPB / 64;
-constexpr uint32_t FEW_RANGE = 1024;           // tokens of a workgroup at most
-constexpr uint32_t FEW_STEP = 4 * 64;          // positions that a wave takes at a time
-
-template <int ID, bool DROP>
-__global__ __launch_bounds__(256) void few_tokens_kernel(Positions P, uint32_t n, uint32_t padded,
-                                                         uint32_t *tokens) {
-    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= padded) return;
-    uint32_t tok = NO_TOKEN;
-    if (i < n) tok = token_at<ID, DROP>(P, i, P.n_columns > 1 ? i % P.n_columns : 0);
-    tokens[i] = tok;
-}
+constexpr uint32_t FEW_RANGE_BITS = 10;  // tokens of a bucket: at most two a thread
+constexpr uint32_t FEW_BUCKET_BITS = 8;
 
 struct Few {
-    const uint32_t *tokens;  // of all positions, padded to FEW_WAVES * steps * FEW_STEP
-    uint32_t n, steps;       // positions; steps of a wave
-    uint32_t n_tokens, range, per_row;
-    uint32_t *keys, *vals;   // by token
+    uint32_t n_tokens, shift;    // 2^shift tokens a bucket
+    const uint32_t *totals;      // of the buckets
+    const uint32_t *part_keys, *part_vals;
+    uint32_t *keys, *vals;
+    uint8_t *table;
+    uint32_t row_bytes;
 };
 
-template <class T, int VEC>
-__global__ __launch_bounds__(FEW_TPB) void few_sort_kernel(Few F, T *table, uint32_t dim,
-                                                           uint32_t n_pieces) {
-    extern __shared__ uint32_t seen[];  // [wave][token]: counts, then places
-    __shared__ uint32_t wave_sum[FEW_WAVES], lower[FEW_WAVES];
+// The sum of the values of lower threads; *all gets the sum of all.
+__device__ __forceinline__ uint32_t sum_below(uint32_t v, uint32_t *wave_sum, uint32_t *all) {
     const uint32_t lane = threadIdx.x & 63, w = threadIdx.x / 64;
-    const uint32_t t0 = blockIdx.x * F.range, range = min(F.range, F.n_tokens - t0);
-    for (uint32_t i = threadIdx.x; i < FEW_WAVES * F.range; i += FEW_TPB) seen[i] = 0;
-    __syncthreads();
-    const uint4 *from = reinterpret_cast<const uint4 *>(F.tokens) + w * F.steps * 64 + lane;
-    uint32_t *mine = seen + w * F.range;
-    uint32_t below_range = 0;
-#pragma unroll 4
-    for (uint32_t k = 0; k < F.steps; k++) {
-        const uint4 q = from[k * 64];
-        const uint32_t tok[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (uint32_t j = 0; j < 4; j++) {
-            below_range += tok[j] < t0;
-            if (tok[j] - t0 < range) atomicAdd(&mine[tok[j] - t0], 1u);
-        }
-    }
-    for (int d = 32; d; d >>= 1) below_range += __shfl_xor(below_range, d);
-    if (lane == 0) lower[w] = below_range;
-    __syncthreads();
-    // places: by token, then by wave. Two tokens a thread.
-    uint32_t c[2] = {0, 0};
-    for (uint32_t j = 0; j < 2; j++)
-        if (2 * threadIdx.x + j < range)
-            for (uint32_t v = 0; v < FEW_WAVES; v++) c[j] += seen[v * F.range + 2 * threadIdx.x + j];
-    uint32_t x = c[0] + c[1];
+    uint32_t x = v;
     for (int d = 1; d < 64; d <<= 1) {
         const uint32_t y = __shfl_up(x, d);
         if (lane >= (uint32_t)d) x += y;
     }
     if (lane == 63) wave_sum[w] = x;
     __syncthreads();
-    uint32_t at = x - c[0] - c[1], end = 0;
-    for (uint32_t v = 0; v < FEW_WAVES; v++) {
-        at += lower[v] + (v < w ? wave_sum[v] : 0);
-        end += lower[v] + wave_sum[v];
+    uint32_t sum = x - v;
+    *all = 0;
+    for (uint32_t k = 0; k < FEW_WAVES; k++) {
+        if (k < w) sum += wave_sum[k];
+        *all += wave_sum[k];
     }
+    return sum;
+}
+
+__global__ __launch_bounds__(FEW_TPB) void few_sort_kernel(Few F) {
+    extern __shared__ uint32_t seen[];  // [wave][token]: counts, then places
+    __shared__ uint32_t wave_sum[FEW_WAVES];
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x / 64;
+    // (token n_tokens, behind the last, are the positions that give nothing)
+    const uint32_t most = 1u << F.shift, t0 = blockIdx.x << F.shift,
+                   range = min(most, F.n_tokens + 1 - t0);
+    uint32_t first;
+    (void)sum_below(threadIdx.x < blockIdx.x ? F.totals[threadIdx.x] : 0, wave_sum, &first);
+    const uint32_t end = first + F.totals[blockIdx.x];
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < FEW_WAVES * most; i += FEW_TPB) seen[i] = 0;
+    __syncthreads();
+    uint32_t *mine = seen + w * most;
+    // a wave's positions, side by side
+    const uint32_t each = ((end - first + FEW_TPB - 1) / FEW_TPB) * 64;
+    const uint32_t i0 = first + w * each, i1 = min(i0 + each, end);
+    for (uint32_t i = i0 + lane; i < i1; i += 64) atomicAdd(&mine[F.part_keys[i] - t0], 1u);
+    __syncthreads();
+    uint32_t c[2] = {0, 0}, all;
+    for (uint32_t j = 0; j < 2; j++)
+        if (2 * threadIdx.x + j < range)
+            for (uint32_t v = 0; v < FEW_WAVES; v++) c[j] += seen[v * most + 2 * threadIdx.x + j];
+    uint32_t at = first + sum_below(c[0] + c[1], wave_sum, &all);
     for (uint32_t j = 0; j < 2; j++)
         if (2 * threadIdx.x + j < range) {
             uint32_t a = at;
             for (uint32_t v = 0; v < FEW_WAVES; v++) {
-                uint32_t *p = &seen[v * F.range + 2 * threadIdx.x + j];
+                uint32_t *p = &seen[v * most + 2 * threadIdx.x + j];
                 const uint32_t m = *p;
                 *p = a;
                 a += m;
@@ -482,56 +487,34 @@ __global__ __launch_bounds__(FEW_TPB) void few_sort_kernel(Few F, T *table, uint
             at += c[j];
         }
     __syncthreads();
-    // Every wave places its positions: the lanes of one token after the other.
-    for (uint32_t k0 = 0; k0 < F.steps; k0 += 4) {
-        uint4 q[4];
-#pragma unroll
-        for (uint32_t i = 0; i < 4; i++) q[i] = from[min(k0 + i, F.steps - 1) * 64];
-#pragma unroll
-        for (uint32_t i = 0; i < 16; i++) {
-            const uint32_t tok = i % 4 == 0   ? q[i / 4].x
-                                 : i % 4 == 1 ? q[i / 4].y
-                                 : i % 4 == 2 ? q[i / 4].z
-                                              : q[i / 4].w;
-            const bool in = k0 + i / 4 < F.steps && tok - t0 < range;
-            uint64_t left = __ballot(in);
-            while (left) {
-                const uint32_t one = __builtin_amdgcn_readlane(tok, __ffsll((long long)left) - 1);
-                const uint64_t same = __ballot(in && tok == one);
-                volatile uint32_t *count = &mine[one - t0];
-                const uint32_t place = *count;
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-                if (lane == 0) *count = place + __popcll(same);
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-                if (in && tok == one) {
-                    const uint32_t to = place + __popcll(same & ((1ull << lane) - 1));
-                    const uint32_t pos = ((w * F.steps + k0 + i / 4) * 64 + lane) * 4 + i % 4;
-                    F.keys[to] = one;
-                    F.vals[to] = F.per_row > 1 ? pos / F.per_row : pos;
-                }
-                left &= ~same;
+    // zeros where a token's first place is the next one's, in pieces of 16 bytes (the last
+    // one of a row over the one before) or, for narrower rows, of 2
+    const uint32_t piece = F.row_bytes < 16 ? 2 : 16, pieces = (F.row_bytes + piece - 1) / piece;
+    const uint32_t lg = pieces >= 64 ? 6 : 32 - __clz(max(pieces, 2u) - 1);  // lanes a row
+    const uint32_t row0 = threadIdx.x >> lg, lane0 = threadIdx.x & ((1u << lg) - 1);
+#pragma unroll 4
+    for (uint32_t t = row0; t < range; t += FEW_TPB >> lg) {
+        if (t0 + t == F.n_tokens || seen[t] != (t + 1 < range ? seen[t + 1] : end)) continue;
+        uint8_t *row = F.table + (uint64_t)(t0 + t) * F.row_bytes;
+        for (uint32_t i = lane0; i < pieces; i += 1u << lg) {
+            if (piece == 2) {
+                reinterpret_cast<uint16_t *>(row)[i] = 0;
+            } else {
+                Piece<uint16_t, 8> o = {};
+                store_piece<uint16_t, 8>(
+                    reinterpret_cast<uint16_t *>(row + min(16 * i, F.row_bytes - 16)), o);
             }
         }
     }
-    // the positions that give nothing, behind all others
-    if (blockIdx.x == gridDim.x - 1)
-        for (uint32_t i = end + threadIdx.x; i < F.n; i += FEW_TPB) F.keys[i] = F.n_tokens;
-    __syncthreads();
-    // seen[last wave][token] is now the place behind the token's last position, and the
-    // token before it ends where it starts
-    uint32_t first_place = 0;
-    for (uint32_t v = 0; v < FEW_WAVES; v++) first_place += lower[v];
-    const uint32_t *ends = seen + (FEW_WAVES - 1) * F.range;
-    for (uint32_t i = threadIdx.x; i < range * n_pieces; i += FEW_TPB) {
-        const uint32_t tok = i / n_pieces;
-        if ((tok ? ends[tok - 1] : first_place) != ends[tok]) continue;
-        const uint32_t cell = min((i - tok * n_pieces) * VEC, dim - VEC);
-        Piece<T, VEC> o;
-#pragma unroll
-        for (int j = 0; j < VEC; j++) o.v[j] = (T)0.0f;
-        store_piece<T, VEC>(table + (uint64_t)(t0 + tok) * dim + cell, o);
+    __syncthreads();  // (the places are read above and moved below)
+    for (uint32_t i = i0; i < i1; i += 64) {
+        const bool in = i + lane < i1;
+        const uint32_t key = in ? F.part_keys[i + lane] : t0, off = key - t0;
+        const uint32_t to = take_places(&mine[off], in, same_digit(in, off, F.shift));
+        if (in) {
+            F.keys[to] = key;
+            F.vals[to] = F.part_vals[i + lane];
+        }
     }
 }
 
@@ -630,11 +613,15 @@ __global__ __launch_bounds__(JOIN_TPB) void grad_join_kernel(Runs R, T *table) {
     if (threadIdx.x == 0) n_longs = 0;
     __syncthreads();
 
-    // the number of chunks behind c whose first position still has this key
-    const auto behind = [&](uint32_t c, uint32_t key, uint32_t most) {
-        uint32_t n = 0;
-        while (n < most && c + 1 + n < chunks && R.keys[(uint64_t)(c + 1 + n) * R.chunk] == key)
-            n++;
+    // the number of chunks behind c, up to JOIN_SHORT, whose first position has this key
+    const auto behind = [&](uint32_t c, uint32_t key) {
+        uint32_t k[JOIN_SHORT], n = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < JOIN_SHORT; i++)
+            k[i] = R.keys[(uint64_t)min(c + 1 + i, chunks - 1) * R.chunk];
+#pragma unroll
+        for (uint32_t i = 0; i < JOIN_SHORT; i++)
+            if (n == i && c + 1 + i < chunks && k[i] == key) n++;
         return n;
     };
     const auto write = [&](uint32_t key, const float *a) {
@@ -650,7 +637,7 @@ __global__ __launch_bounds__(JOIN_TPB) void grad_join_kernel(Runs R, T *table) {
         const uint32_t key = R.keys[c1 - 1];
         const bool starts = R.keys[c0] != key || c0 == 0 || R.keys[c0 - 1] != key;
         if (key < R.n_tokens && starts && R.keys[c1] == key) {
-            const uint32_t n = behind(c, key, JOIN_SHORT);
+            const uint32_t n = behind(c, key);
             if (n == JOIN_SHORT) {
                 if (lane == 0) longs[atomicAdd(&n_longs, 1u)] = c;
             } else if (live) {
@@ -674,33 +661,27 @@ __global__ __launch_bounds__(JOIN_TPB) void grad_join_kernel(Runs R, T *table) {
     for (uint32_t r = 0; r < n_runs; r++) {
         const uint32_t lc = longs[r];
         const uint32_t key = R.keys[(uint64_t)(lc + 1) * R.chunk - 1];
-        // the run's last chunk: doubling steps, then halves
-        uint32_t lo = lc + JOIN_SHORT, hi = lo + 1, step = 1;
-        while (hi < chunks && R.keys[(uint64_t)hi * R.chunk] == key) {
-            lo = hi;
-            step *= 2;
-            hi = min(lo + step, chunks);
+        // (sorted: the chunks that start with this key are the ones right behind)
+        uint32_t n = JOIN_SHORT + 1;
+        for (uint32_t some = JOIN_TPB; some == JOIN_TPB;) {
+            const uint64_t at = (uint64_t)lc + n + threadIdx.x;
+            some = __syncthreads_count(at < chunks && R.keys[at * R.chunk] == key);
+            n += some;
         }
-        while (hi - lo > 1) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if (R.keys[(uint64_t)mid * R.chunk] == key) lo = mid;
-            else hi = mid;
-        }
-        const uint32_t n = lo - lc + 1;
         float a[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; i++) a[i] = 0.0f;
         if (live)
-            for (uint32_t k0 = g; k0 < n; k0 += 4 * groups) {
-                Piece<float, VEC> p[4];
+            for (uint32_t k0 = g; k0 < n; k0 += 8 * groups) {
+                Piece<float, VEC> p[8];
 #pragma unroll
-                for (uint32_t j = 0; j < 4; j++) {
+                for (uint32_t j = 0; j < 8; j++) {
                     const uint32_t k = min(k0 + j * groups, n - 1);
                     p[j] = load_piece<float, VEC>(
                         R.parts + (2ull * (lc + k) + (k ? 0 : 1)) * R.dim + cell);
                 }
 #pragma unroll
-                for (uint32_t j = 0; j < 4; j++)
+                for (uint32_t j = 0; j < 8; j++)
                     if (k0 + j * groups < n)
 #pragma unroll
                         for (int i = 0; i < VEC; i++) a[i] += p[j].v[i];
@@ -1165,9 +1146,12 @@ void with_ids(uint32_t id_type, bool drop, F &&f) {
 }
 
 // The chunks of rows that columns of few ids are summed in; 0: they are sorted by token
-// instead. A chunk of a column has 8 positions an id on average at least, so that the
-// parts are written and read for less than the gradient rows take, and a call has 64k
-// positions at least.
+// instead. One chunk, where a workgroup gets through its column's gradient rows in the
+// time of a launch or two, takes two launches where sorting takes six (64 rows of 100
+// trees, 16 cells of float32: 20 us sorted). Otherwise a chunk of a column has 8
+// positions an id on average at least, so that the parts are written and read for less
+// than the gradient rows take, and a call has 64k positions at least.
+constexpr uint64_t COL_ONE_BYTES = 256 << 10;
 struct ColumnPlan {
     uint32_t chunk = 0, chunks = 0;
     uint64_t padded = 0, local = 0, counts = 0, parts = 0, bytes = 0;
@@ -1178,18 +1162,24 @@ ColumnPlan column_plan(const fbh_embed *e) {
     const uint64_t ids = e->first ? e->most_ids : e->n_tokens;
     const uint64_t columns = e->first ? e->n_columns : 1;
     const uint64_t rows = e->first ? e->n_rows : e->n_rows * e->n_columns;
-    if (ids == 0 || ids > COL_MOST_IDS || rows < 8 * ids || rows > 1u << 29 ||
-        rows * columns < 65536 ||
+    if (rows == 0 || ids == 0 || ids > COL_MOST_IDS || rows > 1u << 29 ||
         (!e->first && e->pooled && e->n_columns > 1))
         return c;
     const uint32_t vec = piece_cells(e->dim, e->dtype);
-    const uint64_t blocks = columns * (((e->dim + vec - 1) / vec + 63) / 64);
-    const uint64_t most = rows / (8 * ids);
-    uint64_t chunks = std::max((rows + COL_MOST_ROWS - 1) / COL_MOST_ROWS,
-                               std::min(most, (1023 + blocks) / blocks));
-    if (chunks > 4) {  // the same on every XCD
-        const uint64_t up = (chunks + 7) / 8 * 8;
-        chunks = up <= std::max<uint64_t>(most, 8) ? up : chunks;
+    const uint64_t cells = e->dtype == FBH_F32 ? 4 : 2;
+    uint64_t chunks;
+    if (rows <= COL_MOST_ROWS && rows * std::min<uint64_t>(e->dim * cells, 1024) <= COL_ONE_BYTES) {
+        chunks = 1;
+    } else {
+        if (rows < 8 * ids || rows * columns < 65536) return c;
+        const uint64_t blocks = columns * (((e->dim + vec - 1) / vec + 63) / 64);
+        const uint64_t most = rows / (8 * ids);
+        chunks = std::max((rows + COL_MOST_ROWS - 1) / COL_MOST_ROWS,
+                          std::min(most, (1023 + blocks) / blocks));
+        if (chunks > 4) {  // the same on every XCD
+            const uint64_t up = (chunks + 7) / 8 * 8;
+            chunks = up <= std::max<uint64_t>(most, 8) ? up : chunks;
+        }
     }
     c.chunk = (uint32_t)(((rows + chunks - 1) / chunks + 63) / 64 * 64);
     c.chunks = (uint32_t)((rows + c.chunk - 1) / c.chunk);
@@ -1209,7 +1199,8 @@ ColumnPlan column_plan(const fbh_embed *e) {
 struct GradPlan {
     uint32_t n = 0, passes = 0, bits = 0, blocks = 0, vec = 0, pieces = 0, lg_g = 0, chunk = 0,
              chunks = 0;
-    uint32_t range = 0, steps = 0, padded = 0;  // few positions: of a workgroup, of a wave
+    bool few = false;    // buckets of 2^shift tokens
+    uint32_t shift = 0;
     uint64_t keys[2], vals[2], counts = 0, totals = 0, parts = 0, bytes = 0;
 };
 
@@ -1220,7 +1211,7 @@ GradPlan grad_plan(const fbh_embed *e) {
     const uint32_t key_bits = lg_at_least((uint64_t)e->n_tokens + 1);  // n_tokens: nothing
     G.passes = (key_bits + 7) / 8;
     G.bits = (key_bits + G.passes - 1) / G.passes;
-    G.blocks = (uint32_t)((n + SORT_ITEMS - 1) / SORT_ITEMS);
+    G.blocks = (uint32_t)((n + SORT_TPB * SORT_ROUNDS - 1) / (SORT_TPB * SORT_ROUNDS));
     G.vec = piece_cells(e->dim, e->dtype);
     G.pieces = (e->dim + G.vec - 1) / G.vec;
     G.lg_g = std::min(lg_at_least(G.pieces), 6u);
@@ -1235,16 +1226,12 @@ GradPlan grad_plan(const fbh_embed *e) {
         G.bytes = (at + bytes + 255) & ~255ull;
         return at;
     };
-    if (n <= FEW_MOST && e->n_tokens <= FEW_RANGE * 1024) {
-        // a workgroup a CU, or more where the tokens are many
-        G.range = std::min((e->n_tokens + 255) / 256, FEW_RANGE);
-        G.steps = (G.n + FEW_WAVES * FEW_STEP - 1) / (FEW_WAVES * FEW_STEP);
-        G.padded = G.steps * FEW_WAVES * FEW_STEP;
-        G.keys[1] = take(4ull * G.padded);  // the tokens
-        G.keys[0] = take(4 * n);
-        G.vals[0] = take(4 * n);
-        G.parts = take(8ull * G.chunks * e->dim);
-        return G;
+    if (n <= FEW_MOST && key_bits <= FEW_RANGE_BITS + FEW_BUCKET_BITS) {
+        G.few = true;
+        G.passes = 1;
+        G.bits = std::min(key_bits, FEW_BUCKET_BITS);
+        G.shift = key_bits - G.bits;
+        G.blocks = (uint32_t)((n + SORT_TPB - 1) / SORT_TPB);
     }
     for (int i = 0; i < 2; i++) {
         G.keys[i] = take(4 * n);
@@ -1331,26 +1318,9 @@ void embed_grad(const fbh_embed *e, const void *grad, void *table, void *work, h
     const GradPlan G = grad_plan(e);
     auto *w = static_cast<uint8_t *>(work);
     const auto list = [&](uint64_t at) { return reinterpret_cast<uint32_t *>(w + at); };
-    const bool few = G.n && G.range;
-    if (few) {
-        with_ids(e->id_type, e->drop > 0.0, [&](auto id, auto drop) {
-            hipLaunchKernelGGL((few_tokens_kernel<decltype(id)::value, decltype(drop)::value>),
-                               dim3(G.padded / 256), dim3(256), 0, s, P, G.n, G.padded,
-                               list(G.keys[1]));
-        });
-        head_check(hipGetLastError(), "tokens");
-        const Few F{list(G.keys[1]), G.n, G.steps, e->n_tokens, G.range,
-                    e->pooled ? e->n_columns : 1, list(G.keys[0]), list(G.vals[0])};
-        with_cells(e->dtype, G.vec, [&](auto one, auto vec) {
-            using T = decltype(one);
-            hipLaunchKernelGGL((few_sort_kernel<T, decltype(vec)::value>),
-                               dim3((e->n_tokens + G.range - 1) / G.range), dim3(FEW_TPB),
-                               FEW_WAVES * G.range * 4, s, F, static_cast<T *>(table), e->dim,
-                               G.pieces);
-        });
-        head_check(hipGetLastError(), "token sort");
-    } else {
-        const uint64_t bytes = (uint64_t)e->n_tokens * e->dim * (e->dtype == FBH_F32 ? 4 : 2);
+    const uint32_t row_bytes = e->dim * (e->dtype == FBH_F32 ? 4 : 2);
+    if (!G.few || G.n == 0) {
+        const uint64_t bytes = (uint64_t)e->n_tokens * row_bytes;
         hipLaunchKernelGGL(zero_kernel,
                            dim3((uint32_t)std::min<uint64_t>((bytes + 4095) / 4096, 4096)),
                            dim3(256), 0, s, static_cast<uint8_t *>(table), bytes);
@@ -1358,28 +1328,38 @@ void embed_grad(const fbh_embed *e, const void *grad, void *table, void *work, h
         if (G.n == 0) return;
     }
     uint32_t *counts = list(G.counts), *totals = list(G.totals);
-    for (uint32_t pass = 0; pass < (few ? 0 : G.passes); pass++) {
+    for (uint32_t pass = 0; pass < G.passes; pass++) {
         const uint32_t to = pass & 1;
-        const SortFrom S{list(G.keys[1 - to]), list(G.vals[1 - to]), G.n, pass * G.bits, G.bits,
-                         e->pooled ? e->n_columns : 1};
+        const SortFrom S{list(G.keys[1 - to]), list(G.vals[1 - to]), G.n,
+                         G.few ? G.shift : pass * G.bits, G.bits, e->pooled ? e->n_columns : 1};
         uint32_t *keys = list(G.keys[to]), *vals = list(G.vals[to]);
-        const auto go = [&](auto id, auto drop, auto first) {
+        const auto go = [&](auto id, auto drop, auto first, auto rounds) {
             constexpr int ID = decltype(id)::value;
             constexpr bool DROP = decltype(drop)::value, FIRST = decltype(first)::value;
-            hipLaunchKernelGGL((sort_count_kernel<ID, DROP, FIRST>), dim3(G.blocks), dim3(SORT_TPB),
-                               0, s, P, S, counts);
+            constexpr uint32_t ROUNDS = decltype(rounds)::value;
+            hipLaunchKernelGGL((sort_count_kernel<ID, DROP, FIRST, ROUNDS>), dim3(G.blocks),
+                               dim3(SORT_TPB), 0, s, P, S, counts);
             hipLaunchKernelGGL(sort_scan_kernel, dim3(1u << G.bits), dim3(SORT_TPB), 0, s, counts,
                                G.blocks, totals);
-            hipLaunchKernelGGL((sort_scatter_kernel<ID, DROP, FIRST>), dim3(G.blocks),
+            hipLaunchKernelGGL((sort_scatter_kernel<ID, DROP, FIRST, ROUNDS>), dim3(G.blocks),
                                dim3(SORT_TPB), 0, s, P, S, counts, totals, keys, vals);
         };
         if (pass == 0)
-            with_ids(e->id_type, e->drop > 0.0,
-                     [&](auto id, auto drop) { go(id, drop, std::true_type{}); });
-        else go(Int<FBH_ID_I32>{}, std::false_type{}, std::false_type{});
+            with_ids(e->id_type, e->drop > 0.0, [&](auto id, auto drop) {
+                if (G.few) go(id, drop, std::true_type{}, Int<1>{});
+                else go(id, drop, std::true_type{}, Int<SORT_ROUNDS>{});
+            });
+        else go(Int<FBH_ID_I32>{}, std::false_type{}, std::false_type{}, Int<SORT_ROUNDS>{});
         head_check(hipGetLastError(), "token sort");
     }
-    const uint32_t at = few ? 0 : (G.passes - 1) & 1;
+    if (G.few) {
+        const Few F{e->n_tokens, G.shift, totals, list(G.keys[0]), list(G.vals[0]),
+                    list(G.keys[1]), list(G.vals[1]), static_cast<uint8_t *>(table), row_bytes};
+        hipLaunchKernelGGL(few_sort_kernel, dim3((e->n_tokens >> G.shift) + 1), dim3(FEW_TPB),
+                           (FEW_WAVES * 4) << G.shift, s, F);
+        head_check(hipGetLastError(), "token sort");
+    }
+    const uint32_t at = G.few ? 1 : (G.passes - 1) & 1;
     const Runs R{list(G.keys[at]), list(G.vals[at]), G.n, G.chunk, e->n_tokens, e->dim, G.pieces,
                  G.lg_g, scale_of(e), reinterpret_cast<float *>(w + G.parts)};
     with_cells(e->dtype, G.vec, [&](auto one, auto vec) {

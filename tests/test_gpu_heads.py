@@ -115,7 +115,8 @@ def test_embed_and_its_gradient(heads, case, dtype):
     (100_000, 5, 24, False), (20_000, 70_000, 7, True), (300_000, 260, 3, True),
     (65_537, 16_777_217, 1, False), (70_000, 3000, 20, True), (200_000, 100_000, 5, False),
     (66_000, 70_000, 260, True), (5000, 600_000, 3, False), (65_536, 1_048_576, 2, True),
-    (65_536, 1_048_577, 2, True)])
+    (65_536, 1_048_577, 2, True), (9000, 262_143, 3, True), (9000, 262_144, 1, False),
+    (300, 1024, 5, True), (16_384, 700, 4, True), (16_385, 700, 4, False)])
 def test_one_vocabulary(heads, n, v, dim, skew):
     """Flat ids without a vocabulary: one to four radix passes, runs over many chunks."""
     rng = np.random.default_rng(n + v)
