@@ -275,7 +275,7 @@ HIP_SYMBOLS = [
     "fbh_shap_model_unpark", "fbh_shap_models_drop",
     "fbh_saabas_contribs", "fbh_predict", "fbh_predict_device", "fbh_shap_contribs_noalloc",
     "fbh_embed_rows", "fbh_embed_grad_bytes", "fbh_embed_grad", "fbh_dropout",
-    "fbh_sample_classes", "fbh_sample_classes_host",
+    "fbh_sample_classes", "fbh_sample_classes_host", "fbh_sample_bytes",
 ]
 TRAIN_SYMBOLS = [
     "fbt_last_error", "fbt_train", "fbt_train_cuts", "fbt_train_rows", "fbt_last_stats",
@@ -406,7 +406,9 @@ def hip() -> C.CDLL:
         L.fbh_dropout.argtypes = [C.c_int, P, P, C.c_uint64, C.c_uint32, C.c_double, C.c_uint64,
                                   C.c_uint64, P]
         L.fbh_sample_classes.argtypes = [C.c_int, P, C.c_uint64, C.c_uint32, C.c_uint32, P, P, P,
-                                         P, P]
+                                         P, P, C.c_uint64, P]
+        L.fbh_sample_bytes.argtypes = [C.c_uint64, C.c_uint32]
+        L.fbh_sample_bytes.restype = C.c_uint64
         L.fbh_sample_classes_host.argtypes = [C.c_int, P, C.c_uint64, C.c_uint32, P, P, P, P]
         _hip = L
     return _hip

@@ -634,9 +634,18 @@ __device__ __forceinline__ uint64_t entry_of(float l, uint32_t c) {
 __device__ __forceinline__ uint32_t entry_key(uint64_t e) { return (uint32_t)(e >> 32); }
 __device__ __forceinline__ uint32_t entry_class(uint64_t e) { return ~(uint32_t)e; }
 
+constexpr uint32_t ROW_BINS = 1024;
+// Bins of max - l: monotone, as each step of it is.
+__device__ __forceinline__ uint32_t weight_bin(float l, float most, float per) {
+    const float d = l == most ? 0.0f : (most - l) * per;
+    return (uint32_t)fminf(d, (float)(ROW_BINS - 1));
+}
+
+struct TileWork;
+
 template <int TPB>
 struct RowShared {
-    static constexpr uint32_t BINS = 1024;
+    static constexpr uint32_t BINS = ROW_BINS;
     static constexpr uint32_t LIST = 2048;
     static constexpr uint32_t MOST_K = TPB / 2;  // of the classes found by the threads' largest
     uint64_t wt[BINS];
@@ -721,10 +730,8 @@ struct SampleRow {
         }
     }
 
-    // Bins of max - l: monotone, as each step of it is.
     __device__ __forceinline__ uint32_t bin_of(float l) const {
-        const float d = l == S.most ? 0.0f : (S.most - l) * per;
-        return (uint32_t)fminf(d, (float)(Shared::BINS - 1));
+        return weight_bin(l, S.most, per);
     }
 
     __device__ __forceinline__ void clear(uint32_t bins) {
@@ -836,6 +843,27 @@ struct SampleRow {
         return cut;
     }
 
+    // From a row's bins of weights: the bin that top-p cuts, with sh.before_* before it, and
+    // the weight that it asks for.
+    template <class W>
+    __device__ __forceinline__ uint32_t weight_cut(const W &work, const RowOptions &O,
+                                                   uint64_t *asked) {
+        clear(Shared::BINS);
+        for (uint32_t b = threadIdx.x; b < Shared::BINS; b += TPB) sh.wt[b] = work.wt[b];
+        return weight_cut(O, asked);
+    }
+    __device__ __forceinline__ uint32_t weight_cut(const RowOptions &O, uint64_t *asked) {
+        before(0, 0);
+        __syncthreads();
+        uint64_t all = 0;
+        for (uint32_t b = threadIdx.x; b < Shared::BINS; b += TPB) all += sh.wt[b];
+        uint64_t weight = share(O.p31, sum(all), 0x7FFFFFFFu);
+        if (weight == 0) weight = 1;
+        find(Shared::BINS, false, 0, weight);
+        if (asked) *asked = weight;
+        return sh.bin;
+    }
+
     // The classes that `take`, in the list; how many they are, NO_BIN if too many.
     template <class F>
     __device__ __forceinline__ uint32_t gather(F &&take) {
@@ -895,8 +923,147 @@ __device__ __forceinline__ void draw_listed(SampleRow<T, TPB> &R, const Draw &D,
     }
 }
 
-template <class T, int TPB>
-__global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D) {
+// ---- Few rows of many classes: a row's tiles (of 1024 pieces) go to a workgroup each. Three
+// launches find what the row's own workgroup finds pass by pass, the largest logit, the
+// histogram of weights, and the tiles' sums with a list of the cut's bin; the row kernel
+// then begins at its last steps. (1 x 50000 bfloat16, top-p: 46 us in one workgroup, whose
+// one CU is bound by the exponentials of doubles.) Rows whose options do not take a
+// histogram of weights (few classes by rank, or more than the row kernel lists) are left to
+// the row kernel altogether.
+constexpr uint32_t TILE_ROWS = 128;  // rows at most: 256 and more fill the device by themselves
+constexpr uint32_t TILE_TPB = 1024;
+constexpr uint32_t TILE_BINS = 1024;
+constexpr uint32_t TILE_LIST = 2048;
+
+struct TileWork {  // of one row
+    uint64_t wt[TILE_BINS];
+    uint64_t list[TILE_LIST];
+    uint64_t tile_w[MOST_TILES];
+    float most[MOST_TILES];
+    uint32_t n_list, reserved;
+};
+
+// Whether the tiles' launches do a row's passes.
+__device__ __forceinline__ bool tiled(const RowOptions &O, uint32_t n) { return O.k >= n; }
+
+__device__ __forceinline__ float row_most(const TileWork &W, uint32_t tiles) {
+    float m = (threadIdx.x & 63) < tiles ? W.most[threadIdx.x & 63] : -INFINITY;
+    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+    return m;
+}
+
+// The thread's piece of a tile, masked classes (and ones behind the last) as -inf.
+template <class T>
+__device__ __forceinline__ void tile_piece(const T *row, uint32_t n, uint32_t i,
+                                           float (&l)[16 / sizeof(T)]) {
+    constexpr int N = 16 / sizeof(T);
+    if (i + N <= n) {
+        const Piece<T, N> p = load_piece<T, N>(row + i);
+#pragma unroll
+        for (int j = 0; j < N; j++) l[j] = masked_nan((float)p.v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j++) l[j] = i + j < n ? masked_nan((float)row[i + j]) : -INFINITY;
+    }
+}
+
+// grid (tiles, rows)
+template <class T>
+__global__ __launch_bounds__(TILE_TPB) void tile_most_kernel(const T *logits, Draw D,
+                                                             TileWork *work) {
+    __shared__ float waves[TILE_TPB / 64];
+    constexpr int N = 16 / sizeof(T);
+    const uint64_t r = blockIdx.y;
+    const RowOptions O = row_options(D, r);
+    if (!tiled(O, D.n_classes)) return;
+    TileWork &W = work[r];
+    if (blockIdx.x == 0) {
+        W.wt[threadIdx.x] = 0;
+        if (threadIdx.x == 0) W.n_list = 0;
+    }
+    float l[N];
+    tile_piece<T>(logits + r * D.n_classes, D.n_classes, (blockIdx.x * TILE_TPB + threadIdx.x) * N, l);
+    float m = l[0];
+#pragma unroll
+    for (int j = 1; j < N; j++) m = fmaxf(m, l[j]);
+    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x / 64] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (uint32_t w = 1; w < TILE_TPB / 64; w++) m = fmaxf(m, waves[w]);
+        W.most[blockIdx.x] = m;
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(TILE_TPB) void tile_weights_kernel(const T *logits, Draw D,
+                                                                TileWork *work) {
+    __shared__ uint64_t wt[TILE_BINS];
+    constexpr int N = 16 / sizeof(T);
+    const uint64_t r = blockIdx.y;
+    const RowOptions O = row_options(D, r);
+    if (!tiled(O, D.n_classes) || O.p31 == 1u << 31) return;
+    TileWork &W = work[r];
+    wt[threadIdx.x] = 0;
+    const float most = row_most(W, gridDim.x);
+    const RowScale S{most, (double)most, O.inv_t};
+    const float per = (float)(O.inv_t * (TILE_BINS / 32));
+    __syncthreads();
+    float l[N];
+    tile_piece<T>(logits + r * D.n_classes, D.n_classes, (blockIdx.x * TILE_TPB + threadIdx.x) * N, l);
+#pragma unroll
+    for (int j = 0; j < N; j++)
+        if (l[j] != -INFINITY) {
+            const uint64_t w = S.weight(l[j]);
+            if (w)
+                atomicAdd(reinterpret_cast<unsigned long long *>(&wt[weight_bin(l[j], most, per)]),
+                          (unsigned long long)w);
+        }
+    __syncthreads();
+    if (wt[threadIdx.x])
+        atomicAdd(reinterpret_cast<unsigned long long *>(&W.wt[threadIdx.x]),
+                  (unsigned long long)wt[threadIdx.x]);
+}
+
+template <class T>
+__global__ __launch_bounds__(TILE_TPB) void tile_sums_kernel(const T *logits, Draw D,
+                                                             TileWork *work) {
+    __shared__ RowShared<TILE_TPB> sh;
+    constexpr int N = 16 / sizeof(T);
+    const uint64_t r = blockIdx.y;
+    const RowOptions O = row_options(D, r);
+    if (!tiled(O, D.n_classes)) return;
+    TileWork &W = work[r];
+    const uint32_t i = (blockIdx.x * TILE_TPB + threadIdx.x) * N;
+    float l[N];
+    tile_piece<T>(logits + r * D.n_classes, D.n_classes, i, l);
+    const float most = row_most(W, gridDim.x);
+    SampleRow<T, TILE_TPB> R{sh, logits + r * D.n_classes, D.n_classes,
+                             RowScale{most, (double)most, O.inv_t},
+                             (float)(O.inv_t * (TILE_BINS / 32))};
+    uint32_t bin = NO_BIN;
+    if (O.p31 < 1u << 31) bin = R.weight_cut(W, O, nullptr);
+    uint64_t w = 0;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        if (l[j] == -INFINITY) continue;
+        const uint32_t b = R.bin_of(l[j]);
+        if (b < bin) {
+            const uint64_t v = R.S.weight(l[j]);
+            if (v >= O.least) w += v;
+        } else if (b == bin) {
+            const uint32_t at = atomicAdd(&W.n_list, 1u);
+            if (at < TILE_LIST) W.list[at] = entry_of(l[j], i + j);
+        }
+    }
+    w = R.sum(w);
+    if (threadIdx.x == 0) W.tile_w[blockIdx.x] = w;
+}
+
+// TILED: rows whose passes the tiles' launches have done take their results.
+template <class T, int TPB, bool TILED>
+__global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D,
+                                                         const TileWork *work) {
     __shared__ RowShared<TPB> sh;
     constexpr int N = 16 / sizeof(T);
     constexpr uint32_t BINS = RowShared<TPB>::BINS;
@@ -904,9 +1071,12 @@ __global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D
     const uint32_t n = D.n_classes;
     const RowOptions O = row_options(D, r);
     SampleRow<T, TPB> R{sh, logits + r * n, n, {}, 0.0f};
+    const uint32_t tiles = (n + TPB * N - 1) / (TPB * N);
+    const bool done = TILED && tiled(O, n);
     float most, own, least;
-    uint32_t most_at;
-    R.largest(most, most_at, own, least);
+    uint32_t most_at = NO_BIN;
+    if (done) most = row_most(work[r], tiles);
+    else R.largest(most, most_at, own, least);
     if (most == -INFINITY || O.k == 1) {
         if (threadIdx.x == 0)
             put_class(D, r, most == -INFINITY ? -1 : (int64_t)most_at, 0.0, WEIGHT_ONE);
@@ -934,9 +1104,8 @@ __global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D
     R.per = (float)(O.inv_t * (BINS / 32));  // 32 (max - l) / T over all bins
 
     // tile sums: TPB pieces of N classes a tile, in class order
-    const uint32_t tiles = (n + TPB * N - 1) / (TPB * N);
     for (uint32_t t = threadIdx.x; t < MOST_TILES; t += TPB) {
-        sh.tile_w[t] = 0;
+        sh.tile_w[t] = done && t < tiles ? work[r].tile_w[t] : 0;
         sh.tile_ties[t] = 0;
     }
     // Adds up, tile by tile, what f(class, logit, weight, ties) finds in a piece.
@@ -1030,32 +1199,33 @@ __global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D
     } else if (O.p31 < 1u << 31) {
         // By weight alone: a histogram finds the cut's bin; one pass then sums the bins
         // before it and lists its own classes, whose digits find the cut.
-        R.clear(BINS);
-        R.each([&](uint32_t, float l) {
-            if (l != -INFINITY) R.add_weight(R.bin_of(l), R.S.weight(l));
-        });
-        R.before(0, 0);
-        __syncthreads();
-        uint64_t all = 0;
-        for (uint32_t b = threadIdx.x; b < BINS; b += TPB) all += sh.wt[b];
-        all = R.sum(all);
-        uint64_t weight = share(O.p31, all, 0x7FFFFFFFu);
-        if (weight == 0) weight = 1;
-        R.find(BINS, false, 0, weight);
-        const uint32_t bin = sh.bin;
-        if (threadIdx.x == 0) sh.n_list = 0;
-        sum_tiles([&](uint32_t c, float l, uint64_t &w, uint32_t &) {
-            if (l == -INFINITY) return;
-            const uint32_t b = R.bin_of(l);
-            if (b < bin) {
-                const uint64_t v = R.S.weight(l);
-                if (v >= O.least) w += v;
-            } else if (b == bin) {
-                const uint32_t at = atomicAdd(&sh.n_list, 1u);
-                if (at < RowShared<TPB>::LIST) sh.list[at] = entry_of(l, c);
-            }
-        });
-        const uint32_t m = sh.n_list <= RowShared<TPB>::LIST ? sh.n_list : NO_BIN;
+        uint64_t weight;
+        uint32_t bin, m;
+        if (done) {
+            bin = R.weight_cut(work[r], O, &weight);
+            m = work[r].n_list <= RowShared<TPB>::LIST ? work[r].n_list : NO_BIN;
+            if (m != NO_BIN)
+                for (uint32_t i = threadIdx.x; i < m; i += TPB) sh.list[i] = work[r].list[i];
+        } else {
+            R.clear(BINS);
+            R.each([&](uint32_t, float l) {
+                if (l != -INFINITY) R.add_weight(R.bin_of(l), R.S.weight(l));
+            });
+            bin = R.weight_cut(O, &weight);
+            if (threadIdx.x == 0) sh.n_list = 0;
+            sum_tiles([&](uint32_t c, float l, uint64_t &w, uint32_t &) {
+                if (l == -INFINITY) return;
+                const uint32_t b = R.bin_of(l);
+                if (b < bin) {
+                    const uint64_t v = R.S.weight(l);
+                    if (v >= O.least) w += v;
+                } else if (b == bin) {
+                    const uint32_t at = atomicAdd(&sh.n_list, 1u);
+                    if (at < RowShared<TPB>::LIST) sh.list[at] = entry_of(l, c);
+                }
+            });
+            m = sh.n_list <= RowShared<TPB>::LIST ? sh.n_list : NO_BIN;
+        }
         cut = R.refine(bin, m, false, 0, weight);
         tie_w = R.S.weight(key_logit(cut.key));
         if (tie_w < O.least) cut.ties = 0;
@@ -1077,6 +1247,8 @@ __global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D
                 if (l != -INFINITY && R.bin_of(l) == bin) one(c, l);
             });
         }
+        __syncthreads();
+    } else if (done) {
         __syncthreads();
     } else {
         sum_tiles([&](uint32_t, float l, uint64_t &w, uint32_t &t) { staying(l, w, t); });
@@ -1142,8 +1314,16 @@ __global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D
     }
 }
 
+// Whether a call's rows may be taken tile by tile.
+bool sample_tiled(uint64_t n_rows, uint32_t n_classes) {
+    return n_rows <= TILE_ROWS && n_classes > 16384;
+}
+uint64_t sample_bytes(uint64_t n_rows, uint32_t n_classes) {
+    return sample_tiled(n_rows, n_classes) ? n_rows * sizeof(TileWork) : 0;
+}
+
 template <class T>
-void launch_sample(const void *logits, const Draw &D, hipStream_t s) {
+void launch_sample(const void *logits, const Draw &D, TileWork *work, hipStream_t s) {
     const auto *l = static_cast<const T *>(logits);
     const uint64_t n = D.n_rows;
     const uint32_t v = D.n_classes;
@@ -1177,16 +1357,31 @@ void launch_sample(const void *logits, const Draw &D, hipStream_t s) {
         head_input(n < 1u << 22, "too many rows");
         const dim3 grid((uint32_t)n);
         if (v <= 16384)
-            hipLaunchKernelGGL((sample_row_kernel<T, 256>), grid, dim3(256), 0, s, l, D);
-        else hipLaunchKernelGGL((sample_row_kernel<T, 1024>), grid, dim3(1024), 0, s, l, D);
+            hipLaunchKernelGGL((sample_row_kernel<T, 256, false>), grid, dim3(256), 0, s, l, D,
+                               nullptr);
+        else if (!sample_tiled(D.n_rows, v) || (!D.own && D.all.k < v))
+            hipLaunchKernelGGL((sample_row_kernel<T, 1024, false>), grid, dim3(1024), 0, s, l, D,
+                               nullptr);
+        else {
+            constexpr uint32_t cells = TILE_TPB * 16 / sizeof(T);
+            const dim3 tiles((v + cells - 1) / cells, (uint32_t)n);
+            hipLaunchKernelGGL((tile_most_kernel<T>), tiles, dim3(TILE_TPB), 0, s, l, D, work);
+            if (D.own || D.all.p31 < 1u << 31)
+                hipLaunchKernelGGL((tile_weights_kernel<T>), tiles, dim3(TILE_TPB), 0, s, l, D,
+                                   work);
+            hipLaunchKernelGGL((tile_sums_kernel<T>), tiles, dim3(TILE_TPB), 0, s, l, D, work);
+            hipLaunchKernelGGL((sample_row_kernel<T, 1024, true>), grid, dim3(1024), 0, s, l, D,
+                               work);
+        }
     }
     head_check(hipGetLastError(), "sampling");
 }
 
-void sample(const void *logits, uint32_t dtype, const Draw &D, hipStream_t s) {
-    if (dtype == FBH_F32) launch_sample<float>(logits, D, s);
-    else if (dtype == FBH_F16) launch_sample<_Float16>(logits, D, s);
-    else launch_sample<__bf16>(logits, D, s);
+void sample(const void *logits, uint32_t dtype, const Draw &D, void *work, hipStream_t s) {
+    auto *w = static_cast<TileWork *>(work);
+    if (dtype == FBH_F32) launch_sample<float>(logits, D, w, s);
+    else if (dtype == FBH_F16) launch_sample<_Float16>(logits, D, w, s);
+    else launch_sample<__bf16>(logits, D, w, s);
 }
 
 Draw draw_of(const float *uniforms, const fbh_sample_options *o, int64_t *classes,
@@ -1210,16 +1405,23 @@ using namespace fbh;
 
 extern "C" {
 
+uint64_t fbh_sample_bytes(uint64_t n_rows, uint32_t n_classes) {
+    return sample_bytes(n_rows, n_classes);
+}
+
 int fbh_sample_classes(int device, const void *logits, uint64_t n_rows, uint32_t n_classes,
                        uint32_t dtype, const float *uniforms, const fbh_sample_options *options,
-                       int64_t *classes, float *log_probs, void *stream) {
+                       int64_t *classes, float *log_probs, void *work, uint64_t work_bytes,
+                       void *stream) {
     return head_guard([&] {
         check_sample(logits, n_rows, n_classes, uniforms, options, classes);
         head_input(dtype <= FBH_BF16, "unknown cell type");
         if (n_rows == 0) return;
+        const uint64_t need = sample_bytes(n_rows, n_classes);
+        head_input(work_bytes >= need && (work || need == 0), "the workspace is too small");
         const OnDevice on(device);
         sample(logits, dtype,
-               draw_of(uniforms, options, classes, log_probs, n_rows, n_classes),
+               draw_of(uniforms, options, classes, log_probs, n_rows, n_classes), work,
                static_cast<hipStream_t>(stream));
     });
 }
@@ -1245,8 +1447,10 @@ int fbh_sample_classes_host(int device, const float *logits, uint64_t n_rows, ui
         const std::unique_ptr<void, decltype(end)> own(s, end);
         const uint64_t l_bytes = (4 * n_rows * n_classes + 255) & ~255ull;
         const uint64_t u_bytes = (4 * n_rows + 255) & ~255ull;
+        const uint64_t c_bytes = (8 * n_rows + 255) & ~255ull;
         head_check(keep_alloc(KeepKind::device, reinterpret_cast<void **>(&block),
-                              l_bytes + 2 * u_bytes + 8 * n_rows),
+                              l_bytes + 2 * u_bytes + c_bytes +
+                                  sample_bytes(n_rows, n_classes)),
                    "device allocation");
         auto *d_u = reinterpret_cast<float *>(block + l_bytes);
         auto *d_p = reinterpret_cast<float *>(block + l_bytes + u_bytes);
@@ -1255,7 +1459,8 @@ int fbh_sample_classes_host(int device, const float *logits, uint64_t n_rows, ui
                    "logit upload");
         head_check(hipMemcpyAsync(d_u, uniforms, 4 * n_rows, hipMemcpyHostToDevice, s),
                    "uniform upload");
-        sample(block, FBH_F32, draw_of(d_u, options, d_c, d_p, n_rows, n_classes), s);
+        sample(block, FBH_F32, draw_of(d_u, options, d_c, d_p, n_rows, n_classes),
+               block + l_bytes + 2 * u_bytes + c_bytes, s);
         head_check(hipMemcpyAsync(classes, d_c, 8 * n_rows, hipMemcpyDeviceToHost, s),
                    "class download");
         if (log_probs)

@@ -376,10 +376,12 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         o = _OPTIONS.pack(*(0 if r is None else r.data_ptr() for r in rows), *numbers)
     classes = logits.new_empty(lead, dtype=torch.int64)
     log_probs = logits.new_empty(lead, dtype=f32)
-    dev = logits.get_device()
-    rc = _L.fbh_sample_classes(dev, logits.data_ptr(), classes.numel(), logits.shape[-1], cells,
-                               uniforms.data_ptr(), o, classes.data_ptr(), log_probs.data_ptr(),
-                               _raw_stream(dev))
+    dev, n, v = logits.get_device(), classes.numel(), logits.shape[-1]
+    size = _L.fbh_sample_bytes(n, v) if v > 1024 else 0
+    work = logits.new_empty(size, dtype=torch.uint8) if size else None
+    rc = _L.fbh_sample_classes(dev, logits.data_ptr(), n, v, cells, uniforms.data_ptr(), o,
+                               classes.data_ptr(), log_probs.data_ptr(),
+                               work.data_ptr() if size else None, size, _raw_stream(dev))
     if rc:
         N.check_hip(rc)
     return classes, log_probs

@@ -762,8 +762,8 @@ typedef struct {
  * an order that depends on the column alone, and rounded once. A model's margins
  * are the pooled embedding of its leaf ids in the table of its leaf values. */
 int fbh_embed_rows(int device, const fbh_embed *e, const void *table, void *out, void *stream);
-/* Device bytes of workspace that fbh_embed_grad takes; 0 for a call that it
- * refuses. */
+/* Device bytes of workspace that fbh_embed_grad takes, 16-byte aligned; 0 for a call
+ * that it refuses. */
 uint64_t fbh_embed_grad_bytes(const fbh_embed *e);
 /* The gradient of fbh_embed_rows by its table: table_grad[v] = scale * the sum
  * over positions of token v of the output's gradient there (grad, laid out as
@@ -811,7 +811,10 @@ typedef struct {
  * most 262144 classes. */
 int fbh_sample_classes(int device, const void *logits, uint64_t n_rows, uint32_t n_classes,
                        uint32_t dtype, const float *uniforms, const fbh_sample_options *options,
-                       int64_t *classes, float *log_probs, void *stream);
+                       int64_t *classes, float *log_probs, void *work, uint64_t work_bytes,
+                       void *stream);
+/* Device bytes of workspace that fbh_sample_classes takes (0: none), 8-byte aligned. */
+uint64_t fbh_sample_bytes(uint64_t n_rows, uint32_t n_classes);
 /* The same with logits (f32), uniforms and results in host memory and one set of
  * options (no pointers in it); returns when the results are there. */
 int fbh_sample_classes_host(int device, const float *logits, uint64_t n_rows, uint32_t n_classes,

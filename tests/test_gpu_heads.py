@@ -286,7 +286,8 @@ def _check_sample(heads, x, u, t, k, p, m):
                                   (257, 8), (40, 9), (33, 16), (20, 17), (50, 33), (40, 64),
                                   (40, 65), (9, 128), (9, 129), (13, 256), (10, 400), (30, 500),
                                   (11, 1000), (6, 1024), (6, 1025), (9, 2048), (7, 2049),
-                                  (3, 16_384), (3, 16_385), (2, 131_071), (1, 262_144)])
+                                  (3, 16_384), (3, 16_385), (2, 131_071), (1, 262_144),
+                                  (129, 16_400)])
 def test_sample(heads, n, v, dtype):
     rng = np.random.default_rng([n, v])
     x = rng.normal(size=(n, v)) * 3

@@ -59,7 +59,13 @@ def test_dropout_and_sampling_refusals_of_the_c_abi():
     for v, dt, u, msg in [(0, 0, 64, "n_classes"), (262145, 0, 64, "n_classes"),
                           (5, 9, 64, "cell type"), (5, 0, None, "null")]:
         with pytest.raises(ValueError, match=msg):
-            N.check_hip(L.fbh_sample_classes(0, 64, 2, v, dt, u, C.byref(o), 64, None, None))
+            N.check_hip(L.fbh_sample_classes(0, 64, 2, v, dt, u, C.byref(o), 64, None, None, 0,
+                                             None))
+    need = L.fbh_sample_bytes(2, 100_000)
+    assert need > 0 and L.fbh_sample_bytes(2, 1000) == L.fbh_sample_bytes(5000, 100_000) == 0
+    with pytest.raises(ValueError, match="workspace"):
+        N.check_hip(L.fbh_sample_classes(0, 64, 2, 100_000, 0, 64, C.byref(o), 64, None, 64,
+                                         need - 1, None))
     o.top_ks = 64
     with pytest.raises(ValueError, match="each row"):
         N.check_hip(L.fbh_sample_classes_host(0, 64, 2, 5, 64, C.byref(o), 64, None))
