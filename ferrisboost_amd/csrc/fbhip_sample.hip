@@ -13,11 +13,15 @@
 #include <algorithm>
 #include <cmath>
 #include <memory>
+#include <type_traits>
 
 #include "fbhip_heads.h"
 
 namespace fbh {
 namespace {
+
+template <int N>
+using Int = std::integral_constant<int, N>;
 
 constexpr uint32_t SAMPLE_MOST = 262144;  // classes: their weights' sum is below 2^63
 constexpr uint32_t NO_BIN = 0xFFFFFFFFu;
@@ -144,21 +148,47 @@ __device__ __forceinline__ uint64_t shfl64_up(uint64_t v, int by, int width = 64
     const uint32_t hi = __shfl_up((uint32_t)(v >> 32), by, width);
     return (uint64_t)hi << 32 | lo;
 }
-__device__ __forceinline__ uint64_t scan64(uint64_t v, uint32_t lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t y = shfl64_up(v, d);
-        if (lane >= (uint32_t)d) v += y;
-    }
+// Sums over a wave's lanes up to each, by moves between lanes that take no LDS: within rows
+// of 16, then the last lane of a row to the next one, then of a half to the other.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t moved(uint64_t v) {
+    return (uint64_t)moved<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 |
+           moved<CTRL, ROWS>((uint32_t)v);
+}
+template <class U>
+__device__ __forceinline__ U scan_wave(U v) {
+    v += moved<0x111, 0xF>(v);
+    v += moved<0x112, 0xF>(v);
+    v += moved<0x114, 0xF>(v);
+    v += moved<0x118, 0xF>(v);
+    v += moved<0x142, 0xA>(v);
+    v += moved<0x143, 0xC>(v);
     return v;
 }
-__device__ __forceinline__ uint32_t scan32(uint32_t v, uint32_t lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t y = __shfl_up(v, d);
-        if (lane >= (uint32_t)d) v += y;
-    }
-    return v;
+__device__ __forceinline__ uint32_t at_lane(uint32_t v, uint32_t lane) {
+    return __builtin_amdgcn_readlane(v, lane);
+}
+__device__ __forceinline__ uint64_t at_lane(uint64_t v, uint32_t lane) {
+    return (uint64_t)at_lane((uint32_t)(v >> 32), lane) << 32 | at_lane((uint32_t)v, lane);
+}
+// The largest of a wave's values.
+__device__ __forceinline__ float most_of_wave(float v) {
+    const auto step = [&](auto ctrl, auto rows) {
+        v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(
+                         __float_as_int(v), __float_as_int(v), decltype(ctrl)::value,
+                         decltype(rows)::value, 0xF, false)));
+    };
+    step(Int<0x111>{}, Int<0xF>{});
+    step(Int<0x112>{}, Int<0xF>{});
+    step(Int<0x114>{}, Int<0xF>{});
+    step(Int<0x118>{}, Int<0xF>{});
+    step(Int<0x142>{}, Int<0xA>{});
+    step(Int<0x143>{}, Int<0xC>{});
+    return __int_as_float((int)at_lane((uint32_t)__float_as_int(v), 63));
 }
 
 // -------------------------------------------------------------- a row a thread
@@ -341,9 +371,7 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const T *logits, Draw 
     float mine = l[0];
 #pragma unroll
     for (int i = 1; i < R; i++) mine = fmaxf(mine, l[i]);
-    float most = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+    const float most = most_of_wave(mine);
     if (most == -INFINITY || O.k == 1) {
         const uint64_t has = __ballot(mine == most);
         if (lane == (uint32_t)__ffsll((long long)has) - 1) {
@@ -357,9 +385,14 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const T *logits, Draw 
     }
     const RowScale S{most, (double)most, O.inv_t};
     const float per_nat = (float)(O.inv_t * (WAVE_BINS / 32));
-    const auto bin_of = [&](float v) {
-        const float d = v == most ? 0.0f : (most - v) * per_nat;
-        return (uint32_t)fminf(d, (float)(WAVE_BINS - 1));
+    uint32_t bins[R];  // of (max - l) / T, 32 over all of them; masked classes behind them
+    const auto set_bins = [&] {
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const float d = l[i] == most ? 0.0f : (most - l[i]) * per_nat;
+            bins[i] = l[i] == -INFINITY ? WAVE_BINS
+                                        : (uint32_t)fminf(d, (float)(WAVE_BINS - 1));
+        }
     };
     const uint32_t target31 = uniform31(D.uniforms[row]);
 
@@ -384,8 +417,8 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const T *logits, Draw 
             cs += c[b];
             vs += v[b];
         }
-        const uint32_t cc = scan32(cs, lane);
-        const uint64_t vv = by_count ? 0 : scan64(vs, lane);
+        const uint32_t cc = scan_wave(cs);
+        const uint64_t vv = by_count ? 0 : scan_wave(vs);
         const uint64_t hits = __ballot(by_count ? cc >= k : vv >= weight);
         if (!hits) return NO_BIN;
         const int who = __ffsll((long long)hits) - 1;
@@ -403,17 +436,17 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const T *logits, Draw 
                     bv += v[b];
                 }
             }
-        before_c = __shfl(bc, who);
-        before_w = shfl64(bv, who);
-        inside = __shfl(inside, who);
-        return (uint32_t)__shfl(bin, who);
+        before_c = at_lane(bc, who);
+        before_w = at_lane(bv, who);
+        inside = at_lane(inside, who);
+        return at_lane(bin, who);
     };
     // Classes with take(i) to lanes, in class order; at most 64 of them.
     const auto gather = [&](auto &&take) {
         uint32_t some = 0;
 #pragma unroll
         for (int i = 0; i < R; i++) some += take(i);
-        uint32_t at = scan32(some, lane) - some;
+        uint32_t at = scan_wave(some) - some;
 #pragma unroll
         for (int i = 0; i < R; i++)
             if (take(i)) {
@@ -426,10 +459,13 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const T *logits, Draw 
     // This lane's place among `members` lanes by falling key, equal ones by lane.
     const auto rank_of = [&](uint32_t key, uint32_t members) {
         uint32_t rank = 0;
-        for (uint32_t j = 0; j < members; j++) {
-            const uint32_t kj = __builtin_amdgcn_readlane(key, j);
-            rank += kj > key || (kj == key && j < lane);
-        }
+        // (lanes behind the last member hold key 0, below any class')
+        for (uint32_t j0 = 0; j0 < members; j0 += 8)
+#pragma unroll
+            for (uint32_t j = j0; j < j0 + 8; j++) {
+                const uint32_t kj = at_lane(key, j);
+                rank += kj > key || (kj == key && j < lane);
+            }
         return rank;
     };
     // The cut among classes of one bin by bisection of their keys, where they are too many
@@ -443,13 +479,13 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const T *logits, Draw 
             uint64_t v = 0;
 #pragma unroll
             for (int i = 0; i < R; i++)
-                if (l[i] != -INFINITY && bin_of(l[i]) == bin && logit_key(l[i]) >= mid) {
+                if (bins[i] == bin && logit_key(l[i]) >= mid) {
                     c++;
                     if (!by_count) v += w[i];
                 }
             const bool enough =
-                by_count ? before_c + __shfl(scan32(c, lane), 63) >= k
-                         : before_w + shfl64(scan64(v, lane), 63) >= weight;
+                by_count ? before_c + at_lane(scan_wave(c), 63) >= k
+                         : before_w + at_lane(scan_wave(v), 63) >= weight;
             if (enough) lo = mid;
             else hi = mid - 1;
         }
@@ -457,15 +493,15 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const T *logits, Draw 
         uint64_t v = 0;
 #pragma unroll
         for (int i = 0; i < R; i++)
-            if (l[i] != -INFINITY && bin_of(l[i]) == bin && logit_key(l[i]) > lo) {
+            if (bins[i] == bin && logit_key(l[i]) > lo) {
                 c++;
                 if (!by_count) v += w[i];
             }
         Cut cut{lo, 0};
-        if (by_count) cut.ties = k - before_c - __shfl(scan32(c, lane), 63);
+        if (by_count) cut.ties = k - before_c - at_lane(scan_wave(c), 63);
         else {
             const uint64_t one = S.weight(key_logit(lo));
-            const uint64_t left = weight - before_w - shfl64(scan64(v, lane), 63);
+            const uint64_t left = weight - before_w - at_lane(scan_wave(v), 63);
             cut.ties = (uint32_t)((left + one - 1) / one);
         }
         return cut;
@@ -473,7 +509,7 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const T *logits, Draw 
     const auto cut_in = [&](uint32_t bin, uint32_t inside, bool by_count, uint32_t k,
                             uint64_t weight, uint32_t before_c, uint64_t before_w) {
         if (inside > 64) return bisect(bin, by_count, k, weight, before_c, before_w);
-        gather([&](int i) { return l[i] != -INFINITY && bin_of(l[i]) == bin; });
+        gather([&](int i) { return bins[i] == bin; });
         const uint32_t key = lane < inside ? sh.keys[lane] : 0;
         const uint32_t rank = rank_of(key, inside);
         wave_fence();
@@ -483,11 +519,11 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const T *logits, Draw 
         const uint32_t sorted = lane < inside ? sh.keys[lane] : 0;
         const uint64_t v =
             lane < inside && !by_count ? S.weight(key_logit(sorted)) : 0;
-        const uint64_t upto = by_count ? 0 : before_w + scan64(v, lane);
+        const uint64_t upto = by_count ? 0 : before_w + scan_wave(v);
         const uint64_t hits = __ballot(
             lane < inside && (by_count ? before_c + lane + 1 >= k : upto >= weight));
         const uint32_t who = (uint32_t)__ffsll((long long)hits) - 1;
-        const uint32_t at = __shfl(sorted, who);
+        const uint32_t at = at_lane(sorted, who);
         const uint64_t same = __ballot(lane < inside && sorted == at);
         wave_fence();
         return Cut{at, who - ((uint32_t)__ffsll((long long)same) - 1) + 1};
@@ -497,16 +533,15 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const T *logits, Draw 
 #pragma unroll
         for (int b = 0; b < (int)WAVE_BINS / 64; b++) {
             sh.ct[lane + 64 * b] = 0;
-            sh.wt[lane + 64 * b] = 0;
+            if (weights) sh.wt[lane + 64 * b] = 0;
         }
         wave_fence();
 #pragma unroll
         for (int i = 0; i < R; i++)
-            if (l[i] != -INFINITY) {
-                const uint32_t b = bin_of(l[i]);
-                atomicAdd(&sh.ct[b], 1u);
+            if (bins[i] < WAVE_BINS) {
+                atomicAdd(&sh.ct[bins[i]], 1u);
                 if (weights)
-                    atomicAdd(reinterpret_cast<unsigned long long *>(&sh.wt[b]),
+                    atomicAdd(reinterpret_cast<unsigned long long *>(&sh.wt[bins[i]]),
                               (unsigned long long)w[i]);
             }
         wave_fence();
@@ -517,13 +552,14 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const T *logits, Draw 
     if (O.cuts(n)) {
         uint32_t before_c = 0, inside = 0;
         uint64_t before_w = 0;
+        set_bins();
         if (O.k <= 64 && O.k < n) {
             histogram(false);
             const uint32_t bin = find(true, O.k, 0, before_c, before_w, inside);
             const uint32_t members = before_c + inside;
             if (bin != NO_BIN && members <= 64) {
                 // All that can stay has a lane each, in class order.
-                gather([&](int i) { return l[i] != -INFINITY && bin_of(l[i]) <= bin; });
+                gather([&](int i) { return bins[i] <= bin; });
                 const uint32_t key = lane < members ? sh.keys[lane] : 0;
                 const uint32_t rank = rank_of(key, members);
                 const float v = key_logit(key);
@@ -532,15 +568,15 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const T *logits, Draw 
                     if (lane < members) sh.wt[rank] = kept;
                     wave_fence();
                     const uint64_t s = lane < members ? sh.wt[lane] : 0;
-                    const uint64_t upto = scan64(s, lane);
-                    uint64_t weight = share(O.p31, shfl64(upto, 63), 0x7FFFFFFFu);
+                    const uint64_t upto = scan_wave(s);
+                    uint64_t weight = share(O.p31, at_lane(upto, 63), 0x7FFFFFFFu);
                     if (weight == 0) weight = 1;
                     const uint32_t stay = __popcll(__ballot(lane < members && upto - s < weight));
                     if (rank >= stay) kept = 0;
                 }
                 if (kept < O.least) kept = 0;
-                const uint64_t cum = scan64(kept, lane);
-                const uint64_t total = shfl64(cum, 63);
+                const uint64_t cum = scan_wave(kept);
+                const uint64_t total = at_lane(cum, 63);
                 const uint64_t hits = __ballot(cum > share(target31, total, 0));
                 if (lane == (uint32_t)__ffsll((long long)hits) - 1)
                     put_class(D, row, sh.classes[lane], S.z(v), total);
@@ -563,7 +599,7 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const T *logits, Draw 
 #pragma unroll
             for (int i = 0; i < R; i++)
                 if (logit_key(l[i]) > cut.key) mine_w += w[i];
-            const uint64_t all = shfl64(scan64(mine_w, lane), 63) + cut.ties * tie_w;
+            const uint64_t all = at_lane(scan_wave(mine_w), 63) + cut.ties * tie_w;
             uint64_t weight = share(O.p31, all, 0x7FFFFFFFu);
             if (weight == 0) weight = 1;
             const uint32_t bin = find(false, 0, weight, before_c, before_w, inside);
@@ -587,11 +623,11 @@ __global__ __launch_bounds__(256) void sample_wave_kernel(const T *logits, Draw 
         }
         sum += w[i];
     }
-    const uint32_t ties0 = scan32(ties, lane) - ties;  // before this lane
+    const uint32_t ties0 = scan_wave(ties) - ties;  // before this lane
     const uint32_t kept = ties0 < cut.ties ? min(cut.ties - ties0, ties) : 0;
     sum += kept * tie_w;
-    const uint64_t cum = scan64(sum, lane);
-    const uint64_t total = shfl64(cum, 63);
+    const uint64_t cum = scan_wave(sum);
+    const uint64_t total = at_lane(cum, 63);
     const uint64_t target = share(target31, total, 0);
     const uint64_t hits = __ballot(cum > target);
     if (lane == (uint32_t)__ffsll((long long)hits) - 1) {
@@ -653,8 +689,7 @@ struct RowShared {
     uint64_t list[LIST];
     uint64_t tile_w[MOST_TILES];
     uint32_t tile_ties[MOST_TILES];
-    float wave_most[TPB / 64], wave_least[TPB / 64];
-    uint32_t wave_at[TPB / 64];
+    float wave_most[TPB / 64];
     uint64_t wave_w[TPB / 64];
     uint32_t wave_ties[TPB / 64];
     uint32_t bin, n_list;
@@ -664,6 +699,21 @@ struct RowShared {
     uint64_t total;
     uint32_t tile, ties;
 };
+
+// The thread's piece of a tile, masked classes (and ones behind the last) as -inf.
+template <class T>
+__device__ __forceinline__ void tile_piece(const T *row, uint32_t n, uint32_t i,
+                                           float (&l)[16 / sizeof(T)]) {
+    constexpr int N = 16 / sizeof(T);
+    if (i + N <= n) {
+        const Piece<T, N> p = load_piece<T, N>(row + i);
+#pragma unroll
+        for (int j = 0; j < N; j++) l[j] = masked_nan((float)p.v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j++) l[j] = i + j < n ? masked_nan((float)row[i + j]) : -INFINITY;
+    }
+}
 
 // One row. All threads of the workgroup call every function; a barrier stands between
 // a write and its readers.
@@ -690,44 +740,48 @@ struct SampleRow {
         }
     }
 
-    // The largest logit and its first class; the thread's own largest, and the least of
-    // those that are not masked.
-    __device__ __forceinline__ void largest(float &most, uint32_t &at, float &own,
-                                            float &least) const {
-        most = -INFINITY;
-        at = NO_BIN;
-        each([&](uint32_t i, float l) {
-            if (l > most) {
-                most = l;
-                at = i;
-            }
-        });
-        own = most;
-        least = most == -INFINITY ? INFINITY : most;
-        for (int d = 1; d < 64; d <<= 1) {
-            const float m = __shfl_xor(most, d);
-            const uint32_t a = __shfl_xor(at, d);
-            least = fminf(least, __shfl_xor(least, d));
-            if (m > most || (m == most && a < at)) {
-                most = m;
-                at = a;
-            }
+    // f(class of the first, logits) for the thread's pieces; ones behind the last class, and
+    // NaN, as -inf.
+    template <class F>
+    __device__ __forceinline__ void pieces(F &&f) const {
+#pragma unroll 4
+        for (uint32_t i = threadIdx.x * N; i < n; i += TPB * N) {
+            float l[N];
+            tile_piece<T>(row, n, i, l);
+            f(i, l);
         }
-        if ((threadIdx.x & 63) == 0) {
-            sh.wave_most[threadIdx.x / 64] = most;
-            sh.wave_least[threadIdx.x / 64] = least;
-            sh.wave_at[threadIdx.x / 64] = at;
-        }
+    }
+    // The least of all threads' values.
+    __device__ __forceinline__ float least(float v) {
+        const float m = -most_of_wave(-v);
         __syncthreads();
-        for (int w = 0; w < TPB / 64; w++) {
-            const float m = sh.wave_most[w];
-            const uint32_t a = sh.wave_at[w];
-            least = fminf(least, sh.wave_least[w]);
-            if (m > most || (m == most && a < at)) {
-                most = m;
-                at = a;
-            }
-        }
+        if ((threadIdx.x & 63) == 0) sh.wave_most[threadIdx.x / 64] = m;
+        __syncthreads();
+        float all = sh.wave_most[0];
+        for (int w = 1; w < TPB / 64; w++) all = fminf(all, sh.wave_most[w]);
+        return all;
+    }
+
+    // The largest logit, and the thread's own largest.
+    __device__ __forceinline__ float largest(float &own) {
+        own = -INFINITY;
+        pieces([&](uint32_t, const float *l) {
+#pragma unroll
+            for (int j = 0; j < N; j++) own = fmaxf(own, l[j]);
+        });
+        return -least(-own);
+    }
+    // The first class of this logit.
+    __device__ __forceinline__ uint32_t first_of(float most) {
+        if (threadIdx.x == 0) sh.n_list = NO_BIN;
+        __syncthreads();
+        pieces([&](uint32_t i, const float *l) {
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                if (l[j] == most) atomicMin(&sh.n_list, i + j);
+        });
+        __syncthreads();
+        return sh.n_list;
     }
 
     __device__ __forceinline__ uint32_t bin_of(float l) const {
@@ -755,7 +809,7 @@ struct SampleRow {
 
     // The sum of all threads' values, and with `upto` that of the threads up to this one.
     __device__ __forceinline__ uint64_t sum(uint64_t v, uint64_t *upto = nullptr) {
-        const uint64_t x = scan64(v, threadIdx.x & 63);
+        const uint64_t x = scan_wave(v);
         __syncthreads();
         if ((threadIdx.x & 63) == 63) sh.wave_w[threadIdx.x / 64] = x;
         __syncthreads();
@@ -782,8 +836,8 @@ struct SampleRow {
                 c += sh.ct[b0 + b];
                 w += sh.wt[b0 + b];
             }
-            const uint32_t cc = scan32(c, threadIdx.x);
-            const uint64_t ww = scan64(w, threadIdx.x);
+            const uint32_t cc = scan_wave(c);
+            const uint64_t ww = scan_wave(w);
             uint32_t bc = sh.before_ct;
             uint64_t bw = sh.before_wt;
             const bool reach = by_count ? bc + cc >= k : bw + ww >= weight;
@@ -864,6 +918,26 @@ struct SampleRow {
         return sh.bin;
     }
 
+    // The classes of logits at or above `from`, in the list; how many, NO_BIN if too many.
+    __device__ __forceinline__ uint32_t gather_from(float from) {
+        if (threadIdx.x == 0) sh.n_list = 0;
+        __syncthreads();
+        pieces([&](uint32_t i, const float *l) {
+            float m = l[0];
+#pragma unroll
+            for (int j = 1; j < N; j++) m = fmaxf(m, l[j]);
+            if (m < from) return;
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                if (l[j] >= from) {
+                    const uint32_t at = atomicAdd(&sh.n_list, 1u);
+                    if (at < Shared::LIST) sh.list[at] = entry_of(l[j], i + j);
+                }
+        });
+        __syncthreads();
+        return sh.n_list <= Shared::LIST ? sh.n_list : NO_BIN;
+    }
+
     // The classes that `take`, in the list; how many they are, NO_BIN if too many.
     template <class F>
     __device__ __forceinline__ uint32_t gather(F &&take) {
@@ -892,6 +966,7 @@ __device__ __forceinline__ void draw_listed(SampleRow<T, TPB> &R, const Draw &D,
     for (uint32_t i = threadIdx.x; i < m; i += TPB) {
         const uint64_t e = sh.list[i];
         uint32_t rank = 0;
+#pragma unroll 8
         for (uint32_t j = 0; j < m; j++) rank += sh.list[j] > e;
         if (rank < O.k) {
             weights[rank] = R.S.weight(key_logit(entry_key(e)));
@@ -916,6 +991,7 @@ __device__ __forceinline__ void draw_listed(SampleRow<T, TPB> &R, const Draw &D,
     const uint64_t target = share(uniform31(D.uniforms[row]), total, 0);
     uint64_t before = 0;
     if (w)
+#pragma unroll 8
         for (uint32_t j = 0; j < k; j++) before += classes[j] < c ? weights[j] : 0;
     if (w && before <= target && target < before + w) {
         const float l = (float)R.row[c];
@@ -948,23 +1024,7 @@ __device__ __forceinline__ bool tiled(const RowOptions &O, uint32_t n) { return 
 
 __device__ __forceinline__ float row_most(const TileWork &W, uint32_t tiles) {
     float m = (threadIdx.x & 63) < tiles ? W.most[threadIdx.x & 63] : -INFINITY;
-    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
-    return m;
-}
-
-// The thread's piece of a tile, masked classes (and ones behind the last) as -inf.
-template <class T>
-__device__ __forceinline__ void tile_piece(const T *row, uint32_t n, uint32_t i,
-                                           float (&l)[16 / sizeof(T)]) {
-    constexpr int N = 16 / sizeof(T);
-    if (i + N <= n) {
-        const Piece<T, N> p = load_piece<T, N>(row + i);
-#pragma unroll
-        for (int j = 0; j < N; j++) l[j] = masked_nan((float)p.v[j]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < N; j++) l[j] = i + j < n ? masked_nan((float)row[i + j]) : -INFINITY;
-    }
+    return most_of_wave(m);
 }
 
 // grid (tiles, rows)
@@ -986,7 +1046,7 @@ __global__ __launch_bounds__(TILE_TPB) void tile_most_kernel(const T *logits, Dr
     float m = l[0];
 #pragma unroll
     for (int j = 1; j < N; j++) m = fmaxf(m, l[j]);
-    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+    m = most_of_wave(m);
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x / 64] = m;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -1073,13 +1133,11 @@ __global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D
     SampleRow<T, TPB> R{sh, logits + r * n, n, {}, 0.0f};
     const uint32_t tiles = (n + TPB * N - 1) / (TPB * N);
     const bool done = TILED && tiled(O, n);
-    float most, own, least;
-    uint32_t most_at = NO_BIN;
-    if (done) most = row_most(work[r], tiles);
-    else R.largest(most, most_at, own, least);
+    float own = -INFINITY;
+    const float most = done ? row_most(work[r], tiles) : R.largest(own);
     if (most == -INFINITY || O.k == 1) {
-        if (threadIdx.x == 0)
-            put_class(D, r, most == -INFINITY ? -1 : (int64_t)most_at, 0.0, WEIGHT_ONE);
+        const int64_t c = most == -INFINITY ? -1 : (int64_t)R.first_of(most);
+        if (threadIdx.x == 0) put_class(D, r, c, 0.0, WEIGHT_ONE);
         return;
     }
     R.S = RowScale{most, (double)most, O.inv_t};
@@ -1087,6 +1145,7 @@ __global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D
     // Few classes by rank: k of the threads' own largest logits are at or above the k-th of
     // them, so the first k classes of the row are too. One more pass lists those.
     if (O.k < n && O.k <= RowShared<TPB>::MOST_K) {
+        const float least = R.least(own == -INFINITY ? INFINITY : own);
         R.per = most > least ? (float)BINS / (most - least) : 0.0f;
         R.clear(BINS);
         if (own != -INFINITY) atomicAdd(&sh.ct[R.bin_of(own)], 1u);
@@ -1094,7 +1153,9 @@ __global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D
         R.find(BINS, true, O.k, 0);
         const uint32_t bin = sh.bin;
         if (bin != NO_BIN) {
-            const uint32_t m = R.gather([&](uint32_t, float l) { return R.bin_of(l) <= bin; });
+            // the least of the largest ones in the bins up to the k-th's
+            const float from = R.least(own != -INFINITY && R.bin_of(own) <= bin ? own : INFINITY);
+            const uint32_t m = R.gather_from(from);
             if (m != NO_BIN) {
                 draw_listed(R, D, r, O, m);
                 return;
@@ -1122,12 +1183,9 @@ __global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D
             } else {
                 for (uint32_t j = i; j < n; j++) f(j, masked_nan((float)R.row[j]), w, ties);
             }
-            for (int d = 32; d; d >>= 1) {
-                w += (uint64_t)__shfl_xor((uint32_t)(w >> 32), d) * 0x100000000ull +
-                     __shfl_xor((uint32_t)w, d);
-                ties += __shfl_xor(ties, d);
-            }
-            if ((threadIdx.x & 63) == 0) {
+            w = scan_wave(w);
+            ties = scan_wave(ties);
+            if ((threadIdx.x & 63) == 63) {
                 if (w)
                     atomicAdd(reinterpret_cast<unsigned long long *>(&sh.tile_w[t]),
                               (unsigned long long)w);
@@ -1284,8 +1342,8 @@ __global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D
     uint64_t w = 0;
     uint32_t ties = 0;
     for (uint32_t j = i0; j < i1; j++) staying(masked_nan((float)R.row[j]), w, ties);
-    uint64_t cw = scan64(w, threadIdx.x & 63);
-    uint32_t ct = scan32(ties, threadIdx.x & 63);
+    uint64_t cw = scan_wave(w);
+    uint32_t ct = scan_wave(ties);
     if ((threadIdx.x & 63) == 63) {
         sh.wave_w[threadIdx.x / 64] = cw;
         sh.wave_ties[threadIdx.x / 64] = ct;
