@@ -727,6 +727,35 @@ struct SampleRow {
     RowScale S;
     float per;  // bins of a unit of logits
 
+    // f(class of the first, logits) for the thread's pieces; ones behind the last class, and
+    // NaN, as -inf.
+    template <class F>
+    __device__ __forceinline__ void pieces(F &&f) const {
+        const uint32_t step = TPB * N, whole = n / step * step;  // (all threads have a piece)
+        uint32_t i = threadIdx.x * N;
+        const auto batch = [&](auto pieces) {
+            constexpr int B = decltype(pieces)::value;
+            Piece<T, N> p[B];
+#pragma unroll
+            for (int b = 0; b < B; b++) p[b] = load_piece<T, N>(row + i + b * step);
+#pragma unroll
+            for (int b = 0; b < B; b++) {
+                float l[N];
+#pragma unroll
+                for (int j = 0; j < N; j++) l[j] = masked_nan((float)p[b].v[j]);
+                f(i + b * step, l);
+            }
+            i += B * step;
+        };
+        while (i + 4 * step <= whole + threadIdx.x * N) batch(Int<4>{});
+        while (i < whole) batch(Int<1>{});
+        if (i < n) {
+            float l[N];
+            tile_piece<T>(row, n, i, l);
+            f(i, l);
+        }
+    }
+    // f(class, logit) for the thread's classes.
     template <class F>
     __device__ __forceinline__ void each(F &&f) const {
         for (uint32_t i = threadIdx.x * N; i < n; i += TPB * N) {
@@ -740,17 +769,6 @@ struct SampleRow {
         }
     }
 
-    // f(class of the first, logits) for the thread's pieces; ones behind the last class, and
-    // NaN, as -inf.
-    template <class F>
-    __device__ __forceinline__ void pieces(F &&f) const {
-#pragma unroll 4
-        for (uint32_t i = threadIdx.x * N; i < n; i += TPB * N) {
-            float l[N];
-            tile_piece<T>(row, n, i, l);
-            f(i, l);
-        }
-    }
     // The least of all threads' values.
     __device__ __forceinline__ float least(float v) {
         const float m = -most_of_wave(-v);
@@ -966,7 +984,7 @@ __device__ __forceinline__ void draw_listed(SampleRow<T, TPB> &R, const Draw &D,
     for (uint32_t i = threadIdx.x; i < m; i += TPB) {
         const uint64_t e = sh.list[i];
         uint32_t rank = 0;
-#pragma unroll 8
+#pragma unroll 16
         for (uint32_t j = 0; j < m; j++) rank += sh.list[j] > e;
         if (rank < O.k) {
             weights[rank] = R.S.weight(key_logit(entry_key(e)));
@@ -991,7 +1009,7 @@ __device__ __forceinline__ void draw_listed(SampleRow<T, TPB> &R, const Draw &D,
     const uint64_t target = share(uniform31(D.uniforms[row]), total, 0);
     uint64_t before = 0;
     if (w)
-#pragma unroll 8
+#pragma unroll 16
         for (uint32_t j = 0; j < k; j++) before += classes[j] < c ? weights[j] : 0;
     if (w && before <= target && target < before + w) {
         const float l = (float)R.row[c];
