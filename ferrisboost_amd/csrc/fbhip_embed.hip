@@ -146,7 +146,7 @@ __global__ __launch_bounds__(EMB_TPB) void embed_sum_kernel(Positions P, const T
                                                             float s) {
     extern __shared__ uint32_t toks[];
     const uint32_t rows = EMB_TPB >> lg_g, cols = 1u << lg_c, pitch = cols + 4;
-    const uint64_t row0 = (uint64_t)blockIdx.x * rows;
+    const uint64_t row0 = (blockIdx.x + (uint64_t)blockIdx.z * gridDim.x) * rows;
     const uint32_t r = threadIdx.x >> lg_g;
     const uint32_t piece = blockIdx.y * (1u << lg_g) + (threadIdx.x & ((1u << lg_g) - 1));
     const bool live = row0 + r < P.n_rows && piece < n_pieces;
@@ -1099,10 +1099,12 @@ void launch_embed(const fbh_embed *e, const void *table, void *out, hipStream_t 
         const uint32_t lg_c =
             std::min(std::max(lg_at_least(P.n_columns), 3u), lg_at_least(4096 / rows));
         const uint64_t blocks = (P.n_rows + rows - 1) / rows;
-        head_input(blocks < 1u << 24, "too many rows");
+        const uint32_t bx = (uint32_t)std::min<uint64_t>(blocks, 1u << 22);
+        const uint64_t bz = (blocks + bx - 1) / bx;
+        head_input(bz <= 65535, "too many rows");
         const auto go = [&](auto buffer) {
             hipLaunchKernelGGL((embed_sum_kernel<T, VEC, ID, DROP, decltype(buffer)::value>),
-                               dim3((uint32_t)blocks, (pieces + (1u << lg_g) - 1) >> lg_g),
+                               dim3(bx, (pieces + (1u << lg_g) - 1) >> lg_g, (uint32_t)bz),
                                dim3(EMB_TPB), (size_t)rows * ((1u << lg_c) + 4) * 4, s, P, tab,
                                to, e->dim, pieces, lg_g, lg_c, sc);
         };
@@ -1415,6 +1417,8 @@ int fbh_embed_grad(int device, const fbh_embed *e, const void *grad, void *table
         head_input(table && (grad || e->n_rows == 0), "null argument");
         const uint64_t need = grad_bytes(e);
         head_input(work_bytes >= need && (work || need == 0), "the workspace is too small");
+        head_input(reinterpret_cast<uintptr_t>(work) % 16 == 0,
+                   "the workspace is not aligned to 16 bytes");
         const OnDevice on(device);
         embed_grad(e, grad, table, work, static_cast<hipStream_t>(stream));
     });

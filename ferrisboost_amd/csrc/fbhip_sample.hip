@@ -1390,6 +1390,8 @@ __global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D
     }
 }
 
+constexpr uint64_t SAMPLE_LAUNCH = 1u << 21;  // rows of a launch at most
+
 // Whether a call's rows may be taken tile by tile.
 bool sample_tiled(uint64_t n_rows, uint32_t n_classes) {
     return n_rows <= TILE_ROWS && n_classes > 16384;
@@ -1400,11 +1402,25 @@ uint64_t sample_bytes(uint64_t n_rows, uint32_t n_classes) {
 
 template <class T>
 void launch_sample(const void *logits, const Draw &D, TileWork *work, hipStream_t s) {
+    const uint32_t v = D.n_classes;
+    if (D.n_rows > SAMPLE_LAUNCH) {  // (a launch has fewer than 2^32 threads)
+        for (uint64_t r = 0; r < D.n_rows; r += SAMPLE_LAUNCH) {
+            Draw d = D;
+            d.n_rows = std::min<uint64_t>(D.n_rows - r, SAMPLE_LAUNCH);
+            d.uniforms += r;
+            d.classes += r;
+            if (d.log_probs) d.log_probs += r;
+            if (d.o.temperatures) d.o.temperatures += r;
+            if (d.o.top_ks) d.o.top_ks += r;
+            if (d.o.top_ps) d.o.top_ps += r;
+            if (d.o.min_ps) d.o.min_ps += r;
+            launch_sample<T>(static_cast<const T *>(logits) + r * v, d, nullptr, s);
+        }
+        return;
+    }
     const auto *l = static_cast<const T *>(logits);
     const uint64_t n = D.n_rows;
-    const uint32_t v = D.n_classes;
     if (v <= THREAD_MOST) {
-        head_input(n <= 1ull << 31, "too many rows");
         const dim3 grid((uint32_t)((n + 255) / 256)), tpb(256);
         if (v == 1) hipLaunchKernelGGL((sample_thread_kernel<T, 1>), grid, tpb, 0, s, l, D);
         else if (v == 2) hipLaunchKernelGGL((sample_thread_kernel<T, 2>), grid, tpb, 0, s, l, D);
@@ -1417,20 +1433,17 @@ void launch_sample(const void *logits, const Draw &D, TileWork *work, hipStream_
     } else if (v <= GROUP_MOST) {
         const uint32_t g = v <= 16 ? 16 : v <= 32 ? 32 : 64;
         const uint64_t blocks = (n + GROUP_TPB / g - 1) / (GROUP_TPB / g);
-        head_input(blocks < 1u << 24, "too many rows");
         const dim3 grid((uint32_t)blocks), tpb(GROUP_TPB);
         if (g == 16) hipLaunchKernelGGL((sample_group_kernel<T, 16>), grid, tpb, 0, s, l, D);
         else if (g == 32) hipLaunchKernelGGL((sample_group_kernel<T, 32>), grid, tpb, 0, s, l, D);
         else hipLaunchKernelGGL((sample_group_kernel<T, 64>), grid, tpb, 0, s, l, D);
     } else if (v <= WAVE_MOST) {
-        head_input(n < 1u << 25, "too many rows");
         const dim3 grid((uint32_t)((n + 3) / 4)), tpb(256);
         if (v <= 128) hipLaunchKernelGGL((sample_wave_kernel<T, 2>), grid, tpb, 0, s, l, D);
         else if (v <= 256) hipLaunchKernelGGL((sample_wave_kernel<T, 4>), grid, tpb, 0, s, l, D);
         else if (v <= 512) hipLaunchKernelGGL((sample_wave_kernel<T, 8>), grid, tpb, 0, s, l, D);
         else hipLaunchKernelGGL((sample_wave_kernel<T, 16>), grid, tpb, 0, s, l, D);
     } else {
-        head_input(n < 1u << 22, "too many rows");
         const dim3 grid((uint32_t)n);
         if (v <= 16384)
             hipLaunchKernelGGL((sample_row_kernel<T, 256, false>), grid, dim3(256), 0, s, l, D,
@@ -1495,6 +1508,8 @@ int fbh_sample_classes(int device, const void *logits, uint64_t n_rows, uint32_t
         if (n_rows == 0) return;
         const uint64_t need = sample_bytes(n_rows, n_classes);
         head_input(work_bytes >= need && (work || need == 0), "the workspace is too small");
+        head_input(need == 0 || reinterpret_cast<uintptr_t>(work) % 8 == 0,
+                   "the workspace is not aligned to 8 bytes");
         const OnDevice on(device);
         sample(logits, dtype,
                draw_of(uniforms, options, classes, log_probs, n_rows, n_classes), work,

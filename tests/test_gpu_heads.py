@@ -350,6 +350,60 @@ def test_sample_follows_the_distribution(heads):
     assert (np.abs(share - p) <= 5 * np.sqrt(p * (1 - p) / n)).all()
 
 
+def test_beyond_32_bits(heads):
+    """More than 2^32 cells, tables beyond the reach of buffer loads, and more rows than one
+    launch takes."""
+    n = (1 << 32) + 4099
+    x = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    out = heads.dropout(x, 0.5, 11)
+    for at in (0, (1 << 31) - 7, (1 << 32) - 33, n - 4100):
+        part = slice(at, min(at + 4100, n))
+        stay = ref.kept(11, 0.5, np.arange(part.start, part.stop))
+        assert np.array_equal(out[part].float().cpu().numpy(), np.where(stay, 2.0, 0.0))
+        assert torch.equal(heads.dropout(x[part], 0.5, 11, at), out[part])
+    del x, out
+    rows, dim = 40_000_003, 32
+    table = torch.zeros((rows, dim), dtype=torch.bfloat16, device="cuda")
+    table[:, 0] = torch.arange(rows, device="cuda") % 128
+    last = torch.arange(rows - 200_000, rows, device="cuda").reshape(-1, 10)
+    want = (last % 128).float().sum(1)
+    pooled = heads.embed(table.float(), last, pooled=True)
+    assert torch.equal(pooled[:, 0], want) and (pooled[:, 1:] == 0).all()
+    assert torch.equal(heads.embed(table, last, pooled=True)[:, 0], want.bfloat16())
+    ids = torch.arange(rows - 1, -1, -1, dtype=torch.int32, device="cuda").repeat(4)
+    out = heads.embed(table, ids)  # 2^32 cells and more
+    assert out.numel() > 1 << 32 and torch.equal(out[-1], table[0])
+    assert torch.equal(out[:rows:10_007], table.flip(0)[::10_007])
+    assert torch.equal(out[3 * rows::10_007], table.flip(0)[::10_007])
+    g = heads.embed_grad(out, ids, rows)  # four positions a row, a chunk's rows far apart
+    assert torch.equal(g[::9973], (4 * table[::9973].float()).bfloat16())
+    del table, out, g, ids
+    u = torch.rand(2_500_000, device="cuda")
+    x = torch.randn(2_500_000, 70, device="cuda")
+    c, p = heads.sample(x, u, top_k=9)
+    at = slice((1 << 21) - 50, (1 << 21) + 50)
+    c2, p2 = heads.sample(x[at], u[at], top_k=9)
+    assert torch.equal(c[at], c2) and torch.equal(p[at], p2) and (c >= 0).all()
+    want, _ = ref.sample(x[-40:].cpu().numpy(), u[-40:].cpu().numpy(), 1.0, 9, 1.0, 0.0)
+    assert np.array_equal(c[-40:].cpu().numpy(), want)
+
+
+def test_captured_calls_with_much_lds(heads):
+    """A gradient whose workgroups take more LDS than a kernel has without asking."""
+    rng = np.random.default_rng(9)
+    voc = heads.Vocabulary([1000, 900])
+    ids = torch.from_numpy(rng.integers(0, 1000, (40_000, 2))).cuda()
+    grad = _cells(rng, (40_000, 2, 40), "bf16")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        g = heads.embed_grad(grad, ids, voc)
+    for _ in range(3):
+        ids.copy_(torch.from_numpy(rng.integers(-1, 950, (40_000, 2))))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(g, heads.embed_grad(grad, ids, voc))
+
+
 def test_empty_calls(heads):
     voc = heads.Vocabulary([3, 4])
     table = torch.ones(7, 5, device="cuda")

@@ -44,6 +44,8 @@ def test_gradient_workspace():
     assert need > 0
     with pytest.raises(ValueError, match="workspace"):
         N.check_hip(L.fbh_embed_grad(0, C.byref(e), 64, 64, 64, need - 1, None))
+    with pytest.raises(ValueError, match="aligned"):
+        N.check_hip(L.fbh_embed_grad(0, C.byref(e), 64, 64, 72, need, None))
     big = _embed(n_rows=1 << 31)
     with pytest.raises(ValueError, match="positions"):
         N.check_hip(L.fbh_embed_grad(0, C.byref(big), 64, 64, 64, 1 << 50, None))
@@ -66,6 +68,9 @@ def test_dropout_and_sampling_refusals_of_the_c_abi():
     with pytest.raises(ValueError, match="workspace"):
         N.check_hip(L.fbh_sample_classes(0, 64, 2, 100_000, 0, 64, C.byref(o), 64, None, 64,
                                          need - 1, None))
+    with pytest.raises(ValueError, match="aligned"):
+        N.check_hip(L.fbh_sample_classes(0, 64, 2, 100_000, 0, 64, C.byref(o), 64, None, 68,
+                                         need, None))
     o.top_ks = 64
     with pytest.raises(ValueError, match="each row"):
         N.check_hip(L.fbh_sample_classes_host(0, 64, 2, 5, 64, C.byref(o), 64, None))
