@@ -56,14 +56,23 @@ __device__ __forceinline__ Part part_of(const Positions &P, uint32_t column) {
 // The table row of a position, or NO_TOKEN.
 template <bool DROP>
 __device__ __forceinline__ uint32_t token_of(const Positions &P, Part part, uint32_t id,
-                                             uint64_t pos) {
-    bool ok = id < part.size;
-    if (DROP) ok = ok && drop_bits(P.key, pos) >= P.threshold;
-    return ok ? part.base + id : NO_TOKEN;
+                                             uint32_t bits) {
+    return id < part.size && (!DROP || bits >= P.threshold) ? part.base + id : NO_TOKEN;
 }
 template <int ID, bool DROP>
 __device__ __forceinline__ uint32_t token_at(const Positions &P, uint64_t pos, uint32_t column) {
-    return token_of<DROP>(P, part_of(P, column), load_id<ID>(P.ids, pos), pos);
+    return token_of<DROP>(P, part_of(P, column), load_id<ID>(P.ids, pos),
+                          DROP ? drop_bits(P.key, pos) : 0);
+}
+// The bits of two positions of a thread whose neighbours in the wave hold the next columns,
+// from an even one on; rows of an even number of columns start with an even position.
+template <bool DROP>
+__device__ __forceinline__ void bits_of_two(const Positions &P, const uint64_t (&pos)[2],
+                                            uint32_t (&bits)[2]) {
+    if (!DROP) return;
+    if (P.n_columns % 2 == 0) drop_bits_of_neighbours(P.key, pos, bits);
+    else
+        for (int k = 0; k < 2; k++) bits[k] = drop_bits(P.key, pos[k]);
 }
 
 // l / d for l + d below 2^31 and l * d below 2^32 (d > 1: m = ceil(2^32 / d)).
@@ -128,11 +137,13 @@ __global__ __launch_bounds__(EMB_TPB) void embed_rows_kernel(Positions P, const 
 }
 
 // ------------------------------------------------------------------- summed
-// out[row] = s * (sum over columns of table[token]). Column t goes to sum t % 8 and the
-// eight sums are added in a tree, in both kernels, so a row's result does not depend on
-// the rows beside it.
-__device__ __forceinline__ float tree8(const float *a) {
-    return ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
+// out[row] = s * (sum over columns of table[token]). Column t goes to sum t % 4 and the
+// four sums are added in pairs, in both kernels, so a row's result does not depend on the
+// rows beside it. (Eight sums take 32 registers more: 100k rows of 100 trees, 64 cells of
+// bfloat16, 92 us against 80.)
+constexpr uint32_t SUMS = 4;
+__device__ __forceinline__ float join_sums(const float *a) {
+    return (a[0] + a[1]) + (a[2] + a[3]);
 }
 
 // A workgroup takes 256 / G rows, G = 2^lg_g lanes a row; the tokens of 2^lg_c columns at
@@ -154,19 +165,33 @@ __global__ __launch_bounds__(EMB_TPB) void embed_sum_kernel(Positions P, const T
     const uint32_t row_bytes = dim * (uint32_t)sizeof(T), cell_bytes = cell * (uint32_t)sizeof(T);
     const auto rsrc = buffer_of(table, BUFFER ? P.n_tokens * row_bytes : 0);
     const T *from = table + cell;
-    float a[VEC][8];
+    float a[VEC][SUMS];
 #pragma unroll
     for (int i = 0; i < VEC; i++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) a[i][j] = 0.0f;
+        for (uint32_t j = 0; j < SUMS; j++) a[i][j] = 0.0f;
     for (uint32_t t0 = 0; t0 < P.n_columns; t0 += cols) {
-        for (uint32_t i = threadIdx.x; i < rows << lg_c; i += EMB_TPB) {
-            const uint32_t rr = i >> lg_c, t = t0 + (i & (cols - 1));
-            uint32_t tok = NO_TOKEN;
-            if (row0 + rr < P.n_rows && t < P.n_columns)
-                tok = token_at<ID, DROP>(P, (row0 + rr) * P.n_columns + t, t);
-            if (BUFFER) tok = tok == NO_TOKEN ? NO_OFFSET : tok * row_bytes;
-            toks[rr * pitch + (i & (cols - 1))] = tok;
+        for (uint32_t i0 = threadIdx.x; i0 < rows << lg_c; i0 += 4 * EMB_TPB) {
+            uint32_t id[4];
+            Part part[4];
+            // (always a load, as in column_ids_kernel; rows << lg_c has whole steps of 256)
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++) {
+                const uint32_t i = i0 + k * EMB_TPB, t = min(t0 + (i & (cols - 1)), P.n_columns - 1);
+                id[k] = load_id<ID>(P.ids, min(row0 + (i >> lg_c), P.n_rows - 1) * P.n_columns + t);
+                part[k] = part_of(P, t);
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < 4; k++) {
+                const uint32_t i = i0 + k * EMB_TPB, rr = i >> lg_c, t = t0 + (i & (cols - 1));
+                if (rr >= rows) break;
+                const uint32_t bits =
+                    DROP ? drop_bits(P.key, (row0 + rr) * P.n_columns + t) : 0;
+                uint32_t tok = token_of<DROP>(P, part[k], id[k], bits);
+                if (row0 + rr >= P.n_rows || t >= P.n_columns) tok = NO_TOKEN;
+                if (BUFFER) tok = tok == NO_TOKEN ? NO_OFFSET : tok * row_bytes;
+                toks[rr * pitch + (i & (cols - 1))] = tok;
+            }
         }
         __syncthreads();
         const uint32_t most = min(cols, P.n_columns - t0);
@@ -185,7 +210,7 @@ __global__ __launch_bounds__(EMB_TPB) void embed_sum_kernel(Positions P, const T
 #pragma unroll
                     for (int j = 0; j < 8; j++)
 #pragma unroll
-                        for (int i = 0; i < VEC; i++) a[i][j] += (float)p[j].v[i];
+                        for (int i = 0; i < VEC; i++) a[i][j % SUMS] += (float)p[j].v[i];
                 } else {
 #pragma unroll
                     for (int j = 0; j < 8; j++)
@@ -195,7 +220,7 @@ __global__ __launch_bounds__(EMB_TPB) void embed_sum_kernel(Positions P, const T
                     for (int j = 0; j < 8; j++)
 #pragma unroll
                         for (int i = 0; i < VEC; i++)
-                            a[i][j] += tok[j] == NO_TOKEN ? 0.0f : (float)p[j].v[i];
+                            a[i][j % SUMS] += tok[j] == NO_TOKEN ? 0.0f : (float)p[j].v[i];
                 }
             }
         __syncthreads();
@@ -203,11 +228,11 @@ __global__ __launch_bounds__(EMB_TPB) void embed_sum_kernel(Positions P, const T
     if (!live) return;
     Piece<T, VEC> o;
 #pragma unroll
-    for (int i = 0; i < VEC; i++) o.v[i] = (T)(tree8(a[i]) * s);
+    for (int i = 0; i < VEC; i++) o.v[i] = (T)(join_sums(a[i]) * s);
     store_piece<T, VEC>(out + (row0 + r) * dim + cell, o);
 }
 
-// Few rows: the eight sums of a row side by side, a workgroup a row and 2^lg_g pieces.
+// Few rows: the sums of a row side by side, a workgroup a row and 2^lg_g pieces.
 template <class T, int VEC, int ID, bool DROP>
 __global__ void embed_sum_few_kernel(Positions P, const T *table, T *out, uint32_t dim,
                                      uint32_t n_pieces, uint32_t lg_g, float s) {
@@ -220,20 +245,22 @@ __global__ void embed_sum_few_kernel(Positions P, const T *table, T *out, uint32
     float a[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; i++) a[i] = 0.0f;
-    for (uint32_t t0 = j; t0 < P.n_columns; t0 += 64) {
-        uint32_t tok[8];
-        Piece<T, VEC> p[8];
+    constexpr uint32_t AHEAD = 16;  // columns requested at once
+    for (uint32_t t0 = j; t0 < P.n_columns; t0 += AHEAD * SUMS) {
+        uint32_t tok[AHEAD];
+        Piece<T, VEC> p[AHEAD];
 #pragma unroll
-        for (uint32_t k = 0; k < 8; k++) {
-            const uint32_t t = t0 + 8 * k;
-            tok[k] = t < P.n_columns ? token_at<ID, DROP>(P, row * P.n_columns + t, t) : NO_TOKEN;
+        for (uint32_t k = 0; k < AHEAD; k++) {
+            const uint32_t t = min(t0 + SUMS * k, P.n_columns - 1);
+            tok[k] = token_at<ID, DROP>(P, row * P.n_columns + t, t);
+            if (t0 + SUMS * k >= P.n_columns) tok[k] = NO_TOKEN;
         }
 #pragma unroll
-        for (uint32_t k = 0; k < 8; k++)
+        for (uint32_t k = 0; k < AHEAD; k++)
             p[k] = load_piece<T, VEC>(table + (uint64_t)(tok[k] == NO_TOKEN ? 0 : tok[k]) * dim +
                                       cell);
 #pragma unroll
-        for (uint32_t k = 0; k < 8; k++)
+        for (uint32_t k = 0; k < AHEAD; k++)
 #pragma unroll
             for (int i = 0; i < VEC; i++) a[i] += tok[k] == NO_TOKEN ? 0.0f : (float)p[k].v[i];
     }
@@ -245,10 +272,10 @@ __global__ void embed_sum_few_kernel(Positions P, const T *table, T *out, uint32
     Piece<T, VEC> o;
 #pragma unroll
     for (int i = 0; i < VEC; i++) {
-        float b[8];
+        float b[SUMS];
 #pragma unroll
-        for (uint32_t k = 0; k < 8; k++) b[k] = sums[((k << lg_g) + lane) * VEC + i];
-        o.v[i] = (T)(tree8(b) * s);
+        for (uint32_t k = 0; k < SUMS; k++) b[k] = sums[((k << lg_g) + lane) * VEC + i];
+        o.v[i] = (T)(join_sums(b) * s);
     }
     store_piece<T, VEC>(out + row * dim + cell, o);
 }
@@ -724,19 +751,25 @@ __global__ __launch_bounds__(256) void column_ids_kernel(Positions P, uint32_t m
     uint32_t id[16];
 #pragma unroll
     for (uint32_t r = 0; r < 16; r++) {
-        const uint64_t row = row0 + w + 4 * r;
-        id[r] = row < P.n_rows && column < P.n_columns
-                    ? load_id<ID>(P.ids, row * P.n_columns + column)
-                    : NO_TOKEN;
+        // (always a load, of the last position where there is none: a branch for each would
+        // have them wait for one another)
+        const uint64_t row = min(row0 + w + 4 * r, P.n_rows - 1);
+        id[r] = load_id<ID>(P.ids, row * P.n_columns + min(column, P.n_columns - 1));
     }
-    Part part{0, 0};
-    if (column < P.n_columns) part = part_of(P, column);
+    Part part = part_of(P, min(column, P.n_columns - 1));
     part.size = min(part.size, most_ids);
 #pragma unroll
-    for (uint32_t r = 0; r < 16; r++) {
-        const uint32_t tok =
-            token_of<DROP>(P, part, id[r], (row0 + w + 4 * r) * P.n_columns + column);
-        tile[w + 4 * r][lane] = tok != NO_TOKEN ? (uint16_t)id[r] : (uint16_t)COL_NONE;
+    for (uint32_t r = 0; r < 16; r += 2) {
+        const uint64_t row = row0 + w + 4 * r;
+        const uint64_t pos[2] = {row * P.n_columns + column, (row + 4) * P.n_columns + column};
+        uint32_t bits[2] = {0, 0};
+        bits_of_two<DROP>(P, pos, bits);
+#pragma unroll
+        for (uint32_t k = 0; k < 2; k++) {
+            const bool some = token_of<DROP>(P, part, id[r + k], bits[k]) != NO_TOKEN &&
+                              row + 4 * k < P.n_rows && column < P.n_columns;
+            tile[w + 4 * (r + k)][lane] = some ? (uint16_t)id[r + k] : (uint16_t)COL_NONE;
+        }
     }
     __syncthreads();
 #pragma unroll 4
@@ -1005,13 +1038,17 @@ __global__ __launch_bounds__(256) void column_join_kernel(Columns C, T *table) {
     for (uint32_t c0 = 0; c0 < C.chunks; c0 += 8) {
         bool some[8];
         Piece<float, VEC> p[8];
+        uint16_t count[8];
 #pragma unroll
         for (uint32_t k = 0; k < 8; k++)
-            some[k] = c0 + k < C.chunks && C.counts[(uint64_t)(c0 + k) * C.n_tokens + tok] != 0;
+            count[k] = C.counts[(uint64_t)min(c0 + k, C.chunks - 1) * C.n_tokens + tok];
 #pragma unroll
-        for (uint32_t k = 0; k < 8; k++)
-            if (some[k])
-                p[k] = load_piece<float, VEC>(part + (uint64_t)(c0 + k) * C.n_tokens * C.dim);
+        for (uint32_t k = 0; k < 8; k++) {
+            // (a chunk without the token has left nothing; the first part is read instead)
+            some[k] = c0 + k < C.chunks && count[k] != 0;
+            p[k] = load_piece<float, VEC>(
+                some[k] ? part + (uint64_t)(c0 + k) * C.n_tokens * C.dim : C.parts);
+        }
 #pragma unroll
         for (uint32_t k = 0; k < 8; k++)
             if (some[k])
@@ -1089,10 +1126,10 @@ void launch_embed(const fbh_embed *e, const void *table, void *out, hipStream_t 
                            divisor(P.n_columns), sc,
                            P.n_rows * P.n_columns * e->dim * sizeof(T) >= STREAM_BYTES);
     } else if (P.n_rows * pieces < 64 * EMB_TPB) {
-        const uint32_t lg_g = std::min(lg_at_least(pieces), 5u);
+        const uint32_t lg_g = std::max(std::min(lg_at_least(pieces), 6u), 4u);
         hipLaunchKernelGGL((embed_sum_few_kernel<T, VEC, ID, DROP>),
                            dim3((uint32_t)P.n_rows, (pieces + (1u << lg_g) - 1) >> lg_g),
-                           dim3(8u << lg_g), (size_t)(8u << lg_g) * VEC * sizeof(float), s, P, tab,
+                           dim3(SUMS << lg_g), (size_t)(SUMS << lg_g) * VEC * sizeof(float), s, P, tab,
                            to, e->dim, pieces, lg_g, sc);
     } else {
         const uint32_t lg_g = std::min(lg_at_least(pieces), 6u), rows = EMB_TPB >> lg_g;
