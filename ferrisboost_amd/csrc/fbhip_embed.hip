@@ -94,13 +94,15 @@ constexpr uint32_t ROW_BLOCK = EMB_TPB * ROW_PIECES;
 // workgroups, whose positions' tokens are found once and kept in LDS. A vector's last
 // piece starts at dim - VEC, so that no piece is partial; the cells it shares with the
 // piece before are written twice, with the same value.
-template <class T, int VEC, int ID, bool DROP>
+// PAST: written past the caches (a parameter, as the compiler would join the two stores of a
+// branch into an ordinary one).
+template <class T, int VEC, int ID, bool DROP, bool PAST>
 __global__ __launch_bounds__(EMB_TPB) void embed_rows_kernel(Positions P, const T *table, T *out,
                                                              uint32_t dim, Divisor pieces,
-                                                             Divisor columns, float s, bool past) {
+                                                             Divisor columns, float s,
+                                                             uint64_t block0) {
     __shared__ uint32_t toks[ROW_BLOCK + 1];
-    const uint64_t block = blockIdx.x + (uint64_t)blockIdx.y * gridDim.x;
-    const uint64_t base = block * ROW_BLOCK;
+    const uint64_t base = (block0 + blockIdx.x) * ROW_BLOCK;
     const uint64_t n_pos = P.n_rows * P.n_columns;
     const uint64_t pos0 = base / pieces.d;
     const uint32_t rem0 = (uint32_t)(base - pos0 * pieces.d);
@@ -127,13 +129,37 @@ __global__ __launch_bounds__(EMB_TPB) void embed_rows_kernel(Positions P, const 
 #pragma unroll
     for (uint32_t k = 0; k < ROW_PIECES; k++) {
         if (pos0 + q[k] >= n_pos) continue;
+        if (tok[k] == NO_TOKEN) p[k] = Piece<T, VEC>{};
+        if (s != 1.0f)  // (the same for all: unscaled vectors are moved as they are)
 #pragma unroll
-        for (int i = 0; i < VEC; i++)
-            p[k].v[i] = tok[k] == NO_TOKEN ? (T)0.0f : (T)((float)p[k].v[i] * s);
+            for (int i = 0; i < VEC; i++) p[k].v[i] = (T)((float)p[k].v[i] * s);
         T *to = out + (pos0 + q[k]) * dim + cell[k];
-        if (past) stream_piece<T, VEC>(to, p[k]);
+        if constexpr (PAST) stream_piece<T, VEC>(to, p[k]);
         else store_piece<T, VEC>(to, p[k]);
     }
+}
+
+// Ids that come from memory while their vectors are written past the caches wait behind
+// those writes, and what is written waits for them. So they are read into the last-level
+// cache first, a part of the rows at a time that it holds (TOUCH_BYTES of ids): 1.28 GB out
+// take 470 -> 320 us as float32 vectors of 32 bytes, 309 -> 236 of 128, 300 -> 234 as
+// bfloat16 of 256.
+constexpr uint64_t TOUCH_BYTES = 160ull << 20;
+
+__global__ __launch_bounds__(256) void touch_kernel(const uint8_t *p, uint64_t pieces) {
+    uint32_t x = 0;
+    const uint64_t step = gridDim.x * 256ull;
+    uint64_t i = blockIdx.x * 256ull + threadIdx.x;
+    for (; i + 3 * step < pieces; i += 4 * step) {
+        Piece<uint32_t, 4> q[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            q[k] = load_piece<uint32_t, 4>(reinterpret_cast<const uint32_t *>(p + 16 * (i + k * step)));
+#pragma unroll
+        for (int k = 0; k < 4; k++) x ^= q[k].v[0] ^ q[k].v[1] ^ q[k].v[2] ^ q[k].v[3];
+    }
+    for (; i < pieces; i += step) x ^= *reinterpret_cast<const uint32_t *>(p + 16 * i);
+    asm volatile("" ::"v"(x));  // (the loads' only use)
 }
 
 // ------------------------------------------------------------------- summed
@@ -1116,15 +1142,32 @@ void launch_embed(const fbh_embed *e, const void *table, void *out, hipStream_t 
     auto *to = static_cast<T *>(out);
     const float sc = scale_of(e);
     if (!e->pooled) {
-        const uint64_t blocks =
-            (P.n_rows * P.n_columns * pieces + ROW_BLOCK - 1) / ROW_BLOCK;
-        const uint32_t bx = (uint32_t)std::min<uint64_t>(blocks, 1u << 22);
-        const uint64_t by = (blocks + bx - 1) / bx;
-        head_input(by <= 65535, "too many cells");
-        hipLaunchKernelGGL((embed_rows_kernel<T, VEC, ID, DROP>), dim3(bx, (uint32_t)by),
-                           dim3(EMB_TPB), 0, s, P, tab, to, e->dim, divisor(pieces),
-                           divisor(P.n_columns), sc,
-                           P.n_rows * P.n_columns * e->dim * sizeof(T) >= STREAM_BYTES);
+        const uint64_t n_pos = P.n_rows * P.n_columns, vector = e->dim * sizeof(T);
+        const uint64_t id_bytes = ID == FBH_ID_I64 ? 8 : 4;
+        const bool past = VEC * sizeof(T) == 16 && n_pos * vector >= STREAM_BYTES;
+        // (workgroups' positions: parts of the call start at a workgroup's first piece)
+        const uint64_t all = (n_pos * pieces + ROW_BLOCK - 1) / ROW_BLOCK;
+        const uint64_t most = past ? TOUCH_BYTES / id_bytes * pieces / ROW_BLOCK : 1ull << 22;
+        for (uint64_t b0 = 0; b0 < all; b0 += most) {
+            const uint64_t blocks = std::min(all - b0, most);
+            if (past) {
+                const uint64_t first = b0 * ROW_BLOCK / pieces * id_bytes;
+                const uint64_t end =
+                    std::min((b0 + blocks) * ROW_BLOCK / pieces + 1, n_pos) * id_bytes;
+                hipLaunchKernelGGL(touch_kernel, dim3(2048), dim3(256), 0, s,
+                                   static_cast<const uint8_t *>(P.ids) + first, (end - first) / 16);
+            }
+            const auto go = [&](auto past_caches) {
+                hipLaunchKernelGGL(
+                    (embed_rows_kernel<T, VEC, ID, DROP, decltype(past_caches)::value>),
+                    dim3((uint32_t)blocks), dim3(EMB_TPB), 0, s, P, tab, to, e->dim,
+                    divisor(pieces), divisor(P.n_columns), sc, b0);
+            };
+            if constexpr (VEC * sizeof(T) == 16) {
+                if (past) go(std::true_type{});
+                else go(std::false_type{});
+            } else go(std::false_type{});
+        }
     } else if (P.n_rows * pieces < 64 * EMB_TPB) {
         const uint32_t lg_g = std::max(std::min(lg_at_least(pieces), 6u), 4u);
         hipLaunchKernelGGL((embed_sum_few_kernel<T, VEC, ID, DROP>),

@@ -80,21 +80,18 @@ __device__ __forceinline__ void store_piece(T *p, const Piece<T, N> &r) {
 }
 
 // Outputs beyond what the caches keep for whoever reads them next are written past them:
-// 2M x 20 vectors of 32 bytes (1.28 GB out) take 196 us so, and 430 through the caches,
-// where the lines wait for their eviction. Smaller ones stay in the cache for the next
-// kernel.
+// 2M x 20 vectors of 32 bytes (1.28 GB out), their ids in the last-level cache, take 220 us
+// so, and 430 through the caches, where lines wait for their eviction. Smaller ones stay in
+// the cache for the next kernel.
 constexpr uint64_t STREAM_BYTES = 128ull << 20;
 template <class T, int N>
 __device__ __forceinline__ void stream_piece(T *p, const Piece<T, N> &r) {
-    if constexpr (sizeof(r) == 16) {
-        typedef uint32_t Words __attribute__((ext_vector_type(4)));
-        typedef Words Loose __attribute__((aligned(2)));
-        Words w;
-        __builtin_memcpy(&w, &r, 16);
-        __builtin_nontemporal_store(w, reinterpret_cast<Loose *>(p));
-    } else {
-        store_piece<T, N>(p, r);
-    }
+    static_assert(sizeof(r) == 16, "whole pieces");
+    typedef uint32_t Words __attribute__((ext_vector_type(4)));
+    typedef Words Loose __attribute__((aligned(2)));
+    Words w;
+    __builtin_memcpy(&w, &r, 16);
+    __builtin_nontemporal_store(w, reinterpret_cast<Loose *>(p));
 }
 
 // Buffer loads: 4-byte aligned pieces at byte offsets of up to 2^31 - 1 from an address
