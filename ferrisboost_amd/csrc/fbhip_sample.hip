@@ -196,8 +196,8 @@ constexpr uint32_t THREAD_MOST = 8;
 
 // Up to 8 classes: a thread a row, whose logits it holds; ranks and the weights before a
 // class from every pair of them. Bound by arithmetic: V exponentials and a logarithm of
-// doubles a row. (500k rows of 4: 17 us with a lane a class, where each row's options and
-// logarithm take a whole wave's instructions.)
+// doubles a row: 500k rows of 4 take 9 us, and 17 with a lane a class, where each row's
+// options and logarithm take a whole wave's instructions.
 template <class T, int V>
 __global__ __launch_bounds__(256) void sample_thread_kernel(const T *logits, Draw D) {
     const uint64_t row = blockIdx.x * 256ull + threadIdx.x;
@@ -331,7 +331,9 @@ constexpr uint32_t WAVE_MOST = 1024;
 // Up to 64 R classes: a wave a row, which lies in registers, R classes side by side a
 // lane. The cut's bin is found from a histogram in LDS; the bin's classes (with top-k of at
 // most 64, all up to the cut) then take a lane each. Four waves a workgroup, with nothing
-// in common: LDS operations of one wave complete in order.
+// in common: LDS operations of one wave complete in order. Bound by instructions, about a
+// thousand a row: 20k rows of 500, top 50, take 35 us (158 with bins and digits in LDS and a
+// row read four times).
 struct WaveShared {
     uint64_t wt[WAVE_BINS];
     uint32_t ct[WAVE_BINS];
@@ -1021,7 +1023,7 @@ __device__ __forceinline__ void draw_listed(SampleRow<T, TPB> &R, const Draw &D,
 // launches find what the row's own workgroup finds pass by pass, the largest logit, the
 // histogram of weights, and the tiles' sums with a list of the cut's bin; the row kernel
 // then begins at its last steps. (1 x 50000 bfloat16, top-p: 46 us in one workgroup, whose
-// one CU is bound by the exponentials of doubles.) Rows whose options do not take a
+// one CU is bound by the exponentials of doubles; 28 in four launches.) Rows whose options do not take a
 // histogram of weights (few classes by rank, or more than the row kernel lists) are left to
 // the row kernel altogether.
 constexpr uint32_t TILE_ROWS = 128;  // rows at most: 256 and more fill the device by themselves
@@ -1138,6 +1140,10 @@ __global__ __launch_bounds__(TILE_TPB) void tile_sums_kernel(const T *logits, Dr
     if (threadIdx.x == 0) W.tile_w[blockIdx.x] = w;
 }
 
+// More classes: a row a workgroup. 256 x 131071 bfloat16, top 200, take 44 us: two passes
+// over 67 MB (12 us each, one row a CU) and the list's ranks and sums; by weight alone 148,
+// bound by two exponentials of doubles a class.
+//
 // TILED: rows whose passes the tiles' launches have done take their results.
 template <class T, int TPB, bool TILED>
 __global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D,
