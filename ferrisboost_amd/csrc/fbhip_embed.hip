@@ -328,7 +328,31 @@ struct SortFrom {
     uint32_t n;       // positions
     uint32_t shift, bits;
     uint32_t per_row; // pooled: the columns of a row, whose positions share its gradient
+    uint32_t blocks;
+    // The table's zeros, for the tokens without a position: a third beside each launch of
+    // the first pass (the blocks behind its own), which leave most of the device idle.
+    // (32768 positions, a table of 102 MB: 17 us by themselves.)
+    uint8_t *zeros;
+    uint64_t zero_bytes;
 };
+
+constexpr uint32_t ZERO_BLOCKS = 1024;
+
+// Part `part` of three of the zeros, by ZERO_BLOCKS workgroups: 16-byte pieces, and what is
+// left before and behind them in bytes.
+__device__ __forceinline__ void zero_part(const SortFrom &S, uint32_t part, uint32_t block) {
+    const uint64_t each = (S.zero_bytes / 3 + 15) & ~15ull, from = min(part * each, S.zero_bytes);
+    uint8_t *p = S.zeros + from;
+    const uint64_t bytes = part == 2 ? S.zero_bytes - from : min(each, S.zero_bytes - from);
+    const uint64_t head = min(bytes, (uint64_t)(-(intptr_t)p & 15));
+    const uint64_t pieces = (bytes - head) / 16;
+    const uint64_t at = block * (uint64_t)SORT_TPB + threadIdx.x,
+                   step = ZERO_BLOCKS * (uint64_t)SORT_TPB;
+    for (uint64_t i = at; i < pieces; i += step)
+        *reinterpret_cast<uint4 *>(p + head + 16 * i) = make_uint4(0, 0, 0, 0);
+    if (at < head) p[at] = 0;
+    if (at < bytes - head - 16 * pieces) p[head + 16 * pieces + at] = 0;
+}
 
 template <int ID, bool DROP, bool FIRST>
 __device__ __forceinline__ uint32_t sort_key(const Positions &P, const SortFrom &S, uint32_t i) {
@@ -341,6 +365,7 @@ __device__ __forceinline__ uint32_t sort_key(const Positions &P, const SortFrom 
 template <int ID, bool DROP, bool FIRST, uint32_t ROUNDS>
 __global__ __launch_bounds__(SORT_TPB) void sort_count_kernel(Positions P, SortFrom S,
                                                               uint32_t *counts) {
+    if (blockIdx.x >= S.blocks) return zero_part(S, 0, blockIdx.x - S.blocks);
     __shared__ uint32_t c[256];
     c[threadIdx.x] = 0;
     __syncthreads();
@@ -352,7 +377,7 @@ __global__ __launch_bounds__(SORT_TPB) void sort_count_kernel(Positions P, SortF
             atomicAdd(&c[(sort_key<ID, DROP, FIRST>(P, S, i) >> S.shift) & mask], 1u);
     }
     __syncthreads();
-    if (threadIdx.x <= mask) counts[(uint64_t)threadIdx.x * gridDim.x + blockIdx.x] = c[threadIdx.x];
+    if (threadIdx.x <= mask) counts[(uint64_t)threadIdx.x * S.blocks + blockIdx.x] = c[threadIdx.x];
 }
 
 // The lanes that are `in` with this lane's digit.
@@ -381,8 +406,10 @@ __device__ __forceinline__ uint32_t take_places(uint32_t *counter, bool in, uint
 }
 
 // A digit's counts to the positions before them in its own part; its total.
-__global__ __launch_bounds__(SORT_TPB) void sort_scan_kernel(uint32_t *counts, uint32_t blocks,
+__global__ __launch_bounds__(SORT_TPB) void sort_scan_kernel(SortFrom S, uint32_t *counts,
                                                              uint32_t *totals) {
+    if (blockIdx.x >> S.bits) return zero_part(S, 1, blockIdx.x - (1u << S.bits));
+    const uint32_t blocks = S.blocks;
     __shared__ uint32_t wave[SORT_WAVES];
     uint32_t *mine = counts + (uint64_t)blockIdx.x * blocks;
     uint32_t before = 0;
@@ -415,6 +442,7 @@ __global__ __launch_bounds__(SORT_TPB) void sort_scatter_kernel(Positions P, Sor
                                                                 const uint32_t *counts,
                                                                 const uint32_t *totals,
                                                                 uint32_t *keys, uint32_t *vals) {
+    if (blockIdx.x >= S.blocks) return zero_part(S, 2, blockIdx.x - S.blocks);
     __shared__ uint32_t base[256];
     __shared__ uint32_t seen[SORT_WAVES][256];
     __shared__ uint32_t wave_sum[SORT_WAVES];
@@ -433,7 +461,7 @@ __global__ __launch_bounds__(SORT_TPB) void sort_scatter_kernel(Positions P, Sor
         for (uint32_t k = 0; k < w; k++) add += wave_sum[k];
         if (threadIdx.x <= mask)
             base[threadIdx.x] =
-                add + x - v + counts[(uint64_t)threadIdx.x * gridDim.x + blockIdx.x];
+                add + x - v + counts[(uint64_t)threadIdx.x * S.blocks + blockIdx.x];
     }
     const uint32_t first = (blockIdx.x * SORT_WAVES + w) * (ROUNDS * 64) + lane;
     uint32_t key[ROUNDS], rank[ROUNDS];
@@ -471,9 +499,8 @@ __global__ __launch_bounds__(SORT_TPB) void sort_scatter_kernel(Positions P, Sor
 
 // ---- Up to 64k positions: one radix pass, of the tokens' high bits and with one position a
 // thread so that its launches are short, parts them into buckets; then each bucket is
-// sorted in a workgroup, which also writes the zeros of the bucket's tokens that have no
-// position, so the table needs no pass of its own. (32768 positions, 50000 tokens of 2 KB:
-// two passes of 16 positions a thread and a pass of zeros took 75 us; workgroups that each
+// sorted in a workgroup. (32768 positions, 50000 tokens of 2 KB: two passes of 16 positions
+// a thread and a pass of zeros took 75 us; workgroups that each
 // look for their own tokens among all positions 39; workgroups that count all positions
 // and place 1024 of them, instead of the pass' three launches, 39 alone.)
 constexpr uint32_t FEW_MOST = 65536;     // positions
@@ -487,8 +514,6 @@ struct Few {
     const uint32_t *totals;      // of the buckets
     const uint32_t *part_keys, *part_vals;
     uint32_t *keys, *vals;
-    uint8_t *table;
-    uint32_t row_bytes;
 };
 
 // The sum of the values of lower threads; *all gets the sum of all.
@@ -527,7 +552,14 @@ __global__ __launch_bounds__(FEW_TPB) void few_sort_kernel(Few F) {
     // a wave's positions, side by side
     const uint32_t each = ((end - first + FEW_TPB - 1) / FEW_TPB) * 64;
     const uint32_t i0 = first + w * each, i1 = min(i0 + each, end);
-    for (uint32_t i = i0 + lane; i < i1; i += 64) atomicAdd(&mine[F.part_keys[i] - t0], 1u);
+    for (uint32_t i = i0 + lane; i < i1; i += 8 * 64) {
+        uint32_t key[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8; j++) key[j] = F.part_keys[min(i + 64 * j, i1 - 1)];
+#pragma unroll
+        for (uint32_t j = 0; j < 8; j++)
+            if (i + 64 * j < i1) atomicAdd(&mine[key[j] - t0], 1u);
+    }
     __syncthreads();
     uint32_t c[2] = {0, 0}, all;
     for (uint32_t j = 0; j < 2; j++)
@@ -546,46 +578,26 @@ __global__ __launch_bounds__(FEW_TPB) void few_sort_kernel(Few F) {
             at += c[j];
         }
     __syncthreads();
-    // zeros where a token's first place is the next one's, in pieces of 16 bytes (the last
-    // one of a row over the one before) or, for narrower rows, of 2
-    const uint32_t piece = F.row_bytes < 16 ? 2 : 16, pieces = (F.row_bytes + piece - 1) / piece;
-    const uint32_t lg = pieces >= 64 ? 6 : 32 - __clz(max(pieces, 2u) - 1);  // lanes a row
-    const uint32_t row0 = threadIdx.x >> lg, lane0 = threadIdx.x & ((1u << lg) - 1);
-#pragma unroll 4
-    for (uint32_t t = row0; t < range; t += FEW_TPB >> lg) {
-        if (t0 + t == F.n_tokens || seen[t] != (t + 1 < range ? seen[t + 1] : end)) continue;
-        uint8_t *row = F.table + (uint64_t)(t0 + t) * F.row_bytes;
-        for (uint32_t i = lane0; i < pieces; i += 1u << lg) {
-            if (piece == 2) {
-                reinterpret_cast<uint16_t *>(row)[i] = 0;
-            } else {
-                Piece<uint16_t, 8> o = {};
-                store_piece<uint16_t, 8>(
-                    reinterpret_cast<uint16_t *>(row + min(16 * i, F.row_bytes - 16)), o);
+    for (uint32_t i = i0; i < i1; i += 8 * 64) {
+        uint32_t key[8], val[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8; j++) {
+            const uint32_t at = min(i + 64 * j + lane, i1 - 1);
+            key[j] = F.part_keys[at];
+            val[j] = F.part_vals[at];
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 8; j++) {
+            if (i + 64 * j >= i1) break;  // (the same for all lanes)
+            const bool in = i + 64 * j + lane < i1;
+            const uint32_t off = key[j] - t0;
+            const uint32_t to = take_places(&mine[off], in, same_digit(in, off, F.shift));
+            if (in) {
+                F.keys[to] = key[j];
+                F.vals[to] = val[j];
             }
         }
     }
-    __syncthreads();  // (the places are read above and moved below)
-    for (uint32_t i = i0; i < i1; i += 64) {
-        const bool in = i + lane < i1;
-        const uint32_t key = in ? F.part_keys[i + lane] : t0, off = key - t0;
-        const uint32_t to = take_places(&mine[off], in, same_digit(in, off, F.shift));
-        if (in) {
-            F.keys[to] = key;
-            F.vals[to] = F.part_vals[i + lane];
-        }
-    }
-}
-
-// 16-byte pieces of zeros, and the rest in bytes.
-__global__ __launch_bounds__(256) void zero_kernel(uint8_t *p, uint64_t bytes) {
-    const uint64_t head = min(bytes, (uint64_t)(-(intptr_t)p & 15));
-    const uint64_t pieces = (bytes - head) / 16;
-    const uint64_t at = blockIdx.x * 256ull + threadIdx.x, step = gridDim.x * 256ull;
-    for (uint64_t i = at; i < pieces; i += step)
-        *reinterpret_cast<uint4 *>(p + head + 16 * i) = make_uint4(0, 0, 0, 0);
-    if (at < head) p[at] = 0;
-    if (at < bytes - head - 16 * pieces) p[head + 16 * pieces + at] = 0;
 }
 
 struct Runs {
@@ -1156,7 +1168,8 @@ void launch_embed(const fbh_embed *e, const void *table, void *out, hipStream_t 
         const bool past = VEC * sizeof(T) == 16 && n_pos * vector >= STREAM_BYTES;
         // (workgroups' positions: parts of the call start at a workgroup's first piece)
         const uint64_t all = (n_pos * pieces + ROW_BLOCK - 1) / ROW_BLOCK;
-        const uint64_t most = past ? TOUCH_BYTES / id_bytes * pieces / ROW_BLOCK : 1ull << 22;
+        const uint64_t most = std::min<uint64_t>(
+            past ? TOUCH_BYTES / id_bytes * pieces / ROW_BLOCK : ~0ull, 1u << 22);
         for (uint64_t b0 = 0; b0 < all; b0 += most) {
             const uint64_t blocks = std::min(all - b0, most);
             if (past) {
@@ -1409,30 +1422,25 @@ void embed_grad(const fbh_embed *e, const void *grad, void *table, void *work, h
     const GradPlan G = grad_plan(e);
     auto *w = static_cast<uint8_t *>(work);
     const auto list = [&](uint64_t at) { return reinterpret_cast<uint32_t *>(w + at); };
-    const uint32_t row_bytes = e->dim * (e->dtype == FBH_F32 ? 4 : 2);
-    if (!G.few || G.n == 0) {
-        const uint64_t bytes = (uint64_t)e->n_tokens * row_bytes;
-        hipLaunchKernelGGL(zero_kernel,
-                           dim3((uint32_t)std::min<uint64_t>((bytes + 4095) / 4096, 4096)),
-                           dim3(256), 0, s, static_cast<uint8_t *>(table), bytes);
-        head_check(hipGetLastError(), "table gradient");
-        if (G.n == 0) return;
-    }
+    const uint64_t zero_bytes =
+        (uint64_t)e->n_tokens * e->dim * (e->dtype == FBH_F32 ? 4 : 2);
     uint32_t *counts = list(G.counts), *totals = list(G.totals);
     for (uint32_t pass = 0; pass < G.passes; pass++) {
         const uint32_t to = pass & 1;
         const SortFrom S{list(G.keys[1 - to]), list(G.vals[1 - to]), G.n,
-                         G.few ? G.shift : pass * G.bits, G.bits, e->pooled ? e->n_columns : 1};
+                         G.few ? G.shift : pass * G.bits, G.bits, e->pooled ? e->n_columns : 1,
+                         G.blocks, static_cast<uint8_t *>(table), zero_bytes};
+        const uint32_t more = pass == 0 ? ZERO_BLOCKS : 0;
         uint32_t *keys = list(G.keys[to]), *vals = list(G.vals[to]);
         const auto go = [&](auto id, auto drop, auto first, auto rounds) {
             constexpr int ID = decltype(id)::value;
             constexpr bool DROP = decltype(drop)::value, FIRST = decltype(first)::value;
             constexpr uint32_t ROUNDS = decltype(rounds)::value;
-            hipLaunchKernelGGL((sort_count_kernel<ID, DROP, FIRST, ROUNDS>), dim3(G.blocks),
+            hipLaunchKernelGGL((sort_count_kernel<ID, DROP, FIRST, ROUNDS>), dim3(G.blocks + more),
                                dim3(SORT_TPB), 0, s, P, S, counts);
-            hipLaunchKernelGGL(sort_scan_kernel, dim3(1u << G.bits), dim3(SORT_TPB), 0, s, counts,
-                               G.blocks, totals);
-            hipLaunchKernelGGL((sort_scatter_kernel<ID, DROP, FIRST, ROUNDS>), dim3(G.blocks),
+            hipLaunchKernelGGL(sort_scan_kernel, dim3((1u << G.bits) + more), dim3(SORT_TPB), 0, s,
+                               S, counts, totals);
+            hipLaunchKernelGGL((sort_scatter_kernel<ID, DROP, FIRST, ROUNDS>), dim3(G.blocks + more),
                                dim3(SORT_TPB), 0, s, P, S, counts, totals, keys, vals);
         };
         if (pass == 0)
@@ -1442,10 +1450,11 @@ void embed_grad(const fbh_embed *e, const void *grad, void *table, void *work, h
             });
         else go(Int<FBH_ID_I32>{}, std::false_type{}, std::false_type{}, Int<SORT_ROUNDS>{});
         head_check(hipGetLastError(), "token sort");
+        if (G.n == 0) return;  // (the table's zeros were all)
     }
     if (G.few) {
         const Few F{e->n_tokens, G.shift, totals, list(G.keys[0]), list(G.vals[0]),
-                    list(G.keys[1]), list(G.vals[1]), static_cast<uint8_t *>(table), row_bytes};
+                    list(G.keys[1]), list(G.vals[1])};
         hipLaunchKernelGGL(few_sort_kernel, dim3((e->n_tokens >> G.shift) + 1), dim3(FEW_TPB),
                            (FEW_WAVES * 4) << G.shift, s, F);
         head_check(hipGetLastError(), "token sort");

@@ -411,6 +411,9 @@ def test_empty_calls(heads):
     assert heads.embed(table, ids, voc, pooled=True).shape == (0, 5)
     assert heads.embed(table, ids, voc).shape == (0, 2, 5)
     assert (heads.embed_grad(torch.ones(0, 5, device="cuda"), ids, voc, pooled=True) == 0).all()
+    for v in (3, 300_000):  # one vocabulary, in one pass and in several
+        g = heads.embed_grad(torch.ones(0, 5, device="cuda"), ids[:, 0], v)
+        assert g.shape == (v, 5) and (g == 0).all()
     none = torch.zeros(3, 0, dtype=torch.int64, device="cuda")
     assert (heads.embed(table, none, pooled=True) == 0).all()
     assert (heads.embed_grad(torch.ones(3, 5, device="cuda"), none, 7, pooled=True) == 0).all()
