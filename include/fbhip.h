@@ -718,12 +718,13 @@ int fbh_shap_contribs_noalloc(fbh_shap_model *m, const float *rows, uint64_t n_r
  * the model has given them: vectors learned for the ids, dropout while they are
  * learned, classes drawn from the margins. No reference counterpart.
  *
- * All pointers are device memory of `device` unless a comment says host, tensors
- * are dense and row-major, and any alignment of their cells' size does. Calls
- * are enqueued on `stream` (a hipStream_t; NULL: the default stream), do not
- * wait, allocate nothing and can be captured into a graph; the caller's current
- * device is the same afterwards. Results are the same in every call. Whatever a
- * call reads must stay unchanged until the stream has passed it. */
+ * Pointers are device memory of `device` unless a comment says host; the structs
+ * themselves are the caller's, read during the call. Tensors are dense and
+ * row-major, and any alignment of their cells' size does. Calls are enqueued on
+ * `stream` (a hipStream_t; NULL: the default stream), do not wait, allocate
+ * nothing and can be captured into a graph; the caller's current device is the
+ * same afterwards. Results are the same in every call. Whatever a call reads must
+ * stay unchanged until the stream has passed it. */
 
 /* Cell types of tables, vectors and logits; types of ids. */
 enum { FBH_F32 = 0, FBH_F16 = 1, FBH_BF16 = 2 };

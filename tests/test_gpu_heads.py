@@ -404,6 +404,32 @@ def test_captured_calls_with_much_lds(heads):
         assert torch.equal(g, heads.embed_grad(grad, ids, voc))
 
 
+def test_captured_large_calls(heads):
+    """Calls of several launches that hand counters and lists to one another."""
+    rng = np.random.default_rng(10)
+    flat = torch.from_numpy(rng.integers(0, 3000, 70_000)).cuda()
+    few = torch.from_numpy(rng.integers(0, 5000, 3000)).cuda()
+    grad = _cells(rng, (70_000, 12), "f32")
+    x = _cells(rng, (3, 40_000), "bf16") * 3
+    u = torch.rand(3, device="cuda")
+
+    def step():
+        return (heads.embed_grad(grad, flat, 3000), heads.embed_grad(grad[:3000], few, 5000),
+                *heads.sample(x, u, top_p=0.9), *heads.sample(x, u))
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(4):
+        flat.random_(0, 3000)
+        few.random_(-1, 5000)
+        x.normal_()
+        u.uniform_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
 def test_empty_calls(heads):
     voc = heads.Vocabulary([3, 4])
     table = torch.ones(7, 5, device="cuda")

@@ -3,6 +3,9 @@
 from __future__ import annotations
 
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -103,3 +106,19 @@ def test_sampling_options(bad):
     with pytest.raises(ValueError, match=next(iter(bad))):
         heads.check_options(**{**{"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0},
                                **bad})
+
+
+def test_torch_after_the_first_call_is_refused():
+    """The package's library has loaded the system's HIP runtime by then, and torch brings
+    its own: pointers of one mean nothing to the other."""
+    code = ("from ferrisboost_amd import _native as N, heads\n"
+            "N.hip()\n"
+            "try:\n"
+            "    heads.Vocabulary([1])\n"
+            "except RuntimeError as e:\n"
+            "    print('refused:', e)\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True,
+                         timeout=300)
+    assert "refused:" in out.stdout and "import torch first" in out.stdout, (out.stdout,
+                                                                            out.stderr[-500:])
