@@ -113,4 +113,25 @@ inline SketchSlots sketch_slots_most(uint64_t m, uint32_t n, uint64_t limit) {
     return s;
 }
 
+// ---- The launches of a sampling call (fbhip_sample.hip). A launch has fewer than 2^32
+// threads, so calls of many rows take several. Few rows of many classes are taken tile by
+// tile, through a workspace of the call's own: that is decided of the whole call, as its
+// workspace is, and never of a launch (the last one of 2^21 + 5 rows has 5 rows and no
+// workspace).
+constexpr uint64_t SAMPLE_LAUNCH = 1u << 21;   // rows of a launch at most
+constexpr uint32_t SAMPLE_TILE_ROWS = 128;     // 256 and more fill the device by themselves
+constexpr uint32_t SAMPLE_TILE_CLASSES = 16384;
+
+// Rows whose tiles' results a call's workspace holds.
+inline uint64_t sample_tiled_rows(uint64_t n_rows, uint32_t n_classes) {
+    return n_rows <= SAMPLE_TILE_ROWS && n_classes > SAMPLE_TILE_CLASSES ? n_rows : 0;
+}
+// f(first row, rows, whether they have a workspace) for every launch.
+template <class F>
+void sample_launches(uint64_t n_rows, uint32_t n_classes, F &&f) {
+    const bool tiled = sample_tiled_rows(n_rows, n_classes) > 0;
+    for (uint64_t r = 0; r < n_rows; r += SAMPLE_LAUNCH)
+        f(r, std::min<uint64_t>(n_rows - r, SAMPLE_LAUNCH), tiled);
+}
+
 }  // namespace fbh

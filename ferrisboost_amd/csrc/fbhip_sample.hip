@@ -1043,7 +1043,6 @@ __device__ __forceinline__ void draw_listed(SampleRow<T, TPB> &R, const Draw &D,
 // one CU is bound by the exponentials of doubles; 28 in four launches.) Rows whose options do not take a
 // histogram of weights (few classes by rank, or more than the row kernel lists) are left to
 // the row kernel altogether.
-constexpr uint32_t TILE_ROWS = 128;  // rows at most: 256 and more fill the device by themselves
 constexpr uint32_t TILE_TPB = 1024;
 constexpr uint32_t TILE_BINS = 1024;
 constexpr uint32_t TILE_LIST = 2048;
@@ -1413,34 +1412,14 @@ __global__ __launch_bounds__(TPB) void sample_row_kernel(const T *logits, Draw D
     }
 }
 
-constexpr uint64_t SAMPLE_LAUNCH = 1u << 21;  // rows of a launch at most
-
-// Whether a call's rows may be taken tile by tile.
-bool sample_tiled(uint64_t n_rows, uint32_t n_classes) {
-    return n_rows <= TILE_ROWS && n_classes > 16384;
-}
 uint64_t sample_bytes(uint64_t n_rows, uint32_t n_classes) {
-    return sample_tiled(n_rows, n_classes) ? n_rows * sizeof(TileWork) : 0;
+    return sample_tiled_rows(n_rows, n_classes) * sizeof(TileWork);
 }
 
+// One launch's rows; work is NULL where the call has no workspace.
 template <class T>
 void launch_sample(const void *logits, const Draw &D, TileWork *work, hipStream_t s) {
     const uint32_t v = D.n_classes;
-    if (D.n_rows > SAMPLE_LAUNCH) {  // (a launch has fewer than 2^32 threads)
-        for (uint64_t r = 0; r < D.n_rows; r += SAMPLE_LAUNCH) {
-            Draw d = D;
-            d.n_rows = std::min<uint64_t>(D.n_rows - r, SAMPLE_LAUNCH);
-            d.uniforms += r;
-            d.classes += r;
-            if (d.log_probs) d.log_probs += r;
-            if (d.o.temperatures) d.o.temperatures += r;
-            if (d.o.top_ks) d.o.top_ks += r;
-            if (d.o.top_ps) d.o.top_ps += r;
-            if (d.o.min_ps) d.o.min_ps += r;
-            launch_sample<T>(static_cast<const T *>(logits) + r * v, d, nullptr, s);
-        }
-        return;
-    }
     const auto *l = static_cast<const T *>(logits);
     const uint64_t n = D.n_rows;
     if (v <= THREAD_MOST) {
@@ -1468,10 +1447,10 @@ void launch_sample(const void *logits, const Draw &D, TileWork *work, hipStream_
         else hipLaunchKernelGGL((sample_wave_kernel<T, 16>), grid, tpb, 0, s, l, D);
     } else {
         const dim3 grid((uint32_t)n);
-        if (v <= 16384)
+        if (v <= SAMPLE_TILE_CLASSES)
             hipLaunchKernelGGL((sample_row_kernel<T, 256, false>), grid, dim3(256), 0, s, l, D,
                                nullptr);
-        else if (!sample_tiled(D.n_rows, v) || (!D.own && D.all.k < v))
+        else if (!work || (!D.own && D.all.k < v))
             hipLaunchKernelGGL((sample_row_kernel<T, 1024, false>), grid, dim3(1024), 0, s, l, D,
                                nullptr);
         else {
@@ -1490,10 +1469,23 @@ void launch_sample(const void *logits, const Draw &D, TileWork *work, hipStream_
 }
 
 void sample(const void *logits, uint32_t dtype, const Draw &D, void *work, hipStream_t s) {
-    auto *w = static_cast<TileWork *>(work);
-    if (dtype == FBH_F32) launch_sample<float>(logits, D, w, s);
-    else if (dtype == FBH_F16) launch_sample<_Float16>(logits, D, w, s);
-    else launch_sample<__bf16>(logits, D, w, s);
+    const uint64_t row_bytes = (uint64_t)D.n_classes * (dtype == FBH_F32 ? 4 : 2);
+    sample_launches(D.n_rows, D.n_classes, [&](uint64_t r, uint64_t rows, bool tiled) {
+        Draw d = D;
+        d.n_rows = rows;
+        d.uniforms += r;
+        d.classes += r;
+        if (d.log_probs) d.log_probs += r;
+        if (d.o.temperatures) d.o.temperatures += r;
+        if (d.o.top_ks) d.o.top_ks += r;
+        if (d.o.top_ps) d.o.top_ps += r;
+        if (d.o.min_ps) d.o.min_ps += r;
+        const auto *from = static_cast<const uint8_t *>(logits) + r * row_bytes;
+        auto *w = tiled ? static_cast<TileWork *>(work) : nullptr;
+        if (dtype == FBH_F32) launch_sample<float>(from, d, w, s);
+        else if (dtype == FBH_F16) launch_sample<_Float16>(from, d, w, s);
+        else launch_sample<__bf16>(from, d, w, s);
+    });
 }
 
 Draw draw_of(const float *uniforms, const fbh_sample_options *o, int64_t *classes,
