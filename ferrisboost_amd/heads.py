@@ -128,7 +128,6 @@ class Vocabulary:
         self.first = torch.from_numpy(first.astype(np.int32)).to(device)
         if self.first.device.type != "cuda":
             raise ValueError(f"device must be a GPU, got {device!r}")
-        self.address = self.first.data_ptr()
 
     def __repr__(self):
         return (f"Vocabulary({self.n_columns} columns, {self.n_tokens} tokens, "
@@ -156,7 +155,9 @@ def _positions(ids, vocabulary, pooled: bool, n_tokens: int, dim: int, cells: in
             n_rows *= s
     else:
         n_rows, columns = ids.numel(), 1
-    first, most = (0, 0) if vocabulary is None else (vocabulary.address, vocabulary.most_ids)
+    # (the address that the tensor has now: a copied or unpickled vocabulary has one of its own)
+    first, most = (0, 0) if vocabulary is None else (vocabulary.first.data_ptr(),
+                                                     vocabulary.most_ids)
     # (a call without columns or positions launches nothing)
     e = _EMBED.pack(n_rows, columns, dim, n_tokens, code, cells, pooled, ids.data_ptr(), first,
                     drop, seed, scale, most) if columns else None

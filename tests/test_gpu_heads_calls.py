@@ -4,6 +4,10 @@ Tolerances are those of tests/test_gpu_heads.py unless a test says otherwise."""
 
 from __future__ import annotations
 
+import copy
+import io
+import pickle
+
 import numpy as np
 import pytest
 import torch
@@ -40,3 +44,28 @@ def test_few_rows_of_many_classes_behind_a_full_launch(heads):
         got = lp[-tail:].cpu().numpy().astype(np.float64)
         assert (np.abs(got - want_lp) <= np.abs(want_lp) * 2.0 ** -24 + 2.0 ** -45).all()
         assert (c[:-tail] == -1).all() and (lp[:-tail] == float("-inf")).all()
+
+
+def test_copied_and_stored_vocabularies(heads):
+    """A copy has a tensor of its own, which the kernels read also when the first one's
+    memory holds something else."""
+    rng = np.random.default_rng(2)
+    voc = heads.Vocabulary([9, 4, 30])
+    table = torch.randn(43, 12, device="cuda")
+    ids = torch.from_numpy(rng.integers(-1, 30, (700, 3))).cuda()
+    want = heads.embed(table, ids, voc, pooled=True)
+    grad = heads.embed_grad(want, ids, voc, pooled=True)
+    stored = io.BytesIO()
+    torch.save({"vocabulary": voc}, stored)
+    stored.seek(0)
+    copies = [copy.deepcopy(voc), pickle.loads(pickle.dumps(voc)),
+              torch.load(stored, weights_only=False)["vocabulary"], copy.copy(voc)]
+    for c in copies[:3]:
+        assert c.first.data_ptr() != voc.first.data_ptr()
+    first, voc = voc.first, None
+    first.zero_()
+    for c in copies[:3]:
+        assert torch.equal(heads.embed(table, ids, c, pooled=True), want)
+        assert torch.equal(heads.embed_grad(want, ids, c, pooled=True), grad)
+    first.copy_(copies[0].first)
+    assert torch.equal(heads.embed(table, ids, copies[3], pooled=True), want)

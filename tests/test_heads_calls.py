@@ -3,6 +3,13 @@ as far as they need no device."""
 
 from __future__ import annotations
 
+import copy
+import pickle
+
+import numpy as np
+import torch
+
+from ferrisboost_amd import heads
 from test_host_rules import run_cpp
 
 
@@ -26,3 +33,22 @@ def test_a_sampling_call_keeps_to_its_workspace(tmp_path):
             });
             CHECK(next == n);
         }""")
+
+
+def _vocabulary(sizes):
+    """A vocabulary in host memory, for what happens before a device is asked for."""
+    voc = object.__new__(heads.Vocabulary)
+    first = np.concatenate([[0], np.cumsum(sizes)])
+    voc.sizes, voc.n_tokens, voc.n_columns = np.asarray(sizes), int(first[-1]), len(sizes)
+    voc.most_ids, voc.first = max(sizes), torch.from_numpy(first.astype(np.int32))
+    return voc
+
+
+def test_a_copied_vocabulary_gives_the_address_of_its_own_tensor():
+    heads._need_torch()
+    voc = _vocabulary([3, 4])
+    ids = torch.zeros((5, 2), dtype=torch.int32)
+    for v in (voc, copy.copy(voc), copy.deepcopy(voc), pickle.loads(pickle.dumps(voc)),
+              copy.deepcopy({"a": [voc]})["a"][0]):
+        e, lead = heads._positions(ids, v, True, 7, 8, 0, 1.0, 0.0, 0)
+        assert heads._EMBED.unpack(e)[8] == v.first.data_ptr() and lead == (5,)
