@@ -107,7 +107,9 @@ def _drop(drop) -> float:
 class Vocabulary:
     """The table rows of several columns' ids: column t's ids 0 .. sizes[t] - 1 are rows
     first[t] .. first[t] + sizes[t] - 1 of a table of n_tokens rows (a model's trees:
-    Model.leaf_vocabulary(); categorical columns: their numbers of codes)."""
+    Model.leaf_vocabulary(); categorical columns: their numbers of codes). It may be copied,
+    stored and used on any stream of its device; a captured graph reads it at every replay,
+    so it has to live as long as the graph does."""
 
     def __init__(self, sizes, device="cuda:0"):
         torch = _need_torch()
@@ -128,6 +130,18 @@ class Vocabulary:
         self.first = torch.from_numpy(first.astype(np.int32)).to(device)
         if self.first.device.type != "cuda":
             raise ValueError(f"device must be a GPU, got {device!r}")
+        self._streams = set()
+
+    def _used_on(self, stream: int):
+        """Keeps the offsets' memory from the allocator until the work now on this stream, the
+        current one, has passed, also when the vocabulary is dropped before."""
+        if stream not in self._streams:
+            self.first.record_stream(_torch.cuda.current_stream(self.first.device))
+            self._streams.add(stream)
+
+    def __getstate__(self):
+        # (a copy's tensor has not been used on any stream yet)
+        return {**self.__dict__, "_streams": set()}
 
     def __repr__(self):
         return (f"Vocabulary({self.n_columns} columns, {self.n_tokens} tokens, "
@@ -171,7 +185,10 @@ def _embed(table, ids, vocabulary, scale, pooled, drop, seed):
     if e is None:
         return out.zero_()
     dev = table.get_device()
-    rc = _L.fbh_embed_rows(dev, e, table.data_ptr(), out.data_ptr(), _raw_stream(dev))
+    stream = _raw_stream(dev)
+    if vocabulary is not None:
+        vocabulary._used_on(stream)
+    rc = _L.fbh_embed_rows(dev, e, table.data_ptr(), out.data_ptr(), stream)
     if rc:
         N.check_hip(rc)
     return out
@@ -260,8 +277,10 @@ def embed_grad(grad, ids, tokens, *, scale: float = 1.0, pooled: bool = False,
     dev = grad.get_device()
     size = _L.fbh_embed_grad_bytes(e)
     work = grad.new_empty(size, dtype=_torch.uint8)
-    rc = _L.fbh_embed_grad(dev, e, grad.data_ptr(), out.data_ptr(), work.data_ptr(), size,
-                           _raw_stream(dev))
+    stream = _raw_stream(dev)
+    if vocabulary is not None:
+        vocabulary._used_on(stream)
+    rc = _L.fbh_embed_grad(dev, e, grad.data_ptr(), out.data_ptr(), work.data_ptr(), size, stream)
     if rc:
         N.check_hip(rc)
     return out

@@ -69,3 +69,32 @@ def test_copied_and_stored_vocabularies(heads):
         assert torch.equal(heads.embed_grad(want, ids, c, pooled=True), grad)
     first.copy_(copies[0].first)
     assert torch.equal(heads.embed(table, ids, copies[3], pooled=True), want)
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_a_vocabulary_dropped_while_a_stream_still_reads_it(heads, backward):
+    """Its memory is not given out again before the stream has passed the call."""
+    voc = heads.Vocabulary([50, 60])
+    table = torch.randn(110, 8, device="cuda")
+    ids = torch.randint(0, 50, (4000, 2), device="cuda")
+    want = heads.embed(table, ids, voc, pooled=True)
+    if backward:
+        grad, want = want, heads.embed_grad(want, ids, voc, pooled=True)
+    a = torch.zeros(1 << 28, device="cuda")  # 1 GiB
+    b = torch.empty_like(a)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        for _ in range(200):  # some 80 ms
+            b.copy_(a)
+        got = (heads.embed_grad(grad, ids, voc, pooled=True) if backward
+               else heads.embed(table, ids, voc, pooled=True))
+        done = s.record_event()
+    at = voc.first.data_ptr()
+    del voc
+    others = [torch.zeros(3, dtype=torch.int32, device="cuda") for _ in range(64)]
+    assert not done.query()  # (else the rest says nothing)
+    assert at not in [o.data_ptr() for o in others]
+    s.synchronize()
+    assert torch.equal(got, want)
