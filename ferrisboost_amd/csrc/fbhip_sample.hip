@@ -30,8 +30,9 @@ constexpr uint64_t WEIGHT_ONE = 1ull << WEIGHT_BITS;
 
 // A row's options, as whole numbers.
 struct RowOptions {
-    double inv_t;       // 1 / temperature, 0: the largest logit
-    uint32_t k;         // classes that stay by rank
+    double inv_t;       // 1 / temperature; 0 where that is infinite, and where k is 1 for the
+                        // largest logit's sake
+    uint32_t k;         // classes that stay by rank (1 for the largest logit)
     uint32_t p31;       // top_p * 2^31
     uint64_t least;     // smallest weight that stays by min_p
     __host__ __device__ bool cuts(uint32_t n) const { return k < n || p31 < 1u << 31; }
@@ -215,9 +216,7 @@ __global__ __launch_bounds__(256) void sample_thread_kernel(const T *logits, Dra
     uint64_t w[V];
 #pragma unroll
     for (int i = 0; i < V; i++)
-        w[i] = l[i] == -INFINITY ? 0
-                                 : (O.inv_t == 0.0 ? (l[i] == most ? WEIGHT_ONE : 0)
-                                                   : S.weight(l[i]));
+        w[i] = l[i] == -INFINITY ? 0 : S.weight(l[i]);
     if (O.cuts(V)) {
         uint32_t rank[V];
         uint64_t all = 0;

@@ -368,7 +368,8 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     the row's uniform number; log_probs is the logarithm of its own share. temperature 0
     takes the largest logit. Each option is a number, or a tensor of one a row (float32;
     top_k int32), whose values the device reads: there 0 or less, and NaN, are
-    temperature 0, no top_k, top_p 0 (NaN: 1) and min_p 0.
+    temperature 0, no top_k, top_p 0 (NaN: 1) and min_p 0, and at an infinite temperature
+    all classes weigh the same.
 
     Logits of -inf or NaN are masked; a row with no others gets class -1 and -inf. At most
     262144 classes. Weights are held as whole numbers of 2^-45 of the largest one, so the

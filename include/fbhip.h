@@ -806,7 +806,9 @@ typedef struct {
  * the staying classes before it exceed the row's uniform number times the sum of
  * all that stay; log_probs[row] (may be NULL) the logarithm of its share of that
  * sum. temperature <= 0 or NaN takes the largest logit (the lowest class of equal
- * ones). Logits of minus infinity or NaN are masked; a row with nothing else
+ * ones); with an infinite one all classes but the masked weigh the same (next to a
+ * logit of plus infinity, finite ones weigh nothing at any temperature). Logits of
+ * minus infinity or NaN are masked; a row with nothing else
  * gets class -1 and minus infinity. top_p is taken to be in 0 .. 1 (0: the first
  * class; NaN: 1), min_p too (NaN: 0), the uniform number in 0 .. 1 - 2^-31. At
  * most 262144 classes. */

@@ -98,3 +98,45 @@ def test_a_vocabulary_dropped_while_a_stream_still_reads_it(heads, backward):
     assert at not in [o.data_ptr() for o in others]
     s.synchronize()
     assert torch.equal(got, want)
+
+
+def _sampled(got, want):
+    """Classes as they must be, log-probabilities to half a step."""
+    (c, lp), (want_c, want_p) = got, want
+    assert np.array_equal(c.cpu().numpy(), want_c)
+    none, got_p = want_c < 0, lp.cpu().numpy().astype(np.float64)
+    assert np.array_equal(got_p[none], want_p[none])
+    tol = np.abs(want_p[~none]) * 2.0 ** -24 + 2.0 ** -45
+    assert (np.abs(got_p[~none] - want_p[~none]) <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("v", [1, 2, 3, 4, 5, 6, 7, 8, 9, 40, 64, 90, 300, 1000, 3000, 20_000])
+def test_infinite_temperatures(heads, v, dtype):
+    """Rows of an infinite temperature beside others, whatever kernel takes them: all that
+    stays weighs the same, ranks still go by logit."""
+    rng = np.random.default_rng(v)
+    n = 40 if v <= 3000 else 8
+    x = torch.from_numpy((rng.normal(size=(n, v)) * 3).astype(np.float32)).to(dtype).cuda()
+    u = torch.from_numpy(rng.random(n).astype(np.float32)).cuda()
+    t = np.where(np.arange(n) % 4 == 3, np.float32(0.5), np.float32(np.inf))
+    k = rng.choice([0, 1, 2, max(1, v // 2), v], n).astype(np.int32)
+    p = rng.choice([0.0, 0.3, 0.9, 1.0], n).astype(np.float32)
+    d_t, d_k, d_p = (torch.from_numpy(o).cuda() for o in (t, k, p))
+    host = x.float().cpu().numpy()
+    for kw, opt in [({}, (t, 0, 1.0, 0.0)), ({"top_k": d_k}, (t, k, 1.0, 0.0)),
+                    ({"top_p": d_p}, (t, 0, p, 0.0)),
+                    ({"top_k": d_k, "top_p": d_p, "min_p": 1.0}, (t, k, p, 1.0))]:
+        _sampled(heads.sample(x, u, temperature=d_t, **kw),
+                 ref.sample(host, u.cpu().numpy(), *opt))
+    # masked classes stay masked: the same as equal logits at temperature 1
+    x[torch.from_numpy(rng.random((n, v)) < 0.3).cuda()] = float("-inf")
+    x[0] = float("-inf")
+    flat = np.where(x.float().cpu().numpy() == -np.inf, -np.inf, 0.0)
+    inf = torch.full((n,), float("inf"), device="cuda")
+    _sampled(heads.sample(x, u, temperature=inf),
+             ref.sample(flat, u.cpu().numpy(), 1.0, 0, 1.0, 0.0))
+    # and next to plus infinity, finite logits weigh nothing
+    x[:, v // 2] = float("inf")
+    _sampled(heads.sample(x, u, temperature=inf),
+             (np.full(n, v // 2), np.zeros(n)))
