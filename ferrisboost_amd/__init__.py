@@ -698,12 +698,7 @@ class Model:
             m = np.stack([np.zeros_like(m), m], axis=1)
         m = np.ascontiguousarray(m, np.float32)
         n, k = m.shape
-        u = np.ascontiguousarray(np.asarray(uniforms, dtype=np.float32))
-        if u.shape != (n,):
-            raise ValueError(f"uniforms must have one value for each of {n} rows, got shape "
-                             f"{u.shape}")
-        if not ((u >= 0.0) & (u < 1.0)).all():
-            raise ValueError("uniforms must be in [0, 1)")
+        u = np.ascontiguousarray(heads.check_uniforms(uniforms, n))
         o = N.SampleOptions()
         o.temperature, o.top_k, o.top_p, o.min_p = options
         classes = np.zeros(n, np.int64)

@@ -357,6 +357,20 @@ def _share(what: str, v) -> float:
     return v
 
 
+def check_uniforms(uniforms, n: int) -> np.ndarray:
+    """Uniform numbers of n rows as float32: what they were given as has to be in [0, 1), and
+    those that float32 rounds to 1 are the largest number below it."""
+    u = np.asarray(uniforms)
+    if u.dtype.kind != "f":
+        u = u.astype(np.float64)
+    if u.shape != (n,):
+        raise ValueError(f"uniforms must have one value for each of {n} rows, got shape "
+                         f"{u.shape}")
+    if not ((u >= 0.0) & (u < 1.0)).all():
+        raise ValueError("uniforms must be in [0, 1)")
+    return np.minimum(u.astype(np.float32), np.float32(1.0 - 2.0 ** -24))
+
+
 def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """One class for every row of `logits` (..., classes), from a uniform float32 number
     in [0, 1) a row: (classes int64, log_probs float32), each of shape (...).

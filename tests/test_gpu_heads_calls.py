@@ -140,3 +140,22 @@ def test_infinite_temperatures(heads, v, dtype):
     x[:, v // 2] = float("inf")
     _sampled(heads.sample(x, u, temperature=inf),
              (np.full(n, v // 2), np.zeros(n)))
+
+
+def test_a_model_takes_uniform_doubles(heads):
+    """Model.sample's default kind of uniform numbers: also ones that float32 rounds to 1."""
+    import ferrisboost_amd as fb
+    from helpers import product_params
+
+    rng = np.random.default_rng(3)
+    x = rng.normal(size=(2000, 4)).astype(np.float32)
+    m = fb.train(product_params({"objective": "multi:softprob", "num_class": 3, "max_depth": 3}),
+                 x, np.digitize(x[:, 0], [-0.5, 0.5]).astype(np.float32), num_boost_round=3)
+    u = rng.random(2000)
+    u[:3] = [1 - 2.0 ** -30, 1 - 2.0 ** -53, 0.0]
+    near = np.minimum(u.astype(np.float32), np.float32(1 - 2.0 ** -24))
+    assert np.array_equal(m.sample(x, u), m.sample(x, near))
+    assert m.sample(x, u)[0] == 2
+    u[5] = 1.0
+    with pytest.raises(ValueError, match="in \\[0, 1\\)"):
+        m.sample(x, u)

@@ -7,6 +7,7 @@ import copy
 import pickle
 
 import numpy as np
+import pytest
 import torch
 
 from ferrisboost_amd import heads
@@ -52,3 +53,27 @@ def test_a_copied_vocabulary_gives_the_address_of_its_own_tensor():
               copy.deepcopy({"a": [voc]})["a"][0]):
         e, lead = heads._positions(ids, v, True, 7, 8, 0, 1.0, 0.0, 0)
         assert heads._EMBED.unpack(e)[8] == v.first.data_ptr() and lead == (5,)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32, np.float64, np.longdouble, np.int64])
+def test_uniforms_are_checked_as_they_are_given(dtype):
+    """Numbers below 1 that float32 rounds to 1 are legal; 1 itself is not."""
+    below = np.nextafter(dtype(1), dtype(0)) if dtype is not np.int64 else 0
+    u = np.array([0, below, 0], dtype)
+    got = heads.check_uniforms(u, 3)
+    assert got.dtype == np.float32 and got.max() < 1 and got[0] == 0
+    assert got[1] == min(np.float32(below), np.nextafter(np.float32(1), np.float32(0)))
+    with pytest.raises(ValueError, match="in \\[0, 1\\)"):
+        heads.check_uniforms(np.array([0, 1], dtype), 2)
+    if dtype is not np.int64:
+        for bad in (-below, np.nan, np.inf):
+            with pytest.raises(ValueError, match="in \\[0, 1\\)"):
+                heads.check_uniforms(np.array([bad], dtype), 1)
+    with pytest.raises(ValueError, match="one value for each of 4 rows"):
+        heads.check_uniforms(u, 4)
+
+
+def test_uniforms_of_a_list_and_of_doubles_near_one():
+    assert (heads.check_uniforms([0.25, 1 - 2.0 ** -30, 1 - 2.0 ** -24], 3)
+            == np.float32([0.25, 1 - 2.0 ** -24, 1 - 2.0 ** -24])).all()
+    assert heads.check_uniforms([], 0).shape == (0,)
