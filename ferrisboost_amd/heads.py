@@ -21,7 +21,9 @@ package's first call, so that both share one HIP runtime. Kernels are hand-writt
 behind the C ABI of include/fbhip.h, enqueued on torch's current stream of the tensors'
 device; nothing waits, results are the same in every call, and all of it can be captured
 into a graph. A tensor that is not contiguous is copied first. embed and dropout take
-part in autograd. Bad arguments are ValueErrors, device failures RuntimeErrors.
+part in autograd, in reverse mode; tensors with a tangent of forward mode are refused. What
+embed_grad and sample give has no gradient. Bad arguments are ValueErrors, device failures
+RuntimeErrors.
 """
 
 from __future__ import annotations
@@ -40,6 +42,7 @@ _L = None
 _CELLS: dict = {}
 _IDS: dict = {}
 _raw_stream = None
+_forward_ad = None
 # fbh_embed and fbh_sample_options (include/fbhip.h), packed in one call: a small
 # operation's time is its host time.
 _EMBED = struct.Struct("QIIIIIIPPdQfI")
@@ -48,7 +51,7 @@ _OPTIONS = struct.Struct("PPPPfiff")
 
 def _need_torch():
     """torch, once it is known to share this package's HIP runtime."""
-    global _torch, _L, _raw_stream
+    global _torch, _L, _raw_stream, _forward_ad
     if _torch is not None:
         return _torch
     import torch
@@ -64,6 +67,7 @@ def _need_torch():
     _IDS.update({torch.int32: 0, torch.int64: 1, torch.float32: 2})
     # the current stream's handle, as torch.cuda.current_stream() wraps it
     _raw_stream = torch._C._cuda_getCurrentRawStream
+    _forward_ad = torch.autograd.forward_ad
     _L = N.hip()
     _torch = torch
     return torch
@@ -72,6 +76,8 @@ def _need_torch():
 def _device_tensor(x, what: str):
     if not isinstance(x, _torch.Tensor):
         raise ValueError(f"{what} must be a torch tensor, got {type(x).__name__}")
+    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(x).tangent is not None:
+        raise ValueError(f"{what} has a tangent: forward-mode derivatives are not available")
     if not x.is_cuda:
         raise ValueError(f"{what} must be on a GPU, it is on {x.device}")
     return x if x.is_contiguous() else x.contiguous()

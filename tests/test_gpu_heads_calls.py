@@ -159,3 +159,21 @@ def test_a_model_takes_uniform_doubles(heads):
     u[5] = 1.0
     with pytest.raises(ValueError, match="in \\[0, 1\\)"):
         m.sample(x, u)
+
+
+def test_tangents_are_refused_and_their_level_is_not(heads):
+    import torch.autograd.forward_ad as fwd
+
+    x = torch.randn(50, 8, device="cuda")
+    ids = torch.arange(50, device="cuda")
+    u = torch.rand(50, device="cuda")
+    with fwd.dual_level():
+        d = fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: heads.embed(d, ids), lambda: heads.embed_grad(d, ids, 50),
+                     lambda: heads.dropout(d, 0.5, 1), lambda: heads.sample(d, u)):
+            with pytest.raises(ValueError, match="has a tangent"):
+                call()
+        assert torch.equal(heads.embed(x, ids), x)
+        y = heads.dropout(x.requires_grad_(), 0.5, 1)
+        (g,) = torch.autograd.grad(y.sum(), x)
+    assert torch.equal(g, heads.dropout(torch.ones_like(x), 0.5, 1))

@@ -77,3 +77,19 @@ def test_uniforms_of_a_list_and_of_doubles_near_one():
     assert (heads.check_uniforms([0.25, 1 - 2.0 ** -30, 1 - 2.0 ** -24], 3)
             == np.float32([0.25, 1 - 2.0 ** -24, 1 - 2.0 ** -24])).all()
     assert heads.check_uniforms([], 0).shape == (0,)
+
+
+def test_tensors_with_a_tangent_are_refused():
+    """Outputs without one would read as derivatives of zero."""
+    import torch.autograd.forward_ad as fwd
+
+    x, ids = torch.ones(4, 8), torch.zeros(4, dtype=torch.int32)
+    with fwd.dual_level():
+        d = fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: heads.embed(d, ids), lambda: heads.embed_grad(d, ids, 4),
+                     lambda: heads.dropout(d, 0.5, 1), lambda: heads.sample(d, x[:, 0]),
+                     lambda: heads.embed(torch.nn.Parameter(x) * d, ids)):
+            with pytest.raises(ValueError, match="has a tangent"):
+                call()
+        with pytest.raises(ValueError, match="on a GPU"):  # a level by itself changes nothing
+            heads.dropout(x, 0.5, 1)
