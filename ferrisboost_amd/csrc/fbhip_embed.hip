@@ -6,6 +6,7 @@
 // position (row, column) whose id is outside its column, or that the counter-based
 // generator drops, takes and gives nothing.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "fbhip_heads.h"
@@ -1115,6 +1116,8 @@ uint32_t lg_at_least(uint64_t n) {
     return l;
 }
 
+float scale_of(const fbh_embed *e) { return (float)((double)e->scale / (1.0 - e->drop)); }
+
 void check_embed(const fbh_embed *e) {
     head_input(e, "null argument");
     head_input(e->dtype <= FBH_BF16, "unknown cell type");
@@ -1129,6 +1132,8 @@ void check_embed(const fbh_embed *e) {
     head_input(e->n_rows <= (1ull << 40) / e->n_columns, "more than 2^40 positions");
     head_input(e->most_ids <= e->n_tokens, "most_ids is larger than the table");
     (void)drop_threshold(e->drop);
+    // (what takes nothing is scaled like the rest, and zero times infinity is none)
+    head_input(std::isfinite(scale_of(e)), "scale / (1 - drop) must be a finite float");
 }
 
 Positions positions_of(const fbh_embed *e) {
@@ -1140,8 +1145,6 @@ Positions positions_of(const fbh_embed *e) {
     }
     return P;
 }
-
-float scale_of(const fbh_embed *e) { return (float)((double)e->scale / (1.0 - e->drop)); }
 
 // Whether buffer loads reach rows of row_bytes from p on: their bytes, in words.
 bool in_buffer(const void *p, uint64_t bytes, uint64_t row_bytes) {

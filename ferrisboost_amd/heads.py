@@ -47,6 +47,7 @@ _forward_ad = None
 # operation's time is its host time.
 _EMBED = struct.Struct("QIIIIIIPPdQfI")
 _OPTIONS = struct.Struct("PPPPfiff")
+_MOST = float(np.finfo(np.float32).max)
 
 
 def _need_torch():
@@ -108,6 +109,13 @@ def _drop(drop) -> float:
     if not 0.0 <= drop < 1.0:
         raise ValueError(f"drop must be in [0, 1), got {drop}")
     return drop
+
+
+def _scale(scale) -> float:
+    scale = float(scale)
+    if not abs(scale) <= _MOST:
+        raise ValueError(f"scale must be a finite float32, got {scale}")
+    return scale
 
 
 class Vocabulary:
@@ -251,7 +259,7 @@ def embed(table, ids, vocabulary: Vocabulary | None = None, *, scale: float = 1.
         raise ValueError(f"table has {table.shape[0]} rows, the vocabulary "
                          f"{vocabulary.n_tokens} tokens")
     ids = _beside(_device_tensor(ids, "ids"), table, "ids")
-    args = (table, ids, vocabulary, float(scale), bool(pooled), _drop(drop), _seed(seed))
+    args = (table, ids, vocabulary, _scale(scale), bool(pooled), _drop(drop), _seed(seed))
     if table.requires_grad and torch.is_grad_enabled():
         return _functions()[0].apply(*args)
     return _embed(*args)
@@ -274,7 +282,7 @@ def embed_grad(grad, ids, tokens, *, scale: float = 1.0, pooled: bool = False,
     if grad.dim() < 1 or grad.shape[-1] < 1:
         raise ValueError(f"grad must have a last axis of cells, got shape {tuple(grad.shape)}")
     e, lead = _positions(ids, vocabulary, bool(pooled), n_tokens, grad.shape[-1],
-                         _cells(grad, "grad"), float(scale), _drop(drop), _seed(seed))
+                         _cells(grad, "grad"), _scale(scale), _drop(drop), _seed(seed))
     if tuple(grad.shape[:-1]) != lead:
         raise ValueError(f"grad has shape {tuple(grad.shape)}, expected {lead} vectors")
     out = grad.new_empty((n_tokens, grad.shape[-1]))
@@ -345,7 +353,7 @@ def check_options(temperature, top_k, top_p, min_p) -> tuple[float, int, float, 
 
 def _temperature(v) -> float:
     v = float(v)
-    if not 0.0 <= v <= float(np.finfo(np.float32).max):
+    if not 0.0 <= v <= _MOST:
         raise ValueError(f"temperature must be a finite float32, not negative, got {v}")
     return v
 

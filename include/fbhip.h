@@ -739,7 +739,8 @@ enum { FBH_ID_I32 = 0, FBH_ID_I64 = 1, FBH_ID_F32 = 2 };
  * whole number) takes and gives nothing; so does one that is dropped: with
  * drop > 0 each position stays with probability 1 - drop, drawn from seed and
  * the position's number (row * n_columns + column) as fbh_dropout draws its
- * elements, and what stays is scaled by 1 / (1 - drop). dim at most 32768. */
+ * elements, and what stays is scaled by 1 / (1 - drop). scale / (1 - drop) has to be
+ * a finite float. dim at most 32768. */
 typedef struct {
     uint64_t n_rows;
     uint32_t n_columns;

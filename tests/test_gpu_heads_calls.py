@@ -177,3 +177,22 @@ def test_tangents_are_refused_and_their_level_is_not(heads):
         y = heads.dropout(x.requires_grad_(), 0.5, 1)
         (g,) = torch.autograd.grad(y.sum(), x)
     assert torch.equal(g, heads.dropout(torch.ones_like(x), 0.5, 1))
+
+
+def test_scales_of_any_finite_size(heads):
+    """Positions that take nothing stay zeros up to the largest scale; beyond it the call is
+    refused."""
+    table = torch.full((4, 8), 2.0 ** -100, device="cuda")
+    ids = torch.tensor([[0, -1], [-1, 3], [4, 9]], device="cuda")
+    most = float(np.finfo(np.float32).max)
+    for scale in (most, -most, 1e-45, 0.0):
+        one = torch.tensor(np.float32(scale)) * 2.0 ** -100
+        out = heads.embed(table, ids, scale=scale).cpu()
+        assert (out[0, 0] == one).all() and (out[1, 1] == one).all()
+        assert (out[0, 1] == 0).all() and (out[1, 0] == 0).all() and (out[2] == 0).all()
+    grad = torch.ones(3, 2, 8, device="cuda")
+    for scale, drop in ((float("inf"), 0.0), (float("nan"), 0.0), (1e39, 0.0), (most, 0.5)):
+        with pytest.raises(ValueError, match="finite"):
+            heads.embed(table, ids, scale=scale, drop=drop)
+        with pytest.raises(ValueError, match="finite"):
+            heads.embed_grad(grad, ids, 4, scale=scale, drop=drop)

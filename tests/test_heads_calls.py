@@ -4,12 +4,14 @@ as far as they need no device."""
 from __future__ import annotations
 
 import copy
+import ctypes as C
 import pickle
 
 import numpy as np
 import pytest
 import torch
 
+from ferrisboost_amd import _native as N
 from ferrisboost_amd import heads
 from test_host_rules import run_cpp
 
@@ -93,3 +95,25 @@ def test_tensors_with_a_tangent_are_refused():
                 call()
         with pytest.raises(ValueError, match="on a GPU"):  # a level by itself changes nothing
             heads.dropout(x, 0.5, 1)
+
+
+@pytest.mark.parametrize("scale, drop", [(float("inf"), 0.0), (float("nan"), 0.0),
+                                         (-float("inf"), 0.5), (3e38, 0.5), (-2e38, 0.9),
+                                         (1e30, 1 - 2.0 ** -53)])
+def test_scales_that_are_not_finite_are_refused(scale, drop):
+    """Positions that take nothing would be zero times infinity."""
+    e = N.Embed()
+    e.n_rows, e.n_columns, e.dim, e.n_tokens, e.ids = 4, 3, 8, 10, 64
+    e.scale, e.drop = scale, drop
+    L = N.hip()
+    with pytest.raises(ValueError, match="finite"):
+        N.check_hip(L.fbh_embed_rows(0, C.byref(e), 64, 64, None))
+    with pytest.raises(ValueError, match="finite"):
+        N.check_hip(L.fbh_embed_grad(0, C.byref(e), 64, 64, 64, 1 << 40, None))
+    assert L.fbh_embed_grad_bytes(C.byref(e)) == 0
+
+
+@pytest.mark.parametrize("scale", [float("inf"), float("nan"), 1e39, -1e300])
+def test_scales_beyond_float32(scale):
+    with pytest.raises(ValueError, match="finite float32"):
+        heads._scale(scale)
