@@ -97,8 +97,15 @@ def _beside(x, other, what: str):
     return x
 
 
+def _whole(v, what: str) -> int:
+    try:
+        return int(v)
+    except (OverflowError, TypeError, ValueError):
+        raise ValueError(f"{what} must be a whole number, got {v!r}") from None
+
+
 def _seed(seed) -> int:
-    seed = int(seed)
+    seed = _whole(seed, "seed")
     if not 0 <= seed < 1 << 64:
         raise ValueError(f"seed must be in 0..=2^64 - 1, got {seed}")
     return seed
@@ -134,6 +141,8 @@ class Vocabulary:
             raise ValueError(f"at most 32768 columns, got {sizes.size}")
         if (sizes < 0).any():
             raise ValueError("sizes must not be negative")
+        if (sizes >= 1 << 31).any():  # (and their sum is below 2^46)
+            raise ValueError("a column has at most 2^31 - 1 ids")
         first = np.concatenate([[0], np.cumsum(sizes, dtype=np.int64)])
         if not 1 <= first[-1] < 1 << 31:
             raise ValueError(f"a table has 1 to 2^31 - 1 rows, these columns {first[-1]}")
@@ -183,6 +192,9 @@ def _positions(ids, vocabulary, pooled: bool, n_tokens: int, dim: int, cells: in
             n_rows *= s
     else:
         n_rows, columns = ids.numel(), 1
+    if max(columns, dim, n_tokens) >> 32:
+        raise ValueError(f"{columns} columns, {n_tokens} table rows and {dim} cells: all must be "
+                         "below 2^32")
     # (the address that the tensor has now: a copied or unpickled vocabulary has one of its own)
     first, most = (0, 0) if vocabulary is None else (vocabulary.first.data_ptr(),
                                                      vocabulary.most_ids)
@@ -276,7 +288,8 @@ def embed_grad(grad, ids, tokens, *, scale: float = 1.0, pooled: bool = False,
     grad = _device_tensor(grad, "grad")
     ids = _beside(_device_tensor(ids, "ids"), grad, "ids")
     vocabulary = tokens if isinstance(tokens, Vocabulary) else None
-    n_tokens = int(tokens if vocabulary is None else vocabulary.n_tokens)
+    n_tokens = vocabulary.n_tokens if vocabulary is not None else _whole(
+        tokens, "tokens, other than a vocabulary,")
     if not 1 <= n_tokens < 1 << 31:
         raise ValueError(f"a table has 1 to 2^31 - 1 rows, got {n_tokens}")
     if grad.dim() < 1 or grad.shape[-1] < 1:
@@ -319,7 +332,7 @@ def dropout(x, drop: float, seed: int, first: int = 0):
     torch = _need_torch()
     x = _device_tensor(x, "x")
     _cells(x, "x")
-    first = int(first)
+    first = _whole(first, "first")
     if not 0 <= first < 1 << 63:
         raise ValueError(f"first must be in 0..=2^63 - 1, got {first}")
     args = (x, _drop(drop), _seed(seed), first)
@@ -359,9 +372,10 @@ def _temperature(v) -> float:
 
 
 def _top_k(v) -> int:
-    if isinstance(v, bool) or int(v) != v or int(v) < 0:
+    k = _whole(v, "top_k")
+    if isinstance(v, bool) or k != v or k < 0:
         raise ValueError(f"top_k must be a whole number, 0 (all) or more, got {v!r}")
-    return min(int(v), 0x7FFFFFFF)
+    return min(k, 0x7FFFFFFF)
 
 
 def _share(what: str, v) -> float:

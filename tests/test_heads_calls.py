@@ -117,3 +117,30 @@ def test_scales_that_are_not_finite_are_refused(scale, drop):
 def test_scales_beyond_float32(scale):
     with pytest.raises(ValueError, match="finite float32"):
         heads._scale(scale)
+
+
+@pytest.mark.parametrize("sizes", [[1 << 62] * 3 + [(1 << 62) + 5], [1 << 31], [3, 1 << 40],
+                                   np.array([2 ** 63, 2 ** 63 - 1, 2], np.uint64)])
+def test_sizes_whose_sum_is_beyond_64_bits(sizes):
+    with pytest.raises(ValueError, match="at most 2\\^31 - 1 ids"):
+        heads.Vocabulary(sizes)
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan"), None, "many"])
+def test_whole_numbers(value):
+    for check in (heads._seed, heads._top_k):
+        with pytest.raises(ValueError, match="whole number"):
+            check(value)
+    assert heads._seed(2 ** 64 - 1) == 2 ** 64 - 1 and heads._top_k(5.0) == 5
+    assert heads._top_k(1 << 40) == 0x7FFFFFFF
+
+
+def test_sizes_beyond_32_bits_are_value_errors():
+    """(tensors of one element, expanded)"""
+    heads._need_torch()
+    wide = torch.zeros((1, 1), dtype=torch.int32).expand(2, 1 << 32)
+    ids = torch.zeros((2, 3), dtype=torch.int32)
+    for args in ((wide, None, True, 5, 8), (ids, None, False, 1 << 32, 1),
+                 (ids, None, False, 1, 1 << 32)):
+        with pytest.raises(ValueError, match="below 2\\^32"):
+            heads._positions(*args, 0, 1.0, 0.0, 0)
