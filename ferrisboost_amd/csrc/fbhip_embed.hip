@@ -318,7 +318,9 @@ __global__ void embed_sum_few_kernel(Positions P, const T *table, T *out, uint32
 // token's positions stand together in their own order; then runs of equal tokens are
 // summed in f32. The sorted positions are cut into chunks of equal length: a run inside
 // one chunk goes to the table, the parts of longer runs are joined in chunk order. All
-// orders are fixed, so the gradient is the same in every call.
+// orders are fixed, so the gradient is the same in every call. A part of a sum is held in
+// f32 (up to 256 positions here, up to 384 blocks of 8 where columns are summed); what joins
+// parts, whose number grows with the positions of a token, is held in f64.
 constexpr uint32_t SORT_TPB = 256;
 constexpr uint32_t SORT_ROUNDS = 16;  // of a thread's positions; 1 where they are few
 constexpr uint32_t SORT_WAVES = SORT_TPB / 64;
@@ -670,12 +672,14 @@ __global__ __launch_bounds__(EMB_TPB) void grad_runs_kernel(Runs R, const T *gra
 
 constexpr uint32_t JOIN_SHORT = 16;  // parts that one chunk's lanes join by themselves
 
-// Joins the parts of the runs that start in a chunk and go on behind it.
+// Joins the parts of the runs that start in a chunk and go on behind it, in doubles: a run
+// over many chunks ends at the error of its parts, not of their number.
 constexpr uint32_t JOIN_TPB = 1024;
 template <class T, int VEC>
 __global__ __launch_bounds__(JOIN_TPB) void grad_join_kernel(Runs R, T *table) {
     __shared__ uint32_t longs[JOIN_TPB], n_longs;
-    __shared__ float sums[JOIN_TPB * VEC];
+    constexpr int H = VEC > 1 ? VEC / 2 : 1;  // cells that the groups join at a time
+    __shared__ double sums[JOIN_TPB * H];
     const uint32_t lanes = 1u << R.lg_g, groups = JOIN_TPB >> R.lg_g;
     const uint32_t g = threadIdx.x >> R.lg_g, lane = threadIdx.x & (lanes - 1);
     const uint32_t piece = (blockIdx.y << R.lg_g) + lane;
@@ -696,10 +700,10 @@ __global__ __launch_bounds__(JOIN_TPB) void grad_join_kernel(Runs R, T *table) {
             if (n == i && c + 1 + i < chunks && k[i] == key) n++;
         return n;
     };
-    const auto write = [&](uint32_t key, const float *a) {
+    const auto write = [&](uint32_t key, const double *a) {
         Piece<T, VEC> o;
 #pragma unroll
-        for (int i = 0; i < VEC; i++) o.v[i] = (T)(a[i] * R.s);
+        for (int i = 0; i < VEC; i++) o.v[i] = (T)(float)(a[i] * R.s);
         store_piece<T, VEC>(table + (uint64_t)key * R.dim + cell, o);
     };
 
@@ -713,7 +717,7 @@ __global__ __launch_bounds__(JOIN_TPB) void grad_join_kernel(Runs R, T *table) {
             if (n == JOIN_SHORT) {
                 if (lane == 0) longs[atomicAdd(&n_longs, 1u)] = c;
             } else if (live) {
-                float a[VEC];
+                double a[VEC];
                 Piece<float, VEC> p = load_piece<float, VEC>(R.parts + (2ull * c + 1) * R.dim + cell);
 #pragma unroll
                 for (int i = 0; i < VEC; i++) a[i] = p.v[i];
@@ -740,9 +744,9 @@ __global__ __launch_bounds__(JOIN_TPB) void grad_join_kernel(Runs R, T *table) {
             some = __syncthreads_count(at < chunks && R.keys[at * R.chunk] == key);
             n += some;
         }
-        float a[VEC];
+        double a[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; i++) a[i] = 0.0f;
+        for (int i = 0; i < VEC; i++) a[i] = 0.0;
         if (live)
             for (uint32_t k0 = g; k0 < n; k0 += 8 * groups) {
                 Piece<float, VEC> p[8];
@@ -759,15 +763,17 @@ __global__ __launch_bounds__(JOIN_TPB) void grad_join_kernel(Runs R, T *table) {
                         for (int i = 0; i < VEC; i++) a[i] += p[j].v[i];
             }
 #pragma unroll
-        for (int i = 0; i < VEC; i++) sums[threadIdx.x * VEC + i] = a[i];
-        __syncthreads();
-        if (g == 0 && live) {
-            for (uint32_t k = 1; k < groups; k++)
+        for (int h = 0; h < VEC; h += H) {
 #pragma unroll
-                for (int i = 0; i < VEC; i++) a[i] += sums[((k << R.lg_g) + lane) * VEC + i];
-            write(key, a);
+            for (int i = 0; i < H; i++) sums[threadIdx.x * H + i] = a[h + i];
+            __syncthreads();
+            if (g == 0)
+                for (uint32_t k = 1; k < groups; k++)
+#pragma unroll
+                    for (int i = 0; i < H; i++) a[h + i] += sums[((k << R.lg_g) + lane) * H + i];
+            __syncthreads();
         }
-        __syncthreads();
+        if (g == 0 && live) write(key, a);
     }
 }
 
@@ -987,17 +993,17 @@ __global__ __launch_bounds__(COL_TPB) void column_sums_kernel(Columns C, const T
     float a[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; i++) a[i] = 0.0f;
-    const auto write = [&](uint32_t id) {
+    const auto write = [&](uint32_t id, const auto *sum) {
         const uint64_t at = (uint64_t)(base + id) * C.dim + cell;
         if (whole) {
             Piece<T, VEC> o;
 #pragma unroll
-            for (int i = 0; i < VEC; i++) o.v[i] = (T)(a[i] * C.s);
+            for (int i = 0; i < VEC; i++) o.v[i] = (T)(float)(sum[i] * C.s);
             store_piece<T, VEC>(table + at, o);
         } else {
             Piece<float, VEC> o;
 #pragma unroll
-            for (int i = 0; i < VEC; i++) o.v[i] = a[i];
+            for (int i = 0; i < VEC; i++) o.v[i] = (float)sum[i];
             store_piece<float, VEC>(C.parts + (uint64_t)chunk * C.n_tokens * C.dim + at, o);
         }
     };
@@ -1027,15 +1033,19 @@ __global__ __launch_bounds__(COL_TPB) void column_sums_kernel(Columns C, const T
                 if constexpr (BUFFER) p[j] = load_offset<T, VEC>(rsrc, row * row_bytes + cell_bytes);
                 else p[j] = load_piece<T, VEC>(rows + (row < C.chunk ? row : 0) * pitch + cell);
             }
-#pragma unroll
-            for (uint32_t j = 0; j < 8; j++) {
+            // The block by itself first, in pairs: a range's sum of up to 3072 rows has an
+            // eighth of the steps, at the same number of additions.
+            const auto at = [&](int j, int i) {
                 const bool none =
                     !BUFFER && ((pair[j / 2] >> (16 * (j & 1))) & 0xFFFFu) >= C.chunk;
+                return none ? 0.0f : (float)p[j].v[i];
+            };
 #pragma unroll
-                for (int i = 0; i < VEC; i++) a[i] += none ? 0.0f : (float)p[j].v[i];
-            }
+            for (int i = 0; i < VEC; i++)
+                a[i] += ((at(0, i) + at(1, i)) + (at(2, i) + at(3, i))) +
+                        ((at(4, i) + at(5, i)) + (at(6, i) + at(7, i)));
             if (b + 1 == end) {
-                if (begun) write(id);
+                if (begun) write(id, a);
                 else leave();
                 begun = true;
 #pragma unroll
@@ -1065,14 +1075,17 @@ __global__ __launch_bounds__(COL_TPB) void column_sums_kernel(Columns C, const T
     }
     __syncthreads();
     if (end) {
+        double b[VEC];  // (ranges are joined in doubles, as chunks are)
+#pragma unroll
+        for (int i = 0; i < VEC; i++) b[i] = a[i];
         for (uint32_t h = g + 1; h * each < end; h++)
 #pragma unroll
-            for (int i = 0; i < VEC; i++) a[i] += sums[((h << C.lg_g) + glane) * VEC + i];
-        write(id);
+            for (int i = 0; i < VEC; i++) b[i] += sums[((h << C.lg_g) + glane) * VEC + i];
+        write(id, b);
     }
 }
 
-// table[token] = s * the sum of its parts, in chunk order.
+// table[token] = s * the sum of its parts, in chunk order and in doubles.
 template <class T, int VEC>
 __global__ __launch_bounds__(256) void column_join_kernel(Columns C, T *table) {
     const uint64_t i = blockIdx.x * 256ull + threadIdx.x;
@@ -1080,9 +1093,9 @@ __global__ __launch_bounds__(256) void column_join_kernel(Columns C, T *table) {
     if (tok >= C.n_tokens) return;
     const uint32_t cell = min((uint32_t)(i - tok * C.n_pieces) * VEC, C.dim - VEC);
     const float *part = C.parts + tok * C.dim + cell;
-    float a[VEC];
+    double a[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; j++) a[j] = 0.0f;
+    for (int j = 0; j < VEC; j++) a[j] = 0.0;
     for (uint32_t c0 = 0; c0 < C.chunks; c0 += 8) {
         bool some[8];
         Piece<float, VEC> p[8];
@@ -1105,7 +1118,7 @@ __global__ __launch_bounds__(256) void column_join_kernel(Columns C, T *table) {
     }
     Piece<T, VEC> o;
 #pragma unroll
-    for (int j = 0; j < VEC; j++) o.v[j] = (T)(a[j] * C.s);
+    for (int j = 0; j < VEC; j++) o.v[j] = (T)(float)(a[j] * C.s);
     store_piece<T, VEC>(table + tok * C.dim + cell, o);
 }
 

@@ -281,8 +281,9 @@ def embed_grad(grad, ids, tokens, *, scale: float = 1.0, pooled: bool = False,
                drop: float = 0.0, seed: int = 0):
     """The gradient of embed()'s table, (n_tokens, dim) in grad's type: `grad` is the
     gradient of embed()'s output, `tokens` its vocabulary or, without one, the number of
-    table rows, and the rest embed()'s arguments. Sums are taken in float32 in a fixed
-    order (the positions sorted by token) and rounded once. (embed() calls this in
+    table rows, and the rest embed()'s arguments. Sums are taken in a fixed order (the
+    positions sorted by token), parts of at most 3072 in float32 and the parts in float64,
+    and rounded once. (embed() calls this in
     backward(); a captured training step can call it by itself.)"""
     _need_torch()
     grad = _device_tensor(grad, "grad")

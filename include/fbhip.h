@@ -770,8 +770,8 @@ uint64_t fbh_embed_grad_bytes(const fbh_embed *e);
 /* The gradient of fbh_embed_rows by its table: table_grad[v] = scale * the sum
  * over positions of token v of the output's gradient there (grad, laid out as
  * out), for every v (zeros where there is no position), in the table's type.
- * Positions are sorted by token and summed in f32 in a fixed order. At most
- * 2^31 - 1 positions. */
+ * Positions are sorted by token and summed in a fixed order, parts of at most 3072
+ * in f32 and the parts in f64, and rounded once. At most 2^31 - 1 positions. */
 int fbh_embed_grad(int device, const fbh_embed *e, const void *grad, void *table_grad, void *work,
                    uint64_t work_bytes, void *stream);
 

@@ -196,3 +196,31 @@ def test_scales_of_any_finite_size(heads):
             heads.embed(table, ids, scale=scale, drop=drop)
         with pytest.raises(ValueError, match="finite"):
             heads.embed_grad(grad, ids, 4, scale=scale, drop=drop)
+
+
+# (positions of one id, table rows, width, distance of the ones): sorted through memory, in
+# buckets, in runs of a few chunks, by columns in chunks of rows, in one chunk, and wide
+LONG_RUNS = [(1 << 20, 70_000, 4, 256), (65_536, 5000, 256, 256), (65_536, 5000, 3, 256),
+             (208, 5000, 8, 16), (208, 5000, 260, 16), (1 << 22, 9, 4, 16_384),
+             (1 << 21, 1000, 2, 16_384), (16_384, 5, 4, 2048), (16_384, 700, 1, 2048),
+             (70_000, 9, 256, 16_384), (140_000, 2, 33, 16_384)]
+
+
+@pytest.mark.parametrize("n, v, dim, every", LONG_RUNS)
+def test_sums_of_frequent_ids(heads, n, v, dim, every):
+    """2^24, then ones so far apart that every part of the sum is a whole number below 2^24
+    or has no other addend: joined in more bits than float32 the sum is exact and rounded
+    once, in float32 each of the ones would be lost."""
+    x = torch.zeros(n, dim, device="cuda")
+    x[::every] = 1.0
+    x[0] = 2.0 ** 24
+    x[:, ::2] *= -1
+    ones = -(-n // every) - 1
+    want = torch.full((dim,), float(np.float32(2 ** 24 + ones)))
+    want[::2] *= -1
+    for token in (0, v - 1):
+        ids = torch.full((n,), token, device="cuda")
+        got = heads.embed_grad(x, ids, v).cpu()
+        assert torch.equal(got[token], want), (got[token][:4], want[:4])
+        got[token] = 0
+        assert (got == 0).all()
