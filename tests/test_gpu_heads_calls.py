@@ -224,3 +224,42 @@ def test_sums_of_frequent_ids(heads, n, v, dim, every):
         assert torch.equal(got[token], want), (got[token][:4], want[:4])
         got[token] = 0
         assert (got == 0).all()
+
+
+def _close(got, want, magnitude, terms, dtype):
+    info = torch.finfo(dtype)
+    tol = (np.abs(want) * info.eps / 2 + info.smallest_normal * info.eps / 2
+           + magnitude * ((np.maximum(terms, 1) + 1) * 2.0 ** -24 * (1 + info.eps)))
+    bad = ~(np.abs(got.detach().cpu().double().numpy() - want) <= tol)
+    assert not bad.any(), (np.argwhere(bad)[:4].tolist(), want[bad][:4])
+
+
+# (rows, columns, table rows, width): few rows and many (both summing kernels), gradients in
+# buckets, in several passes, of a table that columns of their own would take whole, and odd
+SHARED = [(1, 2, 5, 3), (3, 33, 40, 16), (300, 7, 2000, 33), (9000, 7, 300, 8),
+          (1999, 33, 70_000, 5), (20_011, 7, 900, 12), (40_000, 2, 100_000, 20),
+          (30_000, 33, 1000, 1), (5000, 33, 600_000, 2)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n, t, v, dim", SHARED)
+def test_columns_that_share_one_table(heads, n, t, v, dim, dtype):
+    """Sums over columns without a vocabulary, by autograd and by the explicit call."""
+    rng = np.random.default_rng([n, t, v])
+    table = torch.from_numpy(rng.normal(size=(v, dim)).astype(np.float32)).to(dtype).cuda()
+    ids = rng.integers(-1, v + 1, (n, t))
+    ids[:, 0] = np.minimum(rng.pareto(0.5, n), v - 1).astype(np.int64)  # frequent ones
+    d_ids = torch.from_numpy(ids).cuda()
+    for drop in (0.0, 0.25):
+        tok = ref.tokens(ids, None, v, drop, 5)
+        s = 1.5 / (1.0 - drop)
+        leaf = table.clone().requires_grad_()
+        out = heads.embed(leaf, d_ids, scale=1.5, pooled=True, drop=drop, seed=5)
+        want, mag = ref.embed(table.double().cpu().numpy(), tok, s, True)
+        _close(out, want, mag, t, dtype)
+        grad = torch.from_numpy(rng.normal(size=(n, dim)).astype(np.float32)).to(dtype).cuda()
+        out.backward(grad)
+        want, mag, terms = ref.embed_grad(grad.double().cpu().numpy(), tok, v, s, True)
+        _close(leaf.grad, want, mag, terms[:, None], dtype)
+        got = heads.embed_grad(grad, d_ids, v, scale=1.5, pooled=True, drop=drop, seed=5)
+        assert torch.equal(got, leaf.grad)
