@@ -836,13 +836,26 @@ struct Columns {
     const uint16_t *local;
     const uint32_t *first;   // NULL: one column, from row 0
     uint64_t n_rows, padded;
-    uint32_t n_columns, n_tokens, most_ids;
+    uint32_t column0, n_columns;  // of a launch: its parts take the same workspace as the
+                                  // launch's before
+    uint32_t part_tokens;         // tokens that the parts have room for, from column0's on
+    uint32_t n_tokens, most_ids;
     uint32_t chunk, chunks;  // rows of a chunk (a multiple of 64), chunks
     uint32_t per_row;        // gradient vectors of a row: 1 (pooled) or the columns
     uint32_t dim, n_pieces, lg_g;
     float s;
-    float *parts;            // [chunk][token][dim]
-    uint16_t *counts;        // [chunk][token]: positions in the chunk
+    float *parts;            // [chunk][token of the launch][dim]
+    uint16_t *counts;        // [chunk][token of the launch]: positions in the chunk
+
+    bool grouped;            // a launch has not all columns
+
+    // The table rows of the launch's columns: the first, and the one behind the last.
+    __device__ __forceinline__ uint32_t begin() const {
+        return grouped ? min(first[column0], n_tokens) : 0;
+    }
+    __device__ __forceinline__ uint32_t end() const {
+        return grouped ? min(first[column0 + n_columns], n_tokens) : n_tokens;
+    }
 };
 
 // LDS of column_sums_kernel, in byte offsets: the waves' counters and later the ranges'
@@ -869,7 +882,7 @@ __global__ __launch_bounds__(COL_TPB) void column_sums_kernel(Columns C, const T
     // (chunk group, column, chunk of the group): a group's chunks go to one XCD each
     const uint32_t per = min(C.chunks, 8u);
     const uint32_t chunk = blockIdx.x / (C.n_columns * per) * per + blockIdx.x % per;
-    const uint32_t t = blockIdx.x / per % C.n_columns;
+    const uint32_t t = C.column0 + blockIdx.x / per % C.n_columns;
     if (chunk >= C.chunks) return;
     const ColumnLds L = column_lds(C.most_ids, C.chunk, VEC);
     uint16_t *seen = reinterpret_cast<uint16_t *>(lds);
@@ -877,8 +890,12 @@ __global__ __launch_bounds__(COL_TPB) void column_sums_kernel(Columns C, const T
     uint16_t *starts = reinterpret_cast<uint16_t *>(lds + L.starts);
     uint16_t *list = reinterpret_cast<uint16_t *>(lds + L.list);
     const uint32_t base = C.first ? min(C.first[t], C.n_tokens) : 0;
+    const uint32_t part_base = base - C.begin();
     const uint32_t ids = min(C.most_ids, C.first ? min(C.first[t + 1] - base, C.n_tokens - base)
                                                  : C.n_tokens);
+    // (never, but for falling offsets or columns of more than most_ids ids, which the caller
+    // has ruled out)
+    if ((uint64_t)part_base + ids > C.part_tokens) return;
     const uint32_t lane = threadIdx.x & 63, w = threadIdx.x / 64;
     const uint64_t row0 = (uint64_t)chunk * C.chunk;
     const uint16_t *from = C.local + t * C.padded + row0;
@@ -951,7 +968,8 @@ __global__ __launch_bounds__(COL_TPB) void column_sums_kernel(Columns C, const T
             const uint32_t id = 2 * threadIdx.x + j;
             if (id < C.most_ids) {
                 starts[id] = (uint16_t)at;
-                if (id < ids) C.counts[(uint64_t)chunk * C.n_tokens + base + id] = (uint16_t)c[j];
+                if (id < ids)
+                    C.counts[(uint64_t)chunk * C.part_tokens + part_base + id] = (uint16_t)c[j];
                 uint32_t a = 8 * at;
                 for (uint32_t v = 0; v < COL_WAVES; v++) {
                     const uint32_t n = seen[v * C.most_ids + id];
@@ -994,17 +1012,18 @@ __global__ __launch_bounds__(COL_TPB) void column_sums_kernel(Columns C, const T
 #pragma unroll
     for (int i = 0; i < VEC; i++) a[i] = 0.0f;
     const auto write = [&](uint32_t id, const auto *sum) {
-        const uint64_t at = (uint64_t)(base + id) * C.dim + cell;
         if (whole) {
+            const uint64_t at = (uint64_t)(base + id) * C.dim + cell;
             Piece<T, VEC> o;
 #pragma unroll
             for (int i = 0; i < VEC; i++) o.v[i] = (T)(float)(sum[i] * C.s);
             store_piece<T, VEC>(table + at, o);
         } else {
+            const uint64_t at = (uint64_t)chunk * C.part_tokens + (part_base + id);
             Piece<float, VEC> o;
 #pragma unroll
             for (int i = 0; i < VEC; i++) o.v[i] = (float)sum[i];
-            store_piece<float, VEC>(C.parts + (uint64_t)chunk * C.n_tokens * C.dim + at, o);
+            store_piece<float, VEC>(C.parts + at * C.dim + cell, o);
         }
     };
     const auto leave = [&] {
@@ -1089,8 +1108,9 @@ __global__ __launch_bounds__(COL_TPB) void column_sums_kernel(Columns C, const T
 template <class T, int VEC>
 __global__ __launch_bounds__(256) void column_join_kernel(Columns C, T *table) {
     const uint64_t i = blockIdx.x * 256ull + threadIdx.x;
-    const uint64_t tok = i / C.n_pieces;
-    if (tok >= C.n_tokens) return;
+    const uint64_t tok = i / C.n_pieces;  // of the launch
+    const uint64_t begin = C.begin();
+    if (tok >= C.part_tokens || begin + tok >= C.end()) return;
     const uint32_t cell = min((uint32_t)(i - tok * C.n_pieces) * VEC, C.dim - VEC);
     const float *part = C.parts + tok * C.dim + cell;
     double a[VEC];
@@ -1102,13 +1122,13 @@ __global__ __launch_bounds__(256) void column_join_kernel(Columns C, T *table) {
         uint16_t count[8];
 #pragma unroll
         for (uint32_t k = 0; k < 8; k++)
-            count[k] = C.counts[(uint64_t)min(c0 + k, C.chunks - 1) * C.n_tokens + tok];
+            count[k] = C.counts[(uint64_t)min(c0 + k, C.chunks - 1) * C.part_tokens + tok];
 #pragma unroll
         for (uint32_t k = 0; k < 8; k++) {
             // (a chunk without the token has left nothing; the first part is read instead)
             some[k] = c0 + k < C.chunks && count[k] != 0;
             p[k] = load_piece<float, VEC>(
-                some[k] ? part + (uint64_t)(c0 + k) * C.n_tokens * C.dim : C.parts);
+                some[k] ? part + (uint64_t)(c0 + k) * C.part_tokens * C.dim : C.parts);
         }
 #pragma unroll
         for (uint32_t k = 0; k < 8; k++)
@@ -1119,7 +1139,7 @@ __global__ __launch_bounds__(256) void column_join_kernel(Columns C, T *table) {
     Piece<T, VEC> o;
 #pragma unroll
     for (int j = 0; j < VEC; j++) o.v[j] = (T)(float)(a[j] * C.s);
-    store_piece<T, VEC>(table + tok * C.dim + cell, o);
+    store_piece<T, VEC>(table + (begin + tok) * C.dim + cell, o);
 }
 
 // ------------------------------------------------------------------- host side
@@ -1271,9 +1291,16 @@ void with_ids(uint32_t id_type, bool drop, F &&f) {
 // trees, 16 cells of float32: 20 us sorted). Otherwise a chunk of a column has 8
 // positions an id on average at least, so that the parts are written and read for less
 // than the gradient rows take, and a call has 64k positions at least.
+//
+// Where the parts of all columns would take more than COL_PART_BYTES, the columns are taken in
+// groups whose parts do not (a column's by itself may: it has an eighth of a position a row at
+// most, in f32). A group still has some 500 workgroups: 2^28 cells of parts, at most 1024 ids
+// and 512 cells each.
 constexpr uint64_t COL_ONE_BYTES = 256 << 10;
+constexpr uint64_t COL_PART_BYTES = 1ull << 30;
 struct ColumnPlan {
     uint32_t chunk = 0, chunks = 0;
+    uint32_t group = 0, part_tokens = 0;  // columns of a group, and the most tokens of one
     uint64_t padded = 0, local = 0, counts = 0, parts = 0, bytes = 0;
 };
 
@@ -1309,9 +1336,16 @@ ColumnPlan column_plan(const fbh_embed *e) {
         c.bytes = (at + bytes + 255) & ~255ull;
         return at;
     };
+    c.group = (uint32_t)columns;
+    c.part_tokens = e->n_tokens;
+    if (c.chunks > 1 && 4ull * c.chunks * e->n_tokens * e->dim > COL_PART_BYTES) {
+        c.group = (uint32_t)std::clamp<uint64_t>(
+            COL_PART_BYTES / (4ull * c.chunks * ids * e->dim), 1, columns);
+        c.part_tokens = (uint32_t)std::min<uint64_t>(e->n_tokens, c.group * ids);
+    }
     c.local = take(2 * c.padded * columns);
-    c.counts = take(2ull * c.chunks * e->n_tokens);
-    c.parts = take(c.chunks > 1 ? 4ull * c.chunks * e->n_tokens * e->dim : 0);
+    c.counts = take(2ull * c.chunks * c.part_tokens);
+    c.parts = take(c.chunks > 1 ? 4ull * c.chunks * c.part_tokens * e->dim : 0);
     return c;
 }
 
@@ -1389,16 +1423,16 @@ void columns_grad(const fbh_embed *e, const ColumnPlan &G, const void *grad, voi
     head_check(hipGetLastError(), "column ids");
     const uint32_t v = piece_cells(e->dim, e->dtype), pieces = (e->dim + v - 1) / v;
     const uint32_t lg_g = std::min(lg_at_least(pieces), 6u);
-    const Columns C{local, e->first, P.n_rows, G.padded, P.n_columns, e->n_tokens, most_ids,
-                    G.chunk, G.chunks, e->pooled ? 1 : P.n_columns, e->dim, pieces, lg_g,
-                    scale_of(e), reinterpret_cast<float *>(w + G.parts),
-                    reinterpret_cast<uint16_t *>(w + G.counts)};
+    Columns C{local, e->first, P.n_rows, G.padded, 0, 0, G.part_tokens, e->n_tokens, most_ids,
+              G.chunk, G.chunks, e->pooled ? 1 : P.n_columns, e->dim, pieces, lg_g, scale_of(e),
+              reinterpret_cast<float *>(w + G.parts), reinterpret_cast<uint16_t *>(w + G.counts),
+              G.group < P.n_columns};
     with_cells(e->dtype, v, [&](auto one, auto vec) {
         using T = decltype(one);
         constexpr int VEC = decltype(vec)::value;
         const uint32_t lds = column_lds(most_ids, G.chunk, VEC).bytes;
         const uint32_t per = std::min(G.chunks, 8u);
-        const auto go = [&](auto buffer) {
+        const auto sums = [&](auto buffer) {
             const auto kernel = &column_sums_kernel<T, VEC, decltype(buffer)::value>;
             if (lds > 64 * 1024)
                 head_check(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
@@ -1406,24 +1440,29 @@ void columns_grad(const fbh_embed *e, const ColumnPlan &G, const void *grad, voi
                                                128 * 1024),
                            "column sums");
             hipLaunchKernelGGL(kernel,
-                               dim3((G.chunks + per - 1) / per * per * P.n_columns,
+                               dim3((G.chunks + per - 1) / per * per * C.n_columns,
                                     (pieces + (1u << lg_g) - 1) >> lg_g),
                                dim3(COL_TPB), lds, s, C, static_cast<const T *>(grad),
                                static_cast<T *>(table));
         };
         const uint64_t row_bytes = (uint64_t)C.per_row * e->dim * sizeof(T);
-        if constexpr (VEC * sizeof(T) >= 4) {
-            if (row_bytes <= BUFFER_MOST / COL_MOST_ROWS &&
-                in_buffer(grad, G.chunk * row_bytes, e->dim * sizeof(T)))
-                go(std::true_type{});
-            else go(std::false_type{});
-        } else go(std::false_type{});
-        head_check(hipGetLastError(), "column sums");
-        if (G.chunks == 1) return;
-        const uint64_t threads = (uint64_t)e->n_tokens * pieces;
-        hipLaunchKernelGGL((column_join_kernel<T, VEC>), dim3((uint32_t)((threads + 255) / 256)),
-                           dim3(256), 0, s, C, static_cast<T *>(table));
-        head_check(hipGetLastError(), "column sums");
+        for (uint32_t t = 0; t < P.n_columns; t += G.group) {
+            C.column0 = t;
+            C.n_columns = std::min(G.group, P.n_columns - t);
+            if constexpr (VEC * sizeof(T) >= 4) {
+                if (row_bytes <= BUFFER_MOST / COL_MOST_ROWS &&
+                    in_buffer(grad, G.chunk * row_bytes, e->dim * sizeof(T)))
+                    sums(std::true_type{});
+                else sums(std::false_type{});
+            } else sums(std::false_type{});
+            head_check(hipGetLastError(), "column sums");
+            if (G.chunks == 1) return;
+            const uint64_t threads = (uint64_t)G.part_tokens * pieces;
+            hipLaunchKernelGGL((column_join_kernel<T, VEC>),
+                               dim3((uint32_t)((threads + 255) / 256)), dim3(256), 0, s, C,
+                               static_cast<T *>(table));
+            head_check(hipGetLastError(), "column sums");
+        }
     });
 }
 

@@ -765,7 +765,10 @@ typedef struct {
  * are the pooled embedding of its leaf ids in the table of its leaf values. */
 int fbh_embed_rows(int device, const fbh_embed *e, const void *table, void *out, void *stream);
 /* Device bytes of workspace that fbh_embed_grad takes, 16-byte aligned; 0 for a call
- * that it refuses. */
+ * that it refuses. With most_ids up to 1024 (or a table of up to 1024 rows and no
+ * parts): at most 2 bytes a position, and 1 GiB or, if that is more, 1/8 of an f32
+ * vector a row, and little else. Otherwise 17 bytes and at most 1/8 of an f32 vector
+ * a position. */
 uint64_t fbh_embed_grad_bytes(const fbh_embed *e);
 /* The gradient of fbh_embed_rows by its table: table_grad[v] = scale * the sum
  * over positions of token v of the output's gradient there (grad, laid out as

@@ -263,3 +263,37 @@ def test_columns_that_share_one_table(heads, n, t, v, dim, dtype):
         _close(leaf.grad, want, mag, terms[:, None], dtype)
         got = heads.embed_grad(grad, d_ids, v, scale=1.5, pooled=True, drop=drop, seed=5)
         assert torch.equal(got, leaf.grad)
+
+
+@pytest.mark.parametrize("rows, sizes, dim, pooled, dtype", [
+    (40_000, [1000] * 90 + [7, 0, 400], 1024, True, torch.bfloat16),   # 3 groups of columns
+    (70_001, [1000, 3, 0, 1000, 500, 8], 20_000, True, torch.float32),  # a column each
+    (140_000, [0, 1024, 0], 32_768, True, torch.float16),              # all ids in one column
+    (33_000, [900] * 200, 515, False, torch.float16)])                 # 2, an odd width
+def test_columns_whose_parts_take_more_than_one_workspace(heads, rows, sizes, dim, pooled, dtype):
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    voc = heads.Vocabulary(sizes)
+    ids = torch.stack([torch.randint(-1, max(s, 1), (rows,), generator=g, device="cuda")
+                       for s in sizes], 1).int()
+    shape = (rows, dim) if pooled else (rows, len(sizes), dim)
+    grad = torch.randn(shape, generator=g, device="cuda", dtype=dtype)
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = heads.embed_grad(grad, ids, voc, pooled=pooled, scale=0.5)
+    out = got.numel() * got.element_size()
+    parts = max(1 << 30, rows * dim // 2)  # (at least a column's)
+    assert torch.cuda.max_memory_allocated() - before <= out + parts + 8 * ids.numel() + (16 << 20)
+    first = np.concatenate([[0], np.cumsum(sizes)])
+    info = torch.finfo(dtype)
+    for t, s in enumerate(sizes):  # a column at a time, in doubles
+        at = ((ids[:, t] >= 0) & (ids[:, t] < s)).nonzero()[:, 0]
+        tok = ids[at, t].long()
+        x = (grad if pooled else grad[:, t])[at].double()
+        want = torch.zeros(s, dim, dtype=torch.float64, device="cuda").index_add_(0, tok, x) * 0.5
+        mag = torch.zeros_like(want).index_add_(0, tok, x.abs()) * 0.5
+        terms = torch.bincount(tok, minlength=s)[:, None] if s else torch.zeros(0, 1, device="cuda")
+        tol = (want.abs() * info.eps / 2 + info.smallest_normal * info.eps / 2
+               + mag * ((terms + 1) * 2.0 ** -24 * (1 + info.eps)))
+        assert ((got[first[t]:first[t + 1]].double() - want).abs() <= tol).all(), t
+    assert torch.equal(got, heads.embed_grad(grad, ids, voc, pooled=pooled, scale=0.5))
+

@@ -144,3 +144,34 @@ def test_sizes_beyond_32_bits_are_value_errors():
                  (ids, None, False, 1, 1 << 32)):
         with pytest.raises(ValueError, match="below 2\\^32"):
             heads._positions(*args, 0, 1.0, 0.0, 0)
+
+
+def _columns(rows, columns, ids, dim, dtype, pooled=1):
+    e = N.Embed()
+    e.n_rows, e.n_columns, e.dim, e.n_tokens, e.most_ids = rows, columns, dim, columns * ids, ids
+    e.ids, e.first, e.scale, e.dtype, e.pooled = 64, 64, 1.0, dtype, pooled
+    return e
+
+
+@pytest.mark.parametrize("rows, columns, ids, dim, dtype", [
+    (1_000_000, 400, 1000, 160, 2), (100_000, 100, 511, 64, 2), (40_000, 96, 1000, 1024, 2),
+    (9000, 32_768, 1024, 512, 0), (1 << 29, 1, 1024, 64, 0), (1 << 29, 1, 7, 32_768, 0),
+    (65_536, 20, 1024, 32_768, 1), (70_000, 3, 1024, 32_768, 0)])
+def test_workspace_of_column_gradients_is_bounded(rows, columns, ids, dim, dtype):
+    """2 bytes a position (chunks are rounded up to 64 rows), and parts of 1 GiB or an eighth
+    of an f32 vector a row, with two bytes of counts a vector. 1M rows of 400 columns of 1000 ids, 160 cells,
+    took 16 GB."""
+    got = N.hip().fbh_embed_grad_bytes(C.byref(_columns(rows, columns, ids, dim, dtype)))
+    # (at most a chunk for 64 rows and one more)
+    parts = max(1 << 30, rows * dim // 2)
+    assert got <= 2 * (2 * rows + 64) * columns + parts + parts // (2 * dim) + 4096
+    assert got >= 2 * rows * columns
+
+
+@pytest.mark.parametrize("n, tokens, dim", [(1 << 20, 50_000, 64), (60_000, 50_000, 1024),
+                                            ((1 << 31) - 1, 1 << 30, 1), (1 << 25, 4096, 32_768)])
+def test_workspace_of_sorted_gradients(n, tokens, dim):
+    e = _columns(n, 1, tokens, dim, 0)
+    e.first, e.most_ids = None, 0
+    got = N.hip().fbh_embed_grad_bytes(C.byref(e))
+    assert 16 * n <= got <= 17 * n + n * dim // 2 + 16 * dim + (1 << 20)
