@@ -1157,6 +1157,8 @@ void check_embed(const fbh_embed *e) {
     head_input(e->id_type <= FBH_ID_F32, "unknown id type");
     head_input(e->dim >= 1 && e->dim <= EMB_MAX_DIM, "dim must be in 1..=32768");
     head_input(e->n_columns >= 1, "no columns");
+    // (the summing kernels step over a row's columns in 32 bits)
+    head_input(!e->pooled || e->n_columns <= 0x7FFFFFFFu, "at most 2147483647 columns to sum");
     head_input(!e->first || e->n_columns <= EMB_MAX_COLUMNS,
                "at most 32768 columns with parts of their own");
     head_input(e->n_tokens >= 1 && e->n_tokens <= 0x7FFFFFFFu,

@@ -740,7 +740,7 @@ enum { FBH_ID_I32 = 0, FBH_ID_I64 = 1, FBH_ID_F32 = 2 };
  * drop > 0 each position stays with probability 1 - drop, drawn from seed and
  * the position's number (row * n_columns + column) as fbh_dropout draws its
  * elements, and what stays is scaled by 1 / (1 - drop). scale / (1 - drop) has to be
- * a finite float. dim at most 32768. */
+ * a finite float. dim at most 32768; at most 2^31 - 1 columns where they are summed. */
 typedef struct {
     uint64_t n_rows;
     uint32_t n_columns;

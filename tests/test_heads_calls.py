@@ -175,3 +175,12 @@ def test_workspace_of_sorted_gradients(n, tokens, dim):
     e.first, e.most_ids = None, 0
     got = N.hip().fbh_embed_grad_bytes(C.byref(e))
     assert 16 * n <= got <= 17 * n + n * dim // 2 + 16 * dim + (1 << 20)
+
+
+@pytest.mark.parametrize("columns", [1 << 31, (1 << 32) - 1024, (1 << 32) - 1])
+def test_rows_of_too_many_columns_to_sum_are_refused(columns):
+    """The summing kernels' steps over a row would pass 2^32 and never end."""
+    e = _columns(3, 1, 4, 8, 0)
+    e.first, e.n_columns, e.most_ids = None, columns, 0
+    with pytest.raises(ValueError, match="2147483647 columns"):
+        N.check_hip(N.hip().fbh_embed_rows(0, C.byref(e), 64, 64, None))
