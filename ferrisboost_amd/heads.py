@@ -267,6 +267,8 @@ def embed(table, ids, vocabulary: Vocabulary | None = None, *, scale: float = 1.
     table = _device_tensor(table, "table")
     if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
         raise ValueError(f"table must be (tokens, cells), got shape {tuple(table.shape)}")
+    if vocabulary is not None and not isinstance(vocabulary, Vocabulary):
+        raise ValueError(f"vocabulary must be a Vocabulary, got {type(vocabulary).__name__}")
     if vocabulary is not None and vocabulary.n_tokens != table.shape[0]:
         raise ValueError(f"table has {table.shape[0]} rows, the vocabulary "
                          f"{vocabulary.n_tokens} tokens")

@@ -297,3 +297,12 @@ def test_columns_whose_parts_take_more_than_one_workspace(heads, rows, sizes, di
         assert ((got[first[t]:first[t + 1]].double() - want).abs() <= tol).all(), t
     assert torch.equal(got, heads.embed_grad(grad, ids, voc, pooled=pooled, scale=0.5))
 
+
+
+def test_vocabularies_of_another_type(heads):
+    table, ids = torch.zeros(4, 8, device="cuda"), torch.zeros(3, 1, device="cuda")
+    for voc in (4, [4], "4"):
+        with pytest.raises(ValueError, match="must be a Vocabulary"):
+            heads.embed(table, ids, voc)
+    with pytest.raises(ValueError, match="whole number"):
+        heads.embed_grad(table, ids, [4])
