@@ -694,8 +694,8 @@ class Model:
         m = self.predict(data, output_margin=True, n_trees=n_trees,
                          iteration_range=iteration_range, missing=missing,
                          base_margin=base_margin, device=device)
-        if m.ndim == 1:  # binary:logistic: exp(margin) to 1
-            m = np.stack([np.zeros_like(m), m], axis=1)
+        if m.ndim == 1:  # binary:logistic: exp(margin) to 1 (nothing where that is NaN)
+            m = np.stack([np.where(np.isnan(m), m, np.float32(0)), m], axis=1)
         m = np.ascontiguousarray(m, np.float32)
         n, k = m.shape
         u = np.ascontiguousarray(heads.check_uniforms(uniforms, n))

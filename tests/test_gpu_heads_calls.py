@@ -306,3 +306,22 @@ def test_vocabularies_of_another_type(heads):
             heads.embed(table, ids, voc)
     with pytest.raises(ValueError, match="whole number"):
         heads.embed_grad(table, ids, [4])
+
+
+def test_classes_of_margins_that_are_no_numbers(heads):
+    """A row whose margins are all NaN has class -1, in binary models (one margin) too."""
+    import ferrisboost_amd as fb
+    from helpers import product_params
+
+    rng = np.random.default_rng(4)
+    x = rng.normal(size=(900, 3)).astype(np.float32)
+    y = (x[:, 0] > 0).astype(np.float32)
+    u = rng.random(900)
+    for params, outputs in (({}, 1), ({"objective": "multi:softprob", "num_class": 2}, 2)):
+        m = fb.train(product_params({"max_depth": 2, **params}), x, y, num_boost_round=2)
+        base = np.zeros((900, outputs), np.float32)
+        base[5], base[6, -1], base[7, -1] = np.nan, np.inf, -np.inf
+        c, lp = m.sample(x, u, base_margin=base if outputs > 1 else base[:, 0],
+                         return_log_probs=True)
+        assert list(c[5:8]) == [-1, 1, 0] and list(lp[5:8]) == [-np.inf, 0, 0]
+        assert (np.delete(c, 5) >= 0).all()
