@@ -93,10 +93,11 @@ constexpr uint32_t ROW_BLOCK = EMB_TPB * ROW_PIECES;
 
 // out[pos] = s * table[token(pos)]: the output in pieces of VEC cells, flat over the
 // workgroups, whose positions' tokens are found once and kept in LDS. Bound by the output:
-// 2M x 20 ids and vectors of 32 bytes take 200 us (1.44 GB, 7.2 TB/s; a fill reaches 6.9)
-// after 25 us of reading the ids. A vector's last
-// piece starts at dim - VEC, so that no piece is partial; the cells it shares with the
-// piece before are written twice, with the same value.
+// 2M x 20 ids and vectors of 32 bytes take 201 us (1.44 GB, 7.2 TB/s; a fill reaches 6.9)
+// after 26 us of reading the ids where a pass before has left these in the last-level cache,
+// and 320 to 335 in all where they come from memory. A vector's last piece starts at
+// dim - VEC, so that no piece is partial; the cells it shares with the piece before are
+// written twice, with the same value.
 // PAST: written past the caches (a parameter, as the compiler would join the two stores of a
 // branch into an ordinary one).
 template <class T, int VEC, int ID, bool DROP, bool PAST>
@@ -145,8 +146,8 @@ __global__ __launch_bounds__(EMB_TPB) void embed_rows_kernel(Positions P, const 
 // Ids that come from memory while their vectors are written past the caches wait behind
 // those writes, and what is written waits for them. So they are read into the last-level
 // cache first, a part of the rows at a time that it holds (TOUCH_BYTES of ids): 1.28 GB out
-// take 470 -> 320 us as float32 vectors of 32 bytes, 309 -> 236 of 128, 300 -> 234 as
-// bfloat16 of 256.
+// take 405 -> 320 to 335 us as vectors of 32 bytes. Where the ids are few beside the vectors it
+// costs a little: 221 -> 228 us for vectors of 128 bytes, 220 -> 225 for 256.
 constexpr uint64_t TOUCH_BYTES = 160ull << 20;
 
 __global__ __launch_bounds__(256) void touch_kernel(const uint8_t *p, uint64_t pieces) {
@@ -169,7 +170,7 @@ __global__ __launch_bounds__(256) void touch_kernel(const uint8_t *p, uint64_t p
 // out[row] = s * (sum over columns of table[token]). Column t goes to sum t % 4 and the
 // four sums are added in pairs, in both kernels, so a row's result does not depend on the
 // rows beside it. (Eight sums take 32 registers more: 100k rows of 100 trees, 64 cells of
-// bfloat16, 92 us against 80.)
+// bfloat16, 74 us against 66.)
 constexpr uint32_t SUMS = 4;
 __device__ __forceinline__ float join_sums(const float *a) {
     return (a[0] + a[1]) + (a[2] + a[3]);
@@ -207,7 +208,8 @@ __global__ __launch_bounds__(EMB_TPB) void embed_sum_kernel(Positions P, const T
         for (uint32_t i0 = threadIdx.x; i0 < rows << lg_c; i0 += 4 * EMB_TPB) {
             uint32_t id[4];
             Part part[4];
-            // (always a load, as in column_ids_kernel; rows << lg_c has whole steps of 256)
+            // (always a load, as in column_ids_kernel. A workgroup of few rows and columns has
+            // fewer positions than a step takes, 32 at least: the break below keeps to them)
 #pragma unroll
             for (uint32_t k = 0; k < 4; k++) {
                 const uint32_t i = i0 + k * EMB_TPB, t = min(t0 + (i & (cols - 1)), P.n_columns - 1);
@@ -781,11 +783,12 @@ __global__ __launch_bounds__(JOIN_TPB) void grad_join_kernel(Runs R, T *table) {
 // Each column's part of the table is summed over chunks of rows: a workgroup sorts a
 // chunk's ids of one column in LDS, sums the runs, and leaves a part of the table (with
 // the counts of its tokens) that the last kernel adds up chunk by chunk. Nothing is
-// sorted through memory, and the gradient rows that all columns of a chunk gather stay in
-// one XCD's L2: workgroups of one chunk have numbers equal modulo the 8 XCDs. 100k rows of
-// 100 trees, 64 cells of bfloat16: 22 us for the ids (their hashes), 98 for the sums (1.15 GB
-// gathered, 12 TB/s; instructions half of it) and 18 for the last; sorted by token they took
-// 596, and 16 chunks instead of 8 take 110 + 26.
+// sorted through memory, and where the chunks are a multiple of 8 the gradient rows that all
+// columns of a chunk gather stay in one XCD's L2: workgroups of one chunk then have numbers
+// equal modulo the 8 XCDs (column_plan prefers such numbers above 4). 100k rows of 100 trees, 64
+// cells of bfloat16: 22 us for the ids (their hashes), 101 for the sums (1.15 GB gathered, 11.4
+// TB/s; instructions half of it) and 18 for the last; sorted by token they took 596, and 16
+// chunks instead of 8 take 12 and 8 us more.
 constexpr uint32_t COL_TPB = 512;
 constexpr uint32_t COL_WAVES = COL_TPB / 64;
 constexpr uint32_t COL_ITEMS = 32;                       // rows of a thread at most

@@ -80,9 +80,10 @@ __device__ __forceinline__ void store_piece(T *p, const Piece<T, N> &r) {
 }
 
 // Outputs beyond what the caches keep for whoever reads them next are written past them:
-// 2M x 20 vectors of 32 bytes (1.28 GB out), their ids in the last-level cache, take 220 us
-// so, and 430 through the caches, where lines wait for their eviction. Smaller ones stay in
-// the cache for the next kernel.
+// 1.28 GB of vectors of 32 bytes (2M x 20 ids) take 320 to 335 us so, and 428 through the
+// caches, where lines wait for their eviction; of 128 bytes 228 and 291, of 256 as bfloat16
+// 225 and 287 (ids and outputs of another pass before them in the caches). Smaller ones stay
+// in the cache for the next kernel.
 constexpr uint64_t STREAM_BYTES = 128ull << 20;
 template <class T, int N>
 __device__ __forceinline__ void stream_piece(T *p, const Piece<T, N> &r) {

@@ -734,13 +734,14 @@ enum { FBH_ID_I32 = 0, FBH_ID_I64 = 1, FBH_ID_F32 = 2 };
  * table of n_tokens vectors of dim cells that they stand for. Column t's ids are
  * 0 .. first[t + 1] - first[t] - 1 and take table rows from first[t] on (first:
  * n_columns + 1 offsets from 0 to n_tokens, none below the one before, at most
- * 32768 columns); with first NULL every column's ids are the table's rows. FBH_ID_F32 are whole numbers as FBH_PREDICT_LEAF
- * writes them. A position whose id is anything else (negative, too large, no
- * whole number) takes and gives nothing; so does one that is dropped: with
- * drop > 0 each position stays with probability 1 - drop, drawn from seed and
- * the position's number (row * n_columns + column) as fbh_dropout draws its
- * elements, and what stays is scaled by 1 / (1 - drop). scale / (1 - drop) has to be
- * a finite float. dim at most 32768; at most 2^31 - 1 columns where they are summed. */
+ * 32768 columns); with first NULL every column's ids are the table's rows.
+ * FBH_ID_F32 are whole numbers as FBH_PREDICT_LEAF writes them. A position whose id
+ * is anything else (negative, too large, no whole number) takes and gives nothing;
+ * so does one that is dropped: with drop > 0 each position stays with probability
+ * 1 - drop, drawn from seed and the position's number (row * n_columns + column) as
+ * fbh_dropout draws its elements, and what stays is scaled by 1 / (1 - drop).
+ * scale / (1 - drop) has to be a finite float. dim at most 32768; at most 2^31 - 1
+ * columns where they are summed. */
 typedef struct {
     uint64_t n_rows;
     uint32_t n_columns;
