@@ -162,9 +162,9 @@ class Vocabulary:
             self.first.record_stream(_torch.cuda.current_stream(self.first.device))
             self._streams.add(stream)
 
-    def __getstate__(self):
+    def __setstate__(self, state):
         # (a copy's tensor has not been used on any stream yet)
-        return {**self.__dict__, "_streams": set()}
+        self.__dict__.update(state, _streams=set())
 
     def __repr__(self):
         return (f"Vocabulary({self.n_columns} columns, {self.n_tokens} tokens, "

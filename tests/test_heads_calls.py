@@ -184,3 +184,14 @@ def test_rows_of_too_many_columns_to_sum_are_refused(columns):
     e.first, e.n_columns, e.most_ids = None, columns, 0
     with pytest.raises(ValueError, match="2147483647 columns"):
         N.check_hip(N.hip().fbh_embed_rows(0, C.byref(e), 64, 64, None))
+
+
+def test_a_copied_vocabulary_has_been_used_on_no_stream():
+    """Also one that was stored without the streams it had been used on."""
+    voc = _vocabulary([3, 4])
+    voc._streams = {0, 77}
+    for v in (copy.copy(voc), copy.deepcopy(voc), pickle.loads(pickle.dumps(voc))):
+        assert v._streams == set() and torch.equal(v.first, voc.first)
+    assert voc._streams == {0, 77}
+    del voc._streams
+    assert pickle.loads(pickle.dumps(voc))._streams == set()
