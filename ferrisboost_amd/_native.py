@@ -276,6 +276,9 @@ HIP_SYMBOLS = [
     "fbh_saabas_contribs", "fbh_predict", "fbh_predict_device", "fbh_shap_contribs_noalloc",
     "fbh_embed_rows", "fbh_embed_grad_bytes", "fbh_embed_grad", "fbh_dropout",
     "fbh_sample_classes", "fbh_sample_classes_host", "fbh_sample_bytes",
+    "fbh_layer_norm", "fbh_layer_norm_grad_bytes", "fbh_layer_norm_grad", "fbh_route_bytes",
+    "fbh_route", "fbh_to_experts", "fbh_from_experts", "fbh_from_experts_grad",
+    "fbh_adamw_step", "fbh_adamw_moments",
 ]
 TRAIN_SYMBOLS = [
     "fbt_last_error", "fbt_train", "fbt_train_cuts", "fbt_train_rows", "fbt_last_stats",
@@ -410,6 +413,22 @@ def hip() -> C.CDLL:
         L.fbh_sample_bytes.argtypes = [C.c_uint64, C.c_uint32]
         L.fbh_sample_bytes.restype = C.c_uint64
         L.fbh_sample_classes_host.argtypes = [C.c_int, P, C.c_uint64, C.c_uint32, P, P, P, P]
+        L.fbh_layer_norm.argtypes = [C.c_int] + [P] * 7
+        L.fbh_layer_norm_grad_bytes.argtypes = [P]
+        L.fbh_layer_norm_grad_bytes.restype = C.c_uint64
+        L.fbh_layer_norm_grad.argtypes = [C.c_int] + [P] * 9 + [C.c_uint64, P]
+        L.fbh_route_bytes.argtypes = [C.c_uint64, C.c_uint32]
+        L.fbh_route_bytes.restype = C.c_uint64
+        L.fbh_route.argtypes = [C.c_int, P, C.c_uint32, C.c_uint64, C.c_uint32, P, P, P, P,
+                                C.c_uint64, P]
+        L.fbh_to_experts.argtypes = [C.c_int, P, P, C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32,
+                                     P, P]
+        L.fbh_from_experts.argtypes = [C.c_int, P, P, P, C.c_uint64, C.c_uint32, C.c_uint32,
+                                       C.c_uint32, P, P]
+        L.fbh_from_experts_grad.argtypes = [C.c_int, P, P, P, P, C.c_uint64, C.c_uint32,
+                                            C.c_uint32, C.c_uint32, P, P, P]
+        L.fbh_adamw_step.argtypes = [C.c_int, P, P, C.c_uint64, P]
+        L.fbh_adamw_moments.argtypes = [C.c_int, P, P, P, P]
         _hip = L
     return _hip
 

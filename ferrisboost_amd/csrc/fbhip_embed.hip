@@ -14,7 +14,6 @@
 namespace fbh {
 namespace {
 
-constexpr uint32_t NO_TOKEN = 0xFFFFFFFFu;
 constexpr uint32_t EMB_TPB = 256;
 constexpr uint32_t EMB_MAX_DIM = 32768;
 constexpr uint32_t EMB_MAX_COLUMNS = 32768;
@@ -28,21 +27,6 @@ struct Positions {
     uint64_t key;
     uint32_t threshold;
 };
-
-template <int ID>
-__device__ __forceinline__ uint32_t load_id(const void *ids, uint64_t at) {
-    if (ID == FBH_ID_I32) {
-        const int32_t v = static_cast<const int32_t *>(ids)[at];
-        return (uint32_t)v;  // (negative: above any column)
-    } else if (ID == FBH_ID_I64) {
-        const int64_t v = static_cast<const int64_t *>(ids)[at];
-        return (uint64_t)v < NO_TOKEN ? (uint32_t)v : NO_TOKEN;
-    } else {
-        const float v = static_cast<const float *>(ids)[at];
-        const uint32_t u = v >= 0.0f && v < 4294967040.0f ? (uint32_t)v : NO_TOKEN;
-        return (float)u == v ? u : NO_TOKEN;
-    }
-}
 
 // A column's part of the table, inside it whatever `first` says.
 struct Part {
@@ -383,31 +367,6 @@ __global__ __launch_bounds__(SORT_TPB) void sort_count_kernel(Positions P, SortF
     }
     __syncthreads();
     if (threadIdx.x <= mask) counts[(uint64_t)threadIdx.x * S.blocks + blockIdx.x] = c[threadIdx.x];
-}
-
-// The lanes that are `in` with this lane's digit.
-__device__ __forceinline__ uint64_t same_digit(bool in, uint32_t digit, uint32_t bits) {
-    uint64_t same = __ballot(in);
-    for (uint32_t b = 0; b < bits; b++) {
-        const bool one = (digit >> b) & 1;
-        const uint64_t ones = __ballot(one);
-        same &= one ? ones : ~ones;
-    }
-    return same;
-}
-// Takes places from a counter that only this wave uses: what it held, plus the number of
-// lower lanes in `same`.
-__device__ __forceinline__ uint32_t take_places(uint32_t *counter, bool in, uint64_t same) {
-    const uint32_t below = __popcll(same & ((1ull << (threadIdx.x & 63)) - 1));
-    volatile uint32_t *c = counter;
-    uint32_t before = 0;
-    if (in) before = *c;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (in && below == 0) *c = before + __popcll(same);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    return before + below;
 }
 
 // A digit's counts to the positions before them in its own part; its total.
@@ -1187,13 +1146,6 @@ Positions positions_of(const fbh_embed *e) {
 // Whether buffer loads reach rows of row_bytes from p on: their bytes, in words.
 bool in_buffer(const void *p, uint64_t bytes, uint64_t row_bytes) {
     return bytes <= BUFFER_MOST && row_bytes % 4 == 0 && reinterpret_cast<uintptr_t>(p) % 4 == 0;
-}
-
-// Cells of a piece: the largest power of two up to 16 bytes and the vector's width.
-uint32_t piece_cells(uint32_t dim, uint32_t dtype) {
-    uint32_t v = dtype == FBH_F32 ? 4 : 8;
-    while (v > dim) v /= 2;
-    return v;
 }
 
 template <class T, int VEC, int ID, bool DROP>

@@ -1,6 +1,7 @@
 // fbhip_heads.h -- what the kernels of the heads on a model's outputs share
-// (fbhip_embed.hip, fbhip_dropout.hip, fbhip_sample.hip): cell types, 16-byte
-// pieces, the counter-based generator, errors and the calling device.
+// (fbhip_embed.hip, fbhip_dropout.hip, fbhip_sample.hip, fbhip_norm.hip, fbhip_route.hip,
+// fbhip_adamw.hip): cell types, 16-byte pieces, ids, the counter-based generator, errors and
+// the calling device.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -79,6 +80,13 @@ __device__ __forceinline__ void store_piece(T *p, const Piece<T, N> &r) {
     __builtin_memcpy(p, &r, sizeof(r));
 }
 
+// Cells of a piece: the largest power of two up to 16 bytes and the vector's width.
+inline uint32_t piece_cells(uint32_t dim, uint32_t dtype) {
+    uint32_t v = dtype == FBH_F32 ? 4 : 8;
+    while (v > dim) v /= 2;
+    return v;
+}
+
 // Outputs beyond what the caches keep for whoever reads them next are written past them:
 // 1.28 GB of vectors of 32 bytes (2M x 20 ids) take 320 to 335 us so, and 428 through the
 // caches, where lines wait for their eviction; of 128 bytes 228 and 291, of 256 as bfloat16
@@ -119,6 +127,50 @@ __device__ __forceinline__ Piece<T, N> load_offset(__amdgpu_buffer_rsrc_t r, uin
         __builtin_memcpy(&p, &q, 4);
     }
     return p;
+}
+
+// An id as it lies in memory, or a number above any table's rows where it is no whole number
+// of 0 and more.
+constexpr uint32_t NO_TOKEN = 0xFFFFFFFFu;
+template <int ID>
+__device__ __forceinline__ uint32_t load_id(const void *ids, uint64_t at) {
+    if (ID == FBH_ID_I32) {
+        const int32_t v = static_cast<const int32_t *>(ids)[at];
+        return (uint32_t)v;  // (negative: above any column)
+    } else if (ID == FBH_ID_I64) {
+        const int64_t v = static_cast<const int64_t *>(ids)[at];
+        return (uint64_t)v < NO_TOKEN ? (uint32_t)v : NO_TOKEN;
+    } else {
+        const float v = static_cast<const float *>(ids)[at];
+        const uint32_t u = v >= 0.0f && v < 4294967040.0f ? (uint32_t)v : NO_TOKEN;
+        return (float)u == v ? u : NO_TOKEN;
+    }
+}
+
+// ---- Stable ranks of items with equal keys.
+// The lanes that are `in` with this lane's digit.
+__device__ __forceinline__ uint64_t same_digit(bool in, uint32_t digit, uint32_t bits) {
+    uint64_t same = __ballot(in);
+    for (uint32_t b = 0; b < bits; b++) {
+        const bool one = (digit >> b) & 1;
+        const uint64_t ones = __ballot(one);
+        same &= one ? ones : ~ones;
+    }
+    return same;
+}
+// Takes places from a counter that only this wave uses: what it held, plus the number of
+// lower lanes in `same`.
+__device__ __forceinline__ uint32_t take_places(uint32_t *counter, bool in, uint64_t same) {
+    const uint32_t below = __popcll(same & ((1ull << (threadIdx.x & 63)) - 1));
+    volatile uint32_t *c = counter;
+    uint32_t before = 0;
+    if (in) before = *c;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (in && below == 0) *c = before + __popcll(same);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    return before + below;
 }
 
 // ---- The counter-based generator: element e takes half of the 64 bits that the

@@ -7,6 +7,11 @@ device) and class margins, and its rows hold categorical codes. What follows the
                       are or summed over a row's columns, and the table's gradient
   dropout             while they are learned, from (seed, element) alone: no mask
   sample              classes drawn from margins (Model.sample does it on host arrays)
+  layer_norm          a row's cells to mean 0 and variance 1, with its gradients
+  Routes, to_experts, from_experts
+                      rows by their ids (a tree's leaves, say, each with a model of its own)
+                      and back, weighted, with the gradients
+  AdamW               the step of all parameters at once, moments in 32 bits or in 8
 
     model = fb.train({"objective": "multi:softprob", "num_class": 4, ...}, X, label=y)
     leaves = torch.from_numpy(model.predict(X, pred_leaf=True)).cuda()
@@ -14,16 +19,20 @@ device) and class margins, and its rows hold categorical codes. What follows the
     table = torch.zeros(voc.n_tokens, 64, device="cuda", requires_grad=True)
     h = fb.heads.embed(table, leaves, voc, pooled=True, drop=0.1, seed=step)
     h = fb.heads.dropout(h, 0.1, seed=step + 1)
+    h = fb.heads.layer_norm(h, gain, bias)
+    loss = torch.nn.functional.cross_entropy(h @ W, labels)
+    loss.backward()
+    optimizer.step()                           # fb.heads.AdamW([table, gain, bias, W], lr=1e-3)
     classes, log_probs = fb.heads.sample(h @ W, torch.rand(len(h), device="cuda"), top_p=0.9)
 
 Tensors are torch tensors on one gfx950 device; torch must be imported before the
 package's first call, so that both share one HIP runtime. Kernels are hand-written HIP
 behind the C ABI of include/fbhip.h, enqueued on torch's current stream of the tensors'
 device; nothing waits, results are the same in every call, and all of it can be captured
-into a graph. A tensor that is not contiguous is copied first. embed and dropout take
-part in autograd, in reverse mode; tensors with a tangent of forward mode are refused. What
-embed_grad and sample give has no gradient. Bad arguments are ValueErrors, device failures
-RuntimeErrors.
+into a graph. A tensor that is not contiguous is copied first. embed, dropout, layer_norm,
+to_experts and from_experts take part in autograd, in reverse mode; tensors with a tangent of
+forward mode are refused. What embed_grad, layer_norm_grad, from_experts_grad and sample give
+has no gradient. Bad arguments are ValueErrors, device failures RuntimeErrors.
 """
 
 from __future__ import annotations
@@ -35,7 +44,8 @@ import numpy as np
 
 from . import _native as N
 
-__all__ = ["Vocabulary", "embed", "embed_grad", "dropout", "sample"]
+__all__ = ["Vocabulary", "embed", "embed_grad", "dropout", "sample", "layer_norm",
+           "layer_norm_grad", "Routes", "to_experts", "from_experts", "from_experts_grad", "AdamW"]
 
 _torch = None
 _L = None
@@ -47,6 +57,9 @@ _forward_ad = None
 # operation's time is its host time.
 _EMBED = struct.Struct("QIIIIIIPPdQfI")
 _OPTIONS = struct.Struct("PPPPfiff")
+_NORM = struct.Struct("QIIIf")                 # fbh_norm
+_ADAMW = struct.Struct("IfdddPQQPPPP")         # fbh_adamw
+_ADAMW_TENSOR = struct.Struct("PPPQQfI")       # fbh_adamw_tensor
 _MOST = float(np.finfo(np.float32).max)
 
 
@@ -125,7 +138,26 @@ def _scale(scale) -> float:
     return scale
 
 
-class Vocabulary:
+class _Kept:
+    """Device memory that an object keeps for its calls: copies of it have been used on no
+    stream yet."""
+
+    def _tensors(self):
+        raise NotImplementedError
+
+    def _used_on(self, stream: int):
+        """Keeps that memory from the allocator until the work now on this stream, the current
+        one, has passed, also when the object is dropped before."""
+        if stream not in self._streams:
+            for x in self._tensors():
+                x.record_stream(_torch.cuda.current_stream(x.device))
+            self._streams.add(stream)
+
+    def __setstate__(self, state):
+        self.__dict__.update(state, _streams=set())
+
+
+class Vocabulary(_Kept):
     """The table rows of several columns' ids: column t's ids 0 .. sizes[t] - 1 are rows
     first[t] .. first[t] + sizes[t] - 1 of a table of n_tokens rows (a model's trees:
     Model.leaf_vocabulary(); categorical columns: their numbers of codes). It may be copied,
@@ -155,16 +187,8 @@ class Vocabulary:
             raise ValueError(f"device must be a GPU, got {device!r}")
         self._streams = set()
 
-    def _used_on(self, stream: int):
-        """Keeps the offsets' memory from the allocator until the work now on this stream, the
-        current one, has passed, also when the vocabulary is dropped before."""
-        if stream not in self._streams:
-            self.first.record_stream(_torch.cuda.current_stream(self.first.device))
-            self._streams.add(stream)
-
-    def __setstate__(self, state):
-        # (a copy's tensor has not been used on any stream yet)
-        self.__dict__.update(state, _streams=set())
+    def _tensors(self):
+        return (self.first,)
 
     def __repr__(self):
         return (f"Vocabulary({self.n_columns} columns, {self.n_tokens} tokens, "
@@ -249,7 +273,51 @@ def _functions():
         def backward(ctx, grad):
             return (dropout(grad, *ctx.rest),) + (None,) * 3
 
-    return Embed, Dropout
+    class LayerNorm(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, weight, bias, eps):
+            out, stats = _layer_norm(x, weight, bias, eps, True)
+            ctx.save_for_backward(x, stats, weight)
+            ctx.eps = eps
+            ctx.mark_non_differentiable(stats)
+            return out, stats
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, grad, _):
+            x, stats, weight = ctx.saved_tensors
+            return _layer_norm_grad(_device_tensor(grad, "grad"), x, stats, weight,
+                                    ctx.needs_input_grad[:3]) + (None,)
+
+    class ToExperts(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, routes, place):
+            ctx.routes = routes
+            ctx.save_for_backward(place)
+            return _to_experts(x, routes, place)
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, grad):
+            (place,) = ctx.saved_tensors
+            return _from_experts(_device_tensor(grad, "grad"), ctx.routes, place, None), None, None
+
+    class FromExperts(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, y, weights, routes, place):
+            ctx.routes = routes
+            ctx.save_for_backward(y if weights is not None and weights.requires_grad else None,
+                                  weights, place)
+            return _from_experts(y, routes, place, weights)
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, grad):
+            y, weights, place = ctx.saved_tensors
+            return _from_experts_grad(_device_tensor(grad, "grad"), y, ctx.routes, place, weights,
+                                      *ctx.needs_input_grad[:2]) + (None, None)
+
+    return Embed, Dropout, LayerNorm, ToExperts, FromExperts
 
 
 def embed(table, ids, vocabulary: Vocabulary | None = None, *, scale: float = 1.0,
@@ -451,3 +519,487 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if rc:
         N.check_hip(rc)
     return classes, log_probs
+
+
+# ------------------------------------------------------------------- layer norm
+def _eps(eps) -> float:
+    eps = float(eps)
+    if not 2.0 ** -126 <= eps <= _MOST:
+        raise ValueError(f"eps must be a positive normal float32, got {eps}")
+    return eps
+
+
+def _norm_of(x, weight, eps: float) -> bytes:
+    """The call's fbh_norm."""
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 32768:
+        raise ValueError(f"x must be (..., 1 to 32768 cells), got shape {tuple(x.shape)}")
+    return _NORM.pack(x.numel() // x.shape[-1], x.shape[-1], _cells(x, "x"),
+                      0 if weight is None else _cells(weight, "weight"), eps)
+
+
+def _vector(v, x, what: str):
+    v = _beside(_device_tensor(v, what), x, what)
+    if v.dim() != 1 or v.shape[0] != x.shape[-1]:
+        raise ValueError(f"{what} must have shape ({x.shape[-1]},), got {tuple(v.shape)}")
+    return v
+
+
+def _layer_norm(x, weight, bias, eps, stats: bool):
+    a = _norm_of(x, weight, eps)
+    out = _torch.empty_like(x)
+    kept = x.new_empty(x.shape[:-1] + (2,), dtype=_torch.float32) if stats else None
+    dev = x.get_device()
+    rc = _L.fbh_layer_norm(dev, a, x.data_ptr(), 0 if weight is None else weight.data_ptr(),
+                           0 if bias is None else bias.data_ptr(), out.data_ptr(),
+                           kept.data_ptr() if stats else 0, _raw_stream(dev))
+    if rc:
+        N.check_hip(rc)
+    return out, kept
+
+
+def layer_norm(x, weight=None, bias=None, *, eps: float = 1e-5, stats: bool = False):
+    """(x - mean) / sqrt(variance + eps) * weight + bias over the last axis of `x` (up to
+    32768 cells), computed in float32 and rounded once. weight and bias are of x's type or any
+    other of the three, both of the same; bias needs a weight. With stats=True also what
+    layer_norm_grad() takes: each row's mean and 1 / sqrt(variance + eps), (..., 2) float32."""
+    torch = _need_torch()
+    x = _device_tensor(x, "x")
+    _norm_of(x, None, eps := _eps(eps))
+    if weight is not None:
+        weight = _vector(weight, x, "weight")
+        _cells(weight, "weight")
+        if bias is not None:
+            bias = _vector(bias, x, "bias")
+            if bias.dtype != weight.dtype:
+                raise ValueError(f"bias is {bias.dtype}, weight {weight.dtype}")
+    elif bias is not None:
+        raise ValueError("a bias needs a weight")
+    if torch.is_grad_enabled() and (x.requires_grad or
+                                    (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
+        out = _functions()[2].apply(x, weight, bias, eps)
+    else:
+        out = _layer_norm(x, weight, bias, eps, stats)
+    return out if stats else out[0]
+
+
+def _layer_norm_grad(grad, x, stats, weight, wanted):
+    a = _norm_of(x, weight, 1.0)
+    dx = _torch.empty_like(x) if wanted[0] else None
+    dw = _torch.empty_like(weight) if wanted[1] else None
+    db = _torch.empty_like(weight) if wanted[2] else None
+    size = _L.fbh_layer_norm_grad_bytes(a) if wanted[1] or wanted[2] else 0
+    work = grad.new_empty(size, dtype=_torch.uint8) if size else None
+    at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    dev = x.get_device()
+    rc = _L.fbh_layer_norm_grad(dev, a, grad.data_ptr(), x.data_ptr(), stats.data_ptr(),
+                                at(weight), at(dx), at(dw), at(db), at(work), size,
+                                _raw_stream(dev))
+    if rc:
+        N.check_hip(rc)
+    return dx, dw, db
+
+
+def layer_norm_grad(grad, x, stats, weight=None):
+    """The gradients of layer_norm()'s x, weight and bias for `grad`, that of its output:
+    (dx, dweight, dbias), the last two in weight's type and None without one. x, weight and
+    `stats` are those of the call layer_norm(..., stats=True). Sums over rows are taken in a
+    fixed order, a workgroup's in float32 and theirs in float64, and rounded once.
+    (layer_norm() does this in backward(); a captured training step can call it by itself.)"""
+    torch = _need_torch()
+    x = _device_tensor(x, "x")
+    grad = _beside(_device_tensor(grad, "grad"), x, "grad")
+    stats = _beside(_device_tensor(stats, "stats"), x, "stats")
+    _norm_of(x, None, 1.0)
+    if grad.shape != x.shape or grad.dtype != x.dtype:
+        raise ValueError(f"grad is {grad.dtype} of {tuple(grad.shape)}, x {x.dtype} of "
+                         f"{tuple(x.shape)}")
+    if stats.dtype != torch.float32 or stats.shape != x.shape[:-1] + (2,):
+        raise ValueError(f"stats must be float32 of {tuple(x.shape[:-1]) + (2,)}, got "
+                         f"{stats.dtype} of {tuple(stats.shape)}")
+    if weight is not None:
+        weight = _vector(weight, x, "weight")
+        _cells(weight, "weight")
+    return _layer_norm_grad(grad, x, stats, weight, (True, weight is not None,
+                                                     weight is not None))
+
+
+# ------------------------------------------------------------------- experts
+class Routes(_Kept):
+    """The positions of an id matrix `ids` (..., columns) in the order of their ids, each id
+    from 0 to n_experts - 1 an expert (at most 1024): a tree's leaves, say, or a router's
+    choices. An id that is anything else (-1) has no expert; ids are int32, int64, or float32
+    as predict(pred_leaf=True) gives leaf ids.
+
+    order   positions (row * columns + column) by expert, equal ones in their order, those
+            without an expert behind all others; int32
+    place   the row in that order of every position, of ids' shape, or -1 - row of one without
+            an expert; int32
+    starts  expert e's rows are starts[e] .. starts[e + 1] - 1; int32, n_experts + 1 values
+
+    It is used with to_experts() and from_experts(), on any stream of its device that has
+    waited for the one that made it."""
+
+    def __init__(self, ids, n_experts: int):
+        torch = _need_torch()
+        ids = _device_tensor(ids, "ids")
+        code = _IDS.get(ids.dtype)
+        if code is None:
+            raise ValueError(f"ids must be int32, int64 or float32, got {ids.dtype}")
+        if ids.dim() < 1:
+            raise ValueError("ids must have a last axis of columns")
+        n_experts = _whole(n_experts, "n_experts")
+        if not 1 <= n_experts <= 1024:
+            raise ValueError(f"n_experts must be in 1..=1024, got {n_experts}")
+        n = ids.numel()
+        if n >> 31:
+            raise ValueError(f"at most 2^31 - 1 positions, got {n}")
+        self.n_experts = n_experts
+        self.order = ids.new_empty(n, dtype=torch.int32)
+        self.place = ids.new_empty(ids.shape, dtype=torch.int32)
+        self.starts = ids.new_empty(n_experts + 1, dtype=torch.int32)
+        dev = ids.get_device()
+        size = _L.fbh_route_bytes(n, n_experts)
+        work = ids.new_empty(size, dtype=torch.uint8)
+        stream = _raw_stream(dev)
+        rc = _L.fbh_route(dev, ids.data_ptr(), code, n, n_experts, self.order.data_ptr(),
+                          self.place.data_ptr(), self.starts.data_ptr(), work.data_ptr(), size,
+                          stream)
+        if rc:
+            N.check_hip(rc)
+        self._streams = {stream}
+
+    def _tensors(self):
+        return self.order, self.place, self.starts
+
+    def __repr__(self):
+        return f"Routes({tuple(self.place.shape)} ids, {self.n_experts} experts)"
+
+
+def _routes(routes, like):
+    if not isinstance(routes, Routes):
+        raise ValueError(f"routes must be Routes, got {type(routes).__name__}")
+    return _beside(routes.place, like, "the routes")
+
+
+def _vectors(x, what: str, lead):
+    """x as rows of 1 to 32768 cells with that leading shape."""
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 32768 or tuple(x.shape[:-1]) != lead:
+        raise ValueError(f"{what} must have shape {lead} and a last axis of 1 to 32768 cells, got "
+                         f"{tuple(x.shape)}")
+    _cells(x, what)
+    return x
+
+
+def _to_experts(x, routes, place):
+    n = place.numel()
+    out = x.new_empty((n, x.shape[-1]))
+    if n:
+        dev = x.get_device()
+        stream = _raw_stream(dev)
+        routes._used_on(stream)
+        rc = _L.fbh_to_experts(dev, x.data_ptr(), place.data_ptr(), n // place.shape[-1],
+                               place.shape[-1], x.shape[-1], _cells(x, "x"), out.data_ptr(),
+                               stream)
+        if rc:
+            N.check_hip(rc)
+    return out
+
+
+def to_experts(x, routes: Routes):
+    """The rows of `x` (..., cells), with the leading shape of the routes' ids, in the order of
+    the routes: (positions, cells). Expert e's are rows starts[e] .. starts[e + 1] - 1; rows
+    behind the last expert's are zeros."""
+    torch = _need_torch()
+    x = _device_tensor(x, "x")
+    place = _routes(routes, x)
+    _vectors(x, "x", tuple(place.shape[:-1]))
+    if x.requires_grad and torch.is_grad_enabled():
+        return _functions()[3].apply(x, routes, place)
+    return _to_experts(x, routes, place)
+
+
+def _from_experts(y, routes, place, weights):
+    out = y.new_empty(place.shape[:-1] + y.shape[-1:])
+    if not place.numel():
+        return out.zero_()
+    dev = y.get_device()
+    stream = _raw_stream(dev)
+    routes._used_on(stream)
+    rc = _L.fbh_from_experts(dev, y.data_ptr(), place.data_ptr(),
+                             0 if weights is None else weights.data_ptr(),
+                             place.numel() // place.shape[-1], place.shape[-1], y.shape[-1],
+                             _cells(y, "y"), out.data_ptr(), stream)
+    if rc:
+        N.check_hip(rc)
+    return out
+
+
+def _weights(weights, place):
+    weights = _beside(_device_tensor(weights, "weights"), place, "weights")
+    if weights.dtype != _torch.float32 or weights.shape != place.shape:
+        raise ValueError(f"weights must be float32 of {tuple(place.shape)}, got {weights.dtype} of "
+                         f"{tuple(weights.shape)}")
+    return weights
+
+
+def from_experts(y, routes: Routes, weights=None):
+    """What experts have given for the rows of to_experts(), `y` (positions, cells), back at
+    its rows: for each, the sum over its columns of weights[..., column] * the position's row
+    of y, in float32 and rounded once. weights (the shape of ids, float32) may be None: 1. A
+    position without an expert gives nothing, whatever its row of y holds."""
+    torch = _need_torch()
+    y = _device_tensor(y, "y")
+    place = _routes(routes, y)
+    _vectors(y, "y", (place.numel(),))
+    if weights is not None:
+        weights = _weights(weights, place)
+    if torch.is_grad_enabled() and (y.requires_grad or
+                                    (weights is not None and weights.requires_grad)):
+        return _functions()[4].apply(y, weights, routes, place)
+    return _from_experts(y, routes, place, weights)
+
+
+def _from_experts_grad(grad, y, routes, place, weights, want_y: bool, want_weights: bool):
+    n = place.numel()
+    dy = grad.new_empty((n, grad.shape[-1])) if want_y else None
+    dw = _torch.empty_like(weights) if want_weights else None
+    if n and (want_y or want_weights):
+        at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+        dev = grad.get_device()
+        stream = _raw_stream(dev)
+        routes._used_on(stream)
+        rc = _L.fbh_from_experts_grad(dev, grad.data_ptr(), at(y), place.data_ptr(), at(weights),
+                                      n // place.shape[-1], place.shape[-1], grad.shape[-1],
+                                      _cells(grad, "grad"), at(dy), at(dw), stream)
+        if rc:
+            N.check_hip(rc)
+    return dy, dw
+
+
+def from_experts_grad(grad, y, routes: Routes, weights=None):
+    """The gradients of from_experts()'s y and weights for `grad`, that of its output: (dy,
+    dweights), the second None without weights. Rows of dy without an expert are zeros.
+    (from_experts() does this in backward(); a captured training step can call it by itself.
+    to_experts()'s gradient is from_experts() without weights.)"""
+    _need_torch()
+    grad = _device_tensor(grad, "grad")
+    place = _routes(routes, grad)
+    _vectors(grad, "grad", tuple(place.shape[:-1]))
+    y = _beside(_device_tensor(y, "y"), grad, "y")
+    if tuple(y.shape) != (place.numel(), grad.shape[-1]) or y.dtype != grad.dtype:
+        raise ValueError(f"y must be {grad.dtype} of {(place.numel(), grad.shape[-1])}, got "
+                         f"{y.dtype} of {tuple(y.shape)}")
+    if weights is not None:
+        weights = _weights(weights, place)
+    return _from_experts_grad(grad, y, routes, place, weights, True, weights is not None)
+
+
+# ------------------------------------------------------------------- AdamW
+class AdamW(_Kept):
+    """AdamW over `params`, all in one step: for gradient g of a cell w at step t,
+
+        m = beta1 m + (1 - beta1) g,  s = beta2 s + (1 - beta2) g^2
+        w = w (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(s / (1 - beta2^t)) + eps)
+
+    in float32. params are contiguous tensors of one device; one of 16 bits has a float32 copy
+    in `masters`, which is what the steps move and round into it (call take_params() after
+    writing into such a parameter). weight_decay is a number, or a list of one for each
+    parameter; lr, an attribute, a number, or a float32 tensor of one value on the device,
+    which a step reads when it runs. The steps are counted on the device too, so a captured
+    step goes on at each replay.
+
+    bits=32 keeps m and s in float32, bits=8 in a byte each and an exponent for 256 cells:
+    small floats with 3 bits behind the point, rounded up or down at random (from `seed`, the
+    step and the cell, so the same in every run) with the new value as their mean, as a step
+    moves s by less than half the distance of its neighbours. What is not finite is NaN then.
+
+    The state of all parameters is flat: parameter i's cells are first[i] .. first[i] + n - 1
+    of mean and square, first[i] a multiple of 256 and what lies between zeros."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+                 weight_decay=0.01, *, bits: int = 32, seed: int = 0):
+        torch = _need_torch()
+        self.params = [params] if isinstance(params, torch.Tensor) else list(params)
+        if not self.params:
+            raise ValueError("no parameters")
+        betas = tuple(float(b) for b in betas)
+        if len(betas) != 2 or not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError(f"betas must be two numbers in [0, 1), got {betas}")
+        if bits not in (8, 32):
+            raise ValueError(f"bits must be 8 or 32, got {bits!r}")
+        self.lr, self.betas, self.eps, self.bits = lr, betas, _eps(eps), int(bits)
+        self.seed = _seed(seed)
+        n = len(self.params)
+        decays = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else (
+            [weight_decay] * n)
+        self.weight_decay = [float(d) for d in decays]
+        if len(decays) != n or not all(0.0 <= d <= _MOST for d in self.weight_decay):
+            raise ValueError(f"weight_decay must be a number, not negative, or a list of {n}")
+        self.first, at, spans = [], 0, []
+        for i, p in enumerate(self.params):
+            self._check(i, p)
+            self.first.append(at)
+            at += -(-p.numel() // 256) * 256
+            if p.numel():
+                spans.append((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()))
+        if at > 1 << 42:
+            raise ValueError(f"at most 2^42 cells, got {at}")
+        spans.sort()
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("parameters overlap in memory")
+        self._sizes = [p.numel() for p in self.params]
+        self._lr()
+        like = self.params[0]
+        cell = torch.float32 if bits == 32 else torch.uint8
+        self.mean, self.square = (torch.zeros(at, dtype=cell, device=like.device)
+                                  for _ in range(2))
+        self.scales = (torch.zeros((2, at // 256), dtype=torch.uint8, device=like.device)
+                       if bits == 8 else None)
+        self.masters = [None if p.dtype == torch.float32 else p.detach().float()
+                        for p in self.params]
+        self._clock = torch.zeros(3, dtype=torch.int64, device=like.device)
+        self._clock[1:] = 0x3FF0000000000000  # 1.0
+        self._streams = {_raw_stream(like.get_device())}
+
+    def _check(self, i: int, p):
+        if not isinstance(p, _torch.Tensor):
+            raise ValueError(f"parameter {i} must be a torch tensor, got {type(p).__name__}")
+        if not p.is_cuda:
+            raise ValueError(f"parameter {i} must be on a GPU, it is on {p.device}")
+        _cells(p, f"parameter {i}")
+        _beside(p, self.params[0], f"parameter {i}")
+        if not p.is_contiguous():
+            raise ValueError(f"parameter {i} must be contiguous")
+
+    def _tensors(self):
+        return [x for x in (self.mean, self.square, self.scales, self._clock, *self.masters)
+                if x is not None]
+
+    def _lr(self):
+        """The learning rate as a number, and the address of one on the device or 0."""
+        lr = self.lr
+        if isinstance(lr, _torch.Tensor):
+            _beside(_device_tensor(lr, "lr"), self.params[0], "lr")
+            if lr.dtype != _torch.float32 or lr.numel() != 1:
+                raise ValueError(f"lr must be one float32, got {lr.dtype} of {tuple(lr.shape)}")
+            return 0.0, lr.data_ptr()
+        lr = float(lr)
+        if not 0.0 <= lr <= _MOST:
+            raise ValueError(f"lr must be a finite float32, not negative, got {lr}")
+        return lr, 0
+
+    def _packed(self) -> bytes:
+        """The call's fbh_adamw."""
+        lr, lr_at = self._lr()
+        return _ADAMW.pack(self.bits, self.eps, *self.betas, lr, lr_at, self.seed,
+                           self.mean.numel(), self.mean.data_ptr(), self.square.data_ptr(),
+                           0 if self.scales is None else self.scales.data_ptr(),
+                           self._clock.data_ptr())
+
+    def step(self, grads=None):
+        """One step, in place, with the parameters' .grad or with `grads`, a list of one for
+        each parameter, of its shape and type. Every parameter needs one."""
+        torch = _torch
+        params = self.params
+        grads = [p.grad for p in params] if grads is None else list(grads)
+        if len(grads) != len(params):
+            raise ValueError(f"{len(grads)} gradients for {len(params)} parameters")
+        parts = []
+        for i, (p, g) in enumerate(zip(params, grads)):
+            if g is None:
+                raise ValueError(f"parameter {i} has no gradient")
+            g = grads[i] = _device_tensor(g, f"gradient {i}")
+            if g.dtype != p.dtype or g.shape != p.shape or g.device != p.device:
+                raise ValueError(f"gradient {i} is {g.dtype} of {tuple(g.shape)} on {g.device}, "
+                                 f"its parameter {p.dtype} of {tuple(p.shape)} on {p.device}")
+            if p.numel() != self._sizes[i] or not p.is_contiguous():
+                raise ValueError(f"parameter {i} has changed its shape")
+            w = self.masters[i]
+            parts.append(_ADAMW_TENSOR.pack(p.data_ptr(), g.data_ptr(),
+                                            0 if w is None else w.data_ptr(), self._sizes[i],
+                                            self.first[i], self.weight_decay[i], _CELLS[p.dtype]))
+        dev = params[0].get_device()
+        stream = _raw_stream(dev)
+        self._used_on(stream)
+        rc = _L.fbh_adamw_step(dev, self._packed(), b"".join(parts), len(parts), stream)
+        if rc:
+            N.check_hip(rc)
+        torch.autograd.graph.increment_version(params)
+
+    def zero_grad(self):
+        """Drops the parameters' gradients."""
+        for p in self.params:
+            p.grad = None
+
+    def moments(self):
+        """(mean, square) of all parameters, flat, as float32: with bits=32 the state itself,
+        with bits=8 new tensors of what it stands for. split() cuts them by parameter."""
+        if self.bits == 32:
+            return self.mean, self.square
+        out = [self.mean.new_empty(self.mean.numel(), dtype=_torch.float32) for _ in range(2)]
+        dev = self.mean.get_device()
+        stream = _raw_stream(dev)
+        self._used_on(stream)
+        rc = _L.fbh_adamw_moments(dev, self._packed(), out[0].data_ptr(), out[1].data_ptr(),
+                                  stream)
+        if rc:
+            N.check_hip(rc)
+        return out[0], out[1]
+
+    def split(self, flat):
+        """A flat tensor's parts as views in the parameters' shapes."""
+        return [flat[a:a + n].view(p.shape)
+                for a, n, p in zip(self.first, self._sizes, self.params)]
+
+    def take_params(self):
+        """Sets the float32 copies of 16-bit parameters to what these hold now."""
+        with _torch.no_grad():
+            for p, w in zip(self.params, self.masters):
+                if w is not None:
+                    w.copy_(p)
+
+    def state_dict(self) -> dict:
+        """What load_state_dict() takes: the steps done (waits for the device) and the state's
+        own tensors, of which what stores them later makes copies."""
+        clock = self._clock.cpu()
+        return {"step": int(clock[0]), "decays": clock[1:].view(_torch.float64).tolist(),
+                "bits": self.bits, "mean": self.mean, "square": self.square,
+                "scales": self.scales, "masters": list(self.masters)}
+
+    def load_state_dict(self, state: dict):
+        """Takes up a state of as many parameters of the same sizes, copying it. "decays" (the
+        betas' powers) follow from "step" where they are missing, "masters" from the
+        parameters."""
+        step = _whole(state["step"], "step")
+        if not 0 <= step < 1 << 62:
+            raise ValueError(f"step must be in 0..=2^62 - 1, got {step}")
+        if state.get("bits", self.bits) != self.bits:
+            raise ValueError(f"the state has {state['bits']} bits, the optimizer {self.bits}")
+        decays = state.get("decays")
+        decays = [b ** step for b in self.betas] if decays is None else [float(d) for d in decays]
+        if len(decays) != 2 or not all(0.0 <= d <= 1.0 for d in decays):
+            raise ValueError(f"decays must be two numbers in [0, 1], got {decays}")
+        masters = state.get("masters")
+        if masters is None:
+            masters = [None if w is None else p for p, w in zip(self.params, self.masters)]
+        if len(masters) != len(self.masters):
+            raise ValueError(f"{len(masters)} masters for {len(self.masters)} parameters")
+        pairs = [("mean", self.mean, state["mean"]), ("square", self.square, state["square"])]
+        if self.bits == 8:
+            pairs.append(("scales", self.scales, state["scales"]))
+        pairs += [(f"master {i}", to, m) for i, (to, m) in enumerate(zip(self.masters, masters))
+                  if to is not None]
+        for what, to, x in pairs:
+            if not isinstance(x, _torch.Tensor) or x.shape != to.shape or (
+                    x.dtype != to.dtype and not what.startswith("master")):
+                raise ValueError(f"{what} must be {to.dtype} of {tuple(to.shape)}")
+        with _torch.no_grad():
+            for _, to, x in pairs:
+                to.copy_(x)
+            words = struct.unpack("3q", struct.pack("qdd", step, *decays))
+            self._clock.copy_(_torch.tensor(words, dtype=_torch.int64))
+
+    def __repr__(self):
+        return (f"AdamW({len(self.params)} parameters, {sum(self._sizes)} cells, {self.bits} "
+                f"bits)")

@@ -829,6 +829,120 @@ int fbh_sample_classes_host(int device, const float *logits, uint64_t n_rows, ui
                             const float *uniforms, const fbh_sample_options *options,
                             int64_t *classes, float *log_probs);
 
+/* ---- Training heads: layer norm, rows handed to experts, an optimizer's step. */
+
+/* Layer norm over the cells of n_rows rows of dim (1 .. 32768): weight and bias are
+ * [dim] of weight_type. eps is a positive normal float. */
+typedef struct {
+    uint64_t n_rows;
+    uint32_t dim;
+    uint32_t dtype;        /* of rows and their gradients */
+    uint32_t weight_type;  /* of weight, bias and their gradients */
+    float eps;
+} fbh_norm;
+
+/* out = (x - mean) / sqrt(variance + eps) * weight + bias, a row's mean and variance
+ * over its cells (weight NULL: 1, bias NULL: 0). stats (may be NULL) gets each row's
+ * mean and 1 / sqrt(variance + eps), [n_rows][2]. Sums are taken in f32 in an order
+ * that depends on dim alone. out may be x. */
+int fbh_layer_norm(int device, const fbh_norm *a, const void *x, const void *weight,
+                   const void *bias, void *out, float *stats, void *stream);
+/* Device bytes of workspace that fbh_layer_norm_grad takes for dweight or dbias,
+ * 16-byte aligned; 0 for a call that it refuses. */
+uint64_t fbh_layer_norm_grad_bytes(const fbh_norm *a);
+/* The gradients for the output's gradient grad: dx [n_rows][dim] (may be grad or x),
+ * dweight and dbias [dim], summed over all rows (each may be NULL: not wanted); stats
+ * as fbh_layer_norm gave them. The rows of a workgroup are summed in f32, the
+ * workgroups' sums, at most 512, in f64. Orders of sums depend on n_rows and dim
+ * alone. work may be NULL where neither dweight nor dbias is wanted. */
+int fbh_layer_norm_grad(int device, const fbh_norm *a, const void *grad, const void *x,
+                        const float *stats, const void *weight, void *dx, void *dweight,
+                        void *dbias, void *work, uint64_t work_bytes, void *stream);
+
+/* Device bytes of workspace that fbh_route takes, 4-byte aligned; 0 for a call that it
+ * refuses. */
+uint64_t fbh_route_bytes(uint64_t n_positions, uint32_t n_experts);
+/* Positions sorted by the id that they hold, equal ones in their order: an id from 0
+ * to n_experts - 1 (at most 1024) is an expert, a position with anything else
+ * (negative, too large, no whole number) has none and comes behind all others.
+ * order[row] is the position in that row, place[position] its row r, or -1 - r where
+ * it has no expert; expert e has rows starts[e] .. starts[e + 1] - 1 (n_experts + 1
+ * values). At most 2^31 - 1 positions; id_type as in fbh_embed. */
+int fbh_route(int device, const void *ids, uint32_t id_type, uint64_t n_positions,
+              uint32_t n_experts, int32_t *order, int32_t *place, int32_t *starts, void *work,
+              uint64_t work_bytes, void *stream);
+/* Row place[i][j] of out [n_rows * n_columns][dim] is x[i], for every row i and column
+ * j; zeros where place is negative (row -1 - place). place is fbh_route's (places
+ * beyond the rows are taken to the last one). dim at most 32768. */
+int fbh_to_experts(int device, const void *x, const int32_t *place, uint64_t n_rows,
+                   uint32_t n_columns, uint32_t dim, uint32_t dtype, void *out, void *stream);
+/* out[i] = the sum over columns of weights[i][j] * y[place[i][j]] (weights NULL: 1), in
+ * f32 by column and rounded once; what place is negative for gives nothing, whatever y
+ * holds there. Without weights it is also the gradient of fbh_to_experts. */
+int fbh_from_experts(int device, const void *y, const int32_t *place, const float *weights,
+                     uint64_t n_rows, uint32_t n_columns, uint32_t dim, uint32_t dtype, void *out,
+                     void *stream);
+/* The gradients of fbh_from_experts for grad [n_rows][dim]: dy[place[i][j]] =
+ * weights[i][j] * grad[i] (zeros where place is negative), dweights[i][j] = the product
+ * of grad[i] and y[place[i][j]] summed in f32 (0 where place is negative). Either may
+ * be NULL: not wanted; y may be NULL without dweights. */
+int fbh_from_experts_grad(int device, const void *grad, const void *y, const int32_t *place,
+                          const float *weights, uint64_t n_rows, uint32_t n_columns, uint32_t dim,
+                          uint32_t dtype, void *dy, float *dweights, void *stream);
+
+/* One parameter of an AdamW step: n cells of dtype with their gradient, of the same
+ * type; master, of a 16-bit one, its f32 copy, which the step moves and rounds into
+ * param. Its moments are cells first .. first + n - 1 of the state (first a multiple
+ * of 256). */
+typedef struct {
+    void *param;
+    const void *grad;
+    float *master;
+    uint64_t n;
+    uint64_t first;
+    float weight_decay;
+    uint32_t dtype;
+} fbh_adamw_tensor;
+
+/* An AdamW step's numbers and state. mean and square hold n cells (a multiple of 256,
+ * zeros at first) of f32 or, with bits 8, of one byte, 16-byte aligned; scales, with
+ * bits 8, [2][n / 256] bytes. clock: 24 bytes, the steps done (int64) and the products
+ * of as many beta1 and beta2 (f64): 0, 1, 1 at first. lr, or where lr_at is not NULL the
+ * float there when the step runs.
+ *
+ * A byte of mean has a sign, 4 bits of exponent e and 3 of the mantissa f: (1 + f / 8) *
+ * 2^(e - 14 + E - 127), for e = 0 f / 8 * 2^(E - 13 - 127), with E its 256 cells'
+ * byte of scales[0] (at least 1): the exponent field of the largest one as a float. A
+ * byte of square, 5 bits of exponent and 3 of the mantissa: the same with 30 and 29 for
+ * 14 and 13, and scales[1]. 0x7F and 0xFF stand for what is not finite. */
+typedef struct {
+    uint32_t bits;  /* 8 or 32 */
+    float eps;      /* a positive normal float */
+    double beta1;
+    double beta2;
+    double lr;
+    const float *lr_at;
+    uint64_t seed;
+    uint64_t n;
+    void *mean;
+    void *square;
+    void *scales;
+    void *clock;
+} fbh_adamw;
+
+/* Step t (the clock's steps and one) of AdamW on every tensor:
+ *   m = beta1 m + (1 - beta1) g, s = beta2 s + (1 - beta2) g^2,
+ *   w = w (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(s / (1 - beta2^t)) + eps)
+ * in f32, and the clock goes on. With bits 8 the new moments are computed in f64, move w
+ * as f32 and are then rounded to one of the two bytes around them, up with the
+ * probability of what is cut off, to 2^-16: by the bits that fbh_dropout draws for seed
+ * + t and the cell of the state, the low 16 for mean, the high 16 for square; a square
+ * above 0 stays above 0. No two tensors may overlap, in memory or in the state. */
+int fbh_adamw_step(int device, const fbh_adamw *a, const fbh_adamw_tensor *tensors,
+                   uint64_t n_tensors, void *stream);
+/* The f32 values, n each, that moments of 8 bits stand for. */
+int fbh_adamw_moments(int device, const fbh_adamw *a, float *mean, float *square, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
