@@ -8,10 +8,13 @@
 // own sum) is taken out: rows far from 0 keep their cells' accuracy.
 #include "fbhip_heads.h"
 
+#include <algorithm>
+
 namespace fbh {
 namespace {
 
 constexpr uint32_t NORM_MAX_DIM = 32768;
+constexpr uint64_t NORM_BLOCKS = 2048;  // of a launch at most: they go through the rows in turn
 
 struct Norm {
     const void *weight, *bias;
@@ -77,137 +80,184 @@ __device__ __forceinline__ void sum_of_group(float (&v)[K], GroupSum<G, K> &lds,
     }
 }
 
-// A lane's cells: pieces of N that lie G * N cells apart. What is behind the row's end reads
-// as 0.
-template <class T, uint32_t G, uint32_t C>
-struct Cells {
-    static constexpr uint32_t N = 16 / sizeof(T);
-    static constexpr uint32_t P = C / N;
-    float v[C];
-
-    static __device__ __forceinline__ uint32_t column(uint32_t p) {
+// A lane's cells: pieces of N that lie G * N cells apart. A row's last piece starts at dim - N
+// wherever its lane's place is, so that every piece is whole: the `twice` first cells of it
+// are the lane's before it too, take no part in sums, and are stored by both with the same
+// value. Pieces behind the row are empty. (Rows of fewer cells than a piece have N = 1.)
+template <uint32_t N_, uint32_t G, uint32_t C>
+struct Place {
+    static constexpr uint32_t N = N_, P = C / N_;
+    uint32_t dim;
+    __device__ __forceinline__ uint32_t begin(uint32_t p) const {
         return (p * G + threadIdx.x % G) * N;
     }
-    template <class U>
-    __device__ __forceinline__ void load(const U *row, uint32_t dim) {
-#pragma unroll
-        for (uint32_t p = 0; p < P; p++) {
-            const uint32_t c = column(p);
-            if (c + N <= dim) {
-                const Piece<U, N> q = load_piece<U, N>(row + c);
-#pragma unroll
-                for (uint32_t i = 0; i < N; i++) v[p * N + i] = (float)q.v[i];
-            } else {
-#pragma unroll
-                for (uint32_t i = 0; i < N; i++)
-                    v[p * N + i] = c + i < dim ? (float)row[c + i] : 0.0f;
-            }
-        }
+    __device__ __forceinline__ bool empty(uint32_t p) const { return begin(p) >= dim; }
+    __device__ __forceinline__ uint32_t column(uint32_t p) const {
+        return min(begin(p), dim - N);
     }
-    __device__ __forceinline__ void load_typed(const void *p, uint32_t type, uint32_t dim) {
-        if (type == FBH_F32) load(static_cast<const float *>(p), dim);
-        else if (type == FBH_F16) load(static_cast<const _Float16 *>(p), dim);
-        else load(static_cast<const __bf16 *>(p), dim);
+    __device__ __forceinline__ uint32_t twice(uint32_t p) const { return begin(p) - column(p); }
+    // Whether the lane has cells that take no part.
+    __device__ __forceinline__ bool ragged() const {
+        bool r = false;
+#pragma unroll
+        for (uint32_t p = 0; p < P; p++) r |= begin(p) + N > dim;
+        return r;
+    }
+    // (of lanes with such cells)
+    __device__ __forceinline__ bool counts(uint32_t i) const {
+        return !empty(i / N) && i % N >= twice(i / N);
+    }
+};
+
+// Cells as they lie in memory, in words, so that a load is waited for where they are taken.
+template <class T, class L>
+struct Raw {
+    static constexpr uint32_t BYTES = L::N * sizeof(T), WORDS = (BYTES + 3) / 4;
+    uint32_t w[L::P][WORDS];
+
+    __device__ __forceinline__ void load(const T *row, L at) {
+#pragma unroll
+        for (uint32_t p = 0; p < L::P; p++)
+            if (!at.empty(p)) __builtin_memcpy(w[p], row + at.column(p), BYTES);
+    }
+    __device__ __forceinline__ float cell(uint32_t i) const {
+        T t;
+        __builtin_memcpy(&t, reinterpret_cast<const char *>(w[i / L::N]) + i % L::N * sizeof(T),
+                         sizeof(T));
+        return (float)t;
+    }
+};
+
+template <class L, uint32_t C>
+struct Cells {
+    float v[C];
+
+    template <class T>
+    __device__ __forceinline__ void take(const Raw<T, L> &r) {
+#pragma unroll
+        for (uint32_t i = 0; i < C; i++) v[i] = r.cell(i);
+    }
+    __device__ __forceinline__ void load_typed(const void *p, uint32_t type, L at) {
+        const auto load = [&](auto t) {
+            Raw<decltype(t), L> r = {};
+            r.load(static_cast<const decltype(t) *>(p), at);
+            take(r);
+        };
+        if (type == FBH_F32) load(float{});
+        else if (type == FBH_F16) load(_Float16{});
+        else load(__bf16{});
     }
     __device__ __forceinline__ void fill(float f) {
 #pragma unroll
         for (uint32_t i = 0; i < C; i++) v[i] = f;
     }
-    // What lies behind the row's end.
-    __device__ __forceinline__ void fill_behind(float f, uint32_t dim) {
-#pragma unroll
-        for (uint32_t p = 0; p < P; p++) {
-            const uint32_t c = column(p);
-            if (c + N > dim)
-#pragma unroll
-                for (uint32_t i = 0; i < N; i++)
-                    if (c + i >= dim) v[p * N + i] = f;
-        }
-    }
-    __device__ __forceinline__ void store(T *row, uint32_t dim) const {
-#pragma unroll
-        for (uint32_t p = 0; p < P; p++) {
-            const uint32_t c = column(p);
-            if (c + N <= dim) {
-                Piece<T, N> q;
-#pragma unroll
-                for (uint32_t i = 0; i < N; i++) q.v[i] = (T)v[p * N + i];
-                store_piece<T, N>(row + c, q);
-            } else {
-#pragma unroll
-                for (uint32_t i = 0; i < N; i++)
-                    if (c + i < dim) row[c + i] = (T)v[p * N + i];
-            }
-        }
-    }
 };
+
+// f(cell) of the lane's cells to a row.
+template <class T, class L, class F>
+__device__ __forceinline__ void store_cells(T *row, L at, F &&f) {
+#pragma unroll
+    for (uint32_t p = 0; p < L::P; p++)
+        if (!at.empty(p)) {
+            Piece<T, L::N> q;
+#pragma unroll
+            for (uint32_t i = 0; i < L::N; i++) q.v[i] = (T)f(p * L::N + i);
+            store_piece<T, L::N>(row + at.column(p), q);
+        }
+}
+
+// Sums of f(cell) over the lane's cells that take part: of all, and again with care by those
+// few lanes that have others.
+template <uint32_t K, uint32_t C, class L, class F>
+__device__ __forceinline__ void sum_cells(float (&s)[K], L at, bool ragged, F &&f) {
+#pragma unroll
+    for (uint32_t k = 0; k < K; k++) s[k] = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < C; i++) f(i, s);
+    if (ragged) {
+#pragma unroll
+        for (uint32_t k = 0; k < K; k++) s[k] = 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < C; i++)
+            if (at.counts(i)) f(i, s);
+    }
+}
 
 template <uint32_t G>
 constexpr uint32_t norm_threads() {
     return G > 256 ? G : 256;
 }
 
-template <class T, uint32_t G, uint32_t C>
+template <class T, uint32_t N, uint32_t G, uint32_t C>
 __global__ __launch_bounds__(norm_threads<G>()) void norm_kernel(Norm A, const T *x, T *out,
                                                                  float *stats) {
+    using L = Place<N, G, C>;
     constexpr uint32_t ROWS = norm_threads<G>() / G;
     __shared__ GroupSum<G, 1> first;
     __shared__ GroupSum<G, 2> second;
-    Cells<T, G, C> w, b;
-    if (A.weight) w.load_typed(A.weight, A.weight_type, A.dim);
-    else w.fill(1.0f);
-    if (A.bias) b.load_typed(A.bias, A.weight_type, A.dim);
-    else b.fill(0.0f);
-    const float n = (float)A.dim;
-    uint32_t turn = 0;
-    for (uint64_t r = (uint64_t)blockIdx.x * ROWS; r < A.n_rows;
-         r += (uint64_t)gridDim.x * ROWS, turn ^= 1) {
-        const uint64_t row = r + threadIdx.x / G;
-        const bool in = row < A.n_rows;  // (all of a group's lanes, and with G > 64 always)
-        Cells<T, G, C> c;
-        if (in) c.load(x + row * A.dim, A.dim);
-        else c.fill(0.0f);
-        float s1[1] = {0.0f};
-#pragma unroll
-        for (uint32_t i = 0; i < C; i++) s1[0] += c.v[i];
-        sum_of_group<G, 1>(s1, first, turn);
-        const float mean = s1[0] / n;
-        c.fill_behind(mean, A.dim);
-        float s2[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (uint32_t i = 0; i < C; i++) {
-            c.v[i] -= mean;
-            s2[0] += c.v[i];
-            s2[1] += c.v[i] * c.v[i];
+    const L at{A.dim};
+    const bool ragged = at.ragged();
+    const float inv_n = 1.0f / (float)A.dim;
+    const uint64_t step = (uint64_t)gridDim.x * ROWS;
+    uint64_t r = (uint64_t)blockIdx.x * ROWS, row = r + threadIdx.x / G;
+    // the next row's cells are on their way while this one's are worked on, where there are
+    // registers for both
+    constexpr bool AHEAD = C * (2 * sizeof(T) + 8) / 4 <= 208;
+    Raw<T, L> next = {};
+    if (AHEAD && row < A.n_rows) next.load(x + row * A.dim, at);
+    Cells<L, C> w, b;
+    w.fill(1.0f);
+    b.fill(0.0f);
+    if (A.weight) w.load_typed(A.weight, A.weight_type, at);
+    if (A.bias) b.load_typed(A.bias, A.weight_type, at);
+    for (uint32_t turn = 0; r < A.n_rows; r += step, row += step, turn ^= 1) {
+        Raw<T, L> c = {};  // (widened where it is used: half the registers)
+        if constexpr (AHEAD) {
+            c = next;
+            if (row + step < A.n_rows) next.load(x + (row + step) * A.dim, at);
+        } else {
+            if (row < A.n_rows) c.load(x + row * A.dim, at);
         }
+        float s1[1], s2[2];
+        sum_cells<1, C>(s1, at, ragged, [&](uint32_t i, float (&s)[1]) { s[0] += c.cell(i); });
+        sum_of_group<G, 1>(s1, first, turn);
+        const float mean = s1[0] * inv_n;
+        sum_cells<2, C>(s2, at, ragged, [&](uint32_t i, float (&s)[2]) {
+            const float d = c.cell(i) - mean;
+            s[0] += d;
+            s[1] = fmaf(d, d, s[1]);
+        });
         sum_of_group<G, 2>(s2, second, turn);
-        const float rest = s2[0] / n;
-        const float rstd = 1.0f / sqrtf((s2[1] / n - rest * rest) + A.eps);
-#pragma unroll
-        for (uint32_t i = 0; i < C; i++) c.v[i] = (c.v[i] - rest) * rstd * w.v[i] + b.v[i];
-        if (in) {
-            c.store(out + row * A.dim, A.dim);
-            if (stats && threadIdx.x % G == 0) {
-                stats[2 * row] = mean + rest;
-                stats[2 * row + 1] = rstd;
-            }
+        const float rest = s2[0] * inv_n;
+        const float rstd = 1.0f / sqrtf((s2[1] * inv_n - rest * rest) + A.eps);
+        if (row >= A.n_rows) continue;  // (all of a group's lanes, and with G > 64 never)
+        store_cells(out + row * A.dim, at, [&](uint32_t i) {
+            return fmaf((c.cell(i) - mean - rest) * rstd, w.v[i], b.v[i]);
+        });
+        if (stats && threadIdx.x % G == 0) {
+            stats[2 * row] = mean + rest;
+            stats[2 * row + 1] = rstd;
         }
     }
 }
 
-// Lanes and cells a lane of a row, by its cells.
+// f(cells of a piece, lanes of a row, cells of a lane) by the row's cells.
 template <class T, class F>
 void with_shape(uint32_t dim, F &&f) {
-    if (dim <= 4 * 8) f(Int<4>{}, Int<8>{});
-    else if (dim <= 16 * 8) f(Int<16>{}, Int<8>{});
-    else if (dim <= 16 * 16) f(Int<16>{}, Int<16>{});
-    else if (dim <= 64 * 8) f(Int<64>{}, Int<8>{});
-    else if (dim <= 64 * 16) f(Int<64>{}, Int<16>{});
-    else if (dim <= 256 * 8) f(Int<256>{}, Int<8>{});
-    else if (dim <= 256 * 16) f(Int<256>{}, Int<16>{});
-    else if (dim <= 1024 * 8) f(Int<1024>{}, Int<8>{});
-    else if (dim <= 1024 * 16) f(Int<1024>{}, Int<16>{});
-    else f(Int<1024>{}, Int<32>{});
+    constexpr uint32_t N = 16 / sizeof(T);
+    if (dim < N) return f(Int<1>{}, Int<4>{}, Int<2>{});
+    const Int<N> n;
+    if (dim <= 4 * 8) f(n, Int<4>{}, Int<8>{});
+    else if (dim <= 8 * 8) f(n, Int<8>{}, Int<8>{});
+    else if (dim <= 16 * 8) f(n, Int<16>{}, Int<8>{});
+    else if (dim <= 16 * 16) f(n, Int<16>{}, Int<16>{});
+    else if (dim <= 64 * 8) f(n, Int<64>{}, Int<8>{});
+    else if (dim <= 64 * 16) f(n, Int<64>{}, Int<16>{});
+    else if (dim <= 256 * 8) f(n, Int<256>{}, Int<8>{});
+    else if (dim <= 256 * 16) f(n, Int<256>{}, Int<16>{});
+    else if (dim <= 512 * 16) f(n, Int<512>{}, Int<16>{});
+    else if (dim <= 512 * 32) f(n, Int<512>{}, Int<32>{});
+    else f(n, Int<512>{}, Int<64>{});
 }
 template <class F>
 void with_type(uint32_t dtype, F &&f) {
@@ -219,7 +269,6 @@ void with_type(uint32_t dtype, F &&f) {
 // ------------------------------------------------------------------- gradient
 // Workgroups go through rows in turn and hold their sums of dw and db in registers; each
 // writes its part, and the parts are added in order.
-constexpr uint32_t GRAD_GROUPS = 512;
 constexpr uint32_t SPLIT_DIM = 16384;  // wider rows' sums have no room in registers
 
 struct NormGrad {
@@ -230,134 +279,179 @@ struct NormGrad {
     float *parts;  // [groups][2][dim], or for wide rows [n_rows]: what the mean leaves out
 };
 
-template <class T, uint32_t G, uint32_t C, bool SUMS>
+template <class T, uint32_t N, uint32_t G, uint32_t C, bool SUMS>
 __global__ __launch_bounds__(norm_threads<G>()) void norm_grad_kernel(NormGrad A, const T *g,
                                                                       const T *x, T *dx) {
+    using L = Place<N, G, C>;
     constexpr uint32_t ROWS = norm_threads<G>() / G;
+    constexpr bool AHEAD = C * (4 * sizeof(T) + (SUMS ? 12 : 4)) / 4 <= 208;
     __shared__ GroupSum<G, 3> lds;
-    Cells<T, G, C> w, dw, db;
-    if (A.weight) w.load_typed(A.weight, A.weight_type, A.dim);
-    else w.fill(1.0f);
+    const L at{A.dim};
+    const bool ragged = at.ragged();
+    const float inv_n = 1.0f / (float)A.dim;
+    const uint64_t step = (uint64_t)gridDim.x * ROWS;
+    uint64_t r = (uint64_t)blockIdx.x * ROWS, row = r + threadIdx.x / G;
+    Raw<T, L> next_x = {}, next_g = {};
+    float next_mean = 0.0f, next_rstd = 0.0f;
+    const auto load = [&](uint64_t row, Raw<T, L> &c, Raw<T, L> &d, float &mean, float &rstd) {
+        if (row < A.n_rows) {
+            c.load(x + row * A.dim, at);
+            d.load(g + row * A.dim, at);
+            mean = A.stats[2 * row];
+            rstd = A.stats[2 * row + 1];
+        }
+    };
+    if (AHEAD) load(row, next_x, next_g, next_mean, next_rstd);
+    Cells<L, C> w, dw, db;
+    w.fill(1.0f);
+    if (A.weight) w.load_typed(A.weight, A.weight_type, at);
     if (SUMS) {
         dw.fill(0.0f);
         db.fill(0.0f);
     }
-    const float n = (float)A.dim;
-    uint32_t turn = 0;
-    for (uint64_t r = (uint64_t)blockIdx.x * ROWS; r < A.n_rows;
-         r += (uint64_t)gridDim.x * ROWS, turn ^= 1) {
-        const uint64_t row = r + threadIdx.x / G;
-        const bool in = row < A.n_rows;
-        Cells<T, G, C> c, d;
+    for (uint32_t turn = 0; r < A.n_rows; r += step, row += step, turn ^= 1) {
+        Raw<T, L> c = {}, d = {};  // (widened where they are used)
         float mean = 0.0f, rstd = 0.0f;
-        if (in) {
-            c.load(x + row * A.dim, A.dim);
-            d.load(g + row * A.dim, A.dim);
-            mean = A.stats[2 * row];
-            rstd = A.stats[2 * row + 1];
+        if constexpr (AHEAD) {
+            c = next_x;
+            d = next_g;
+            mean = next_mean;
+            rstd = next_rstd;
+            load(row + step, next_x, next_g, next_mean, next_rstd);
         } else {
-            c.fill(0.0f);
-            d.fill(0.0f);
+            load(row, c, d, mean, rstd);
         }
-        c.fill_behind(mean, A.dim);
-        float s[3] = {0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (uint32_t i = 0; i < C; i++) {
-            c.v[i] -= mean;
-            const float e = d.v[i] * w.v[i];
-            s[0] += c.v[i];
+        float s[3];
+        sum_cells<3, C>(s, at, ragged, [&](uint32_t i, float (&s)[3]) {
+            const float e = d.cell(i) * w.v[i], f = c.cell(i) - mean;
+            s[0] += f;
             s[1] += e;
-            s[2] += e * c.v[i];
-        }
+            s[2] = fmaf(e, f, s[2]);
+        });
         sum_of_group<G, 3>(s, lds, turn);
-        const float rest = s[0] / n, a = s[1] / n;
-        const float b = (s[2] / n - a * rest) * rstd;  // mean(d * h)
-        if (!SUMS && A.parts && in && threadIdx.x % G == 0) A.parts[row] = rest;
+        if (row >= A.n_rows) continue;  // (all of a group's lanes, and with G > 64 never)
+        const float rest = s[0] * inv_n, a = s[1] * inv_n;
+        const float b = (s[2] * inv_n - a * rest) * rstd;  // mean(d * h)
+        if (!SUMS && A.parts && threadIdx.x % G == 0) A.parts[row] = rest;
+        if (SUMS)
 #pragma unroll
-        for (uint32_t i = 0; i < C; i++) {
-            const float h = (c.v[i] - rest) * rstd;
-            if (SUMS) {
-                dw.v[i] += d.v[i] * h;
-                db.v[i] += d.v[i];
+            for (uint32_t i = 0; i < C; i++) {
+                const float h = (c.cell(i) - mean - rest) * rstd;
+                dw.v[i] = fmaf(d.cell(i), h, dw.v[i]);
+                db.v[i] += d.cell(i);
             }
-            c.v[i] = (d.v[i] * w.v[i] - a - h * b) * rstd;
-        }
-        if (in && dx) c.store(dx + row * A.dim, A.dim);
+        if (dx)
+            store_cells(dx + row * A.dim, at, [&](uint32_t i) {
+                const float h = (c.cell(i) - mean - rest) * rstd;
+                return fmaf(-h, b, d.cell(i) * w.v[i] - a) * rstd;
+            });
     }
     if constexpr (SUMS) {
         if (!A.parts) return;
-        constexpr uint32_t N = Cells<T, G, C>::N;
         float *out = A.parts + (uint64_t)blockIdx.x * 2 * A.dim;
         if constexpr (ROWS == 1) {
 #pragma unroll
-            for (uint32_t i = 0; i < C; i++) {
-                const uint32_t col = Cells<T, G, C>::column(i / N) + i % N;
-                if (col < A.dim) {
-                    out[col] = dw.v[i];
-                    out[A.dim + col] = db.v[i];
+            for (uint32_t i = 0; i < C; i++)
+                if (!at.empty(i / N)) {
+                    out[at.column(i / N) + i % N] = dw.v[i];
+                    out[A.dim + at.column(i / N) + i % N] = db.v[i];
                 }
-            }
         } else {
-            // the workgroup's rows, added in their order
-            __shared__ float sums[2][ROWS][G * C / 4];
+            // the workgroup's rows, added in their order, a quarter of the cells at a time
+            constexpr uint32_t Q = C > 4 ? C / 4 : 1;
+            __shared__ float sums[2][ROWS][G * Q];
 #pragma unroll
-            for (uint32_t q = 0; q < 4; q++) {  // a quarter of the cells at a time
+            for (uint32_t q = 0; q < C / Q; q++) {
                 __syncthreads();
 #pragma unroll
-                for (uint32_t k = 0; k < C / 4; k++) {
-                    const uint32_t at = k * G + threadIdx.x % G;
-                    sums[0][threadIdx.x / G][at] = dw.v[q * (C / 4) + k];
-                    sums[1][threadIdx.x / G][at] = db.v[q * (C / 4) + k];
+                for (uint32_t k = 0; k < Q; k++) {
+                    sums[0][threadIdx.x / G][k * G + threadIdx.x % G] = dw.v[q * Q + k];
+                    sums[1][threadIdx.x / G][k * G + threadIdx.x % G] = db.v[q * Q + k];
                 }
                 __syncthreads();
-                for (uint32_t j = threadIdx.x; j < 2 * G * C / 4; j += norm_threads<G>()) {
-                    const uint32_t at = j % (G * C / 4), which = j / (G * C / 4);
+                for (uint32_t j = threadIdx.x; j < 2 * G * Q; j += norm_threads<G>()) {
+                    const uint32_t slot = j % (G * Q), which = j / (G * Q);
                     float t = 0.0f;
-                    for (uint32_t k = 0; k < ROWS; k++) t += sums[which][k][at];
-                    const uint32_t i = q * (C / 4) + at / G;
-                    const uint32_t col = ((i / N) * G + at % G) * N + i % N;
-                    if (col < A.dim) out[which * A.dim + col] = t;
+                    for (uint32_t k = 0; k < ROWS; k++) t += sums[which][k][slot];
+                    const uint32_t i = q * Q + slot / G;
+                    const uint32_t begin = ((i / N) * G + slot % G) * N;
+                    if (begin < A.dim) out[which * A.dim + min(begin, A.dim - N) + i % N] = t;
                 }
             }
         }
     }
 }
 
-// dw and db of wide rows: a thread a column, the rows cut into `groups` equal parts.
+// dw and db of wide rows: four columns a thread, four rows at a time, the rows cut into `groups`
+// equal parts. A thread's columns start at dim - 4 at the latest.
 template <class T>
 __global__ __launch_bounds__(256) void norm_columns_kernel(NormGrad A, const T *g, const T *x,
                                                            const float *rests, float *parts) {
-    const uint32_t col = blockIdx.x * 256 + threadIdx.x;
-    if (col >= A.dim) return;
+    const uint32_t begin = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if (begin >= A.dim) return;
+    const uint32_t col = min(begin, A.dim - 4);
     const uint64_t each = (A.n_rows + A.groups - 1) / A.groups;
-    const uint64_t begin = blockIdx.y * each, end = min(begin + each, A.n_rows);
-    float dw = 0.0f, db = 0.0f;
-    for (uint64_t r = begin; r < end; r++) {
-        const float d = (float)g[r * A.dim + col];
-        const float h = ((float)x[r * A.dim + col] - A.stats[2 * r] - rests[r]) *
-                        A.stats[2 * r + 1];
-        dw += d * h;
-        db += d;
+    const uint64_t first = blockIdx.y * each, end = min(first + each, A.n_rows);
+    float dw[4] = {}, db[4] = {};
+    const auto add = [&](const Piece<T, 4> &gp, const Piece<T, 4> &xp, uint64_t r) {
+        const float mean = A.stats[2 * r], rstd = A.stats[2 * r + 1], rest = rests[r];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float d = (float)gp.v[i];
+            dw[i] = fmaf(d, ((float)xp.v[i] - mean - rest) * rstd, dw[i]);
+            db[i] += d;
+        }
+    };
+    uint64_t r = first;
+    for (; r + 4 <= end; r += 4) {
+        Piece<T, 4> gp[4], xp[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            gp[k] = load_piece<T, 4>(g + (r + k) * A.dim + col);
+            xp[k] = load_piece<T, 4>(x + (r + k) * A.dim + col);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) add(gp[k], xp[k], r + k);
     }
+    for (; r < end; r++)
+        add(load_piece<T, 4>(g + r * A.dim + col), load_piece<T, 4>(x + r * A.dim + col), r);
     float *out = parts + (uint64_t)blockIdx.y * 2 * A.dim;
-    out[col] = dw;
-    out[A.dim + col] = db;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        out[col + i] = dw[i];
+        out[A.dim + col + i] = db[i];
+    }
 }
 
-// The parts' sums, in doubles: 16 columns a workgroup, each part's cells to one of 16 threads.
+// The parts' sums, in doubles: COLUMNS columns a workgroup, 256 / COLUMNS threads a column, each
+// of which takes a part in as many; their sums are then added in order. Few columns need many
+// threads each (64 cells and 1024 parts: 4.0 us, 8 columns a workgroup), many whole cache lines
+// (16384 cells and 512 parts, 67 MB: 41.7 us with 8 columns).
+template <uint32_t COLUMNS>
 __global__ __launch_bounds__(256) void norm_join_kernel(const float *parts, uint32_t dim,
                                                         uint32_t groups, uint32_t weight_type,
                                                         void *dweight, void *dbias) {
-    __shared__ double sums[16][17];
-    const uint32_t lane = threadIdx.x % 16, k = threadIdx.x / 16;
-    const uint32_t j = blockIdx.x * 16 + lane;  // of 2 * dim
+    constexpr uint32_t THREADS = 256 / COLUMNS;
+    __shared__ double sums[THREADS][COLUMNS + 1];
+    const uint32_t lane = threadIdx.x % COLUMNS, k = threadIdx.x / COLUMNS;
+    const uint32_t j = blockIdx.x * COLUMNS + lane;  // of 2 * dim
     double t = 0.0;
-    if (j < 2 * dim)
-        for (uint32_t p = k; p < groups; p += 16) t += (double)parts[(uint64_t)p * 2 * dim + j];
+    if (j < 2 * dim) {
+        uint32_t p = k;
+        for (; p + 7 * THREADS < groups; p += 8 * THREADS) {
+            float v[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++)
+                v[i] = parts[(uint64_t)(p + i * THREADS) * 2 * dim + j];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) t += (double)v[i];
+        }
+        for (; p < groups; p += THREADS) t += (double)parts[(uint64_t)p * 2 * dim + j];
+    }
     sums[k][lane] = t;
     __syncthreads();
     if (k != 0 || j >= 2 * dim) return;
-    for (uint32_t i = 1; i < 16; i++) t += sums[i][lane];
+    for (uint32_t i = 1; i < THREADS; i++) t += sums[i][lane];
     void *out = j < dim ? dweight : dbias;
     const uint32_t at = j < dim ? j : j - dim;
     if (!out) return;
@@ -369,16 +463,19 @@ __global__ __launch_bounds__(256) void norm_join_kernel(const float *parts, uint
 // ------------------------------------------------------------------- host side
 uint32_t rows_of_group(uint32_t dim) {
     uint32_t rows = 1;
-    with_shape<float>(dim, [&](auto g, auto) {
+    with_shape<float>(dim, [&](auto, auto g, auto) {
         constexpr uint32_t G = decltype(g)::value;
         rows = norm_threads<G>() / G;
     });
     return rows;
 }
 
+// Parts of the weights' sums: as many workgroups as the device holds at a time, or fewer where
+// the parts would be large beside the rows.
 uint32_t grad_groups(uint64_t n_rows, uint32_t dim) {
-    const uint64_t most = (n_rows + rows_of_group(dim) - 1) / rows_of_group(dim);
-    return (uint32_t)(most < GRAD_GROUPS ? (most ? most : 1) : GRAD_GROUPS);
+    const uint64_t most = dim <= 256 ? 1024 : dim <= 4096 ? 512 : dim <= SPLIT_DIM ? 256 : 64;
+    const uint64_t n = (n_rows + rows_of_group(dim) - 1) / rows_of_group(dim);
+    return (uint32_t)(n < most ? (n ? n : 1) : most);
 }
 
 uint64_t padded_rows(uint64_t n) { return (n + 3) / 4 * 4; }
@@ -409,11 +506,11 @@ template <class T>
 void launch_norm(const fbh_norm *a, const void *x, const void *weight, const void *bias, void *out,
                  float *stats, hipStream_t s) {
     const Norm A{weight, bias, a->n_rows, a->dim, a->weight_type, a->eps};
-    with_shape<T>(a->dim, [&](auto g, auto c) {
-        constexpr uint32_t G = decltype(g)::value, C = decltype(c)::value;
+    with_shape<T>(a->dim, [&](auto n, auto g, auto c) {
+        constexpr uint32_t N = decltype(n)::value, G = decltype(g)::value, C = decltype(c)::value;
         constexpr uint32_t ROWS = norm_threads<G>() / G;
         const uint64_t blocks = (a->n_rows + ROWS - 1) / ROWS;
-        launch(norm_kernel<T, G, C>, blocks < 2048 ? blocks : 2048, norm_threads<G>(), s, A,
+        launch(norm_kernel<T, N, G, C>, std::min<uint64_t>(blocks, NORM_BLOCKS), norm_threads<G>(), s, A,
                static_cast<const T *>(x), static_cast<T *>(out), stats);
     });
 }
@@ -425,21 +522,25 @@ void launch_norm_grad(const fbh_norm *a, const T *g, const T *x, const float *st
     const bool sums = dweight || dbias, split = a->dim > SPLIT_DIM;
     const uint32_t groups = grad_groups(a->n_rows, a->dim);
     NormGrad A{a->n_rows, a->dim, a->weight_type, groups, weight, stats, sums ? work : nullptr};
-    with_shape<T>(a->dim, [&](auto gg, auto cc) {
-        constexpr uint32_t G = decltype(gg)::value, C = decltype(cc)::value;
+    with_shape<T>(a->dim, [&](auto nn, auto gg, auto cc) {
+        constexpr uint32_t N = decltype(nn)::value, G = decltype(gg)::value;
+        constexpr uint32_t C = decltype(cc)::value;
         constexpr bool SUMS = G * C <= SPLIT_DIM;
-        launch(norm_grad_kernel<T, G, C, SUMS>, groups, norm_threads<G>(), s, A, g, x, dx);
+        const uint64_t blocks = SUMS ? groups : std::clamp<uint64_t>(a->n_rows, 1, 512);
+        launch(norm_grad_kernel<T, N, G, C, SUMS>, blocks, norm_threads<G>(), s, A, g, x, dx);
     });
     if (!sums) return;
     float *parts = work;
     if (split) {
         parts = work + padded_rows(a->n_rows);
-        hipLaunchKernelGGL(norm_columns_kernel<T>, dim3((a->dim + 255) / 256, groups), dim3(256),
+        hipLaunchKernelGGL(norm_columns_kernel<T>, dim3((a->dim + 1023) / 1024, groups), dim3(256),
                            0, s, A, g, x, work, parts);
         head_check(hipGetLastError(), "layer norm");
     }
-    launch(norm_join_kernel, (2 * a->dim + 15) / 16, 256, s, parts, a->dim, groups,
-           a->weight_type, dweight, dbias);
+    const uint32_t columns = a->dim <= 512 ? 8 : 32;
+    launch(columns == 8 ? norm_join_kernel<8> : norm_join_kernel<32>,
+           (2 * a->dim + columns - 1) / columns, 256, s, parts, a->dim, groups, a->weight_type,
+           dweight, dbias);
 }
 
 }  // namespace

@@ -853,7 +853,7 @@ uint64_t fbh_layer_norm_grad_bytes(const fbh_norm *a);
 /* The gradients for the output's gradient grad: dx [n_rows][dim] (may be grad or x),
  * dweight and dbias [dim], summed over all rows (each may be NULL: not wanted); stats
  * as fbh_layer_norm gave them. The rows of a workgroup are summed in f32, the
- * workgroups' sums, at most 512, in f64. Orders of sums depend on n_rows and dim
+ * workgroups' sums, at most 1024, in f64. Orders of sums depend on n_rows and dim
  * alone. work may be NULL where neither dweight nor dbias is wanted. */
 int fbh_layer_norm_grad(int device, const fbh_norm *a, const void *grad, const void *x,
                         const float *stats, const void *weight, void *dx, void *dweight,
