@@ -25,13 +25,16 @@ constexpr uint32_t ADAM_CHUNKS = 4;                 // of a wave in a tile
 constexpr uint32_t ADAM_TILE = ADAM_TPB / 64 * ADAM_CHUNKS * ADAM_CHUNK;
 constexpr uint32_t ADAM_TENSORS = 64;               // of a launch
 constexpr uint64_t ADAM_BLOCKS = 1u << 16;          // of a launch at most
+constexpr uint64_t ADAM_TICKS = 256;  // workgroups up to which they move the clock themselves
 constexpr uint32_t ADAM_TOP_M = 14, ADAM_TOP_S = 30;
 constexpr uint32_t ADAM_NAN_M = 0x7F, ADAM_NAN_S = 0xFF;
 
-// What a program keeps on the device: the steps done, and the products of as many betas.
+// What a program keeps on the device: the steps done, the products of as many betas, and how
+// many workgroups of a step's last launch are through (0 between steps).
 struct Clock {
     int64_t step;
     double decay1, decay2;
+    uint64_t done;
 };
 
 struct AdamTensor {
@@ -41,7 +44,6 @@ struct AdamTensor {
     uint64_t n, first;
     uint64_t tiles_before;
     float decay;
-    uint32_t dtype;
 };
 
 struct Adam {
@@ -55,6 +57,7 @@ struct Adam {
     uint64_t tiles;
     float eps;
     uint32_t n_tensors;
+    uint32_t ticks;  // whether this launch moves the clock on
 };
 
 struct AdamLaunch {
@@ -70,6 +73,7 @@ struct AdamStep {
     double lr;
     float size, root;  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
     float eps;
+    bool tiny_eps;
     uint64_t key;
 };
 
@@ -87,163 +91,249 @@ __device__ __forceinline__ AdamStep adam_step(const Adam &A) {
     s.size = (float)(s.lr / (1.0 - A.clock->decay1 * A.beta1));
     s.root = (float)(1.0 / sqrt(1.0 - A.clock->decay2 * A.beta2));
     s.eps = A.eps;
+    s.tiny_eps = A.eps < 0x1p-38f;  // (2^25 times the root of the largest subnormal)
     s.key = drop_mix((A.seed + (uint64_t)A.clock->step + 1) ^ 0x9E3779B97F4A7C15ull);
     return s;
 }
 
-__global__ void adam_clock_kernel(Clock *clock, double beta1, double beta2) {
+__device__ __forceinline__ void tick(Clock *clock, double beta1, double beta2) {
     clock->step++;
     clock->decay1 *= beta1;
     clock->decay2 *= beta2;
 }
+__global__ void adam_clock_kernel(Clock *clock, double beta1, double beta2) {
+    tick(clock, beta1, beta2);
+}
 
-// ---- The 8-bit floats.
-__device__ __forceinline__ double widen_mean(uint32_t code, double scale) {
-    const uint32_t mag = code & 0x7F;
-    const double v = (double)__uint_as_float(mag << 20) * scale;
-    return mag == ADAM_NAN_M ? (double)NAN : (code & 0x80) ? -v : v;
-}
-__device__ __forceinline__ double widen_square(uint32_t code, double scale) {
-    const double v = (double)__uint_as_float(code << 20) * scale;
-    return code == ADAM_NAN_S ? (double)NAN : v;
-}
-// 2^(field - top): what a block's codes are multiplied by.
+// ---- The 8-bit floats. A block's exponent field is in a scalar register, so is what its codes
+// are multiplied by: 2^(field - top).
 __device__ __forceinline__ double scale_of(uint32_t field, uint32_t top) {
     const int e = (int)max(field, 1u) - (int)top;
     return __longlong_as_double((long long)(1023 + e) << 52);
 }
-__device__ __forceinline__ uint32_t finite_bits(float v) {
-    const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
-    return b < 0x7F800000u ? b : 0;
+// Byte k of a word as a float under the exponents 14 and 30.
+__device__ __forceinline__ float mean_float(uint32_t codes, int k) {
+    return __uint_as_float((uint32_t)((int32_t)(codes << (24 - 8 * k)) >> 4) & 0x87F00000u);
 }
-// random: 16 bits.
-__device__ __forceinline__ uint32_t narrow(float v, uint32_t field, uint32_t top,
-                                           uint32_t random) {
-    const float y = ldexpf(fabsf(v), (int)top - (int)max(field, 1u));
-    return (__float_as_uint(y) + (random << 4)) >> 20;
+__device__ __forceinline__ float square_float(uint32_t codes, int k) {
+    return __uint_as_float((codes >> 8 * k & 0xFF) << 20);
 }
-__device__ __forceinline__ uint32_t narrow_mean(float v, uint32_t field, uint32_t random) {
-    const uint32_t b = __float_as_uint(v);
-    const uint32_t code = narrow(v, field, ADAM_TOP_M, random);
-    return ((b & 0x7FFFFFFFu) < 0x7F800000u ? code : ADAM_NAN_M) | (b >> 31 << 7);
+// Whether one of four bytes stands for what is not finite.
+__device__ __forceinline__ bool has_nan_mean(uint32_t codes) {
+    return ((codes & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
 }
-// (a square above 0 stays above it)
-__device__ __forceinline__ uint32_t narrow_square(float v, uint32_t field, uint32_t random) {
-    const uint32_t code = narrow(v, field, ADAM_TOP_S, random);
-    return !(v < __builtin_huge_valf()) ? ADAM_NAN_S : v > 0.0f ? max(code, 1u) : 0;
+__device__ __forceinline__ bool has_nan_square(uint32_t codes) {
+    return (~codes - 0x01010101u) & codes & 0x80808080u;
 }
-
-// The largest of a wave's values, in every lane.
-__device__ __forceinline__ uint32_t most_of_lanes(uint32_t v) {
-    for (int d = 32; d; d >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d));
-    return v;
+__device__ __forceinline__ bool is_nan_mean(uint32_t codes, int k) {
+    return (codes >> 8 * k & 0x7F) == ADAM_NAN_M;
+}
+__device__ __forceinline__ bool is_nan_square(uint32_t codes, int k) {
+    return (codes >> 8 * k & 0xFF) == ADAM_NAN_S;
 }
 
-// ---- Four cells of a lane.
-template <class T>
-__device__ __forceinline__ void load_four(const T *p, uint64_t i, uint64_t n, float (&v)[4]) {
-    if (i + 4 <= n) {
-        const Piece<T, 4> q = load_piece<T, 4>(p + i);
+// The largest of a wave's values, in a scalar register.
+__device__ __forceinline__ uint32_t most_of_wave(uint32_t v) {
+#define FBH_MOST(CTRL, ROWS)                                                                     \
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false))
+    FBH_MOST(0x111, 0xF);
+    FBH_MOST(0x112, 0xF);
+    FBH_MOST(0x114, 0xF);
+    FBH_MOST(0x118, 0xF);
+    FBH_MOST(0x142, 0xA);
+    FBH_MOST(0x143, 0xC);
+#undef FBH_MOST
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ uint32_t size_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_huge_valf(); }
+// In branches that hardly ever run: the compiler must not run them for everyone.
+__device__ __forceinline__ void seldom() { asm volatile(""); }
+
+// The top bytes of four words.
+__device__ __forceinline__ uint32_t top_bytes(const uint32_t (&t)[4]) {
+    const uint32_t lo = __builtin_amdgcn_perm(t[1], t[0], 0x0C0C0703u);
+    const uint32_t hi = __builtin_amdgcn_perm(t[3], t[2], 0x07030C0Cu);
+    return lo | hi;
+}
+
+// ---- Four cells of a lane; WHOLE: all of them are the tensor's.
+template <bool WHOLE, class T>
+__device__ __forceinline__ void load_four(const T *p, uint32_t left, float (&v)[4]) {
+    if (WHOLE || left >= 4) {
+        const Piece<T, 4> q = load_piece<T, 4>(p);
 #pragma unroll
         for (int k = 0; k < 4; k++) v[k] = (float)q.v[k];
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; k++) v[k] = i + k < n ? (float)p[i + k] : 0.0f;
+        for (int k = 0; k < 4; k++) v[k] = (uint32_t)k < left ? (float)p[k] : 0.0f;
     }
 }
-template <class T>
-__device__ __forceinline__ void store_four(T *p, uint64_t i, uint64_t n, const float (&v)[4]) {
-    if (i + 4 <= n) {
+template <bool WHOLE, class T>
+__device__ __forceinline__ void store_four(T *p, uint32_t left, const float (&v)[4]) {
+    if (WHOLE || left >= 4) {
         Piece<T, 4> q;
 #pragma unroll
         for (int k = 0; k < 4; k++) q.v[k] = (T)v[k];
-        store_piece<T, 4>(p + i, q);
+        store_piece<T, 4>(p, q);
     } else {
 #pragma unroll
         for (int k = 0; k < 4; k++)
-            if (i + k < n) p[i + k] = (T)v[k];
+            if ((uint32_t)k < left) p[k] = (T)v[k];
     }
 }
 
-template <class T, bool SMALL>
+// m / (sqrt(s) root + eps), by the reciprocal and the square root of the hardware, one unit in
+// the last place each: the step is small beside the weight that takes it. The square root may
+// lose subnormals, which eps covers unless it is tiny. (Divided and rooted to half a unit the
+// 8-bit step was bound by its instructions: 120M cells in 484 us.)
+__device__ __forceinline__ void move_by(float (&m)[4], const float (&s)[4], const AdamStep &S) {
+    float root[4];
+    if (S.tiny_eps) {
+        seldom();
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const bool low = s[k] < 0x1p-96f;
+            root[k] = __builtin_amdgcn_sqrtf(low ? s[k] * 0x1p64f : s[k]) *
+                      (low ? 0x1p-32f : 1.0f);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) root[k] = __builtin_amdgcn_sqrtf(s[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+        m[k] *= __builtin_amdgcn_rcpf(root[k] * S.root + S.eps);
+}
+
+// A wave's block of 256 cells, `at` of a tensor's; word: the generator's step times the first
+// pair's number of this lane.
+template <class T, bool SMALL, bool WHOLE>
 __device__ __forceinline__ void adam_chunk(const Adam &A, const AdamStep &S, const AdamTensor &t,
-                                           uint64_t at) {
+                                           float shrink, uint64_t at, uint64_t word) {
     const uint32_t lane = threadIdx.x & 63;
-    const uint64_t i = at + lane * 4, flat = t.first + i;
+    const uint64_t flat = t.first + at;
+    const uint32_t here = (uint32_t)min(t.n - at, (uint64_t)ADAM_CHUNK);
+    const uint32_t left = WHOLE ? 4 : here - min(here, lane * 4);
     constexpr bool MASTER = sizeof(T) == 2;
-    float *weights = MASTER ? t.master : static_cast<float *>(t.param);
+    float *weights = (MASTER ? t.master : static_cast<float *>(t.param)) + at + lane * 4;
+    T *param = static_cast<T *>(t.param) + at + lane * 4;
     float g[4], w[4], m[4], s[4];
-    load_four(static_cast<const T *>(t.grad), i, t.n, g);
-    load_four(weights, i, t.n, w);
+    load_four<WHOLE>(static_cast<const T *>(t.grad) + at + lane * 4, left, g);
+    load_four<WHOLE>(weights, left, w);
     uint32_t *codes_m = nullptr, *codes_s = nullptr;
+    float *mean = nullptr, *square = nullptr;
+    const uint64_t block = flat / ADAM_CHUNK;
+    bool odd = false;  // something of this lane's is not finite
     if constexpr (SMALL) {
-        codes_m = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(A.mean) + flat);
-        codes_s = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(A.square) + flat);
+        codes_m = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(A.mean) + flat) + lane;
+        codes_s = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(A.square) + flat) + lane;
         const uint32_t cm = *codes_m, cs = *codes_s;
-        const uint64_t block = (t.first + at) / ADAM_CHUNK;
-        const double scale_m = scale_of(A.scales[block], ADAM_TOP_M);
-        const double scale_s = scale_of(A.scales[A.blocks + block], ADAM_TOP_S);
+        const double scale_m = scale_of(__builtin_amdgcn_readfirstlane(A.scales[block]),
+                                        ADAM_TOP_M) * S.b1;
+        const double scale_s = scale_of(__builtin_amdgcn_readfirstlane(A.scales[A.blocks + block]),
+                                        ADAM_TOP_S) * S.b2;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const double gd = (double)g[k];
-            m[k] = (float)(widen_mean(cm >> 8 * k & 0xFF, scale_m) * S.b1 + gd * S.c1);
-            s[k] = (float)(widen_square(cs >> 8 * k & 0xFF, scale_s) * S.b2 + gd * gd * S.c2);
+            m[k] = (float)fma((double)mean_float(cm, k), scale_m, gd * S.c1);
+            s[k] = (float)fma((double)square_float(cs, k), scale_s, gd * gd * S.c2);
+        }
+        odd = has_nan_mean(cm) || has_nan_square(cs);
+        if (odd) {
+            seldom();
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (is_nan_mean(cm, k)) m[k] = NAN;
+                if (is_nan_square(cs, k)) s[k] = NAN;
+            }
         }
     } else {
-        load_four(static_cast<float *>(A.mean), flat, ~0ull, m);
-        load_four(static_cast<float *>(A.square), flat, ~0ull, s);
+        mean = static_cast<float *>(A.mean) + flat + lane * 4;
+        square = static_cast<float *>(A.square) + flat + lane * 4;
+        load_four<true>(mean, 4, m);
+        load_four<true>(square, 4, s);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             m[k] = m[k] * S.fb1 + g[k] * S.fc1;
             s[k] = s[k] * S.fb2 + g[k] * g[k] * S.fc2;
         }
     }
+    if (!WHOLE)
 #pragma unroll
-    for (int k = 0; k < 4; k++)
-        if (i + k >= t.n) m[k] = s[k] = 0.0f;
-    const float shrink = (float)(1.0 - S.lr * (double)t.decay);
+        for (int k = 0; k < 4; k++)
+            if ((uint32_t)k >= left) m[k] = s[k] = 0.0f;
+    float by[4] = {m[0], m[1], m[2], m[3]};
+    move_by(by, s, S);
 #pragma unroll
-    for (int k = 0; k < 4; k++)
-        w[k] = w[k] * shrink - S.size * (m[k] / (sqrtf(s[k]) * S.root + S.eps));
-    store_four(weights, i, t.n, w);
-    if constexpr (MASTER) store_four(static_cast<T *>(t.param), i, t.n, w);
+    for (int k = 0; k < 4; k++) {
+        w[k] = fmaf(-S.size, by[k], w[k] * shrink);
+        // the 16-bit parameter is this float rounded, not the sum before
+        if (MASTER) asm volatile("" : "+v"(w[k]));
+    }
+    store_four<WHOLE>(weights, left, w);
+    if constexpr (MASTER) store_four<WHOLE>(param, left, w);
     if constexpr (SMALL) {
-        uint32_t most_m = 0, most_s = 0;
+        // (m is finite where s is, or its byte was odd already)
+        odd = odd || !finite((s[0] + s[1]) + (s[2] + s[3]));
+        uint32_t most_m = max(max(size_bits(m[0]), size_bits(m[1])),
+                              max(size_bits(m[2]), size_bits(m[3])));
+        uint32_t most_s = max(max(size_bits(s[0]), size_bits(s[1])),
+                              max(size_bits(s[2]), size_bits(s[3])));
+        if (odd) {
+            seldom();
+            most_m = most_s = 0;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            most_m = max(most_m, finite_bits(m[k]));
-            most_s = max(most_s, finite_bits(s[k]));
-        }
-        const uint32_t field_m = most_of_lanes(most_m) >> 23;
-        const uint32_t field_s = most_of_lanes(most_s) >> 23;
-        uint32_t cm = 0, cs = 0;
-#pragma unroll
-        for (int k = 0; k < 4; k += 2) {
-            const uint64_t bits = drop_word(S.key, (flat + k) >> 1);
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const uint32_t r = (uint32_t)(bits >> 32 * j);
-                cm |= narrow_mean(m[k + j], field_m, r & 0xFFFF) << 8 * (k + j);
-                cs |= narrow_square(s[k + j], field_s, r >> 16) << 8 * (k + j);
+            for (int k = 0; k < 4; k++) {
+                if (finite(m[k])) most_m = max(most_m, size_bits(m[k]));
+                if (finite(s[k])) most_s = max(most_s, size_bits(s[k]));
             }
         }
-        *codes_m = cm;
-        *codes_s = cs;
+        const uint32_t field_m = most_of_wave(most_m) >> 23;
+        const uint32_t field_s = most_of_wave(most_s) >> 23;
+        const int up_m = (int)ADAM_TOP_M - (int)max(field_m, 1u);
+        const int up_s = (int)ADAM_TOP_S - (int)max(field_s, 1u);
+        uint32_t tm[4], ts[4];  // codes in the top bytes
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+            const uint64_t bits = drop_mix(S.key ^ (word + k / 2 * DROP_STEP));
+#pragma unroll
+            for (int j = k; j < k + 2; j++) {
+                const uint32_t r = (uint32_t)(bits >> 32 * (j - k));
+                const uint32_t ym = __float_as_uint(ldexpf(fabsf(m[j]), up_m));
+                const uint32_t ys = __float_as_uint(ldexpf(s[j], up_s));
+                tm[j] = (ym << 4) + (r << 8 & 0xFFFF00u);
+                ts[j] = (ys << 4) + (r >> 8 & 0xFFFF00u);
+                // the sign; a square above 0 stays above it
+                tm[j] = (tm[j] & 0x7FFFFFFFu) | (__float_as_uint(m[j]) & 0x80000000u);
+                ts[j] = max(ts[j], s[j] > 0.0f ? 1u << 24 : 0u);
+            }
+        }
+        if (odd) {
+            seldom();
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (!finite(m[k])) tm[k] = ADAM_NAN_M << 24;
+                if (!finite(s[k])) ts[k] = ADAM_NAN_S << 24;
+            }
+        }
+        *codes_m = top_bytes(tm);
+        *codes_s = top_bytes(ts);
         if (lane == 0) {
-            const uint64_t block = (t.first + at) / ADAM_CHUNK;
             A.scales[block] = (uint8_t)field_m;
             A.scales[A.blocks + block] = (uint8_t)field_s;
         }
     } else {
-        store_four(static_cast<float *>(A.mean), flat, ~0ull, m);
-        store_four(static_cast<float *>(A.square), flat, ~0ull, s);
+        store_four<true>(mean, 4, m);
+        store_four<true>(square, 4, s);
     }
 }
 
-template <bool SMALL>
+template <class T, bool SMALL>
 __global__ __launch_bounds__(ADAM_TPB) void adam_kernel(AdamLaunch L) {
     const Adam &A = L.a;
     const AdamStep S = adam_step(A);
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     for (uint64_t tile = blockIdx.x; tile < A.tiles; tile += gridDim.x) {
         uint32_t lo = 0, hi = A.n_tensors;  // the last one that begins at the tile or before
         while (hi - lo > 1) {
@@ -253,14 +343,23 @@ __global__ __launch_bounds__(ADAM_TPB) void adam_kernel(AdamLaunch L) {
         }
         const AdamTensor &t = L.t[lo];
         const uint64_t begin = (tile - t.tiles_before) * ADAM_TILE +
-                               (threadIdx.x / 64) * (ADAM_CHUNKS * ADAM_CHUNK);
+                               wave * (ADAM_CHUNKS * ADAM_CHUNK);
+        const float shrink = (float)(1.0 - S.lr * (double)t.decay);
+        const uint64_t word = ((t.first + begin) / 2 + (threadIdx.x & 63) * 2) * DROP_STEP;
         for (uint32_t c = 0; c < ADAM_CHUNKS; c++) {
-            const uint64_t at = begin + c * ADAM_CHUNK;
-            if (at >= t.n) break;
-            if (t.dtype == FBH_F32) adam_chunk<float, SMALL>(A, S, t, at);
-            else if (t.dtype == FBH_F16) adam_chunk<_Float16, SMALL>(A, S, t, at);
-            else adam_chunk<__bf16, SMALL>(A, S, t, at);
+            const uint64_t at = begin + c * ADAM_CHUNK, w = word + c * (ADAM_CHUNK / 2) * DROP_STEP;
+            if (at + ADAM_CHUNK <= t.n) adam_chunk<T, SMALL, true>(A, S, t, shrink, at, w);
+            else if (at < t.n) adam_chunk<T, SMALL, false>(A, S, t, shrink, at, w);
         }
+    }
+    if (!A.ticks) return;
+    // the last workgroup that is through moves the clock on: all have read it by then
+    __syncthreads();
+    if (threadIdx.x == 0 &&
+        __hip_atomic_fetch_add(&A.clock->done, 1ull, __ATOMIC_ACQ_REL,
+                               __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1) {
+        A.clock->done = 0;
+        tick(A.clock, A.beta1, A.beta2);
     }
 }
 
@@ -279,12 +378,25 @@ __global__ __launch_bounds__(ADAM_TPB) void adam_moments_kernel(const uint8_t *m
         Piece<float, 4> m, s;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            m.v[k] = (float)widen_mean(cm >> 8 * k & 0xFF, scale_m);
-            s.v[k] = (float)widen_square(cs >> 8 * k & 0xFF, scale_s);
+            m.v[k] = is_nan_mean(cm, k) ? NAN : (float)((double)mean_float(cm, k) * scale_m);
+            s.v[k] = is_nan_square(cs, k) ? NAN
+                                          : (float)((double)square_float(cs, k) * scale_s);
         }
         store_piece<float, 4>(out_m + i, m);
         store_piece<float, 4>(out_s + i, s);
     }
+}
+
+void launch_adamw(uint32_t dtype, uint32_t bits, const AdamLaunch &L, hipStream_t s) {
+    const auto kernel = dtype == FBH_F32   ? (bits == 8 ? adam_kernel<float, true>
+                                                        : adam_kernel<float, false>)
+                        : dtype == FBH_F16 ? (bits == 8 ? adam_kernel<_Float16, true>
+                                                        : adam_kernel<_Float16, false>)
+                                           : (bits == 8 ? adam_kernel<__bf16, true>
+                                                        : adam_kernel<__bf16, false>);
+    const uint64_t blocks = L.a.tiles < ADAM_BLOCKS ? L.a.tiles : ADAM_BLOCKS;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(ADAM_TPB), 0, s, L);
+    head_check(hipGetLastError(), "adamw");
 }
 
 bool aligned(const void *p, uintptr_t by) { return reinterpret_cast<uintptr_t>(p) % by == 0; }
@@ -333,25 +445,34 @@ int fbh_adamw_step(int device, const fbh_adamw *a, const fbh_adamw_tensor *tenso
         AdamLaunch L{};
         L.a = Adam{a->beta1, a->beta2, a->lr, a->lr_at, a->seed, a->mean, a->square,
                    static_cast<uint8_t *>(a->scales), static_cast<Clock *>(a->clock),
-                   a->n / ADAM_CHUNK, 0, a->eps, 0};
-        const auto flush = [&] {
-            if (L.a.n_tensors == 0) return;
-            const uint64_t blocks = L.a.tiles < ADAM_BLOCKS ? L.a.tiles : ADAM_BLOCKS;
-            hipLaunchKernelGGL((a->bits == 8 ? adam_kernel<true> : adam_kernel<false>),
-                               dim3((uint32_t)blocks), dim3(ADAM_TPB), 0, s, L);
-            head_check(hipGetLastError(), "adamw");
+                   a->n / ADAM_CHUNK, 0, a->eps, 0, 0};
+        // a launch for every 64 tensors of a type; the clock goes on in the last one, or in a
+        // launch of its own
+        bool ticked = false;
+        uint64_t left = 0;
+        for (uint64_t i = 0; i < n_tensors; i++) left += tensors[i].n != 0;
+        for (uint32_t dtype = FBH_F32; dtype <= FBH_BF16 && left; dtype++) {
             L.a.n_tensors = 0;
             L.a.tiles = 0;
-        };
-        for (uint64_t i = 0; i < n_tensors; i++) {
-            const fbh_adamw_tensor &t = tensors[i];
-            if (t.n == 0) continue;
-            L.t[L.a.n_tensors++] = AdamTensor{t.param, t.grad, t.master, t.n, t.first, L.a.tiles,
-                                              t.weight_decay, t.dtype};
-            L.a.tiles += (t.n + ADAM_TILE - 1) / ADAM_TILE;
-            if (L.a.n_tensors == ADAM_TENSORS) flush();
+            const auto launch = [&] {
+                if (L.a.n_tensors == 0) return;
+                ticked = L.a.ticks = left == 0 && L.a.tiles <= ADAM_TICKS;
+                launch_adamw(dtype, a->bits, L, s);
+                L.a.n_tensors = 0;
+                L.a.tiles = 0;
+            };
+            for (uint64_t i = 0; i < n_tensors; i++) {
+                const fbh_adamw_tensor &t = tensors[i];
+                if (t.n == 0 || t.dtype != dtype) continue;
+                L.t[L.a.n_tensors++] = AdamTensor{t.param, t.grad, t.master, t.n, t.first,
+                                                  L.a.tiles, t.weight_decay};
+                L.a.tiles += (t.n + ADAM_TILE - 1) / ADAM_TILE;
+                left--;
+                if (L.a.n_tensors == ADAM_TENSORS) launch();
+            }
+            launch();
         }
-        flush();
+        if (ticked) return;
         hipLaunchKernelGGL(adam_clock_kernel, dim3(1), dim3(1), 0, s, L.a.clock, a->beta1,
                            a->beta2);
         head_check(hipGetLastError(), "adamw");

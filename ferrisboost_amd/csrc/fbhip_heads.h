@@ -147,16 +147,40 @@ __device__ __forceinline__ uint32_t load_id(const void *ids, uint64_t at) {
     }
 }
 
+// Sums over a wave's lanes up to each, by moves between lanes that take no LDS: within rows
+// of 16, then the last lane of a row to the next one, then of a half to the other.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t moved(uint64_t v) {
+    return (uint64_t)moved<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 |
+           moved<CTRL, ROWS>((uint32_t)v);
+}
+template <class U>
+__device__ __forceinline__ U scan_wave(U v) {
+    v += moved<0x111, 0xF>(v);
+    v += moved<0x112, 0xF>(v);
+    v += moved<0x114, 0xF>(v);
+    v += moved<0x118, 0xF>(v);
+    v += moved<0x142, 0xA>(v);
+    v += moved<0x143, 0xC>(v);
+    return v;
+}
+
 // ---- Stable ranks of items with equal keys.
 // The lanes that are `in` with this lane's digit.
 __device__ __forceinline__ uint64_t same_digit(bool in, uint32_t digit, uint32_t bits) {
-    uint64_t same = __ballot(in);
+    const uint64_t all = __ballot(in);
+    uint32_t lo = (uint32_t)all, hi = (uint32_t)(all >> 32);
     for (uint32_t b = 0; b < bits; b++) {
-        const bool one = (digit >> b) & 1;
-        const uint64_t ones = __ballot(one);
-        same &= one ? ones : ~ones;
+        const uint32_t bit = (uint32_t)((int32_t)(digit << (31 - b)) >> 31);  // 0 or all ones
+        const uint64_t ones = __ballot(bit != 0);
+        lo &= ~((uint32_t)ones ^ bit);
+        hi &= ~((uint32_t)(ones >> 32) ^ bit);
     }
-    return same;
+    return (uint64_t)hi << 32 | lo;
 }
 // Takes places from a counter that only this wave uses: what it held, plus the number of
 // lower lanes in `same`.

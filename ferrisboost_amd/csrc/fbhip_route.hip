@@ -8,116 +8,184 @@
 // positions, their sums over the chunks before, and places from both. All orders are fixed.
 #include "fbhip_heads.h"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace fbh {
 namespace {
 
 constexpr uint32_t ROUTE_MAX_EXPERTS = 1024;
 constexpr uint32_t ROUTE_TPB = 512;
 constexpr uint32_t ROUTE_WAVES = ROUTE_TPB / 64;
-constexpr uint32_t ROUTE_CHUNK = 4096;   // positions of a chunk at least
-constexpr uint32_t ROUTE_CHUNKS = 1024;  // chunks at most
+constexpr uint32_t ROUTE_ONE = 4096;     // positions that one workgroup sorts by itself
 constexpr uint32_t ROUTE_MAX_DIM = 32768;
 constexpr uint64_t ROUTE_BLOCKS = 1u << 20;  // of a launch at most
 
 struct Route {
     const void *ids;
-    uint32_t n, n_experts, bits;
-    uint32_t chunks, each;  // chunks, and positions of a wave of one
+    uint32_t id_type, n, n_experts, chunks;
     int32_t *order, *place, *starts;
     uint32_t *counts;  // [n_experts + 1][chunks]
     uint32_t *totals;  // [n_experts + 1]
 };
 
-template <int ID>
-__device__ __forceinline__ uint32_t expert_at(const Route &R, uint32_t pos) {
-    return min(load_id<ID>(R.ids, pos), R.n_experts);
+// The experts of ROUNDS positions from `first` on, `apart` from one another (behind the last
+// one: `none`).
+template <uint32_t ROUNDS>
+__device__ __forceinline__ void load_experts(const Route &R, uint64_t first, uint32_t apart,
+                                             uint32_t none, uint32_t (&e)[ROUNDS]) {
+    const auto load = [&](auto id) {
+#pragma unroll
+        for (uint32_t r = 0; r < ROUNDS; r++) {
+            const uint64_t i = first + r * apart;
+            e[r] = i < R.n ? min(load_id<decltype(id)::value>(R.ids, i), R.n_experts) : none;
+        }
+    };
+    if (R.id_type == FBH_ID_I32) load(std::integral_constant<int, FBH_ID_I32>{});
+    else if (R.id_type == FBH_ID_I64) load(std::integral_constant<int, FBH_ID_I64>{});
+    else load(std::integral_constant<int, FBH_ID_F32>{});
 }
 
-template <int ID>
+// A workgroup's chunk has ROUNDS positions a thread; a wave's follow one another, 64 a round.
+template <uint32_t ROUNDS>
 __global__ __launch_bounds__(ROUTE_TPB) void route_count_kernel(Route R) {
     __shared__ uint32_t c[ROUTE_MAX_EXPERTS + 1];
-    for (uint32_t e = threadIdx.x; e <= R.n_experts; e += ROUTE_TPB) c[e] = 0;
+    uint32_t e[ROUNDS];
+    load_experts<ROUNDS>(R, (uint64_t)blockIdx.x * (ROUTE_TPB * ROUNDS) + threadIdx.x, ROUTE_TPB,
+                         ~0u, e);
+    for (uint32_t x = threadIdx.x; x <= R.n_experts; x += ROUTE_TPB) c[x] = 0;
     __syncthreads();
-    const uint64_t begin = (uint64_t)blockIdx.x * ROUTE_WAVES * R.each;
-    const uint32_t end = (uint32_t)min(begin + ROUTE_WAVES * R.each, (uint64_t)R.n);
-    for (uint64_t i = begin + threadIdx.x; i < end; i += ROUTE_TPB)
-        atomicAdd(&c[expert_at<ID>(R, (uint32_t)i)], 1u);
+#pragma unroll
+    for (uint32_t r = 0; r < ROUNDS; r++)
+        if (e[r] != ~0u) atomicAdd(&c[e[r]], 1u);
     __syncthreads();
-    for (uint32_t e = threadIdx.x; e <= R.n_experts; e += ROUTE_TPB)
-        R.counts[(uint64_t)e * R.chunks + blockIdx.x] = c[e];
+    for (uint32_t x = threadIdx.x; x <= R.n_experts; x += ROUTE_TPB)
+        R.counts[(uint64_t)x * R.chunks + blockIdx.x] = c[x];
 }
 
-// The sum of the values of lower lanes.
-__device__ __forceinline__ uint32_t before_in_wave(uint32_t v, uint32_t *all) {
-    uint32_t x = v;
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t y = __shfl_up(x, d);
-        if ((threadIdx.x & 63) >= (uint32_t)d) x += y;
-    }
-    *all = __shfl(x, 63);
-    return x - v;
-}
-
-// An expert's counts to the positions before them among its own; its total.
+// An expert's counts to the positions before them among its own, 8 chunks a lane; its total.
 __global__ __launch_bounds__(64) void route_scan_kernel(Route R) {
     uint32_t *c = R.counts + (uint64_t)blockIdx.x * R.chunks;
     uint32_t sum = 0;
-    for (uint32_t b = 0; b < R.chunks; b += 64) {
-        const uint32_t i = b + threadIdx.x;
-        uint32_t all;
-        const uint32_t at = before_in_wave(i < R.chunks ? c[i] : 0, &all);
-        if (i < R.chunks) c[i] = sum + at;
-        sum += all;
+    for (uint32_t b = 0; b < R.chunks; b += 512) {
+        const uint32_t i = b + threadIdx.x * 8;
+        uint32_t v[8], own = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k++) v[k] = i + k < R.chunks ? c[i + k] : 0;
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k++) own += v[k];
+        const uint32_t upto = scan_wave(own);
+        uint32_t at = sum + upto - own;
+#pragma unroll
+        for (uint32_t k = 0; k < 8; k++) {
+            if (i + k < R.chunks) c[i + k] = at;
+            at += v[k];
+        }
+        sum += __builtin_amdgcn_readlane(upto, 63);
     }
     if (threadIdx.x == 0) R.totals[blockIdx.x] = sum;
 }
 
-template <int ID>
-__global__ __launch_bounds__(ROUTE_TPB) void route_place_kernel(Route R) {
-    __shared__ uint32_t base[ROUTE_MAX_EXPERTS + 1];
-    __shared__ uint32_t seen[ROUTE_WAVES][ROUTE_MAX_EXPERTS + 1];
+// The sums of lower threads' values, of two at a time.
+__device__ __forceinline__ void before_in_group(uint32_t (&v)[2], uint32_t (*sums)[2]) {
     const uint32_t lane = threadIdx.x & 63, w = threadIdx.x / 64;
-    for (uint32_t e = threadIdx.x; e <= R.n_experts; e += ROUTE_TPB)
-        for (uint32_t k = 0; k < ROUTE_WAVES; k++) seen[k][e] = 0;
-    if (w == 0) {  // where each expert's positions begin
-        uint32_t sum = 0;
-        for (uint32_t b = 0; b <= R.n_experts; b += 64) {
-            const uint32_t e = b + lane;
-            uint32_t all;
-            const uint32_t at = before_in_wave(e <= R.n_experts ? R.totals[e] : 0, &all);
-            if (e <= R.n_experts) {
-                base[e] = sum + at;
-                if (blockIdx.x == 0) R.starts[e] = (int32_t)(sum + at);
+    uint32_t upto[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) upto[k] = scan_wave(v[k]);
+    if (lane == 63)
+#pragma unroll
+        for (int k = 0; k < 2; k++) sums[w][k] = upto[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        v[k] = upto[k] - v[k];
+        for (uint32_t u = 0; u < w; u++) v[k] += sums[u][k];
+    }
+}
+
+// A chunk is sorted in LDS first: what a wave then writes of `order` are a few runs and not 64
+// cells apart (16M positions of 64 experts: 70 us straight from the ranks). ONE: the only
+// workgroup, which needs no counts. BITS: of the experts' numbers, known so that the search for
+// equal ones in a wave has no loop.
+template <uint32_t ROUNDS, uint32_t BITS, bool ONE>
+__global__ __launch_bounds__(ROUTE_TPB) void route_place_kernel(Route R) {
+    constexpr uint32_t EACH = (ROUTE_MAX_EXPERTS + ROUTE_TPB) / ROUTE_TPB;  // experts a thread
+    constexpr uint32_t CHUNK = ROUTE_TPB * ROUNDS;
+    __shared__ uint32_t seen[ROUTE_WAVES][ROUTE_MAX_EXPERTS + 1];
+    __shared__ uint32_t shift[ROUTE_MAX_EXPERTS + 1];  // from places in the chunk to those in all
+    __shared__ uint32_t sorted[CHUNK];  // a position's number in the chunk, and its expert
+    __shared__ uint32_t sums[ROUTE_WAVES][2];
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x / 64;
+    const uint64_t begin = (uint64_t)blockIdx.x * CHUNK;
+    const uint32_t here = (uint32_t)min((uint64_t)CHUNK, R.n - min(begin, (uint64_t)R.n));
+    const uint32_t first = w * (64 * ROUNDS) + lane;
+    uint32_t e[ROUNDS], rank[ROUNDS], total[EACH], before[EACH], own[EACH];
+    load_experts<ROUNDS>(R, begin + first, 64, 0, e);
+    if (!ONE)
+#pragma unroll
+        for (uint32_t k = 0; k < EACH; k++) {
+            const uint32_t x = threadIdx.x * EACH + k;
+            total[k] = x <= R.n_experts ? R.totals[x] : 0;
+            before[k] = x <= R.n_experts ? R.counts[(uint64_t)x * R.chunks + blockIdx.x] : 0;
+        }
+    for (uint32_t x = lane; x <= R.n_experts; x += 64) seen[w][x] = 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    // (a wave's LDS operations complete in order, and only it touches its counters)
+#pragma unroll
+    for (uint32_t r = 0; r < ROUNDS; r++) {
+        const bool in = first + r * 64 < here;
+        rank[r] = take_places(&seen[w][e[r]], in, same_digit(in, e[r], BITS));
+    }
+    __syncthreads();
+    // where the experts begin, in the chunk and in all, and each wave's positions of them
+    uint32_t at[2] = {0, 0};
+#pragma unroll
+    for (uint32_t k = 0; k < EACH; k++) {
+        const uint32_t x = threadIdx.x * EACH + k;
+        own[k] = 0;
+        if (x <= R.n_experts)
+#pragma unroll
+            for (uint32_t v = 0; v < ROUTE_WAVES; v++) own[k] += seen[v][x];
+        if (ONE) {
+            total[k] = own[k];
+            before[k] = 0;
+        }
+        at[0] += own[k];
+        at[1] += total[k];
+    }
+    before_in_group(at, sums);
+#pragma unroll
+    for (uint32_t k = 0; k < EACH; k++) {
+        const uint32_t x = threadIdx.x * EACH + k;
+        if (x <= R.n_experts) {
+            if (blockIdx.x == 0) R.starts[x] = (int32_t)at[1];
+            shift[x] = at[1] + before[k] - at[0];
+            uint32_t to = at[0], c[ROUTE_WAVES];
+#pragma unroll
+            for (uint32_t v = 0; v < ROUTE_WAVES; v++) c[v] = seen[v][x];
+#pragma unroll
+            for (uint32_t v = 0; v < ROUTE_WAVES; v++) {
+                seen[v][x] = to;
+                to += c[v];
             }
-            sum += all;
         }
+        at[0] += own[k];
+        at[1] += total[k];
     }
     __syncthreads();
-    const uint64_t begin = ((uint64_t)blockIdx.x * ROUTE_WAVES + w) * R.each;
-    const uint64_t end = min(begin + R.each, (uint64_t)R.n);
-    for (uint64_t i = begin + lane; i < end; i += 64)
-        atomicAdd(&seen[w][expert_at<ID>(R, (uint32_t)i)], 1u);
-    __syncthreads();
-    for (uint32_t e = threadIdx.x; e <= R.n_experts; e += ROUTE_TPB) {
-        uint32_t at = base[e] + R.counts[(uint64_t)e * R.chunks + blockIdx.x];
-        for (uint32_t k = 0; k < ROUTE_WAVES; k++) {
-            const uint32_t c = seen[k][e];
-            seen[k][e] = at;
-            at += c;
-        }
+#pragma unroll
+    for (uint32_t r = 0; r < ROUNDS; r++) {
+        const uint32_t i = first + r * 64;
+        if (i >= here) continue;
+        const uint32_t to = seen[w][e[r]] + rank[r], row = to + shift[e[r]];
+        sorted[to] = i | e[r] << 16;
+        R.place[begin + i] = e[r] < R.n_experts ? (int32_t)row : -1 - (int32_t)row;
     }
     __syncthreads();
-    // a wave's rounds are one after the other, a lane's place in its round is the number of
-    // lower lanes with its expert
-    for (uint64_t i0 = begin; i0 < end; i0 += 64) {
-        const uint64_t i = i0 + lane;
-        const bool in = i < end;
-        const uint32_t e = in ? expert_at<ID>(R, (uint32_t)i) : 0;
-        const uint32_t at = take_places(&seen[w][e], in, same_digit(in, e, R.bits));
-        if (in) {
-            R.order[at] = (int32_t)i;
-            R.place[i] = e < R.n_experts ? (int32_t)at : -1 - (int32_t)at;
-        }
+    for (uint32_t j = threadIdx.x; j < here; j += ROUTE_TPB) {
+        const uint32_t v = sorted[j];
+        R.order[j + shift[v >> 16]] = (int32_t)(begin + (v & 0xFFFF));
     }
 }
 
@@ -167,64 +235,105 @@ __global__ __launch_bounds__(256) void to_experts_kernel(Rows R, const T *x, T *
     });
 }
 
-template <class T, int VEC>
-__device__ __forceinline__ void from_experts_row(Rows R, const T *y, T *out, uint64_t row, uint32_t lane) {
-    const int32_t *place = R.place + row * R.n_columns;
-    const float *weights = R.weights + row * R.n_columns;
+// K columns of a row side by side, so that their pieces are on their way together.
+template <int K>
+struct Columns {
+    uint64_t at[K];   // the first cells of the places
+    float weight[K];  // 0 without a place
+    bool is[K];
+
+    __device__ __forceinline__ Columns(const Rows &R, uint64_t row, uint32_t first) {
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const uint64_t i = row * R.n_columns + first + k;
+            const bool in = first + k < R.n_columns;
+            const int32_t a = in ? R.place[i] : -1;
+            is[k] = a >= 0;
+            at[k] = (uint64_t)place_row(R, a) * R.dim;
+            weight[k] = !is[k] ? 0.0f : R.weights ? R.weights[i] : 1.0f;
+        }
+    }
+};
+
+template <class T, int VEC, int K>
+__device__ __forceinline__ void from_experts_row(const Rows &R, const T *y, T *out, uint64_t row,
+                                                 uint32_t lane) {
+    // (one batch of columns: their places are read once)
+    const Columns<K> only(R, row, 0);
     for (uint32_t p = lane; p < R.pieces; p += 1u << R.lg_g) {
         const uint32_t c = min(p * VEC, R.dim - VEC);
         float s[VEC] = {};
-        for (uint32_t j = 0; j < R.n_columns; j++) {
-            const int32_t a = place[j];
-            if (a < 0) continue;
-            const Piece<T, VEC> v = load_piece<T, VEC>(y + (uint64_t)place_row(R, a) * R.dim + c);
-            const float f = R.weights ? weights[j] : 1.0f;
+        const auto add = [&](const Columns<K> &C) {
+            Piece<T, VEC> v[K] = {};
 #pragma unroll
-            for (int i = 0; i < VEC; i++) s[i] += f * (float)v.v[i];
-        }
+            for (int k = 0; k < K; k++)
+                if (C.is[k]) v[k] = load_piece<T, VEC>(y + C.at[k] + c);
+#pragma unroll
+            for (int k = 0; k < K; k++)
+#pragma unroll
+                for (int i = 0; i < VEC; i++) s[i] += C.weight[k] * (float)v[k].v[i];
+        };
+        add(only);
+        for (uint32_t j = K; j < R.n_columns; j += K) add(Columns<K>(R, row, j));
         Piece<T, VEC> o;
 #pragma unroll
         for (int i = 0; i < VEC; i++) o.v[i] = (T)s[i];
         store_piece<T, VEC>(out + row * R.dim + c, o);
     }
 }
-template <class T, int VEC>
+template <class T, int VEC, int K>
 __global__ __launch_bounds__(256) void from_experts_kernel(Rows R, const T *y, T *out) {
     for_rows(R, [&](uint64_t row, uint32_t lane) {
-        from_experts_row<T, VEC>(R, y, out, row, lane);
+        from_experts_row<T, VEC, K>(R, y, out, row, lane);
     });
 }
 
 // The gradients of from_experts: dy = weight * g to the place, dweight = <g, y> there.
-template <class T, int VEC>
-__device__ __forceinline__ void from_experts_grad_row(Rows R, const T *g, const T *y, T *dy, float *dweights, uint64_t row, uint32_t lane) {
-    for (uint32_t j = 0; j < R.n_columns; j++) {
-        const int32_t a = R.place[row * R.n_columns + j];
-        const float w = R.weights ? R.weights[row * R.n_columns + j] : 1.0f;
-        const uint64_t at = (uint64_t)place_row(R, a) * R.dim;
-        float dot = 0.0f;
+template <class T, int VEC, int K>
+__device__ __forceinline__ void from_experts_grad_row(const Rows &R, const T *g, const T *y, T *dy,
+                                                      float *dweights, uint64_t row,
+                                                      uint32_t lane) {
+    for (uint32_t j = 0; j < R.n_columns; j += K) {
+        const Columns<K> C(R, row, j);
+        float dot[K] = {};
         for (uint32_t p = lane; p < R.pieces; p += 1u << R.lg_g) {
-            const uint32_t c = min(p * VEC, R.dim - VEC);
+            const uint32_t c = min(p * VEC, R.dim - VEC), twice = p * VEC - c;
             const Piece<T, VEC> v = load_piece<T, VEC>(g + row * R.dim + c);
-            Piece<T, VEC> o;
+            Piece<T, VEC> u[K] = {};
+            if (dweights)
 #pragma unroll
-            for (int i = 0; i < VEC; i++) o.v[i] = a < 0 ? (T)0.0f : (T)(w * (float)v.v[i]);
-            if (dy) store_piece<T, VEC>(dy + at + c, o);
-            if (!dweights || a < 0) continue;
-            const Piece<T, VEC> u = load_piece<T, VEC>(y + at + c);
+                for (int k = 0; k < K; k++)
+                    if (C.is[k]) u[k] = load_piece<T, VEC>(y + C.at[k] + c);
 #pragma unroll
-            for (int i = 0; i < VEC; i++)
-                if (c + i >= p * VEC) dot += (float)v.v[i] * (float)u.v[i];
+            for (int k = 0; k < K; k++) {
+                if (j + k >= R.n_columns) continue;
+                if (dy) {
+                    Piece<T, VEC> o;
+#pragma unroll
+                    for (int i = 0; i < VEC; i++)
+                        o.v[i] = C.is[k] ? (T)(C.weight[k] * (float)v.v[i]) : (T)0.0f;
+                    store_piece<T, VEC>(dy + C.at[k] + c, o);
+                }
+                // (cells that the piece before has too count once)
+                if (C.is[k])
+#pragma unroll
+                    for (int i = 0; i < VEC; i++)
+                        if ((uint32_t)i >= twice) dot[k] += (float)v.v[i] * (float)u[k].v[i];
+            }
         }
         if (!dweights) continue;
-        for (uint32_t d = 1u << R.lg_g; d >>= 1;) dot += __shfl_xor(dot, d);
-        if (lane == 0) dweights[row * R.n_columns + j] = dot;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            for (uint32_t d = 1u << R.lg_g; d >>= 1;) dot[k] += __shfl_xor(dot[k], d);
+            if (lane == 0 && j + k < R.n_columns) dweights[row * R.n_columns + j + k] = dot[k];
+        }
     }
 }
-template <class T, int VEC>
-__global__ __launch_bounds__(256) void from_experts_grad_kernel(Rows R, const T *g, const T *y, T *dy, float *dweights) {
+template <class T, int VEC, int K>
+__global__ __launch_bounds__(256) void from_experts_grad_kernel(Rows R, const T *g, const T *y,
+                                                                T *dy, float *dweights) {
     for_rows(R, [&](uint64_t row, uint32_t lane) {
-        from_experts_grad_row<T, VEC>(R, g, y, dy, dweights, row, lane);
+        from_experts_grad_row<T, VEC, K>(R, g, y, dy, dweights, row, lane);
     });
 }
 
@@ -240,20 +349,40 @@ void check_route(uint64_t n, uint32_t n_experts) {
     head_input(n_experts >= 1 && n_experts <= ROUTE_MAX_EXPERTS, "n_experts must be in 1..=1024");
 }
 
+// Positions a thread: more of them where the device is full without, as a chunk's counts are
+// written and read besides.
+uint32_t route_rounds(uint64_t n) {
+    if (n <= ROUTE_ONE) return n <= ROUTE_TPB ? 1 : n <= 2 * ROUTE_TPB ? 2 : 8;
+    return n <= 512 * 2 * ROUTE_TPB ? 2 : 8;
+}
 uint64_t route_chunks(uint64_t n) {
-    const uint64_t c = (n + ROUTE_CHUNK - 1) / ROUTE_CHUNK;
-    return c < 1 ? 1 : c > ROUTE_CHUNKS ? ROUTE_CHUNKS : c;
+    const uint64_t chunk = (uint64_t)ROUTE_TPB * route_rounds(n);
+    return (n + chunk - 1) / chunk;
 }
-
 uint64_t route_bytes(uint64_t n, uint32_t n_experts) {
-    return (n_experts + 1) * (route_chunks(n) + 1) * 4;
+    return n <= ROUTE_ONE ? 0 : (n_experts + 1) * (route_chunks(n) + 1) * 4;
 }
 
-template <int ID>
 void launch_route(const Route &R, hipStream_t s) {
-    launch(route_count_kernel<ID>, R.chunks, ROUTE_TPB, s, R);
-    launch(route_scan_kernel, R.n_experts + 1, 64, s, R);
-    launch(route_place_kernel<ID>, R.chunks, ROUTE_TPB, s, R);
+    const uint32_t rounds = route_rounds(R.n);
+    if (R.n > ROUTE_ONE) {
+        launch(rounds == 2 ? route_count_kernel<2> : route_count_kernel<8>, R.chunks, ROUTE_TPB,
+               s, R);
+        launch(route_scan_kernel, R.n_experts + 1, 64, s, R);
+    }
+    const auto place = [&](auto b) {
+        constexpr uint32_t B = decltype(b)::value;
+        launch(R.n > ROUTE_ONE ? (rounds == 2 ? route_place_kernel<2, B, false>
+                                              : route_place_kernel<8, B, false>)
+               : rounds == 1   ? route_place_kernel<1, B, true>
+               : rounds == 2   ? route_place_kernel<2, B, true>
+                               : route_place_kernel<8, B, true>,
+               R.chunks, ROUTE_TPB, s, R);
+    };
+    // (numbers up to n_experts, which stands for none)
+    if (R.n_experts < 16) place(std::integral_constant<uint32_t, 4>{});
+    else if (R.n_experts < 128) place(std::integral_constant<uint32_t, 7>{});
+    else place(std::integral_constant<uint32_t, 11>{});
 }
 
 Rows rows_of(const int32_t *place, const float *weights, uint64_t n_rows, uint32_t n_columns,
@@ -286,6 +415,14 @@ void with_pieces(uint32_t dim, uint32_t dtype, F &&f) {
     else vec(__bf16{});
 }
 
+// f(columns side by side)
+template <class F>
+void with_columns(uint32_t n_columns, F &&f) {
+    if (n_columns == 1) f(std::integral_constant<int, 1>{});
+    else if (n_columns == 2) f(std::integral_constant<int, 2>{});
+    else f(std::integral_constant<int, 4>{});
+}
+
 uint64_t row_blocks(const Rows &R) {
     const uint32_t rows = 256 >> R.lg_g;
     const uint64_t blocks = (R.n_rows + rows - 1) / rows;
@@ -316,23 +453,16 @@ int fbh_route(int device, const void *ids, uint32_t id_type, uint64_t n_position
         head_input(id_type <= FBH_ID_F32, "unknown id type");
         head_input((ids && order && place) || n_positions == 0, "null argument");
         head_input(starts, "null argument");
-        head_input(work && work_bytes >= route_bytes(n_positions, n_experts),
-                   "the workspace is too small");
-        head_input(reinterpret_cast<uintptr_t>(work) % 4 == 0,
+        const uint64_t need = route_bytes(n_positions, n_experts);
+        head_input(need == 0 || (work && work_bytes >= need), "the workspace is too small");
+        head_input(need == 0 || reinterpret_cast<uintptr_t>(work) % 4 == 0,
                    "the workspace must be 4-byte aligned");
         const OnDevice on(device);
-        Route R{ids, (uint32_t)n_positions, n_experts, 0, 0, 0, order, place, starts, nullptr,
-                nullptr};
-        while ((1u << R.bits) <= n_experts) R.bits++;
-        R.chunks = (uint32_t)route_chunks(n_positions);
-        const uint64_t waves = (uint64_t)R.chunks * ROUTE_WAVES;
-        R.each = (uint32_t)(((n_positions + waves - 1) / waves + 63) / 64 * 64);
-        R.counts = static_cast<uint32_t *>(work);
-        R.totals = R.counts + (uint64_t)(n_experts + 1) * R.chunks;
-        const auto s = static_cast<hipStream_t>(stream);
-        if (id_type == FBH_ID_I32) launch_route<FBH_ID_I32>(R, s);
-        else if (id_type == FBH_ID_I64) launch_route<FBH_ID_I64>(R, s);
-        else launch_route<FBH_ID_F32>(R, s);
+        Route R{ids, id_type, (uint32_t)n_positions, n_experts,
+                (uint32_t)std::max<uint64_t>(route_chunks(n_positions), 1), order, place, starts,
+                static_cast<uint32_t *>(work), nullptr};
+        if (need) R.totals = R.counts + (uint64_t)(n_experts + 1) * R.chunks;
+        launch_route(R, static_cast<hipStream_t>(stream));
     });
 }
 
@@ -362,9 +492,11 @@ int fbh_from_experts(int device, const void *y, const int32_t *place, const floa
         const OnDevice on(device);
         with_pieces(dim, dtype, [&](auto t, auto v) {
             using T = decltype(t);
-            launch(from_experts_kernel<T, decltype(v)::value>, row_blocks(R), 256,
-                   static_cast<hipStream_t>(stream), R, static_cast<const T *>(y),
-                   static_cast<T *>(out));
+            with_columns(n_columns, [&](auto k) {
+                launch(from_experts_kernel<T, decltype(v)::value, decltype(k)::value>,
+                       row_blocks(R), 256, static_cast<hipStream_t>(stream), R,
+                       static_cast<const T *>(y), static_cast<T *>(out));
+            });
         });
     });
 }
@@ -379,9 +511,12 @@ int fbh_from_experts_grad(int device, const void *grad, const void *y, const int
         const OnDevice on(device);
         with_pieces(dim, dtype, [&](auto t, auto v) {
             using T = decltype(t);
-            launch(from_experts_grad_kernel<T, decltype(v)::value>, row_blocks(R), 256,
-                   static_cast<hipStream_t>(stream), R, static_cast<const T *>(grad),
-                   static_cast<const T *>(y), static_cast<T *>(dy), dweights);
+            with_columns(n_columns, [&](auto k) {
+                launch(from_experts_grad_kernel<T, decltype(v)::value, decltype(k)::value>,
+                       row_blocks(R), 256, static_cast<hipStream_t>(stream), R,
+                       static_cast<const T *>(grad), static_cast<const T *>(y),
+                       static_cast<T *>(dy), dweights);
+            });
         });
     });
 }

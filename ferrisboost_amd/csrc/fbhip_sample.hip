@@ -149,27 +149,6 @@ __device__ __forceinline__ uint64_t shfl64_up(uint64_t v, int by, int width = 64
     const uint32_t hi = __shfl_up((uint32_t)(v >> 32), by, width);
     return (uint64_t)hi << 32 | lo;
 }
-// Sums over a wave's lanes up to each, by moves between lanes that take no LDS: within rows
-// of 16, then the last lane of a row to the next one, then of a half to the other.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t moved(uint32_t v) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
-}
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint64_t moved(uint64_t v) {
-    return (uint64_t)moved<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 |
-           moved<CTRL, ROWS>((uint32_t)v);
-}
-template <class U>
-__device__ __forceinline__ U scan_wave(U v) {
-    v += moved<0x111, 0xF>(v);
-    v += moved<0x112, 0xF>(v);
-    v += moved<0x114, 0xF>(v);
-    v += moved<0x118, 0xF>(v);
-    v += moved<0x142, 0xA>(v);
-    v += moved<0x143, 0xC>(v);
-    return v;
-}
 __device__ __forceinline__ uint32_t at_lane(uint32_t v, uint32_t lane) {
     return __builtin_amdgcn_readlane(v, lane);
 }

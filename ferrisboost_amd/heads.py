@@ -59,7 +59,6 @@ _EMBED = struct.Struct("QIIIIIIPPdQfI")
 _OPTIONS = struct.Struct("PPPPfiff")
 _NORM = struct.Struct("QIIIf")                 # fbh_norm
 _ADAMW = struct.Struct("IfdddPQQPPPP")         # fbh_adamw
-_ADAMW_TENSOR = struct.Struct("PPPQQfI")       # fbh_adamw_tensor
 _MOST = float(np.finfo(np.float32).max)
 
 
@@ -660,11 +659,11 @@ class Routes(_Kept):
         self.starts = ids.new_empty(n_experts + 1, dtype=torch.int32)
         dev = ids.get_device()
         size = _L.fbh_route_bytes(n, n_experts)
-        work = ids.new_empty(size, dtype=torch.uint8)
+        work = ids.new_empty(size, dtype=torch.uint8) if size else None
         stream = _raw_stream(dev)
         rc = _L.fbh_route(dev, ids.data_ptr(), code, n, n_experts, self.order.data_ptr(),
-                          self.place.data_ptr(), self.starts.data_ptr(), work.data_ptr(), size,
-                          stream)
+                          self.place.data_ptr(), self.starts.data_ptr(),
+                          work.data_ptr() if size else 0, size, stream)
         if rc:
             N.check_hip(rc)
         self._streams = {stream}
@@ -849,6 +848,11 @@ class AdamW(_Kept):
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("parameters overlap in memory")
         self._sizes = [p.numel() for p in self.params]
+        self._types = [p.dtype for p in self.params]
+        # an fbh_adamw_tensor a parameter, whose addresses are filled in at each step
+        self._parts = [x for i, p in enumerate(self.params) for x in
+                       (0, 0, 0, self._sizes[i], self.first[i], self.weight_decay[i],
+                        _CELLS[p.dtype])]
         self._lr()
         like = self.params[0]
         cell = torch.float32 if bits == 32 else torch.uint8
@@ -858,8 +862,8 @@ class AdamW(_Kept):
                        if bits == 8 else None)
         self.masters = [None if p.dtype == torch.float32 else p.detach().float()
                         for p in self.params]
-        self._clock = torch.zeros(3, dtype=torch.int64, device=like.device)
-        self._clock[1:] = 0x3FF0000000000000  # 1.0
+        self._clock = torch.zeros(4, dtype=torch.int64, device=like.device)
+        self._clock[1:3] = 0x3FF0000000000000  # 1.0
         self._streams = {_raw_stream(like.get_device())}
 
     def _check(self, i: int, p):
@@ -897,35 +901,45 @@ class AdamW(_Kept):
                            0 if self.scales is None else self.scales.data_ptr(),
                            self._clock.data_ptr())
 
+    def _gradient(self, i: int, p, g):
+        """The gradient of parameter i, checked and contiguous."""
+        if g is None:
+            raise ValueError(f"parameter {i} has no gradient")
+        g = _device_tensor(g, f"gradient {i}")
+        if g.dtype != p.dtype or g.shape != p.shape or g.device != p.device:
+            raise ValueError(f"gradient {i} is {g.dtype} of {tuple(g.shape)} on {g.device}, "
+                             f"its parameter {p.dtype} of {tuple(p.shape)} on {p.device}")
+        return g
+
     def step(self, grads=None):
         """One step, in place, with the parameters' .grad or with `grads`, a list of one for
         each parameter, of its shape and type. Every parameter needs one."""
-        torch = _torch
         params = self.params
         grads = [p.grad for p in params] if grads is None else list(grads)
         if len(grads) != len(params):
             raise ValueError(f"{len(grads)} gradients for {len(params)} parameters")
-        parts = []
-        for i, (p, g) in enumerate(zip(params, grads)):
-            if g is None:
-                raise ValueError(f"parameter {i} has no gradient")
-            g = grads[i] = _device_tensor(g, f"gradient {i}")
-            if g.dtype != p.dtype or g.shape != p.shape or g.device != p.device:
-                raise ValueError(f"gradient {i} is {g.dtype} of {tuple(g.shape)} on {g.device}, "
-                                 f"its parameter {p.dtype} of {tuple(p.shape)} on {p.device}")
-            if p.numel() != self._sizes[i] or not p.is_contiguous():
-                raise ValueError(f"parameter {i} has changed its shape")
-            w = self.masters[i]
-            parts.append(_ADAMW_TENSOR.pack(p.data_ptr(), g.data_ptr(),
-                                            0 if w is None else w.data_ptr(), self._sizes[i],
-                                            self.first[i], self.weight_decay[i], _CELLS[p.dtype]))
+        parts = self._parts
         dev = params[0].get_device()
+        plain = _forward_ad._current_level < 0
+        k = 0
+        for p, g, w, n, cell in zip(params, grads, self.masters, self._sizes, self._types):
+            # (a small step's time is what this loop takes)
+            if not (plain and type(g) is _torch.Tensor and g.get_device() == dev and
+                    g.is_contiguous() and g.dtype is p.dtype and g.shape == p.shape):
+                g = grads[k // 7] = self._gradient(k // 7, p, g)
+            if not (p.dtype is cell and p.numel() == n and p.get_device() == dev and
+                    p.is_contiguous()):
+                raise ValueError(f"parameter {k // 7} has changed its type, size or place")
+            parts[k], parts[k + 1] = p.data_ptr(), g.data_ptr()
+            parts[k + 2] = 0 if w is None else w.data_ptr()
+            k += 7
         stream = _raw_stream(dev)
         self._used_on(stream)
-        rc = _L.fbh_adamw_step(dev, self._packed(), b"".join(parts), len(parts), stream)
+        rc = _L.fbh_adamw_step(dev, self._packed(), struct.pack("PPPQQfI" * len(params), *parts),
+                               len(params), stream)
         if rc:
             N.check_hip(rc)
-        torch.autograd.graph.increment_version(params)
+        _torch.autograd.graph.increment_version(params)
 
     def zero_grad(self):
         """Drops the parameters' gradients."""
@@ -963,7 +977,7 @@ class AdamW(_Kept):
         """What load_state_dict() takes: the steps done (waits for the device) and the state's
         own tensors, of which what stores them later makes copies."""
         clock = self._clock.cpu()
-        return {"step": int(clock[0]), "decays": clock[1:].view(_torch.float64).tolist(),
+        return {"step": int(clock[0]), "decays": clock[1:3].view(_torch.float64).tolist(),
                 "bits": self.bits, "mean": self.mean, "square": self.square,
                 "scales": self.scales, "masters": list(self.masters)}
 
@@ -997,7 +1011,7 @@ class AdamW(_Kept):
         with _torch.no_grad():
             for _, to, x in pairs:
                 to.copy_(x)
-            words = struct.unpack("3q", struct.pack("qdd", step, *decays))
+            words = struct.unpack("4q", struct.pack("qddq", step, *decays, 0))
             self._clock.copy_(_torch.tensor(words, dtype=_torch.int64))
 
     def __repr__(self):

@@ -859,8 +859,8 @@ int fbh_layer_norm_grad(int device, const fbh_norm *a, const void *grad, const v
                         const float *stats, const void *weight, void *dx, void *dweight,
                         void *dbias, void *work, uint64_t work_bytes, void *stream);
 
-/* Device bytes of workspace that fbh_route takes, 4-byte aligned; 0 for a call that it
- * refuses. */
+/* Device bytes of workspace that fbh_route takes, 4-byte aligned; 0 for up to 4096
+ * positions and for a call that it refuses. */
 uint64_t fbh_route_bytes(uint64_t n_positions, uint32_t n_experts);
 /* Positions sorted by the id that they hold, equal ones in their order: an id from 0
  * to n_experts - 1 (at most 1024) is an expert, a position with anything else
@@ -906,8 +906,9 @@ typedef struct {
 
 /* An AdamW step's numbers and state. mean and square hold n cells (a multiple of 256,
  * zeros at first) of f32 or, with bits 8, of one byte, 16-byte aligned; scales, with
- * bits 8, [2][n / 256] bytes. clock: 24 bytes, the steps done (int64) and the products
- * of as many beta1 and beta2 (f64): 0, 1, 1 at first. lr, or where lr_at is not NULL the
+ * bits 8, [2][n / 256] bytes. clock: 32 bytes, the steps done (int64), the products of
+ * as many beta1 and beta2 (f64), and 8 bytes that are 0 between steps: 0, 1, 1, 0 at
+ * first. lr, or where lr_at is not NULL the
  * float there when the step runs.
  *
  * A byte of mean has a sign, 4 bits of exponent e and 3 of the mantissa f: (1 + f / 8) *
