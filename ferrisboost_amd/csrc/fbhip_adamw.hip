@@ -224,7 +224,6 @@ __device__ __forceinline__ void adam_chunk(const Adam &A, const AdamStep &S, con
     uint32_t *codes_m = nullptr, *codes_s = nullptr;
     float *mean = nullptr, *square = nullptr;
     const uint64_t block = flat / ADAM_CHUNK;
-    bool odd = false;  // something of this lane's is not finite
     if constexpr (SMALL) {
         codes_m = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(A.mean) + flat) + lane;
         codes_s = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(A.square) + flat) + lane;
@@ -239,8 +238,7 @@ __device__ __forceinline__ void adam_chunk(const Adam &A, const AdamStep &S, con
             m[k] = (float)fma((double)mean_float(cm, k), scale_m, gd * S.c1);
             s[k] = (float)fma((double)square_float(cs, k), scale_s, gd * gd * S.c2);
         }
-        odd = has_nan_mean(cm) || has_nan_square(cs);
-        if (odd) {
+        if (has_nan_mean(cm) || has_nan_square(cs)) {
             seldom();
 #pragma unroll
             for (int k = 0; k < 4; k++) {
@@ -274,12 +272,11 @@ __device__ __forceinline__ void adam_chunk(const Adam &A, const AdamStep &S, con
     store_four<WHOLE>(weights, left, w);
     if constexpr (MASTER) store_four<WHOLE>(param, left, w);
     if constexpr (SMALL) {
-        // (m is finite where s is, or its byte was odd already)
-        odd = odd || !finite((s[0] + s[1]) + (s[2] + s[3]));
         uint32_t most_m = max(max(size_bits(m[0]), size_bits(m[1])),
                               max(size_bits(m[2]), size_bits(m[3])));
         uint32_t most_s = max(max(size_bits(s[0]), size_bits(s[1])),
                               max(size_bits(s[2]), size_bits(s[3])));
+        const bool odd = max(most_m, most_s) >= 0x7F800000u;  // some are not finite
         if (odd) {
             seldom();
             most_m = most_s = 0;

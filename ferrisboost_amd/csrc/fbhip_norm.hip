@@ -584,6 +584,7 @@ int fbh_layer_norm_grad(int device, const fbh_norm *a, const void *grad, const v
             head_input(reinterpret_cast<uintptr_t>(work) % 16 == 0,
                        "the workspace must be 16-byte aligned");
         }
+        head_input(!dx || (dx != grad && dx != x), "dx must not be grad or x");
         if (!dx && !dweight && !dbias) return;
         const OnDevice on(device);
         const auto s = static_cast<hipStream_t>(stream);

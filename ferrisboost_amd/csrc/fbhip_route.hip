@@ -25,7 +25,7 @@ struct Route {
     const void *ids;
     uint32_t id_type, n, n_experts, chunks;
     int32_t *order, *place, *starts;
-    uint32_t *counts;  // [n_experts + 1][chunks]
+    uint32_t *counts;  // [chunks][n_experts + 1]
     uint32_t *totals;  // [n_experts + 1]
 };
 
@@ -60,30 +60,50 @@ __global__ __launch_bounds__(ROUTE_TPB) void route_count_kernel(Route R) {
         if (e[r] != ~0u) atomicAdd(&c[e[r]], 1u);
     __syncthreads();
     for (uint32_t x = threadIdx.x; x <= R.n_experts; x += ROUTE_TPB)
-        R.counts[(uint64_t)x * R.chunks + blockIdx.x] = c[x];
+        R.counts[(uint64_t)blockIdx.x * (R.n_experts + 1) + x] = c[x];
 }
 
-// An expert's counts to the positions before them among its own, 8 chunks a lane; its total.
-__global__ __launch_bounds__(64) void route_scan_kernel(Route R) {
-    uint32_t *c = R.counts + (uint64_t)blockIdx.x * R.chunks;
-    uint32_t sum = 0;
-    for (uint32_t b = 0; b < R.chunks; b += 512) {
-        const uint32_t i = b + threadIdx.x * 8;
-        uint32_t v[8], own = 0;
+// The experts' counts to the positions before them among their own, and their totals: 16 experts
+// a workgroup, its threads a 64th of the chunks of one each.
+constexpr uint32_t SCAN_EXPERTS = 16, SCAN_PARTS = 64;
+__global__ __launch_bounds__(SCAN_EXPERTS *SCAN_PARTS) void route_scan_kernel(Route R) {
+    __shared__ uint32_t sums[SCAN_PARTS][SCAN_EXPERTS + 1];
+    const uint32_t part = threadIdx.x / SCAN_EXPERTS, mine = threadIdx.x % SCAN_EXPERTS;
+    const uint32_t x = blockIdx.x * SCAN_EXPERTS + mine, row = R.n_experts + 1;
+    const uint32_t each = (R.chunks + SCAN_PARTS - 1) / SCAN_PARTS;
+    const uint32_t begin = min(part * each, R.chunks), end = min(begin + each, R.chunks);
+    uint32_t sum = 0, first[8];
+    if (x < row) {
 #pragma unroll
-        for (uint32_t k = 0; k < 8; k++) v[k] = i + k < R.chunks ? c[i + k] : 0;
+        for (uint32_t k = 0; k < 8; k++)
+            first[k] = begin + k < end ? R.counts[(uint64_t)(begin + k) * row + x] : 0;
 #pragma unroll
-        for (uint32_t k = 0; k < 8; k++) own += v[k];
-        const uint32_t upto = scan_wave(own);
-        uint32_t at = sum + upto - own;
-#pragma unroll
-        for (uint32_t k = 0; k < 8; k++) {
-            if (i + k < R.chunks) c[i + k] = at;
-            at += v[k];
-        }
-        sum += __builtin_amdgcn_readlane(upto, 63);
+        for (uint32_t k = 0; k < 8; k++) sum += first[k];
+#pragma unroll 8
+        for (uint32_t c = begin + 8; c < end; c++) sum += R.counts[(uint64_t)c * row + x];
     }
-    if (threadIdx.x == 0) R.totals[blockIdx.x] = sum;
+    sums[part][mine] = sum;
+    __syncthreads();
+    {  // a wave an expert, a lane a part
+        const uint32_t lane = threadIdx.x % SCAN_PARTS, e = threadIdx.x / SCAN_PARTS;
+        const uint32_t v = sums[lane][e], upto = scan_wave(v);
+        sums[lane][e] = upto - v;
+        const uint32_t y = blockIdx.x * SCAN_EXPERTS + e;
+        if (lane == SCAN_PARTS - 1 && y < row) R.totals[y] = upto;
+    }
+    __syncthreads();
+    if (x >= row) return;
+    uint32_t at = sums[part][mine];
+#pragma unroll
+    for (uint32_t k = 0; k < 8; k++) {
+        if (begin + k < end) R.counts[(uint64_t)(begin + k) * row + x] = at;
+        at += first[k];
+    }
+    for (uint32_t c = begin + 8; c < end; c++) {
+        const uint32_t v = R.counts[(uint64_t)c * row + x];
+        R.counts[(uint64_t)c * row + x] = at;
+        at += v;
+    }
 }
 
 // The sums of lower threads' values, of two at a time.
@@ -126,7 +146,7 @@ __global__ __launch_bounds__(ROUTE_TPB) void route_place_kernel(Route R) {
         for (uint32_t k = 0; k < EACH; k++) {
             const uint32_t x = threadIdx.x * EACH + k;
             total[k] = x <= R.n_experts ? R.totals[x] : 0;
-            before[k] = x <= R.n_experts ? R.counts[(uint64_t)x * R.chunks + blockIdx.x] : 0;
+            before[k] = x <= R.n_experts ? R.counts[(uint64_t)blockIdx.x * (R.n_experts + 1) + x] : 0;
         }
     for (uint32_t x = lane; x <= R.n_experts; x += 64) seen[w][x] = 0;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -368,7 +388,7 @@ void launch_route(const Route &R, hipStream_t s) {
     if (R.n > ROUTE_ONE) {
         launch(rounds == 2 ? route_count_kernel<2> : route_count_kernel<8>, R.chunks, ROUTE_TPB,
                s, R);
-        launch(route_scan_kernel, R.n_experts + 1, 64, s, R);
+        launch(route_scan_kernel, R.n_experts / SCAN_EXPERTS + 1, SCAN_EXPERTS * SCAN_PARTS, s, R);
     }
     const auto place = [&](auto b) {
         constexpr uint32_t B = decltype(b)::value;

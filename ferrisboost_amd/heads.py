@@ -104,7 +104,7 @@ def _cells(x, what: str) -> int:
 
 
 def _beside(x, other, what: str):
-    if x.device != other.device:
+    if x.get_device() != other.get_device():
         raise ValueError(f"{what} is on {x.device}, the call's other tensors on {other.device}")
     return x
 
@@ -274,10 +274,9 @@ def _functions():
 
     class LayerNorm(torch.autograd.Function):
         @staticmethod
-        def forward(ctx, x, weight, bias, eps):
-            out, stats = _layer_norm(x, weight, bias, eps, True)
+        def forward(ctx, x, weight, bias, a):
+            out, stats = _layer_norm(a, x, weight, bias, True)
             ctx.save_for_backward(x, stats, weight)
-            ctx.eps = eps
             ctx.mark_non_differentiable(stats)
             return out, stats
 
@@ -538,13 +537,12 @@ def _norm_of(x, weight, eps: float) -> bytes:
 
 def _vector(v, x, what: str):
     v = _beside(_device_tensor(v, what), x, what)
-    if v.dim() != 1 or v.shape[0] != x.shape[-1]:
+    if v.shape != x.shape[-1:]:
         raise ValueError(f"{what} must have shape ({x.shape[-1]},), got {tuple(v.shape)}")
     return v
 
 
-def _layer_norm(x, weight, bias, eps, stats: bool):
-    a = _norm_of(x, weight, eps)
+def _layer_norm(a: bytes, x, weight, bias, stats: bool):
     out = _torch.empty_like(x)
     kept = x.new_empty(x.shape[:-1] + (2,), dtype=_torch.float32) if stats else None
     dev = x.get_device()
@@ -563,22 +561,21 @@ def layer_norm(x, weight=None, bias=None, *, eps: float = 1e-5, stats: bool = Fa
     layer_norm_grad() takes: each row's mean and 1 / sqrt(variance + eps), (..., 2) float32."""
     torch = _need_torch()
     x = _device_tensor(x, "x")
-    _norm_of(x, None, eps := _eps(eps))
     if weight is not None:
-        weight = _vector(weight, x, "weight")
-        _cells(weight, "weight")
-        if bias is not None:
-            bias = _vector(bias, x, "bias")
-            if bias.dtype != weight.dtype:
-                raise ValueError(f"bias is {bias.dtype}, weight {weight.dtype}")
-    elif bias is not None:
-        raise ValueError("a bias needs a weight")
+        weight = _vector(weight, x, "weight") if x.dim() else weight
+    a = _norm_of(x, weight, _eps(eps))
+    if bias is not None:
+        if weight is None:
+            raise ValueError("a bias needs a weight")
+        bias = _vector(bias, x, "bias")
+        if bias.dtype != weight.dtype:
+            raise ValueError(f"bias is {bias.dtype}, weight {weight.dtype}")
     if torch.is_grad_enabled() and (x.requires_grad or
                                     (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
-        out = _functions()[2].apply(x, weight, bias, eps)
+        out = _functions()[2].apply(x, weight, bias, a)
     else:
-        out = _layer_norm(x, weight, bias, eps, stats)
+        out = _layer_norm(a, x, weight, bias, stats)
     return out if stats else out[0]
 
 
@@ -806,7 +803,8 @@ class AdamW(_Kept):
     writing into such a parameter). weight_decay is a number, or a list of one for each
     parameter; lr, an attribute, a number, or a float32 tensor of one value on the device,
     which a step reads when it runs. The steps are counted on the device too, so a captured
-    step goes on at each replay.
+    step goes on at each replay. Steps of one optimizer follow one another: on another stream
+    only when that has waited.
 
     bits=32 keeps m and s in float32, bits=8 in a byte each and an exponent for 256 cells:
     small floats with 3 bits behind the point, rounded up or down at random (from `seed`, the
@@ -985,6 +983,10 @@ class AdamW(_Kept):
         """Takes up a state of as many parameters of the same sizes, copying it. "decays" (the
         betas' powers) follow from "step" where they are missing, "masters" from the
         parameters."""
+        missing = {"step", "mean", "square"} | ({"scales"} if self.bits == 8 else set())
+        missing -= state.keys()
+        if missing:
+            raise ValueError(f"the state has no {', '.join(sorted(missing))}")
         step = _whole(state["step"], "step")
         if not 0 <= step < 1 << 62:
             raise ValueError(f"step must be in 0..=2^62 - 1, got {step}")

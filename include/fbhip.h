@@ -850,9 +850,9 @@ int fbh_layer_norm(int device, const fbh_norm *a, const void *x, const void *wei
 /* Device bytes of workspace that fbh_layer_norm_grad takes for dweight or dbias,
  * 16-byte aligned; 0 for a call that it refuses. */
 uint64_t fbh_layer_norm_grad_bytes(const fbh_norm *a);
-/* The gradients for the output's gradient grad: dx [n_rows][dim] (may be grad or x),
- * dweight and dbias [dim], summed over all rows (each may be NULL: not wanted); stats
- * as fbh_layer_norm gave them. The rows of a workgroup are summed in f32, the
+/* The gradients for the output's gradient grad: dx [n_rows][dim] (not grad or x: wide
+ * rows are read again), dweight and dbias [dim], summed over all rows (each may be NULL:
+ * not wanted); stats as fbh_layer_norm gave them. The rows of a workgroup are summed in f32, the
  * workgroups' sums, at most 1024, in f64. Orders of sums depend on n_rows and dim
  * alone. work may be NULL where neither dweight nor dbias is wanted. */
 int fbh_layer_norm_grad(int device, const fbh_norm *a, const void *grad, const void *x,
@@ -938,7 +938,8 @@ typedef struct {
  * as f32 and are then rounded to one of the two bytes around them, up with the
  * probability of what is cut off, to 2^-16: by the bits that fbh_dropout draws for seed
  * + t and the cell of the state, the low 16 for mean, the high 16 for square; a square
- * above 0 stays above 0. No two tensors may overlap, in memory or in the state. */
+ * above 0 stays above 0. No two tensors may overlap, in memory or in the state, and no
+ * gradient another tensor; steps of one state follow one another. */
 int fbh_adamw_step(int device, const fbh_adamw *a, const fbh_adamw_tensor *tensors,
                    uint64_t n_tensors, void *stream);
 /* The f32 values, n each, that moments of 8 bits stand for. */

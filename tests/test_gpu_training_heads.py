@@ -556,3 +556,54 @@ def test_adamw_of_more_than_2_32_bytes(heads):
     for part in (p[:5], p[-5:], opt.params[1]):
         assert (part.float() + 0.5).abs().max() <= 0.5 * 2.0 ** -8
     assert int((p != 0).sum()) == 10 and int((opt.square != 0).sum()) == 13
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_copies(heads, bits):
+    """A copy has parameters and a state of its own and goes on as the first one would."""
+    import copy
+    import pickle
+
+    p = [torch.randn(900, device="cuda"), torch.randn(5, device="cuda").bfloat16()]
+    grads = [[torch.randn_like(x) for x in p] for _ in range(4)]
+    opt = heads.AdamW(p, lr=0.1, bits=bits)
+    opt.step(grads[0])
+    copies = [copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))]
+    for g in grads[1:]:
+        opt.step(g)
+    for c in copies:
+        assert c.params[0].data_ptr() != p[0].data_ptr()
+        for g in grads[1:]:
+            c.step(g)
+        for x, y in zip(opt.params + opt._tensors(), c.params + c._tensors()):
+            assert torch.equal(x, y)
+    shared = copy.copy(opt)
+    shared.step(grads[0])
+    assert opt.state_dict()["step"] == 5 and shared.params[0] is p[0]
+
+
+def test_adamw_states_without_parts(heads):
+    opt = heads.AdamW([torch.zeros(5, device="cuda").half()], bits=8)
+    state = opt.state_dict()
+    for k in ("step", "mean", "square", "scales"):
+        with pytest.raises(ValueError, match=f"has no {k}"):
+            opt.load_state_dict({a: b for a, b in state.items() if a != k})
+    opt.params[0].fill_(2.0)
+    opt.load_state_dict({k: state[k] for k in ("step", "mean", "square", "scales")})
+    assert (opt.masters[0] == 2.0).all()
+
+
+def test_adamw_8_bit_moments_near_the_end_of_the_range(heads):
+    """A mean of 2^128, which rounding up gives, that a beta near 1 keeps beyond float32: its
+    cells are NaN. 2^127 (1 - 2^-30) is 2^127 as a float, whose exponent field is 254."""
+    n = 256
+    p = torch.zeros(n, device="cuda")
+    opt = heads.AdamW([p], lr=0.0, betas=(1.0 - 2.0 ** -30, 0.999), bits=8)
+    state = opt.state_dict()
+    state["mean"][:3] = torch.tensor([0x78, 0xF8, 0x70], dtype=torch.uint8)
+    state["scales"][0] = 254
+    opt.load_state_dict(state)
+    opt.step([torch.zeros(n, device="cuda")])
+    m = opt.moments()[0]
+    assert torch.isnan(m[:2]).all() and float(m[2]) == 2.0 ** 127
+    assert (m[3:] == 0).all() and int(opt.scales[0, 0]) == 254

@@ -31,7 +31,7 @@ def test_layer_norm_refusals_of_the_c_abi(bad, msg):
     with pytest.raises(ValueError, match=msg):
         N.check_hip(L.fbh_layer_norm(0, a, 64, None, None, 64, None, None))
     with pytest.raises(ValueError, match=msg):
-        N.check_hip(L.fbh_layer_norm_grad(0, a, 64, 64, 64, None, 64, None, None, None, 0, None))
+        N.check_hip(L.fbh_layer_norm_grad(0, a, 64, 64, 64, None, 72, None, None, None, 0, None))
     assert L.fbh_layer_norm_grad_bytes(a) == 0
 
 
@@ -42,6 +42,10 @@ def test_layer_norm_null_arguments_and_workspace():
             N.check_hip(L.fbh_layer_norm(0, a, *args, None))
     with pytest.raises(ValueError, match="null"):
         N.check_hip(L.fbh_layer_norm_grad(0, a, 64, 64, None, None, 64, None, None, None, 0, None))
+    for dx in (64, 128):
+        with pytest.raises(ValueError, match="must not be grad or x"):
+            N.check_hip(L.fbh_layer_norm_grad(0, a, 64, 128, 64, None, dx, None, None, None, 0,
+                                              None))
     need = L.fbh_layer_norm_grad_bytes(a)
     assert need > 0
     for work, size, msg in ((64, need - 1, "workspace"), (None, 0, "workspace"),
