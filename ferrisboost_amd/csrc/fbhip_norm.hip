@@ -2,10 +2,16 @@
 // and its gradients. With h = (x - mean) * r and d = g * w for the output's gradient g:
 //   dx = r * (d - mean(d) - h * mean(d * h)),  dw = sum over rows of g * h,  db = sum of g.
 //
-// A row is held in registers by G lanes of C cells each, so that every cell is read once. Its
-// sums are taken in f32 in a tree whose shape depends on the width alone; the variance is the
-// mean square of differences from the mean, and what the mean's rounding leaves in them (their
-// own sum) is taken out: rows far from 0 keep their cells' accuracy.
+// A row is held in registers by G lanes of C cells each, so that every cell is read once, and
+// the next one is on its way meanwhile: bound by memory (bfloat16, against 4.84 TB/s of a large
+// copy: forward 32768 x 4096 in 102 us, 5.3 TB/s, 1M x 60 in 47, 4096 x 30000 in 109; gradients
+// of 32768 x 4096 in 154 us and 5 for the parts of the weights' sums, 5.2 TB/s, 100k x 64 in 11
+// and 4). Loads that were widened as they came, and cells read one by one at a row's end, had
+// the gradient of 32768 x 4096 wait for each row: 258 us.
+//
+// A row's sums are taken in f32 in a tree whose shape depends on the width alone; the variance
+// is the mean square of differences from the mean, and what the mean's rounding leaves in them
+// (their own sum) is taken out: rows far from 0 keep their cells' accuracy.
 #include "fbhip_heads.h"
 
 #include <algorithm>
@@ -14,7 +20,6 @@ namespace fbh {
 namespace {
 
 constexpr uint32_t NORM_MAX_DIM = 32768;
-constexpr uint64_t NORM_BLOCKS = 2048;  // of a launch at most: they go through the rows in turn
 
 struct Norm {
     const void *weight, *bias;
@@ -166,17 +171,17 @@ __device__ __forceinline__ void store_cells(T *row, L at, F &&f) {
         }
 }
 
-// Sums of f(cell) over the lane's cells that take part: of all, and again with care by those
-// few lanes that have others.
+// Sums of f(cell) over the lane's cells that take part; with care in those few lanes that have
+// others.
 template <uint32_t K, uint32_t C, class L, class F>
 __device__ __forceinline__ void sum_cells(float (&s)[K], L at, bool ragged, F &&f) {
 #pragma unroll
     for (uint32_t k = 0; k < K; k++) s[k] = 0.0f;
+    if (!ragged) {
 #pragma unroll
-    for (uint32_t i = 0; i < C; i++) f(i, s);
-    if (ragged) {
-#pragma unroll
-        for (uint32_t k = 0; k < K; k++) s[k] = 0.0f;
+        for (uint32_t i = 0; i < C; i++) f(i, s);
+    } else {
+        asm volatile("" : "+s"(at.dim));  // (what is asked of it here is not kept in registers)
 #pragma unroll
         for (uint32_t i = 0; i < C; i++)
             if (at.counts(i)) f(i, s);
@@ -382,7 +387,7 @@ __global__ __launch_bounds__(norm_threads<G>()) void norm_grad_kernel(NormGrad A
     }
 }
 
-// dw and db of wide rows: four columns a thread, four rows at a time, the rows cut into `groups`
+// dw and db of rows of more than 16384 cells, from the rows once more: four columns a thread, four rows at a time, the rows cut into `groups`
 // equal parts. A thread's columns start at dim - 4 at the latest.
 template <class T>
 __global__ __launch_bounds__(256) void norm_columns_kernel(NormGrad A, const T *g, const T *x,
@@ -470,12 +475,15 @@ uint32_t rows_of_group(uint32_t dim) {
     return rows;
 }
 
-// Parts of the weights' sums: as many workgroups as the device holds at a time, or fewer where
-// the parts would be large beside the rows.
+// Parts of the weights' sums, a workgroup's each: as many workgroups as the device holds at a
+// time, fewer where their parts would be large beside the rows (in us, bfloat16 gradients of
+// 4096 cells: 512 rows with 512 parts 24.2, with 128 14.4; 2048 rows with 512 parts 25.9, with
+// 256 21.8), and 128 while there are rows for them (128 rows: 10.2, with 32 parts 12.7).
 uint32_t grad_groups(uint64_t n_rows, uint32_t dim) {
     const uint64_t most = dim <= 256 ? 1024 : dim <= 4096 ? 512 : dim <= SPLIT_DIM ? 256 : 64;
-    const uint64_t n = (n_rows + rows_of_group(dim) - 1) / rows_of_group(dim);
-    return (uint32_t)(n < most ? (n ? n : 1) : most);
+    const uint32_t rows = rows_of_group(dim);
+    const uint64_t n = std::max<uint64_t>((n_rows + rows - 1) / rows, 1);
+    return (uint32_t)std::min({n, most, std::max<uint64_t>(n / (rows == 1 ? 8 : 4), 128)});
 }
 
 uint64_t padded_rows(uint64_t n) { return (n + 3) / 4 * 4; }
@@ -485,6 +493,11 @@ uint64_t grad_bytes(const fbh_norm *a) {
     if (a->dim > SPLIT_DIM) b += padded_rows(a->n_rows) * 4;
     return b;
 }
+
+// Workgroups of a launch at most: they go through the rows in turn, and the more of them there
+// are the more often the weights are read (4096 x 30000 bfloat16: 109 us with 256, 155 with
+// 4096), but small rows' latencies overlap better (1M x 60: 114 and 47).
+uint64_t norm_blocks(uint32_t dim) { return dim <= 8192 ? 4096 : dim <= SPLIT_DIM ? 1024 : 256; }
 
 void check_norm(const fbh_norm *a) {
     head_input(a, "null argument");
@@ -510,7 +523,7 @@ void launch_norm(const fbh_norm *a, const void *x, const void *weight, const voi
         constexpr uint32_t N = decltype(n)::value, G = decltype(g)::value, C = decltype(c)::value;
         constexpr uint32_t ROWS = norm_threads<G>() / G;
         const uint64_t blocks = (a->n_rows + ROWS - 1) / ROWS;
-        launch(norm_kernel<T, N, G, C>, std::min<uint64_t>(blocks, NORM_BLOCKS), norm_threads<G>(), s, A,
+        launch(norm_kernel<T, N, G, C>, std::min(blocks, norm_blocks(a->dim)), norm_threads<G>(), s, A,
                static_cast<const T *>(x), static_cast<T *>(out), stats);
     });
 }
@@ -526,7 +539,7 @@ void launch_norm_grad(const fbh_norm *a, const T *g, const T *x, const float *st
         constexpr uint32_t N = decltype(nn)::value, G = decltype(gg)::value;
         constexpr uint32_t C = decltype(cc)::value;
         constexpr bool SUMS = G * C <= SPLIT_DIM;
-        const uint64_t blocks = SUMS ? groups : std::clamp<uint64_t>(a->n_rows, 1, 512);
+        const uint64_t blocks = SUMS ? groups : std::clamp<uint64_t>(a->n_rows, 1, norm_blocks(a->dim));
         launch(norm_grad_kernel<T, N, G, C, SUMS>, blocks, norm_threads<G>(), s, A, g, x, dx);
     });
     if (!sums) return;

@@ -5,7 +5,10 @@
 //   starts  the first row of every expert, and the end of the last one's
 //
 // The sort is one counting pass, as there are at most 1024 ids: counts of the ids in chunks of
-// positions, their sums over the chunks before, and places from both. All orders are fixed.
+// positions, their sums over the chunks before, and places from both; up to 4096 positions take
+// one workgroup and launch (2.6 us for 8, 7.5 for 4000). All orders are fixed. 2M positions of
+// 511 ids take 5.6 + 3.6 + 14.6 us where memory would take 5: each launch's workgroups are all
+// on the device at once, and its time is what one of them takes from its loads to its stores.
 #include "fbhip_heads.h"
 
 #include <algorithm>
@@ -210,8 +213,11 @@ __global__ __launch_bounds__(ROUTE_TPB) void route_place_kernel(Route R) {
 }
 
 // ------------------------------------------------------------------- rows
-// A row's pieces go to G = 2^lg_g lanes; the last one starts at dim - VEC, so that no piece is
-// partial: the cells it shares with the one before are written twice, with the same value.
+// Bound by memory (65,536 rows of 1024 bfloat16 cells with 2 columns: to the experts 63 us, 402
+// MB, 6.4 TB/s, most of them writes that the last-level cache takes; back 94 us, 4.3 TB/s, rows
+// read from everywhere; a copy reaches 4.84). A row's pieces go to G = 2^lg_g lanes; the last one
+// starts at dim - VEC, so that no piece is partial: the cells it shares with the one before are
+// written twice, with the same value.
 struct Rows {
     const int32_t *place;
     const float *weights;
@@ -308,7 +314,9 @@ __global__ __launch_bounds__(256) void from_experts_kernel(Rows R, const T *y, T
     });
 }
 
-// The gradients of from_experts: dy = weight * g to the place, dweight = <g, y> there.
+// The gradients of from_experts: dy = weight * g to the place, dweight = <g, y> there; a row of
+// g is read once for K columns, and not once for each (30,001 rows of 515 float32 cells with 4
+// columns: 141 -> 124 us, 4.5 TB/s).
 template <class T, int VEC, int K>
 __device__ __forceinline__ void from_experts_grad_row(const Rows &R, const T *g, const T *y, T *dy,
                                                       float *dweights, uint64_t row,

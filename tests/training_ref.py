@@ -34,8 +34,10 @@ def layer_norm(x, w, b, eps):
 def layer_norm_grad(g, x, w, eps, groups=512):
     """((dx, off), (dw, off), (db, off)). The means over a row are trees as above, 48 half steps
     of their terms' magnitudes; h is off by 64 of |h| + 1, the statistics kept in float32 among
-    them, r by 30. A weight's sum is a chain over the rows of a workgroup, in turn and then side
-    by side (at most 64), and exact from there on."""
+    them, r by 30. A weight's sum is a chain over the rows of a workgroup, in turn (a group of
+    lanes has at most one in 512 of a few thousand rows, or one in 64 of up to 600 wide ones) and
+    then side by side (at most 64 groups, of which wide rows have one), and exact from there
+    on."""
     g, n = g.astype(np.float64), x.shape[0]
     w = np.ones(x.shape[-1]) if w is None else w.astype(np.float64)
     h, r = norm_parts(x, eps)
