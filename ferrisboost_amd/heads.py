@@ -801,8 +801,8 @@ class AdamW(_Kept):
     in float32. params are contiguous tensors of one device; one of 16 bits has a float32 copy
     in `masters`, which is what the steps move and round into it (call take_params() after
     writing into such a parameter). weight_decay is a number, or a list of one for each
-    parameter; lr, an attribute, a number, or a float32 tensor of one value on the device,
-    which a step reads when it runs. The steps are counted on the device too, so a captured
+    parameter; lr a number, or a float32 tensor of one value on the device, which a step reads
+    when it runs. Both are attributes that may be set between steps. The steps are counted on the device too, so a captured
     step goes on at each replay. Steps of one optimizer follow one another: on another stream
     only when that has waited.
 
@@ -827,12 +827,8 @@ class AdamW(_Kept):
             raise ValueError(f"bits must be 8 or 32, got {bits!r}")
         self.lr, self.betas, self.eps, self.bits = lr, betas, _eps(eps), int(bits)
         self.seed = _seed(seed)
-        n = len(self.params)
-        decays = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else (
-            [weight_decay] * n)
-        self.weight_decay = [float(d) for d in decays]
-        if len(decays) != n or not all(0.0 <= d <= _MOST for d in self.weight_decay):
-            raise ValueError(f"weight_decay must be a number, not negative, or a list of {n}")
+        self._parts = None
+        self.weight_decay = weight_decay
         self.first, at, spans = [], 0, []
         for i, p in enumerate(self.params):
             self._check(i, p)
@@ -849,7 +845,7 @@ class AdamW(_Kept):
         self._types = [p.dtype for p in self.params]
         # an fbh_adamw_tensor a parameter, whose addresses are filled in at each step
         self._parts = [x for i, p in enumerate(self.params) for x in
-                       (0, 0, 0, self._sizes[i], self.first[i], self.weight_decay[i],
+                       (0, 0, 0, self._sizes[i], self.first[i], self._decays[i],
                         _CELLS[p.dtype])]
         self._lr()
         like = self.params[0]
@@ -863,6 +859,22 @@ class AdamW(_Kept):
         self._clock = torch.zeros(4, dtype=torch.int64, device=like.device)
         self._clock[1:3] = 0x3FF0000000000000  # 1.0
         self._streams = {_raw_stream(like.get_device())}
+
+    @property
+    def weight_decay(self) -> tuple:
+        """Each parameter's weight decay; it is set as a number or a list of one for each."""
+        return self._decays
+
+    @weight_decay.setter
+    def weight_decay(self, value):
+        n = len(self.params)
+        decays = tuple(float(d) for d in value) if isinstance(value, (list, tuple)) else (
+            (float(value),) * n)
+        if len(decays) != n or not all(0.0 <= d <= _MOST for d in decays):
+            raise ValueError(f"weight_decay must be a number, not negative, or a list of {n}")
+        self._decays = decays
+        if self._parts is not None:
+            self._parts[5::7] = decays
 
     def _check(self, i: int, p):
         if not isinstance(p, _torch.Tensor):

@@ -582,6 +582,21 @@ def test_adamw_copies(heads, bits):
     assert opt.state_dict()["step"] == 5 and shared.params[0] is p[0]
 
 
+def test_adamw_weight_decay_between_steps(heads):
+    p = [torch.ones(300, device="cuda"), torch.ones(7, device="cuda")]
+    zeros = [torch.zeros_like(x) for x in p]
+    opt = heads.AdamW(p, lr=0.5, weight_decay=0.0)
+    opt.step(zeros)
+    assert (p[0] == 1.0).all() and opt.weight_decay == (0.0, 0.0)
+    opt.weight_decay = [0.5, 0.25]
+    opt.step(zeros)
+    assert (p[0] == 0.75).all() and (p[1] == 0.875).all()
+    for bad in ([0.1], -1.0, float("inf")):
+        with pytest.raises(ValueError, match="weight_decay"):
+            opt.weight_decay = bad
+    assert opt.weight_decay == (0.5, 0.25)
+
+
 def test_adamw_states_without_parts(heads):
     opt = heads.AdamW([torch.zeros(5, device="cuda").half()], bits=8)
     state = opt.state_dict()
