@@ -239,9 +239,11 @@ __device__ __forceinline__ void adam_chunk(const Adam &A, const AdamStep &S, con
                                         ADAM_TOP_S) * S.b2;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
+            // (each product rounded by itself, so that whoever computes them in doubles has
+            // the same bytes)
             const double gd = (double)g[k];
-            m[k] = (float)fma((double)mean_float(cm, k), scale_m, gd * S.c1);
-            s[k] = (float)fma((double)square_float(cs, k), scale_s, gd * gd * S.c2);
+            m[k] = (float)((double)mean_float(cm, k) * scale_m + gd * S.c1);
+            s[k] = (float)((double)square_float(cs, k) * scale_s + gd * gd * S.c2);
         }
         if (has_nan_mean(cm) || has_nan_square(cs)) {
             seldom();
