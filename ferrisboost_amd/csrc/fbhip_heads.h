@@ -175,7 +175,7 @@ __device__ __forceinline__ uint64_t same_digit(bool in, uint32_t digit, uint32_t
     const uint64_t all = __ballot(in);
     uint32_t lo = (uint32_t)all, hi = (uint32_t)(all >> 32);
     for (uint32_t b = 0; b < bits; b++) {
-        const uint32_t bit = (uint32_t)((int32_t)(digit << (31 - b)) >> 31);  // 0 or all ones
+        const uint32_t bit = (uint32_t)__builtin_amdgcn_sbfe((int)digit, b, 1);  // 0 or all ones
         const uint64_t ones = __ballot(bit != 0);
         lo &= ~((uint32_t)ones ^ bit);
         hi &= ~((uint32_t)(ones >> 32) ^ bit);

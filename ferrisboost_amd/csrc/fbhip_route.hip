@@ -129,13 +129,15 @@ __device__ __forceinline__ void before_in_group(uint32_t (&v)[2], uint32_t (*sum
 // A chunk is sorted in LDS first: what a wave then writes of `order` are a few runs and not 64
 // cells apart (16M positions of 64 experts: 70 us straight from the ranks). ONE: the only
 // workgroup, which needs no counts. BITS: of the experts' numbers, known so that the search for
-// equal ones in a wave has no loop.
+// equal ones in a wave has no loop, a thread has one of up to 512 experts (2M positions of 511
+// with room for 1024: 14.7 us), and workgroups of few take little LDS.
 template <uint32_t ROUNDS, uint32_t BITS, bool ONE>
 __global__ __launch_bounds__(ROUTE_TPB) void route_place_kernel(Route R) {
-    constexpr uint32_t EACH = (ROUTE_MAX_EXPERTS + ROUTE_TPB) / ROUTE_TPB;  // experts a thread
+    constexpr uint32_t ROOM = BITS > 10 ? ROUTE_MAX_EXPERTS + 1 : 1u << BITS;
+    constexpr uint32_t EACH = (ROOM + ROUTE_TPB - 1) / ROUTE_TPB;  // experts a thread
     constexpr uint32_t CHUNK = ROUTE_TPB * ROUNDS;
-    __shared__ uint32_t seen[ROUTE_WAVES][ROUTE_MAX_EXPERTS + 1];
-    __shared__ uint32_t shift[ROUTE_MAX_EXPERTS + 1];  // from places in the chunk to those in all
+    __shared__ uint32_t seen[ROUTE_WAVES][ROOM];
+    __shared__ uint32_t shift[ROOM];  // from places in the chunk to those in all
     __shared__ uint32_t sorted[CHUNK];  // a position's number in the chunk, and its expert
     __shared__ uint32_t sums[ROUTE_WAVES][2];
     const uint32_t lane = threadIdx.x & 63, w = threadIdx.x / 64;
@@ -410,6 +412,7 @@ void launch_route(const Route &R, hipStream_t s) {
     // (numbers up to n_experts, which stands for none)
     if (R.n_experts < 16) place(std::integral_constant<uint32_t, 4>{});
     else if (R.n_experts < 128) place(std::integral_constant<uint32_t, 7>{});
+    else if (R.n_experts < 512) place(std::integral_constant<uint32_t, 9>{});
     else place(std::integral_constant<uint32_t, 11>{});
 }
 
