@@ -70,6 +70,7 @@ struct AdamLaunch {
     AdamTensor t[ADAM_TENSORS];
 };
 static_assert(sizeof(AdamLaunch) <= 4096, "kernel arguments");
+static_assert(ADAM_TENSORS == 64, "a lane each");
 
 // A step's numbers.
 struct AdamStep {
@@ -339,12 +340,10 @@ __global__ __launch_bounds__(ADAM_TPB) void adam_kernel(AdamLaunch L) {
     const AdamStep S = adam_step(A);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     for (uint64_t tile = blockIdx.x; tile < A.tiles; tile += gridDim.x) {
-        uint32_t lo = 0, hi = A.n_tensors;  // the last one that begins at the tile or before
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (L.t[mid].tiles_before <= tile) lo = mid;
-            else hi = mid;
-        }
+        // the last tensor that begins at the tile or before, by a lane each
+        const uint32_t lane = threadIdx.x & 63;
+        const uint64_t before = lane < A.n_tensors ? L.t[lane].tiles_before : ~0ull;
+        const uint32_t lo = __popcll(__ballot(before <= tile)) - 1;
         const AdamTensor &t = L.t[lo];
         const uint64_t begin = (tile - t.tiles_before) * ADAM_TILE +
                                wave * (ADAM_CHUNKS * ADAM_CHUNK);
@@ -357,10 +356,11 @@ __global__ __launch_bounds__(ADAM_TPB) void adam_kernel(AdamLaunch L) {
         }
     }
     if (!A.ticks) return;
-    // the last workgroup that is through moves the clock on: all have read it by then
+    // the last workgroup that is through moves the clock on: all have read it by then (which
+    // is all that the count has to order, and no load passes the barrier)
     __syncthreads();
     if (threadIdx.x == 0 &&
-        __hip_atomic_fetch_add(&A.clock->done, 1ull, __ATOMIC_ACQ_REL,
+        __hip_atomic_fetch_add(&A.clock->done, 1ull, __ATOMIC_RELAXED,
                                __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1) {
         A.clock->done = 0;
         tick(A.clock, A.beta1, A.beta2);
