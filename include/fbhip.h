@@ -873,7 +873,8 @@ int fbh_route(int device, const void *ids, uint32_t id_type, uint64_t n_position
               uint64_t work_bytes, void *stream);
 /* Row place[i][j] of out [n_rows * n_columns][dim] is x[i], for every row i and column
  * j; zeros where place is negative (row -1 - place). place is fbh_route's (places
- * beyond the rows are taken to the last one). dim at most 32768. */
+ * beyond the rows are taken to the last one). dim at most 32768. Here and below no
+ * output overlaps an input. */
 int fbh_to_experts(int device, const void *x, const int32_t *place, uint64_t n_rows,
                    uint32_t n_columns, uint32_t dim, uint32_t dtype, void *out, void *stream);
 /* out[i] = the sum over columns of weights[i][j] * y[place[i][j]] (weights NULL: 1), in
