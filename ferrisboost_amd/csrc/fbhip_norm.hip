@@ -234,7 +234,9 @@ __global__ __launch_bounds__(norm_threads<G>()) void norm_kernel(Norm A, const T
         });
         sum_of_group<G, 2>(s2, second, turn);
         const float rest = s2[0] * inv_n;
-        const float rstd = 1.0f / sqrtf((s2[1] * inv_n - rest * rest) + A.eps);
+        // (of equal cells, by rounding, the variance may be below 0; NaN stays)
+        const float var = s2[1] * inv_n - rest * rest;
+        const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + A.eps);
         if (row >= A.n_rows) continue;  // (all of a group's lanes, and with G > 64 never)
         store_cells(out + row * A.dim, at, [&](uint32_t i) {
             return fmaf((c.cell(i) - mean - rest) * rstd, w.v[i], b.v[i]);
@@ -387,8 +389,9 @@ __global__ __launch_bounds__(norm_threads<G>()) void norm_grad_kernel(NormGrad A
     }
 }
 
-// dw and db of rows of more than 16384 cells, from the rows once more: four columns a thread, four rows at a time, the rows cut into `groups`
-// equal parts. A thread's columns start at dim - 4 at the latest.
+// dw and db of rows of more than 16384 cells, from the rows once more: four columns a thread,
+// four rows at a time, the rows cut into `groups` equal parts. A thread's columns start at
+// dim - 4 at the latest.
 template <class T>
 __global__ __launch_bounds__(256) void norm_columns_kernel(NormGrad A, const T *g, const T *x,
                                                            const float *rests, float *parts) {
@@ -523,8 +526,8 @@ void launch_norm(const fbh_norm *a, const void *x, const void *weight, const voi
         constexpr uint32_t N = decltype(n)::value, G = decltype(g)::value, C = decltype(c)::value;
         constexpr uint32_t ROWS = norm_threads<G>() / G;
         const uint64_t blocks = (a->n_rows + ROWS - 1) / ROWS;
-        launch(norm_kernel<T, N, G, C>, std::min(blocks, norm_blocks(a->dim)), norm_threads<G>(), s, A,
-               static_cast<const T *>(x), static_cast<T *>(out), stats);
+        launch(norm_kernel<T, N, G, C>, std::min(blocks, norm_blocks(a->dim)), norm_threads<G>(),
+               s, A, static_cast<const T *>(x), static_cast<T *>(out), stats);
     });
 }
 
@@ -539,7 +542,8 @@ void launch_norm_grad(const fbh_norm *a, const T *g, const T *x, const float *st
         constexpr uint32_t N = decltype(nn)::value, G = decltype(gg)::value;
         constexpr uint32_t C = decltype(cc)::value;
         constexpr bool SUMS = G * C <= SPLIT_DIM;
-        const uint64_t blocks = SUMS ? groups : std::clamp<uint64_t>(a->n_rows, 1, norm_blocks(a->dim));
+        const uint64_t most = norm_blocks(a->dim);
+        const uint64_t blocks = SUMS ? groups : std::clamp<uint64_t>(a->n_rows, 1, most);
         launch(norm_grad_kernel<T, N, G, C, SUMS>, blocks, norm_threads<G>(), s, A, g, x, dx);
     });
     if (!sums) return;

@@ -151,7 +151,8 @@ __global__ __launch_bounds__(ROUTE_TPB) void route_place_kernel(Route R) {
         for (uint32_t k = 0; k < EACH; k++) {
             const uint32_t x = threadIdx.x * EACH + k;
             total[k] = x <= R.n_experts ? R.totals[x] : 0;
-            before[k] = x <= R.n_experts ? R.counts[(uint64_t)blockIdx.x * (R.n_experts + 1) + x] : 0;
+            before[k] = x <= R.n_experts
+                            ? R.counts[(uint64_t)blockIdx.x * (R.n_experts + 1) + x] : 0;
         }
     for (uint32_t x = lane; x <= R.n_experts; x += 64) seen[w][x] = 0;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -242,7 +243,8 @@ __device__ __forceinline__ void for_rows(const Rows &R, F &&f) {
 }
 
 template <class T, int VEC>
-__device__ __forceinline__ void to_experts_row(Rows R, const T *x, T *out, uint64_t row, uint32_t lane) {
+__device__ __forceinline__ void to_experts_row(const Rows &R, const T *x, T *out, uint64_t row,
+                                               uint32_t lane) {
     const int32_t *place = R.place + row * R.n_columns;
     for (uint32_t p = lane; p < R.pieces; p += 1u << R.lg_g) {
         const uint32_t c = min(p * VEC, R.dim - VEC);

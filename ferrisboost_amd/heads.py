@@ -802,9 +802,9 @@ class AdamW(_Kept):
     in `masters`, which is what the steps move and round into it (call take_params() after
     writing into such a parameter). weight_decay is a number, or a list of one for each
     parameter; lr a number, or a float32 tensor of one value on the device, which a step reads
-    when it runs. Both are attributes that may be set between steps. The steps are counted on the device too, so a captured
-    step goes on at each replay. Steps of one optimizer follow one another: on another stream
-    only when that has waited.
+    when it runs. Both are attributes that may be set between steps. The steps are counted on
+    the device too, so a captured step goes on at each replay. Steps of one optimizer follow
+    one another: on another stream only when that has waited.
 
     bits=32 keeps m and s in float32, bits=8 in a byte each and an exponent for 256 cells:
     small floats with 3 bits behind the point, rounded up or down at random (from `seed`, the

@@ -124,6 +124,31 @@ def test_layer_norm_rows_do_not_depend_on_their_neighbours(heads):
         assert torch.equal(heads.layer_norm(x[:n]), y[:n])
 
 
+@pytest.mark.parametrize("dim", [3, 31, 100, 1000, 5000, 12_000, 30_000])
+def test_layer_norm_of_equal_cells_with_a_tiny_eps(heads, dim):
+    """What rounding leaves of a variance of 0 may be below it, never a NaN: cells are off from
+    their mean by at most 46 half steps of it, and by 46 of that once it is taken out."""
+    x = torch.full((64, dim), 1.0, device="cuda") * (torch.rand(64, 1, device="cuda") * 1000 + 0.1)
+    for eps in (2.0 ** -126, 1e-30, 1e-12):
+        y, stats = heads.layer_norm(x, eps=eps, stats=True)
+        assert torch.isfinite(y).all() and torch.isfinite(stats).all()
+        off = x.abs().max().double() * (46 * 2.0 ** -24) ** 2 * stats[:, 1:].double()
+        assert (y.double().abs() <= off * 1.01).all()
+
+
+@pytest.mark.parametrize("n, dim", [(700, 3), (700, 33), (300, 513), (40, 4097), (300, 16_385)])
+def test_layer_norm_in_place(heads, n, dim):
+    """The C entry allows an output over its input."""
+    from ferrisboost_amd import _native as N
+
+    x = torch.randn(n, dim, device="cuda")
+    want = heads.layer_norm(x)
+    a = heads._norm_of(x, None, EPS)
+    N.check_hip(heads._L.fbh_layer_norm(0, a, x.data_ptr(), None, None, x.data_ptr(), None,
+                                        heads._raw_stream(0)))
+    assert torch.equal(x, want)
+
+
 def test_layer_norm_shapes(heads):
     """Leading axes, no rows, slices that no 16-byte piece begins at, transposed tensors."""
     x = torch.randn(3, 4, 50, device="cuda")
