@@ -248,7 +248,11 @@ __global__ __launch_bounds__(norm_threads<G>()) void norm_kernel(Norm A, const T
     }
 }
 
-// f(cells of a piece, lanes of a row, cells of a lane) by the row's cells.
+// f(cells of a piece, lanes of a row, cells of a lane) by the row's cells: few lanes, so that all
+// of them have cells (1M rows of 60 bfloat16 in 16 lanes 68 us, in 8 41 to 47), but no more than
+// 16 cells of a lane while rows still fit the device's workgroups, as sums over more cells cost
+// their registers: waves or, from 512 lanes on, the next row on its way (gradients of 8192 x
+// 16384 bfloat16: 512 lanes of 32 cells 170 us, 1024 of 16, with half the registers each, 208).
 template <class T, class F>
 void with_shape(uint32_t dim, F &&f) {
     constexpr uint32_t N = 16 / sizeof(T);

@@ -277,6 +277,7 @@ def _functions():
         def forward(ctx, x, weight, bias, a):
             out, stats = _layer_norm(a, x, weight, bias, True)
             ctx.save_for_backward(x, stats, weight)
+            ctx.a = a
             ctx.mark_non_differentiable(stats)
             return out, stats
 
@@ -284,7 +285,7 @@ def _functions():
         @torch.autograd.function.once_differentiable
         def backward(ctx, grad, _):
             x, stats, weight = ctx.saved_tensors
-            return _layer_norm_grad(_device_tensor(grad, "grad"), x, stats, weight,
+            return _layer_norm_grad(ctx.a, _device_tensor(grad, "grad"), x, stats, weight,
                                     ctx.needs_input_grad[:3]) + (None,)
 
     class ToExperts(torch.autograd.Function):
@@ -579,8 +580,7 @@ def layer_norm(x, weight=None, bias=None, *, eps: float = 1e-5, stats: bool = Fa
     return out if stats else out[0]
 
 
-def _layer_norm_grad(grad, x, stats, weight, wanted):
-    a = _norm_of(x, weight, 1.0)
+def _layer_norm_grad(a: bytes, grad, x, stats, weight, wanted):
     dx = _torch.empty_like(x) if wanted[0] else None
     dw = _torch.empty_like(weight) if wanted[1] else None
     db = _torch.empty_like(weight) if wanted[2] else None
@@ -606,18 +606,17 @@ def layer_norm_grad(grad, x, stats, weight=None):
     x = _device_tensor(x, "x")
     grad = _beside(_device_tensor(grad, "grad"), x, "grad")
     stats = _beside(_device_tensor(stats, "stats"), x, "stats")
-    _norm_of(x, None, 1.0)
+    if weight is not None:
+        weight = _vector(weight, x, "weight") if x.dim() else weight
+    a = _norm_of(x, weight, 1.0)
     if grad.shape != x.shape or grad.dtype != x.dtype:
         raise ValueError(f"grad is {grad.dtype} of {tuple(grad.shape)}, x {x.dtype} of "
                          f"{tuple(x.shape)}")
     if stats.dtype != torch.float32 or stats.shape != x.shape[:-1] + (2,):
         raise ValueError(f"stats must be float32 of {tuple(x.shape[:-1]) + (2,)}, got "
                          f"{stats.dtype} of {tuple(stats.shape)}")
-    if weight is not None:
-        weight = _vector(weight, x, "weight")
-        _cells(weight, "weight")
-    return _layer_norm_grad(grad, x, stats, weight, (True, weight is not None,
-                                                     weight is not None))
+    both = weight is not None
+    return _layer_norm_grad(a, grad, x, stats, weight, (True, both, both))
 
 
 # ------------------------------------------------------------------- experts

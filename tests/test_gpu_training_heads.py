@@ -297,6 +297,24 @@ def test_rows_to_experts_and_back(heads, n, k, e, dim, dtype):
         assert torch.equal(got[1], weights.grad)
 
 
+def test_positions_without_an_expert_take_any_weight(heads):
+    """NaN and infinity there reach neither outputs nor gradients."""
+    rng = np.random.default_rng(8)
+    for k in (1, 2, 5):
+        ids = torch.from_numpy(rng.integers(-1, 4, (500, k))).cuda()
+        ids[7] = -1  # a row of none
+        r = heads.Routes(ids, 4)
+        y = torch.randn(500 * k, 70, device="cuda")
+        g = torch.randn(500, 70, device="cuda")
+        w = torch.rand(500, k, device="cuda")
+        bad = torch.where(ids < 0, torch.tensor(float("nan"), device="cuda"), w)
+        bad[7] = float("inf")
+        assert torch.equal(heads.from_experts(y, r, bad), heads.from_experts(y, r, w))
+        got, want = (heads.from_experts_grad(g, y, r, a) for a in (bad, w))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert (want[1][ids < 0] == 0).all() and (heads.from_experts(y, r, bad)[7] == 0).all()
+
+
 def test_experts_leading_axes_and_odd_addresses(heads):
     rng = np.random.default_rng(3)
     ids = torch.from_numpy(rng.integers(-1, 6, (3, 5, 2))).cuda()
