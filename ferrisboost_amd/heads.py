@@ -38,6 +38,7 @@ has no gradient. Bad arguments are ValueErrors, device failures RuntimeErrors.
 from __future__ import annotations
 
 import functools
+import operator
 import struct
 
 import numpy as np
@@ -60,6 +61,7 @@ _OPTIONS = struct.Struct("PPPPfiff")
 _NORM = struct.Struct("QIIIf")                 # fbh_norm
 _ADAMW = struct.Struct("IfdddPQQPPPP")         # fbh_adamw
 _MOST = float(np.finfo(np.float32).max)
+_dtype_of, _shape_of = operator.attrgetter("dtype"), operator.attrgetter("shape")
 
 
 def _need_torch():
@@ -791,6 +793,12 @@ def from_experts_grad(grad, y, routes: Routes, weights=None):
 
 
 # ------------------------------------------------------------------- AdamW
+@functools.lru_cache(maxsize=64)
+def _adamw_tensors(n: int) -> struct.Struct:
+    """n of fbh_adamw_tensor."""
+    return struct.Struct("PPPQQfI" * n)
+
+
 class AdamW(_Kept):
     """AdamW over `params`, all in one step: for gradient g of a cell w at step t,
 
@@ -927,24 +935,26 @@ class AdamW(_Kept):
         grads = [p.grad for p in params] if grads is None else list(grads)
         if len(grads) != len(params):
             raise ValueError(f"{len(grads)} gradients for {len(params)} parameters")
-        parts = self._parts
+        # (a small step's time is what the host takes for these)
+        T = _torch.Tensor
         dev = params[0].get_device()
-        plain = _forward_ad._current_level < 0
-        k = 0
-        for p, g, w, n, cell in zip(params, grads, self.masters, self._sizes, self._types):
-            # (a small step's time is what this loop takes)
-            if not (plain and type(g) is _torch.Tensor and g.get_device() == dev and
-                    g.is_contiguous() and g.dtype is p.dtype and g.shape == p.shape):
-                g = grads[k // 7] = self._gradient(k // 7, p, g)
-            if not (p.dtype is cell and p.numel() == n and p.get_device() == dev and
-                    p.is_contiguous()):
-                raise ValueError(f"parameter {k // 7} has changed its type, size or place")
-            parts[k], parts[k + 1] = p.data_ptr(), g.data_ptr()
-            parts[k + 2] = 0 if w is None else w.data_ptr()
-            k += 7
+        devices = [dev] * len(params)
+        if not (_forward_ad._current_level < 0 and all(type(g) is T for g in grads) and
+                list(map(T.get_device, grads)) == devices and all(map(T.is_contiguous, grads)) and
+                list(map(_dtype_of, grads)) == self._types and
+                list(map(_shape_of, grads)) == list(map(_shape_of, params))):
+            grads = [self._gradient(i, p, g) for i, (p, g) in enumerate(zip(params, grads))]
+        if not (list(map(_dtype_of, params)) == self._types and
+                list(map(T.numel, params)) == self._sizes and
+                list(map(T.get_device, params)) == devices and all(map(T.is_contiguous, params))):
+            raise ValueError("a parameter has changed its type, size or place")
+        parts = self._parts
+        parts[0::7] = map(T.data_ptr, params)
+        parts[1::7] = map(T.data_ptr, grads)
+        parts[2::7] = [0 if w is None else w.data_ptr() for w in self.masters]
         stream = _raw_stream(dev)
         self._used_on(stream)
-        rc = _L.fbh_adamw_step(dev, self._packed(), struct.pack("PPPQQfI" * len(params), *parts),
+        rc = _L.fbh_adamw_step(dev, self._packed(), _adamw_tensors(len(params)).pack(*parts),
                                len(params), stream)
         if rc:
             N.check_hip(rc)
