@@ -292,31 +292,32 @@ def _functions():
 
     class ToExperts(torch.autograd.Function):
         @staticmethod
-        def forward(ctx, x, routes, place):
-            ctx.routes = routes
+        def forward(ctx, x, routes, place, *size):
+            ctx.routes, ctx.size = routes, size
             ctx.save_for_backward(place)
-            return _to_experts(x, routes, place)
+            return _to_experts(x, routes, place, *size)
 
         @staticmethod
         @torch.autograd.function.once_differentiable
         def backward(ctx, grad):
             (place,) = ctx.saved_tensors
-            return _from_experts(_device_tensor(grad, "grad"), ctx.routes, place, None), None, None
+            dx = _from_experts(_device_tensor(grad, "grad"), ctx.routes, place, None, *ctx.size)
+            return dx, None, None, None, None
 
     class FromExperts(torch.autograd.Function):
         @staticmethod
-        def forward(ctx, y, weights, routes, place):
-            ctx.routes = routes
+        def forward(ctx, y, weights, routes, place, *size):
+            ctx.routes, ctx.size = routes, size
             ctx.save_for_backward(y if weights is not None and weights.requires_grad else None,
                                   weights, place)
-            return _from_experts(y, routes, place, weights)
+            return _from_experts(y, routes, place, weights, *size)
 
         @staticmethod
         @torch.autograd.function.once_differentiable
         def backward(ctx, grad):
             y, weights, place = ctx.saved_tensors
             return _from_experts_grad(_device_tensor(grad, "grad"), y, ctx.routes, place, weights,
-                                      *ctx.needs_input_grad[:2]) + (None, None)
+                                      *ctx.needs_input_grad[:2], *ctx.size) + (None,) * 4
 
     return Embed, Dropout, LayerNorm, ToExperts, FromExperts
 
@@ -531,18 +532,18 @@ def _eps(eps) -> float:
 
 
 def _norm_of(x, weight, eps: float) -> bytes:
-    """The call's fbh_norm."""
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= 32768:
-        raise ValueError(f"x must be (..., 1 to 32768 cells), got shape {tuple(x.shape)}")
-    return _NORM.pack(x.numel() // x.shape[-1], x.shape[-1], _cells(x, "x"),
-                      0 if weight is None else _cells(weight, "weight"), eps)
-
-
-def _vector(v, x, what: str):
-    v = _beside(_device_tensor(v, what), x, what)
-    if v.shape != x.shape[-1:]:
-        raise ValueError(f"{what} must have shape ({x.shape[-1]},), got {tuple(v.shape)}")
-    return v
+    """The call's fbh_norm, after checking x and weight."""
+    shape = x.shape
+    dim = shape[-1] if shape else 0
+    if not 1 <= dim <= 32768:
+        raise ValueError(f"x must be (..., 1 to 32768 cells), got shape {tuple(shape)}")
+    kind = 0
+    if weight is not None:
+        _beside(weight, x, "weight")
+        if weight.shape != (dim,):
+            raise ValueError(f"weight must have shape ({dim},), got {tuple(weight.shape)}")
+        kind = _cells(weight, "weight")
+    return _NORM.pack(x.numel() // dim, dim, _cells(x, "x"), kind, eps)
 
 
 def _layer_norm(a: bytes, x, weight, bias, stats: bool):
@@ -565,14 +566,15 @@ def layer_norm(x, weight=None, bias=None, *, eps: float = 1e-5, stats: bool = Fa
     torch = _need_torch()
     x = _device_tensor(x, "x")
     if weight is not None:
-        weight = _vector(weight, x, "weight") if x.dim() else weight
+        weight = _device_tensor(weight, "weight")
     a = _norm_of(x, weight, _eps(eps))
     if bias is not None:
         if weight is None:
             raise ValueError("a bias needs a weight")
-        bias = _vector(bias, x, "bias")
-        if bias.dtype != weight.dtype:
-            raise ValueError(f"bias is {bias.dtype}, weight {weight.dtype}")
+        bias = _beside(_device_tensor(bias, "bias"), x, "bias")
+        if bias.dtype != weight.dtype or bias.shape != weight.shape:
+            raise ValueError(f"bias is {bias.dtype} of {tuple(bias.shape)}, weight "
+                             f"{weight.dtype} of {tuple(weight.shape)}")
     if torch.is_grad_enabled() and (x.requires_grad or
                                     (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
@@ -609,7 +611,7 @@ def layer_norm_grad(grad, x, stats, weight=None):
     grad = _beside(_device_tensor(grad, "grad"), x, "grad")
     stats = _beside(_device_tensor(stats, "stats"), x, "stats")
     if weight is not None:
-        weight = _vector(weight, x, "weight") if x.dim() else weight
+        weight = _device_tensor(weight, "weight")
     a = _norm_of(x, weight, 1.0)
     if grad.shape != x.shape or grad.dtype != x.dtype:
         raise ValueError(f"grad is {grad.dtype} of {tuple(grad.shape)}, x {x.dtype} of "
@@ -679,25 +681,26 @@ def _routes(routes, like):
     return _beside(routes.place, like, "the routes")
 
 
-def _vectors(x, what: str, lead):
-    """x as rows of 1 to 32768 cells with that leading shape."""
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= 32768 or tuple(x.shape[:-1]) != lead:
-        raise ValueError(f"{what} must have shape {lead} and a last axis of 1 to 32768 cells, got "
-                         f"{tuple(x.shape)}")
-    _cells(x, what)
-    return x
+def _rows_of(x, what: str, lead):
+    """The cells of a row of x, whose leading shape is `lead`: 1 to 32768."""
+    shape = x.shape
+    dim = shape[-1] if shape else 0
+    if not 1 <= dim <= 32768 or shape[:-1] != lead:
+        raise ValueError(f"{what} must have shape {tuple(lead)} and a last axis of 1 to 32768 "
+                         f"cells, got {tuple(shape)}")
+    return dim
 
 
-def _to_experts(x, routes, place):
+def _to_experts(x, routes, place, dim: int, cells: int):
     n = place.numel()
-    out = x.new_empty((n, x.shape[-1]))
+    out = x.new_empty((n, dim))
     if n:
         dev = x.get_device()
         stream = _raw_stream(dev)
         routes._used_on(stream)
-        rc = _L.fbh_to_experts(dev, x.data_ptr(), place.data_ptr(), n // place.shape[-1],
-                               place.shape[-1], x.shape[-1], _cells(x, "x"), out.data_ptr(),
-                               stream)
+        columns = place.shape[-1]
+        rc = _L.fbh_to_experts(dev, x.data_ptr(), place.data_ptr(), n // columns, columns, dim,
+                               cells, out.data_ptr(), stream)
         if rc:
             N.check_hip(rc)
     return out
@@ -710,23 +713,24 @@ def to_experts(x, routes: Routes):
     torch = _need_torch()
     x = _device_tensor(x, "x")
     place = _routes(routes, x)
-    _vectors(x, "x", tuple(place.shape[:-1]))
+    dim, cells = _rows_of(x, "x", place.shape[:-1]), _cells(x, "x")
     if x.requires_grad and torch.is_grad_enabled():
-        return _functions()[3].apply(x, routes, place)
-    return _to_experts(x, routes, place)
+        return _functions()[3].apply(x, routes, place, dim, cells)
+    return _to_experts(x, routes, place, dim, cells)
 
 
-def _from_experts(y, routes, place, weights):
-    out = y.new_empty(place.shape[:-1] + y.shape[-1:])
-    if not place.numel():
+def _from_experts(y, routes, place, weights, dim: int, cells: int):
+    shape = place.shape
+    out = y.new_empty(shape[:-1] + (dim,))
+    n = place.numel()
+    if not n:
         return out.zero_()
     dev = y.get_device()
     stream = _raw_stream(dev)
     routes._used_on(stream)
     rc = _L.fbh_from_experts(dev, y.data_ptr(), place.data_ptr(),
-                             0 if weights is None else weights.data_ptr(),
-                             place.numel() // place.shape[-1], place.shape[-1], y.shape[-1],
-                             _cells(y, "y"), out.data_ptr(), stream)
+                             0 if weights is None else weights.data_ptr(), n // shape[-1],
+                             shape[-1], dim, cells, out.data_ptr(), stream)
     if rc:
         N.check_hip(rc)
     return out
@@ -734,7 +738,7 @@ def _from_experts(y, routes, place, weights):
 
 def _weights(weights, place):
     weights = _beside(_device_tensor(weights, "weights"), place, "weights")
-    if weights.dtype != _torch.float32 or weights.shape != place.shape:
+    if weights.dtype is not _torch.float32 or weights.shape != place.shape:
         raise ValueError(f"weights must be float32 of {tuple(place.shape)}, got {weights.dtype} of "
                          f"{tuple(weights.shape)}")
     return weights
@@ -744,31 +748,33 @@ def from_experts(y, routes: Routes, weights=None):
     """What experts have given for the rows of to_experts(), `y` (positions, cells), back at
     its rows: for each, the sum over its columns of weights[..., column] * the position's row
     of y, in float32 and rounded once. weights (the shape of ids, float32) may be None: 1. A
-    position without an expert gives nothing, whatever its row of y holds."""
+    position without an expert gives nothing, whatever its row of y and its weight hold."""
     torch = _need_torch()
     y = _device_tensor(y, "y")
     place = _routes(routes, y)
-    _vectors(y, "y", (place.numel(),))
+    dim, cells = _rows_of(y, "y", (place.numel(),)), _cells(y, "y")
     if weights is not None:
         weights = _weights(weights, place)
-    if torch.is_grad_enabled() and (y.requires_grad or
-                                    (weights is not None and weights.requires_grad)):
-        return _functions()[4].apply(y, weights, routes, place)
-    return _from_experts(y, routes, place, weights)
+    if (y.requires_grad or (weights is not None and weights.requires_grad)) and (
+            torch.is_grad_enabled()):
+        return _functions()[4].apply(y, weights, routes, place, dim, cells)
+    return _from_experts(y, routes, place, weights, dim, cells)
 
 
-def _from_experts_grad(grad, y, routes, place, weights, want_y: bool, want_weights: bool):
+def _from_experts_grad(grad, y, routes, place, weights, want_y: bool, want_weights: bool,
+                       dim: int, cells: int):
     n = place.numel()
-    dy = grad.new_empty((n, grad.shape[-1])) if want_y else None
+    dy = grad.new_empty((n, dim)) if want_y else None
     dw = _torch.empty_like(weights) if want_weights else None
     if n and (want_y or want_weights):
-        at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
         dev = grad.get_device()
         stream = _raw_stream(dev)
         routes._used_on(stream)
-        rc = _L.fbh_from_experts_grad(dev, grad.data_ptr(), at(y), place.data_ptr(), at(weights),
-                                      n // place.shape[-1], place.shape[-1], grad.shape[-1],
-                                      _cells(grad, "grad"), at(dy), at(dw), stream)
+        columns = place.shape[-1]
+        rc = _L.fbh_from_experts_grad(
+            dev, grad.data_ptr(), 0 if y is None else y.data_ptr(), place.data_ptr(),
+            0 if weights is None else weights.data_ptr(), n // columns, columns, dim, cells,
+            dy.data_ptr() if want_y else 0, dw.data_ptr() if want_weights else 0, stream)
         if rc:
             N.check_hip(rc)
     return dy, dw
@@ -782,14 +788,15 @@ def from_experts_grad(grad, y, routes: Routes, weights=None):
     _need_torch()
     grad = _device_tensor(grad, "grad")
     place = _routes(routes, grad)
-    _vectors(grad, "grad", tuple(place.shape[:-1]))
+    dim, cells = _rows_of(grad, "grad", place.shape[:-1]), _cells(grad, "grad")
     y = _beside(_device_tensor(y, "y"), grad, "y")
-    if tuple(y.shape) != (place.numel(), grad.shape[-1]) or y.dtype != grad.dtype:
-        raise ValueError(f"y must be {grad.dtype} of {(place.numel(), grad.shape[-1])}, got "
-                         f"{y.dtype} of {tuple(y.shape)}")
+    if y.shape != (place.numel(), dim) or y.dtype is not grad.dtype:
+        raise ValueError(f"y must be {grad.dtype} of {(place.numel(), dim)}, got {y.dtype} of "
+                         f"{tuple(y.shape)}")
     if weights is not None:
         weights = _weights(weights, place)
-    return _from_experts_grad(grad, y, routes, place, weights, True, weights is not None)
+    return _from_experts_grad(grad, y, routes, place, weights, True, weights is not None, dim,
+                              cells)
 
 
 # ------------------------------------------------------------------- AdamW
