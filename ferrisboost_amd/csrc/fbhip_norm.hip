@@ -288,7 +288,16 @@ struct NormGrad {
     const void *weight;
     const float *stats;
     float *parts;  // [groups][2][dim], or for wide rows [n_rows]: what the mean leaves out
+    void *dweight, *dbias;  // of the only workgroup, which needs no parts
 };
+
+// Cell `at` of a weight's or bias' gradient, where one is wanted.
+__device__ __forceinline__ void store_weight(void *out, uint32_t type, uint32_t at, float v) {
+    if (!out) return;
+    if (type == FBH_F32) static_cast<float *>(out)[at] = v;
+    else if (type == FBH_F16) static_cast<_Float16 *>(out)[at] = (_Float16)v;
+    else static_cast<__bf16 *>(out)[at] = (__bf16)v;
+}
 
 template <class T, uint32_t N, uint32_t G, uint32_t C, bool SUMS>
 __global__ __launch_bounds__(norm_threads<G>()) void norm_grad_kernel(NormGrad A, const T *g,
@@ -358,14 +367,17 @@ __global__ __launch_bounds__(norm_threads<G>()) void norm_grad_kernel(NormGrad A
             });
     }
     if constexpr (SUMS) {
-        if (!A.parts) return;
-        float *out = A.parts + (uint64_t)blockIdx.x * 2 * A.dim;
+        if (!A.parts && !A.dweight && !A.dbias) return;
+        const auto put = [&](uint32_t which, uint32_t col, float v) {
+            if (A.parts) A.parts[((uint64_t)blockIdx.x * 2 + which) * A.dim + col] = v;
+            else store_weight(which ? A.dbias : A.dweight, A.weight_type, col, v);
+        };
         if constexpr (ROWS == 1) {
 #pragma unroll
             for (uint32_t i = 0; i < C; i++)
                 if (!at.empty(i / N)) {
-                    out[at.column(i / N) + i % N] = dw.v[i];
-                    out[A.dim + at.column(i / N) + i % N] = db.v[i];
+                    put(0, at.column(i / N) + i % N, dw.v[i]);
+                    put(1, at.column(i / N) + i % N, db.v[i]);
                 }
         } else {
             // the workgroup's rows, added in their order, a quarter of the cells at a time
@@ -386,7 +398,7 @@ __global__ __launch_bounds__(norm_threads<G>()) void norm_grad_kernel(NormGrad A
                     for (uint32_t k = 0; k < ROWS; k++) t += sums[which][k][slot];
                     const uint32_t i = q * Q + slot / G;
                     const uint32_t begin = ((i / N) * G + slot % G) * N;
-                    if (begin < A.dim) out[which * A.dim + min(begin, A.dim - N) + i % N] = t;
+                    if (begin < A.dim) put(which, min(begin, A.dim - N) + i % N, t);
                 }
             }
         }
@@ -464,12 +476,8 @@ __global__ __launch_bounds__(256) void norm_join_kernel(const float *parts, uint
     __syncthreads();
     if (k != 0 || j >= 2 * dim) return;
     for (uint32_t i = 1; i < THREADS; i++) t += sums[i][lane];
-    void *out = j < dim ? dweight : dbias;
-    const uint32_t at = j < dim ? j : j - dim;
-    if (!out) return;
-    if (weight_type == FBH_F32) static_cast<float *>(out)[at] = (float)t;
-    else if (weight_type == FBH_F16) static_cast<_Float16 *>(out)[at] = (_Float16)(float)t;
-    else static_cast<__bf16 *>(out)[at] = (__bf16)(float)t;
+    if (j < dim) store_weight(dweight, weight_type, j, (float)t);
+    else store_weight(dbias, weight_type, j - dim, (float)t);
 }
 
 // ------------------------------------------------------------------- host side
@@ -482,11 +490,20 @@ uint32_t rows_of_group(uint32_t dim) {
     return rows;
 }
 
+// Whether one workgroup takes all rows, twice as many as it holds at once, and writes the
+// weights' gradients itself, without a second launch (in us on the device, and with: 64 x 60
+// 5.0 and 5.9, 128 x 60 6.5 and 5.8; 8 x 1000 6.8 and 6.7, 16 x 1000 9.6 and 6.7; 2 x 4000 7.9
+// and 8.6, 4 x 4000 10.8 and 8.5; a launch less is 5 us less of the host's).
+bool grad_alone(uint64_t n_rows, uint32_t dim) {
+    return dim <= 4096 && n_rows <= 2 * rows_of_group(dim);
+}
+
 // Parts of the weights' sums, a workgroup's each: as many workgroups as the device holds at a
 // time, fewer where their parts would be large beside the rows (in us, bfloat16 gradients of
 // 4096 cells: 512 rows with 512 parts 24.2, with 128 14.4; 2048 rows with 512 parts 25.9, with
 // 256 21.8), and 128 while there are rows for them (128 rows: 10.2, with 32 parts 12.7).
 uint32_t grad_groups(uint64_t n_rows, uint32_t dim) {
+    if (grad_alone(n_rows, dim)) return 1;
     const uint64_t most = dim <= 256 ? 1024 : dim <= 4096 ? 512 : dim <= SPLIT_DIM ? 256 : 64;
     const uint32_t rows = rows_of_group(dim);
     const uint64_t n = std::max<uint64_t>((n_rows + rows - 1) / rows, 1);
@@ -496,6 +513,7 @@ uint32_t grad_groups(uint64_t n_rows, uint32_t dim) {
 uint64_t padded_rows(uint64_t n) { return (n + 3) / 4 * 4; }
 
 uint64_t grad_bytes(const fbh_norm *a) {
+    if (grad_alone(a->n_rows, a->dim)) return 0;
     uint64_t b = (uint64_t)grad_groups(a->n_rows, a->dim) * 2 * a->dim * 4;
     if (a->dim > SPLIT_DIM) b += padded_rows(a->n_rows) * 4;
     return b;
@@ -541,7 +559,10 @@ void launch_norm_grad(const fbh_norm *a, const T *g, const T *x, const float *st
                       hipStream_t s) {
     const bool sums = dweight || dbias, split = a->dim > SPLIT_DIM;
     const uint32_t groups = grad_groups(a->n_rows, a->dim);
-    NormGrad A{a->n_rows, a->dim, a->weight_type, groups, weight, stats, sums ? work : nullptr};
+    const bool alone = grad_alone(a->n_rows, a->dim);
+    NormGrad A{a->n_rows, a->dim, a->weight_type, groups, weight, stats,
+               sums && !alone ? work : nullptr, alone ? dweight : nullptr,
+               alone ? dbias : nullptr};
     with_shape<T>(a->dim, [&](auto nn, auto gg, auto cc) {
         constexpr uint32_t N = decltype(nn)::value, G = decltype(gg)::value;
         constexpr uint32_t C = decltype(cc)::value;
@@ -550,7 +571,7 @@ void launch_norm_grad(const fbh_norm *a, const T *g, const T *x, const float *st
         const uint64_t blocks = SUMS ? groups : std::clamp<uint64_t>(a->n_rows, 1, most);
         launch(norm_grad_kernel<T, N, G, C, SUMS>, blocks, norm_threads<G>(), s, A, g, x, dx);
     });
-    if (!sums) return;
+    if (!sums || alone) return;
     float *parts = work;
     if (split) {
         parts = work + padded_rows(a->n_rows);
@@ -601,8 +622,9 @@ int fbh_layer_norm_grad(int device, const fbh_norm *a, const void *grad, const v
         check_norm(a);
         head_input((grad && x && stats) || a->n_rows == 0, "null argument");
         if (dweight || dbias) {
-            head_input(work && work_bytes >= grad_bytes(a), "the workspace is too small");
-            head_input(reinterpret_cast<uintptr_t>(work) % 16 == 0,
+            const uint64_t need = grad_bytes(a);
+            head_input(need == 0 || (work && work_bytes >= need), "the workspace is too small");
+            head_input(need == 0 || reinterpret_cast<uintptr_t>(work) % 16 == 0,
                        "the workspace must be 16-byte aligned");
         }
         head_input(!dx || (dx != grad && dx != x), "dx must not be grad or x");

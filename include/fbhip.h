@@ -848,7 +848,8 @@ typedef struct {
 int fbh_layer_norm(int device, const fbh_norm *a, const void *x, const void *weight,
                    const void *bias, void *out, float *stats, void *stream);
 /* Device bytes of workspace that fbh_layer_norm_grad takes for dweight or dbias,
- * 16-byte aligned; 0 for a call that it refuses. */
+ * 16-byte aligned; 0 for a few rows (up to 2 to 128 by their width) and for a call that it
+ * refuses. */
 uint64_t fbh_layer_norm_grad_bytes(const fbh_norm *a);
 /* The gradients for the output's gradient grad: dx [n_rows][dim] (not grad or x: wide
  * rows are read again), dweight and dbias [dim], summed over all rows (each may be NULL:

@@ -36,7 +36,7 @@ def test_layer_norm_refusals_of_the_c_abi(bad, msg):
 
 
 def test_layer_norm_null_arguments_and_workspace():
-    L, a = N.hip(), _norm()
+    L, a = N.hip(), _norm(n_rows=1000)
     for args in ((None, None, None, 64, None), (64, None, None, None, None)):
         with pytest.raises(ValueError, match="null"):
             N.check_hip(L.fbh_layer_norm(0, a, *args, None))
@@ -59,10 +59,12 @@ def test_layer_norm_null_arguments_and_workspace():
 @pytest.mark.parametrize("dim", [1, 3, 8, 33, 256, 257, 4096, 4097, 16_384, 16_385, 32_768])
 def test_layer_norm_workspace_is_bounded(n, dim):
     """At most 1024 parts of two float32 vectors, fewer of wider ones (32 MiB but for the
-    widest rows, which take 4 bytes a row besides), and no more parts than rows."""
+    widest rows, which take 4 bytes a row besides), and no more parts than rows; none for a
+    few rows."""
     got = N.hip().fbh_layer_norm_grad_bytes(_norm(n_rows=n, dim=dim))
     rows = 4 * n + 16 if dim > 16_384 else 0
-    assert 8 * dim <= got <= min(32 << 20, 8 * dim * max(n, 1)) + rows
+    assert got <= min(32 << 20, 8 * dim * max(n, 1)) + rows
+    assert got >= 8 * dim or (got == 0 and n <= 128 and dim <= 4096)
 
 
 def test_experts_refusals_of_the_c_abi():
