@@ -28,7 +28,7 @@ constexpr uint32_t ADAM_TPB = 256;
 constexpr uint32_t ADAM_CHUNK = 256;                // cells of a wave at a time: a block
 constexpr uint32_t ADAM_CHUNKS = 4;                 // of a wave in a tile
 constexpr uint32_t ADAM_TILE = ADAM_TPB / 64 * ADAM_CHUNKS * ADAM_CHUNK;
-constexpr uint32_t ADAM_TENSORS = 64;               // of a launch
+constexpr uint32_t ADAM_TENSORS = 64, ADAM_FEW = 16;  // of a launch
 constexpr uint64_t ADAM_BLOCKS = 1u << 16;          // of a launch at most
 // Workgroups up to which they move the clock themselves: 25 of them take 4.6 us so and 5.3 with a
 // launch of its own for it, 122 6.2 and 6.1, 244, which queue up at one counter, 8.4 and 7.0.
@@ -67,11 +67,13 @@ struct Adam {
     uint32_t ticks;  // whether this launch moves the clock on
 };
 
+// (room for few tensors or many: 3.7 KB of arguments take 0.9 us more of the host than 64 bytes)
+template <uint32_t MOST>
 struct AdamLaunch {
     Adam a;
-    AdamTensor t[ADAM_TENSORS];
+    AdamTensor t[MOST];
 };
-static_assert(sizeof(AdamLaunch) <= 4096, "kernel arguments");
+static_assert(sizeof(AdamLaunch<ADAM_TENSORS>) <= 4096, "kernel arguments");
 static_assert(ADAM_TENSORS == 64, "a lane each");
 
 // A step's numbers.
@@ -336,8 +338,8 @@ __device__ __forceinline__ void adam_chunk(const Adam &A, const AdamStep &S, con
     }
 }
 
-template <class T, bool SMALL>
-__global__ __launch_bounds__(ADAM_TPB) void adam_kernel(AdamLaunch L) {
+template <class T, bool SMALL, uint32_t MOST>
+__global__ __launch_bounds__(ADAM_TPB) void adam_kernel(AdamLaunch<MOST> L) {
     const Adam &A = L.a;
     const AdamStep S = adam_step(A);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -393,16 +395,26 @@ __global__ __launch_bounds__(ADAM_TPB) void adam_moments_kernel(const uint8_t *m
     }
 }
 
-void launch_adamw(uint32_t dtype, uint32_t bits, const AdamLaunch &L, hipStream_t s) {
-    const auto kernel = dtype == FBH_F32   ? (bits == 8 ? adam_kernel<float, true>
-                                                        : adam_kernel<float, false>)
-                        : dtype == FBH_F16 ? (bits == 8 ? adam_kernel<_Float16, true>
-                                                        : adam_kernel<_Float16, false>)
-                                           : (bits == 8 ? adam_kernel<__bf16, true>
-                                                        : adam_kernel<__bf16, false>);
+template <uint32_t MOST>
+void launch_most(uint32_t dtype, uint32_t bits, const AdamLaunch<MOST> &L, hipStream_t s) {
+    const auto kernel =
+        dtype == FBH_F32   ? (bits == 8 ? adam_kernel<float, true, MOST>
+                                        : adam_kernel<float, false, MOST>)
+        : dtype == FBH_F16 ? (bits == 8 ? adam_kernel<_Float16, true, MOST>
+                                        : adam_kernel<_Float16, false, MOST>)
+                           : (bits == 8 ? adam_kernel<__bf16, true, MOST>
+                                        : adam_kernel<__bf16, false, MOST>);
     const uint64_t blocks = L.a.tiles < ADAM_BLOCKS ? L.a.tiles : ADAM_BLOCKS;
     hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(ADAM_TPB), 0, s, L);
     head_check(hipGetLastError(), "adamw");
+}
+void launch_adamw(uint32_t dtype, uint32_t bits, const AdamLaunch<ADAM_TENSORS> &L,
+                  hipStream_t s) {
+    if (L.a.n_tensors > ADAM_FEW) return launch_most(dtype, bits, L, s);
+    AdamLaunch<ADAM_FEW> few{};
+    few.a = L.a;
+    for (uint32_t i = 0; i < L.a.n_tensors; i++) few.t[i] = L.t[i];
+    launch_most(dtype, bits, few, s);
 }
 
 bool aligned(const void *p, uintptr_t by) { return reinterpret_cast<uintptr_t>(p) % by == 0; }
@@ -448,7 +460,7 @@ int fbh_adamw_step(int device, const fbh_adamw *a, const fbh_adamw_tensor *tenso
         }
         const OnDevice on(device);
         const auto s = static_cast<hipStream_t>(stream);
-        AdamLaunch L{};
+        AdamLaunch<ADAM_TENSORS> L{};
         L.a = Adam{a->beta1, a->beta2, a->lr, a->lr_at, a->seed, a->mean, a->square,
                    static_cast<uint8_t *>(a->scales), static_cast<Clock *>(a->clock),
                    a->n / ADAM_CHUNK, 0, a->eps, 0, 0};

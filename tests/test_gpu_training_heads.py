@@ -124,6 +124,42 @@ def test_layer_norm_rows_do_not_depend_on_their_neighbours(heads):
         assert torch.equal(heads.layer_norm(x[:n]), y[:n])
 
 
+def test_gradients_of_broadcast_and_strided_inputs(heads):
+    """Copies of one cell, of one row, and transposed ones: their gradients are summed, or laid
+    out, as those of what they are views of."""
+    rng = np.random.default_rng(9)
+    x, g = _cells(rng, (40, 60), "f32"), _cells(rng, (40, 60), "f32")
+    w, b = _cells(rng, 60, "f32"), _cells(rng, 60, "f32")
+
+    def grads(make, *leaves):
+        leaves = [a.detach().clone().requires_grad_() for a in leaves]
+        return torch.autograd.grad(heads.layer_norm(*make(*leaves)), leaves, g)
+
+    base = grads(lambda *a: a, x, w, b)
+    got = grads(lambda x, w, b: (x.t(), w, b), x.t().contiguous(), w, b)
+    assert torch.equal(got[0].t(), base[0]) and torch.equal(got[1], base[1])
+    one = grads(lambda *a: a, x[:1].expand(40, 60).contiguous(), w, b)
+    got = grads(lambda x, w, b: (x.expand(40, 60), w, b), x[:1], w, b)
+    assert torch.equal(got[0], one[0].sum(0, keepdim=True)) and torch.equal(got[1], one[1])
+    one = grads(lambda *a: a, x, w[:1].expand(60).contiguous(), b)
+    got = grads(lambda x, w, b: (x, w.expand(60), b), x, w[:1], b)
+    assert torch.equal(got[1], one[1].sum(0, keepdim=True))
+    # experts: one weight for all, rows of a transposed output, an expanded gradient
+    ids = torch.from_numpy(rng.integers(-1, 5, (40, 2))).cuda()
+    r = heads.Routes(ids, 5)
+    y = _cells(rng, (80, 60), "f32").requires_grad_()
+    v = torch.tensor(0.5, device="cuda", requires_grad=True)
+    out = heads.from_experts(y, r, v.expand(40, 2))
+    out.backward(g[:, :1].expand(40, 60))
+    dy, dw = heads.from_experts_grad(g[:, :1].expand(40, 60).contiguous(), y.detach(), r,
+                                     torch.full((40, 2), 0.5, device="cuda"))
+    assert torch.equal(y.grad, dy) and torch.equal(v.grad, dw.sum())
+    t = y.detach().t().contiguous().requires_grad_()
+    heads.from_experts(t.t(), r, torch.full((40, 2), 0.5, device="cuda")).backward(
+        g[:, :1].expand(40, 60))
+    assert torch.equal(t.grad.t(), dy)
+
+
 @pytest.mark.parametrize("dim", [3, 31, 100, 1000, 5000, 12_000, 30_000])
 def test_layer_norm_of_equal_cells_with_a_tiny_eps(heads, dim):
     """What rounding leaves of a variance of 0 may be below it, never a NaN: cells are off from
