@@ -19,7 +19,11 @@
 // tensors in its arguments, so nothing is copied to the device before it.
 #include "fbhip_heads.h"
 
+#include <algorithm>
 #include <cmath>
+#include <iterator>
+#include <utility>
+#include <vector>
 
 namespace fbh {
 namespace {
@@ -436,6 +440,31 @@ void check_adamw(const fbh_adamw *a) {
     head_input(a->n == 0 || a->bits == 32 || a->scales, "moments of 8 bits need scales");
 }
 
+// That no parameter shares memory with another one or with a gradient: steps of both would run
+// side by side.
+void check_overlaps(const fbh_adamw_tensor *tensors, uint64_t n_tensors) {
+    using Span = std::pair<uintptr_t, uintptr_t>;
+    const auto span = [](const fbh_adamw_tensor &t, const void *p) {
+        const auto at = reinterpret_cast<uintptr_t>(p);
+        return Span{at, at + t.n * (t.dtype == FBH_F32 ? 4 : 2)};
+    };
+    std::vector<Span> params;
+    params.reserve(n_tensors);
+    for (uint64_t i = 0; i < n_tensors; i++)
+        if (tensors[i].n) params.push_back(span(tensors[i], tensors[i].param));
+    std::sort(params.begin(), params.end());
+    for (size_t i = 1; i < params.size(); i++)
+        head_input(params[i - 1].second <= params[i].first, "parameters overlap in memory");
+    for (uint64_t i = 0; i < n_tensors; i++) {
+        if (!tensors[i].n) continue;
+        const Span g = span(tensors[i], tensors[i].grad);
+        // the first parameter that begins behind the gradient; the one before ends last
+        const auto behind = std::lower_bound(params.begin(), params.end(), Span{g.second, 0});
+        head_input(behind == params.begin() || std::prev(behind)->second <= g.first,
+                   "a gradient overlaps a parameter in memory");
+    }
+}
+
 }  // namespace
 }  // namespace fbh
 
@@ -458,6 +487,7 @@ int fbh_adamw_step(int device, const fbh_adamw *a, const fbh_adamw_tensor *tenso
             head_input(std::isfinite(t.weight_decay) && t.weight_decay >= 0.0f,
                        "weight_decay must be finite and not negative");
         }
+        check_overlaps(tensors, n_tensors);
         const OnDevice on(device);
         const auto s = static_cast<hipStream_t>(stream);
         AdamLaunch<ADAM_TENSORS> L{};

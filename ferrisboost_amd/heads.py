@@ -937,7 +937,8 @@ class AdamW(_Kept):
 
     def step(self, grads=None):
         """One step, in place, with the parameters' .grad or with `grads`, a list of one for
-        each parameter, of its shape and type. Every parameter needs one."""
+        each parameter, of its shape and type. Every parameter needs one, in memory that is no
+        parameter's."""
         params = self.params
         grads = [p.grad for p in params] if grads is None else list(grads)
         if len(grads) != len(params):
@@ -994,6 +995,7 @@ class AdamW(_Kept):
 
     def take_params(self):
         """Sets the float32 copies of 16-bit parameters to what these hold now."""
+        self._used_on(_raw_stream(self.mean.get_device()))
         with _torch.no_grad():
             for p, w in zip(self.params, self.masters):
                 if w is not None:
@@ -1038,6 +1040,7 @@ class AdamW(_Kept):
             if not isinstance(x, _torch.Tensor) or x.shape != to.shape or (
                     x.dtype != to.dtype and not what.startswith("master")):
                 raise ValueError(f"{what} must be {to.dtype} of {tuple(to.shape)}")
+        self._used_on(_raw_stream(self.mean.get_device()))
         with _torch.no_grad():
             for _, to, x in pairs:
                 to.copy_(x)

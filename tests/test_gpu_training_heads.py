@@ -701,3 +701,24 @@ def test_adamw_8_bit_moments_near_the_end_of_the_range(heads):
     m = opt.moments()[0]
     assert torch.isnan(m[:2]).all() and float(m[2]) == 2.0 ** 127
     assert (m[3:] == 0).all() and int(opt.scales[0, 0]) == 254
+
+
+def test_adamw_gradients_in_parameters_memory(heads):
+    """A gradient that is another parameter, or one moved onto another's memory later, is
+    refused before anything moves; neighbours in one buffer are not."""
+    flat = torch.randn(4, 256, device="cuda")
+    p, q, g, h = flat
+    opt = heads.AdamW([p, q], lr=0.1)
+    before = flat.clone()
+    for grads in ([q, p], [g, flat.view(-1)[255:511]], [p, h]):
+        with pytest.raises(ValueError, match="overlaps a parameter"):
+            opt.step(grads)
+    moved = [torch.nn.Parameter(torch.zeros(256, device="cuda")) for _ in range(2)]
+    other = heads.AdamW(moved)
+    moved[1].data = moved[0].data
+    with pytest.raises(ValueError, match="parameters overlap"):
+        other.step([g, h])
+    assert torch.equal(flat, before) and opt.state_dict()["step"] == 0
+    opt.step([h, g])
+    assert torch.equal(flat[2:], before[2:]) and (flat[:2] != before[:2]).all()
+    assert opt.state_dict()["step"] == 1

@@ -146,6 +146,22 @@ def test_adamw_tensor_refusals_of_the_c_abi():
         N.check_hip(L.fbh_adamw_moments(0, _adamw(), 64, None, None))
 
 
+@pytest.mark.parametrize("tensors, msg", [
+    # (256 cells of float32: 1024 bytes each)
+    ([(0x1000, 0x9000), (0x13FC, 0xA000)], "parameters overlap"),
+    ([(0x1400, 0x9000), (0x3000, 0xA000), (0x1001, 0xB000)], "parameters overlap"),
+    ([(0x1000, 0x9000), (0x1000, 0xA000)], "parameters overlap"),
+    ([(0x1000, 0x1000)], "gradient overlaps"),
+    ([(0x1000, 0x3000), (0x3000, 0x1000)], "gradient overlaps"),
+    ([(0x1000, 0x9000), (0x3000, 0x33FF)], "gradient overlaps"),
+    ([(0x1000, 0x9000), (0x3000, 0x0C01), (0x5000, 0xA000)], "gradient overlaps")])
+def test_adamw_refuses_overlapping_tensors(tensors, msg):
+    packed = b"".join(_tensor(param=p, grad=g, first=256 * i, dtype=0)
+                      for i, (p, g) in enumerate(tensors))
+    with pytest.raises(ValueError, match=msg):
+        N.check_hip(N.hip().fbh_adamw_step(0, _adamw(n=1024), packed, len(tensors), None))
+
+
 def test_structs_have_the_header_s_sizes():
     """8-byte fields first and 4-byte ones in pairs: no padding but the norm's last word."""
     assert heads._ADAMW.size == 88 and len(_tensor()) == 48
