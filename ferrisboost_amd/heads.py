@@ -888,7 +888,9 @@ class AdamW(_Kept):
             raise ValueError(f"weight_decay must be a number, not negative, or a list of {n}")
         self._decays = decays
         if self._parts is not None:
-            self._parts[5::7] = decays
+            parts = list(self._parts)  # (a copy of the optimizer shares the list)
+            parts[5::7] = decays
+            self._parts = parts
 
     def _check(self, i: int, p):
         if not isinstance(p, _torch.Tensor):

@@ -1,0 +1,48 @@
+"""Calls of the training heads that need no device: what they refuse, and what they leave to
+others that share their tensors."""
+
+from __future__ import annotations
+
+import copy
+import pickle
+
+import pytest
+import torch
+
+from ferrisboost_amd import heads
+
+
+def _optimizer(sizes=(3, 300), bits=32, **kw):
+    """An optimizer of float32 parameters on the host, which can do everything but step."""
+    heads._need_torch()
+    opt = object.__new__(heads.AdamW)
+    opt.params = [torch.zeros(n) for n in sizes]
+    opt.lr, opt.betas, opt.eps, opt.bits, opt.seed = 0.1, (0.9, 0.999), 1e-8, bits, 0
+    opt._parts, opt.weight_decay = None, kw.pop("weight_decay", 0.1)
+    blocks = [-(-n // 256) for n in sizes]
+    opt.first = [256 * sum(blocks[:i]) for i in range(len(sizes))]
+    opt._sizes, opt._types = list(sizes), [torch.float32] * len(sizes)
+    opt._parts = [x for i, n in enumerate(sizes)
+                  for x in (0, 0, 0, n, opt.first[i], opt.weight_decay[i], 0)]
+    opt.mean, opt.square = (torch.zeros(256 * sum(blocks),
+                                        dtype=torch.uint8 if bits == 8 else torch.float32)
+                            for _ in range(2))
+    opt.scales = torch.zeros((2, sum(blocks)), dtype=torch.uint8) if bits == 8 else None
+    opt.masters = [None] * len(sizes)
+    opt._clock = torch.tensor([0, 0x3FF0000000000000, 0x3FF0000000000000, 0])
+    opt._streams = set()
+    for k, v in kw.items():
+        setattr(opt, k, v)
+    return opt
+
+
+@pytest.mark.parametrize("how", [copy.copy, copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o))])
+def test_weight_decay_of_a_copy_is_its_own(how):
+    """What a step packs for the first one stays, whichever of the two is set."""
+    opt = _optimizer()
+    c = how(opt)
+    c.weight_decay = 0.75
+    assert opt.weight_decay == (0.1, 0.1) and opt._parts[5::7] == [0.1, 0.1]
+    assert c.weight_decay == (0.75, 0.75) and c._parts[5::7] == [0.75, 0.75]
+    opt.weight_decay = [0.5, 0.25]
+    assert opt._parts[5::7] == [0.5, 0.25] and c._parts[5::7] == [0.75, 0.75]
