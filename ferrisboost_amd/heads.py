@@ -947,7 +947,7 @@ class AdamW(_Kept):
             raise ValueError(f"{len(grads)} gradients for {len(params)} parameters")
         # (a small step's time is what the host takes for these)
         T = _torch.Tensor
-        dev = params[0].get_device()
+        dev = self.mean.get_device()
         devices = [dev] * len(params)
         if not (_forward_ad._current_level < 0 and all(type(g) is T for g in grads) and
                 list(map(T.get_device, grads)) == devices and all(map(T.is_contiguous, grads)) and

@@ -46,3 +46,17 @@ def test_weight_decay_of_a_copy_is_its_own(how):
     assert c.weight_decay == (0.75, 0.75) and c._parts[5::7] == [0.75, 0.75]
     opt.weight_decay = [0.5, 0.25]
     assert opt._parts[5::7] == [0.5, 0.25] and c._parts[5::7] == [0.75, 0.75]
+
+
+def test_parameters_that_left_the_optimizer_s_device():
+    """Parameters and gradients moved together: the state has not."""
+    opt = _optimizer()
+
+    class On0:
+        @staticmethod
+        def get_device():
+            return 0
+
+    opt.mean = On0()
+    with pytest.raises(ValueError, match="on a GPU"):
+        opt.step([torch.ones_like(p) for p in opt.params])
