@@ -88,11 +88,15 @@ def _need_torch():
     return torch
 
 
+def _no_tangent(x, what: str):
+    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(x).tangent is not None:
+        raise ValueError(f"{what} has a tangent: forward-mode derivatives are not available")
+
+
 def _device_tensor(x, what: str):
     if not isinstance(x, _torch.Tensor):
         raise ValueError(f"{what} must be a torch tensor, got {type(x).__name__}")
-    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(x).tangent is not None:
-        raise ValueError(f"{what} has a tangent: forward-mode derivatives are not available")
+    _no_tangent(x, what)
     if not x.is_cuda:
         raise ValueError(f"{what} must be on a GPU, it is on {x.device}")
     return x if x.is_contiguous() else x.contiguous()
@@ -895,6 +899,7 @@ class AdamW(_Kept):
     def _check(self, i: int, p):
         if not isinstance(p, _torch.Tensor):
             raise ValueError(f"parameter {i} must be a torch tensor, got {type(p).__name__}")
+        _no_tangent(p, f"parameter {i}")
         if not p.is_cuda:
             raise ValueError(f"parameter {i} must be on a GPU, it is on {p.device}")
         _cells(p, f"parameter {i}")
@@ -953,6 +958,8 @@ class AdamW(_Kept):
                 list(map(T.get_device, grads)) == devices and all(map(T.is_contiguous, grads)) and
                 list(map(_dtype_of, grads)) == self._types and
                 list(map(_shape_of, grads)) == list(map(_shape_of, params))):
+            for i, p in enumerate(params):
+                _no_tangent(p, f"parameter {i}")
             grads = [self._gradient(i, p, g) for i, (p, g) in enumerate(zip(params, grads))]
         if not (list(map(_dtype_of, params)) == self._types and
                 list(map(T.numel, params)) == self._sizes and
@@ -997,6 +1004,8 @@ class AdamW(_Kept):
 
     def take_params(self):
         """Sets the float32 copies of 16-bit parameters to what these hold now."""
+        for i, p in enumerate(self.params):
+            _no_tangent(p, f"parameter {i}")
         self._used_on(_raw_stream(self.mean.get_device()))
         with _torch.no_grad():
             for p, w in zip(self.params, self.masters):
@@ -1042,6 +1051,7 @@ class AdamW(_Kept):
             if not isinstance(x, _torch.Tensor) or x.shape != to.shape or (
                     x.dtype != to.dtype and not what.startswith("master")):
                 raise ValueError(f"{what} must be {to.dtype} of {tuple(to.shape)}")
+            _no_tangent(x, what)
         self._used_on(_raw_stream(self.mean.get_device()))
         with _torch.no_grad():
             for _, to, x in pairs:

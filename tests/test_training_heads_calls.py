@@ -60,3 +60,20 @@ def test_parameters_that_left_the_optimizer_s_device():
     opt.mean = On0()
     with pytest.raises(ValueError, match="on a GPU"):
         opt.step([torch.ones_like(p) for p in opt.params])
+
+
+def test_a_parameter_with_a_tangent_is_refused():
+    """A step would move its value and leave its tangent as it was."""
+    import torch.autograd.forward_ad as fwd
+
+    opt = _optimizer()
+    with fwd.dual_level():
+        d = fwd.make_dual(opt.params[1], torch.ones_like(opt.params[1]))
+        opt.params[1] = d
+        with pytest.raises(ValueError, match="parameter 1 has a tangent"):
+            opt.step([torch.ones_like(p) for p in opt.params])
+        with pytest.raises(ValueError, match="parameter 0 has a tangent"):
+            heads.AdamW([d])
+        mean = fwd.make_dual(opt.mean, torch.ones_like(opt.mean))
+        with pytest.raises(ValueError, match="mean has a tangent"):
+            opt.load_state_dict({"step": 0, "mean": mean, "square": opt.square})
