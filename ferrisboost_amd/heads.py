@@ -40,6 +40,7 @@ from __future__ import annotations
 import functools
 import operator
 import struct
+from collections.abc import Mapping
 
 import numpy as np
 
@@ -122,6 +123,22 @@ def _whole(v, what: str) -> int:
         raise ValueError(f"{what} must be a whole number, got {v!r}") from None
 
 
+def _number(v, what: str) -> float:
+    try:
+        if _torch is not None and isinstance(v, _torch.Tensor) and v.numel() != 1:
+            raise ValueError
+        return float(v)
+    except (OverflowError, TypeError, ValueError):
+        raise ValueError(f"{what} must be a number, got {v!r}") from None
+
+
+def _list(v, what: str) -> list:
+    try:
+        return list(v)
+    except TypeError:
+        raise ValueError(f"{what} must be a list, got {type(v).__name__}") from None
+
+
 def _seed(seed) -> int:
     seed = _whole(seed, "seed")
     if not 0 <= seed < 1 << 64:
@@ -130,14 +147,14 @@ def _seed(seed) -> int:
 
 
 def _drop(drop) -> float:
-    drop = float(drop)
+    drop = _number(drop, "drop")
     if not 0.0 <= drop < 1.0:
         raise ValueError(f"drop must be in [0, 1), got {drop}")
     return drop
 
 
 def _scale(scale) -> float:
-    scale = float(scale)
+    scale = _number(scale, "scale")
     if not abs(scale) <= _MOST:
         raise ValueError(f"scale must be a finite float32, got {scale}")
     return scale
@@ -442,7 +459,7 @@ def check_options(temperature, top_k, top_p, min_p) -> tuple[float, int, float, 
 
 
 def _temperature(v) -> float:
-    v = float(v)
+    v = _number(v, "temperature")
     if not 0.0 <= v <= _MOST:
         raise ValueError(f"temperature must be a finite float32, not negative, got {v}")
     return v
@@ -456,7 +473,7 @@ def _top_k(v) -> int:
 
 
 def _share(what: str, v) -> float:
-    v = float(v)
+    v = _number(v, what)
     if not 0.0 <= v <= 1.0:
         raise ValueError(f"{what} must be in [0, 1], got {v}")
     return v
@@ -529,7 +546,7 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
 
 # ------------------------------------------------------------------- layer norm
 def _eps(eps) -> float:
-    eps = float(eps)
+    eps = _number(eps, "eps")
     if not 2.0 ** -126 <= eps <= _MOST:
         raise ValueError(f"eps must be a positive normal float32, got {eps}")
     return eps
@@ -835,10 +852,12 @@ class AdamW(_Kept):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay=0.01, *, bits: int = 32, seed: int = 0):
         torch = _need_torch()
-        self.params = [params] if isinstance(params, torch.Tensor) else list(params)
+        self.params = [params] if isinstance(params, torch.Tensor) else _list(
+            params, "params")
         if not self.params:
             raise ValueError("no parameters")
-        betas = tuple(float(b) for b in betas)
+        betas = tuple(_number(b, "betas must be two numbers in [0, 1): each")
+                      for b in _list(betas, "betas must be two numbers in [0, 1): they"))
         if len(betas) != 2 or not all(0.0 <= b < 1.0 for b in betas):
             raise ValueError(f"betas must be two numbers in [0, 1), got {betas}")
         if bits not in (8, 32):
@@ -886,8 +905,8 @@ class AdamW(_Kept):
     @weight_decay.setter
     def weight_decay(self, value):
         n = len(self.params)
-        decays = tuple(float(d) for d in value) if isinstance(value, (list, tuple)) else (
-            (float(value),) * n)
+        decays = tuple(_number(d, "weight_decay") for d in value) if (
+            isinstance(value, (list, tuple))) else (_number(value, "weight_decay"),) * n
         if len(decays) != n or not all(0.0 <= d <= _MOST for d in decays):
             raise ValueError(f"weight_decay must be a number, not negative, or a list of {n}")
         self._decays = decays
@@ -919,7 +938,7 @@ class AdamW(_Kept):
             if lr.dtype != _torch.float32 or lr.numel() != 1:
                 raise ValueError(f"lr must be one float32, got {lr.dtype} of {tuple(lr.shape)}")
             return 0.0, lr.data_ptr()
-        lr = float(lr)
+        lr = _number(lr, "lr")
         if not 0.0 <= lr <= _MOST:
             raise ValueError(f"lr must be a finite float32, not negative, got {lr}")
         return lr, 0
@@ -947,7 +966,8 @@ class AdamW(_Kept):
         each parameter, of its shape and type. Every parameter needs one, in memory that is no
         parameter's."""
         params = self.params
-        grads = [p.grad for p in params] if grads is None else list(grads)
+        grads = [p.grad for p in params] if grads is None else _list(
+            grads, "grads")
         if len(grads) != len(params):
             raise ValueError(f"{len(grads)} gradients for {len(params)} parameters")
         # (a small step's time is what the host takes for these)
@@ -1024,6 +1044,8 @@ class AdamW(_Kept):
         """Takes up a state of as many parameters of the same sizes, copying it. "decays" (the
         betas' powers) follow from "step" where they are missing, "masters" from the
         parameters."""
+        if not isinstance(state, Mapping):
+            raise ValueError(f"a state must be a dict, got {type(state).__name__}")
         missing = {"step", "mean", "square"} | ({"scales"} if self.bits == 8 else set())
         missing -= state.keys()
         if missing:
@@ -1034,12 +1056,15 @@ class AdamW(_Kept):
         if state.get("bits", self.bits) != self.bits:
             raise ValueError(f"the state has {state['bits']} bits, the optimizer {self.bits}")
         decays = state.get("decays")
-        decays = [b ** step for b in self.betas] if decays is None else [float(d) for d in decays]
+        decays = [b ** step for b in self.betas] if decays is None else [
+            _number(d, "decays must be two numbers in [0, 1]: each")
+            for d in _list(decays, "decays must be two numbers in [0, 1]: they")]
         if len(decays) != 2 or not all(0.0 <= d <= 1.0 for d in decays):
             raise ValueError(f"decays must be two numbers in [0, 1], got {decays}")
         masters = state.get("masters")
         if masters is None:
             masters = [None if w is None else p for p, w in zip(self.params, self.masters)]
+        masters = _list(masters, "masters")
         if len(masters) != len(self.masters):
             raise ValueError(f"{len(masters)} masters for {len(self.masters)} parameters")
         pairs = [("mean", self.mean, state["mean"]), ("square", self.square, state["square"])]

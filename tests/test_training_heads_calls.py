@@ -6,6 +6,7 @@ from __future__ import annotations
 import copy
 import pickle
 
+import numpy as np
 import pytest
 import torch
 
@@ -77,3 +78,29 @@ def test_a_parameter_with_a_tangent_is_refused():
         mean = fwd.make_dual(opt.mean, torch.ones_like(opt.mean))
         with pytest.raises(ValueError, match="mean has a tangent"):
             opt.load_state_dict({"step": 0, "mean": mean, "square": opt.square})
+
+
+@pytest.mark.parametrize("call, msg", [
+    (lambda o: heads._eps(None), "eps must be a number"),
+    (lambda o: heads._drop("half"), "drop must be a number"),
+    (lambda o: heads._scale([1.0, 2.0]), "scale must be a number"),
+    (lambda o: heads._scale(10 ** 400), "scale must be a number"),
+    (lambda o: heads.check_options(None, 0, 1.0, 0.0), "temperature must be a number"),
+    (lambda o: heads.check_options(1.0, 0, torch.ones(2), 0.0), "top_p must be a number"),
+    (lambda o: heads.AdamW([torch.zeros(3)], betas=0.9), "betas must be two numbers"),
+    (lambda o: heads.AdamW([torch.zeros(3)], betas=(0.9, None)), "betas must be two numbers"),
+    (lambda o: heads.AdamW([torch.zeros(3)], eps=None), "eps must be a number"),
+    (lambda o: heads.AdamW(3), "params must be"),
+    (lambda o: setattr(o, "weight_decay", np.array([0.1, 0.1])), "weight_decay must be"),
+    (lambda o: setattr(o, "weight_decay", None), "weight_decay must be"),
+    (lambda o: setattr(o, "weight_decay", [0.1, None]), "weight_decay must be"),
+    (lambda o: (setattr(o, "lr", None), o._lr()), "lr must be a number"),
+    (lambda o: o.step(5), "grads must be a list"),
+    (lambda o: o.load_state_dict(None), "a state must be a dict"),
+    (lambda o: o.load_state_dict({"step": 0, "mean": o.mean, "square": o.square, "decays": 1.0}),
+     "decays must be two numbers"),
+    (lambda o: o.load_state_dict({"step": 0, "mean": o.mean, "square": o.square, "masters": 1}),
+     "masters must be a list")])
+def test_arguments_of_another_kind_are_value_errors(call, msg):
+    with pytest.raises(ValueError, match=msg):
+        call(_optimizer())
