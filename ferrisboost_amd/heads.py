@@ -94,10 +94,17 @@ def _no_tangent(x, what: str):
         raise ValueError(f"{what} has a tangent: forward-mode derivatives are not available")
 
 
+def _dense(x, what: str):
+    if x.layout is not _torch.strided or x.is_nested:
+        raise ValueError(f"{what} must be dense, got "
+                         f"{'a nested tensor' if x.is_nested else x.layout}")
+
+
 def _device_tensor(x, what: str):
     if not isinstance(x, _torch.Tensor):
         raise ValueError(f"{what} must be a torch tensor, got {type(x).__name__}")
     _no_tangent(x, what)
+    _dense(x, what)
     if not x.is_cuda:
         raise ValueError(f"{what} must be on a GPU, it is on {x.device}")
     return x if x.is_contiguous() else x.contiguous()
@@ -919,6 +926,7 @@ class AdamW(_Kept):
         if not isinstance(p, _torch.Tensor):
             raise ValueError(f"parameter {i} must be a torch tensor, got {type(p).__name__}")
         _no_tangent(p, f"parameter {i}")
+        _dense(p, f"parameter {i}")
         if not p.is_cuda:
             raise ValueError(f"parameter {i} must be on a GPU, it is on {p.device}")
         _cells(p, f"parameter {i}")
@@ -985,9 +993,15 @@ class AdamW(_Kept):
                 list(map(T.numel, params)) == self._sizes and
                 list(map(T.get_device, params)) == devices and all(map(T.is_contiguous, params))):
             raise ValueError("a parameter has changed its type, size or place")
+        try:
+            at = list(map(T.data_ptr, grads))
+        except RuntimeError:  # (of a sparse one, whose address is the first thing that it lacks)
+            for i, (p, g) in enumerate(zip(params, grads)):
+                self._gradient(i, p, g)
+            raise
         parts = self._parts
         parts[0::7] = map(T.data_ptr, params)
-        parts[1::7] = map(T.data_ptr, grads)
+        parts[1::7] = at
         parts[2::7] = [0 if w is None else w.data_ptr() for w in self.masters]
         stream = _raw_stream(dev)
         self._used_on(stream)

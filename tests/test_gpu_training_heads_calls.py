@@ -39,3 +39,23 @@ def test_parameters_that_left_the_device(heads):
     with pytest.raises(ValueError, match="changed its type, size or place"):
         opt.step([torch.zeros(300, device="cuda")])
     assert opt.state_dict()["step"] == 0
+
+
+def test_sparse_gradients_are_refused(heads):
+    table = torch.nn.Embedding(50, 8, sparse=True, device="cuda")
+    bias = torch.nn.Parameter(torch.zeros(8, device="cuda"))
+    opt = heads.AdamW([bias, table.weight])
+    before = table.weight.detach().clone()
+    (table(torch.tensor([3, 4, 3], device="cuda")) + bias).sum().backward()
+    assert table.weight.grad.is_sparse
+    with pytest.raises(ValueError, match="gradient 1 must be dense"):
+        opt.step()
+    assert opt.state_dict()["step"] == 0 and torch.equal(table.weight, before)
+    table.weight.grad = table.weight.grad.to_dense()
+    opt.step()
+    moved = (table.weight != before).any(1)
+    assert moved[3] and moved[4]
+    with pytest.raises(ValueError, match="x must be dense"):
+        heads.layer_norm(before.to_sparse())
+    with pytest.raises(ValueError, match="x must be dense"):
+        heads.layer_norm(before.to_sparse_csr())

@@ -104,3 +104,25 @@ def test_a_parameter_with_a_tangent_is_refused():
 def test_arguments_of_another_kind_are_value_errors(call, msg):
     with pytest.raises(ValueError, match=msg):
         call(_optimizer())
+
+
+@pytest.mark.parametrize("sparse", [
+    lambda x: x.to_sparse(), lambda x: x.to_sparse_csr(),
+    lambda x: torch.nested.nested_tensor([x[0], x[1]])])
+def test_tensors_that_are_not_dense_are_refused(sparse):
+    x = sparse(torch.ones(4, 3))
+    for call in (lambda: heads.layer_norm(x), lambda: heads.dropout(x, 0.5, 1),
+                 lambda: heads.AdamW([x])):
+        with pytest.raises(ValueError, match="must be dense"):
+            call()
+
+
+def test_sparse_gradients_are_refused():
+    """What an embedding with sparse=True leaves in .grad, say."""
+    opt = _optimizer()
+    grads = [torch.ones(3), torch.ones(300).to_sparse()]
+    opt.mean = grads[0]  # (on the gradients' device, as it is on a GPU)
+    with pytest.raises(ValueError, match="gradient 1 must be dense"):
+        opt._gradient(1, opt.params[1], grads[1])
+    with pytest.raises(ValueError, match="gradient"):
+        opt.step(grads)
