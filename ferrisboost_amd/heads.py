@@ -982,23 +982,24 @@ class AdamW(_Kept):
         T = _torch.Tensor
         dev = self.mean.get_device()
         devices = [dev] * len(params)
-        if not (_forward_ad._current_level < 0 and all(type(g) is T for g in grads) and
-                list(map(T.get_device, grads)) == devices and all(map(T.is_contiguous, grads)) and
-                list(map(_dtype_of, grads)) == self._types and
-                list(map(_shape_of, grads)) == list(map(_shape_of, params))):
+        try:
+            plain = (_forward_ad._current_level < 0 and all(type(g) is T for g in grads) and
+                     list(map(T.get_device, grads)) == devices and
+                     all(map(T.is_contiguous, grads)) and
+                     list(map(_dtype_of, grads)) == self._types and
+                     list(map(_shape_of, grads)) == list(map(_shape_of, params)))
+            at = list(map(T.data_ptr, grads)) if plain else None
+        except RuntimeError:  # (sparse ones have no address)
+            plain = False
+        if not plain:
             for i, p in enumerate(params):
                 _no_tangent(p, f"parameter {i}")
             grads = [self._gradient(i, p, g) for i, (p, g) in enumerate(zip(params, grads))]
+            at = list(map(T.data_ptr, grads))
         if not (list(map(_dtype_of, params)) == self._types and
                 list(map(T.numel, params)) == self._sizes and
                 list(map(T.get_device, params)) == devices and all(map(T.is_contiguous, params))):
             raise ValueError("a parameter has changed its type, size or place")
-        try:
-            at = list(map(T.data_ptr, grads))
-        except RuntimeError:  # (of a sparse one, whose address is the first thing that it lacks)
-            for i, (p, g) in enumerate(zip(params, grads)):
-                self._gradient(i, p, g)
-            raise
         parts = self._parts
         parts[0::7] = map(T.data_ptr, params)
         parts[1::7] = at

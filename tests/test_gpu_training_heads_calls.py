@@ -51,6 +51,8 @@ def test_sparse_gradients_are_refused(heads):
     with pytest.raises(ValueError, match="gradient 1 must be dense"):
         opt.step()
     assert opt.state_dict()["step"] == 0 and torch.equal(table.weight, before)
+    with pytest.raises(ValueError, match="gradient 1 must be dense"):
+        opt.step([bias.grad, table.weight.grad.to_dense().to_sparse_csr()])
     table.weight.grad = table.weight.grad.to_dense()
     opt.step()
     moved = (table.weight != before).any(1)
