@@ -125,7 +125,12 @@ def _beside(x, other, what: str):
 
 def _whole(v, what: str) -> int:
     try:
-        return int(v)
+        if _torch is not None and isinstance(v, _torch.Tensor) and v.numel() != 1:
+            raise ValueError
+        whole = int(v)
+        if whole != v and not isinstance(v, str):
+            raise ValueError
+        return whole
     except (OverflowError, TypeError, ValueError):
         raise ValueError(f"{what} must be a whole number, got {v!r}") from None
 

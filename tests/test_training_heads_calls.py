@@ -126,3 +126,12 @@ def test_sparse_gradients_are_refused():
         opt._gradient(1, opt.params[1], grads[1])
     with pytest.raises(ValueError, match="gradient"):
         opt.step(grads)
+
+
+@pytest.mark.parametrize("v", [2.5, 1e-3, np.float32(7.25), torch.tensor(0.5), -0.1,
+                               torch.tensor([1, 2])])
+def test_whole_numbers_have_no_fraction(v):
+    with pytest.raises(ValueError, match="n must be a whole number"):
+        heads._whole(v, "n")
+    assert heads._whole(3.0, "n") == heads._whole(np.int64(3), "n") == 3
+    assert heads._whole(torch.tensor(3), "n") == heads._whole(True, "n") + 2 == 3
