@@ -28,6 +28,12 @@ inline void head_input(bool ok, const char *message) {
     if (!ok) throw HeadError(FBH_INPUT_ERROR, message);
 }
 
+// Whether two pieces of memory share a byte.
+inline bool overlap(const void *a, uint64_t a_bytes, const void *b, uint64_t b_bytes) {
+    const auto p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+    return a && b && (p < q ? q - p < a_bytes : p - q < b_bytes) && a_bytes && b_bytes;
+}
+
 template <class F>
 int head_guard(F &&f) {
     try {

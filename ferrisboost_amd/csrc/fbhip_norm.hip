@@ -534,6 +534,12 @@ void check_norm(const fbh_norm *a) {
                "eps must be a positive normal float");
 }
 
+// Bytes of the rows, of their statistics and of a weight.
+uint64_t cell_bytes(uint32_t type) { return type == FBH_F32 ? 4 : 2; }
+uint64_t row_bytes(const fbh_norm *a) { return a->n_rows * a->dim * cell_bytes(a->dtype); }
+uint64_t stats_bytes(const fbh_norm *a) { return a->n_rows * 8; }
+uint64_t weight_bytes(const fbh_norm *a) { return a->dim * cell_bytes(a->weight_type); }
+
 template <class K, class... A>
 void launch(K kernel, uint64_t blocks, uint32_t threads, hipStream_t s, A... args) {
     hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(threads), 0, s, args...);
@@ -598,6 +604,13 @@ int fbh_layer_norm(int device, const fbh_norm *a, const void *x, const void *wei
         check_norm(a);
         head_input((x && out) || a->n_rows == 0, "null argument");
         if (a->n_rows == 0) return;
+        const uint64_t rows = row_bytes(a), each = stats_bytes(a), cells = weight_bytes(a);
+        head_input(out == x || !overlap(out, rows, x, rows), "out must be x or apart from it");
+        head_input(!overlap(out, rows, weight, cells) && !overlap(out, rows, bias, cells),
+                   "out must not overlap a weight");
+        head_input(!overlap(stats, each, x, rows) && !overlap(stats, each, out, rows) &&
+                       !overlap(stats, each, weight, cells) && !overlap(stats, each, bias, cells),
+                   "stats must not overlap another tensor");
         const OnDevice on(device);
         const auto s = static_cast<hipStream_t>(stream);
         with_type(a->dtype, [&](auto t) {
@@ -627,7 +640,12 @@ int fbh_layer_norm_grad(int device, const fbh_norm *a, const void *grad, const v
             head_input(need == 0 || reinterpret_cast<uintptr_t>(work) % 16 == 0,
                        "the workspace must be 16-byte aligned");
         }
-        head_input(!dx || (dx != grad && dx != x), "dx must not be grad or x");
+        const uint64_t rows = row_bytes(a);
+        head_input(!overlap(dx, rows, grad, rows) && !overlap(dx, rows, x, rows),
+                   "dx must not be grad or x, nor overlap them");
+        head_input(!overlap(dx, rows, stats, stats_bytes(a)) &&
+                       !overlap(dx, rows, weight, weight_bytes(a)),
+                   "dx must not overlap stats or weight");
         if (!dx && !dweight && !dbias) return;
         const OnDevice on(device);
         const auto s = static_cast<hipStream_t>(stream);

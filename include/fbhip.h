@@ -844,15 +844,16 @@ typedef struct {
 /* out = (x - mean) / sqrt(variance + eps) * weight + bias, a row's mean and variance
  * over its cells (weight NULL: 1, bias NULL: 0). stats (may be NULL) gets each row's
  * mean and 1 / sqrt(variance + eps), [n_rows][2]. Sums are taken in f32 in an order
- * that depends on dim alone. out may be x. */
+ * that depends on dim alone. out may be x; apart from that no output overlaps another
+ * tensor of the call. */
 int fbh_layer_norm(int device, const fbh_norm *a, const void *x, const void *weight,
                    const void *bias, void *out, float *stats, void *stream);
 /* Device bytes of workspace that fbh_layer_norm_grad takes for dweight or dbias,
  * 16-byte aligned; 0 for a few rows (up to 2 to 128 by their width) and for a call that it
  * refuses. */
 uint64_t fbh_layer_norm_grad_bytes(const fbh_norm *a);
-/* The gradients for the output's gradient grad: dx [n_rows][dim] (not grad or x: wide
- * rows are read again), dweight and dbias [dim], summed over all rows (each may be NULL:
+/* The gradients for the output's gradient grad: dx [n_rows][dim] (apart from the inputs:
+ * wide rows are read again), dweight and dbias [dim], summed over all rows (each may be NULL:
  * not wanted); stats as fbh_layer_norm gave them. The rows of a workgroup are summed in f32, the
  * workgroups' sums, at most 1024, in f64. Orders of sums depend on n_rows and dim
  * alone. work may be NULL where neither dweight nor dbias is wanted. */

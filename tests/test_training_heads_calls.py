@@ -10,6 +10,7 @@ import numpy as np
 import pytest
 import torch
 
+from ferrisboost_amd import _native as N
 from ferrisboost_amd import heads
 
 
@@ -135,3 +136,41 @@ def test_whole_numbers_have_no_fraction(v):
         heads._whole(v, "n")
     assert heads._whole(3.0, "n") == heads._whole(np.int64(3), "n") == 3
     assert heads._whole(torch.tensor(3), "n") == heads._whole(True, "n") + 2 == 3
+
+
+# 100 rows of 8 float32: 3200 bytes; their statistics 800, weights 32
+ROWS, CELLS = 100, 8
+
+
+@pytest.mark.parametrize("over", ["dx", "out", "stats"])
+@pytest.mark.parametrize("shift", [-3196, -4, 4, 3196])
+def test_layer_norm_outputs_that_overlap_an_input_in_part(over, shift):
+    """Rows would be read after others have been written over them."""
+    L, a = N.hip(), heads._NORM.pack(ROWS, CELLS, 0, 0, 1e-5)
+    x, g = 0x10000, 0x20000
+    if over == "dx":
+        for dx, msg in ((x + shift, "dx must not"), (g + shift, "dx must not")):
+            with pytest.raises(ValueError, match=msg):
+                N.check_hip(L.fbh_layer_norm_grad(0, a, g, x, 0x30000, None, dx, None, None, None,
+                                                  0, None))
+    elif over == "out":
+        with pytest.raises(ValueError, match="out must be x or apart"):
+            N.check_hip(L.fbh_layer_norm(0, a, x, None, None, x + shift, None, None))
+    else:
+        at = x + (shift if shift > 0 else shift % 800 - 800)
+        with pytest.raises(ValueError, match="stats must not"):
+            N.check_hip(L.fbh_layer_norm(0, a, x, None, None, 0x30000, at, None))
+        with pytest.raises(ValueError, match="stats must not"):
+            N.check_hip(L.fbh_layer_norm(0, a, x, None, None, x, at, None))
+
+
+def test_layer_norm_outputs_that_overlap_weights_or_statistics():
+    L, a = N.hip(), heads._NORM.pack(ROWS, CELLS, 0, 0, 1e-5)
+    x, g, out = 0x10000, 0x20000, 0x30000
+    for w, b in ((out + 3196, None), (out - 28, None), (0x40000, out)):
+        with pytest.raises(ValueError, match="out must not overlap a weight"):
+            N.check_hip(L.fbh_layer_norm(0, a, x, w, b, out, None, None))
+    for stats, w in ((out - 796, None), (out + 3196, None), (0x40000, out + 3196)):
+        with pytest.raises(ValueError, match="dx must not"):
+            N.check_hip(L.fbh_layer_norm_grad(0, a, g, x, stats, w, out, None, None, None, 0,
+                                              None))
