@@ -1057,13 +1057,14 @@ class AdamW(_Kept):
         own tensors, of which what stores them later makes copies."""
         clock = self._clock.cpu()
         return {"step": int(clock[0]), "decays": clock[1:3].view(_torch.float64).tolist(),
-                "bits": self.bits, "mean": self.mean, "square": self.square,
-                "scales": self.scales, "masters": list(self.masters)}
+                "bits": self.bits, "sizes": list(self._sizes), "mean": self.mean,
+                "square": self.square, "scales": self.scales, "masters": list(self.masters)}
 
     def load_state_dict(self, state: dict):
         """Takes up a state of as many parameters of the same sizes, copying it. "decays" (the
         betas' powers) follow from "step" where they are missing, "masters" from the
-        parameters."""
+        parameters; without "sizes", the parameters' numbers of cells, only their padded sum
+        is checked."""
         if not isinstance(state, Mapping):
             raise ValueError(f"a state must be a dict, got {type(state).__name__}")
         missing = {"step", "mean", "square"} | ({"scales"} if self.bits == 8 else set())
@@ -1075,6 +1076,10 @@ class AdamW(_Kept):
             raise ValueError(f"step must be in 0..=2^62 - 1, got {step}")
         if state.get("bits", self.bits) != self.bits:
             raise ValueError(f"the state has {state['bits']} bits, the optimizer {self.bits}")
+        sizes = state.get("sizes")
+        if sizes is not None and _list(sizes, "sizes") != self._sizes:
+            raise ValueError(f"the state is one of parameters of {list(sizes)} cells, these have "
+                             f"{self._sizes}")
         decays = state.get("decays")
         decays = [b ** step for b in self.betas] if decays is None else [
             _number(d, "decays must be two numbers in [0, 1]: each")

@@ -61,3 +61,18 @@ def test_sparse_gradients_are_refused(heads):
         heads.layer_norm(before.to_sparse())
     with pytest.raises(ValueError, match="x must be dense"):
         heads.layer_norm(before.to_sparse_csr())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_states_of_other_sizes_are_refused(heads, bits):
+    """Of parameters whose padded sizes add up to the same."""
+    a = heads.AdamW([torch.ones(n, device="cuda") for n in (300, 100)], bits=bits)
+    b = heads.AdamW([torch.ones(n, device="cuda") for n in (100, 300)], bits=bits)
+    a.step([torch.ones_like(p) for p in a.params])
+    with pytest.raises(ValueError, match="parameters of"):
+        b.load_state_dict(a.state_dict())
+    assert b.state_dict()["step"] == 0 and (b.mean == 0).all()
+    state = a.state_dict()
+    del state["sizes"]  # (one that was stored before states held them)
+    heads.AdamW([torch.ones(n, device="cuda") for n in (300, 100)],
+                bits=bits).load_state_dict(state)

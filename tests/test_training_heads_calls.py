@@ -174,3 +174,16 @@ def test_layer_norm_outputs_that_overlap_weights_or_statistics():
         with pytest.raises(ValueError, match="dx must not"):
             N.check_hip(L.fbh_layer_norm_grad(0, a, g, x, stats, w, out, None, None, None, 0,
                                               None))
+
+
+def test_states_of_other_sizes_are_refused():
+    """Sizes of the same padded total: moments would land in other cells."""
+    for sizes, other in (((300, 100), (100, 300)), ((1,), (256,)), ((300, 5), (300, 6))):
+        a, b = _optimizer(sizes), _optimizer(other)
+        assert a.mean.shape == b.mean.shape
+        state = a.state_dict()
+        assert state["sizes"] == list(sizes)
+        with pytest.raises(ValueError, match="parameters of"):
+            b.load_state_dict(state)
+        with pytest.raises(ValueError, match="sizes must be a list"):
+            b.load_state_dict({**state, "sizes": 3})
