@@ -1054,17 +1054,19 @@ class AdamW(_Kept):
 
     def state_dict(self) -> dict:
         """What load_state_dict() takes: the steps done (waits for the device) and the state's
-        own tensors, of which what stores them later makes copies."""
+        own tensors, of which what stores them later makes copies. The numbers that the
+        optimizer was made with or given since (lr, betas, eps, weight_decay) are not in it."""
         clock = self._clock.cpu()
         return {"step": int(clock[0]), "decays": clock[1:3].view(_torch.float64).tolist(),
-                "bits": self.bits, "sizes": list(self._sizes), "mean": self.mean,
-                "square": self.square, "scales": self.scales, "masters": list(self.masters)}
+                "bits": self.bits, "sizes": list(self._sizes), "seed": self.seed,
+                "mean": self.mean, "square": self.square, "scales": self.scales,
+                "masters": list(self.masters)}
 
     def load_state_dict(self, state: dict):
         """Takes up a state of as many parameters of the same sizes, copying it. "decays" (the
         betas' powers) follow from "step" where they are missing, "masters" from the
         parameters; without "sizes", the parameters' numbers of cells, only their padded sum
-        is checked."""
+        is checked, and without "seed" the optimizer keeps its own."""
         if not isinstance(state, Mapping):
             raise ValueError(f"a state must be a dict, got {type(state).__name__}")
         missing = {"step", "mean", "square"} | ({"scales"} if self.bits == 8 else set())
@@ -1080,6 +1082,7 @@ class AdamW(_Kept):
         if sizes is not None and _list(sizes, "sizes") != self._sizes:
             raise ValueError(f"the state is one of parameters of {list(sizes)} cells, these have "
                              f"{self._sizes}")
+        seed = self.seed if state.get("seed") is None else _seed(state["seed"])
         decays = state.get("decays")
         decays = [b ** step for b in self.betas] if decays is None else [
             _number(d, "decays must be two numbers in [0, 1]: each")
@@ -1108,6 +1111,7 @@ class AdamW(_Kept):
                 to.copy_(x)
             words = struct.unpack("4q", struct.pack("qddq", step, *decays, 0))
             self._clock.copy_(_torch.tensor(words, dtype=_torch.int64))
+        self.seed = seed
 
     def __repr__(self):
         return (f"AdamW({len(self.params)} parameters, {sum(self._sizes)} cells, {self.bits} "

@@ -76,3 +76,26 @@ def test_states_of_other_sizes_are_refused(heads, bits):
     del state["sizes"]  # (one that was stored before states held them)
     heads.AdamW([torch.ones(n, device="cuda") for n in (300, 100)],
                 bits=bits).load_state_dict(state)
+
+
+def test_a_resumed_run_rounds_as_the_first_one_would(heads):
+    """Moments of 8 bits are rounded by bits of the seed, which a state brings with it."""
+    grads = [torch.randn(3000, device="cuda") for _ in range(6)]
+    p = torch.randn(3000, device="cuda")
+    opt = heads.AdamW([p], lr=0.01, bits=8, seed=77)
+    for g in grads[:3]:
+        opt.step([g])
+    q = p.clone()
+    again = heads.AdamW([q], lr=0.01, bits=8)
+    again.load_state_dict(opt.state_dict())
+    assert again.seed == 77
+    for g in grads[3:]:
+        opt.step([g])
+        again.step([g])
+    assert torch.equal(p, q) and torch.equal(opt.mean, again.mean)
+    assert torch.equal(opt.square, again.square) and torch.equal(opt.scales, again.scales)
+    old = opt.state_dict()
+    del old["seed"]  # (one that was stored before states held it)
+    other = heads.AdamW([q], bits=8, seed=5)
+    other.load_state_dict(old)
+    assert other.seed == 5

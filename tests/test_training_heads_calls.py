@@ -187,3 +187,12 @@ def test_states_of_other_sizes_are_refused():
             b.load_state_dict(state)
         with pytest.raises(ValueError, match="sizes must be a list"):
             b.load_state_dict({**state, "sizes": 3})
+
+
+def test_states_hold_their_seed():
+    for bits in (8, 32):
+        state = _optimizer(bits=bits, seed=2 ** 64 - 1).state_dict()
+        assert state["seed"] == 2 ** 64 - 1
+        for bad in (-1, 1 << 64, "none"):
+            with pytest.raises(ValueError, match="seed"):
+                _optimizer(bits=bits).load_state_dict({**state, "seed": bad})
