@@ -909,6 +909,12 @@ class AdamW(_Kept):
         self._clock[1:3] = 0x3FF0000000000000  # 1.0
         self._streams = {_raw_stream(like.get_device())}
 
+    # the learning rate's tensor and the stream that the last step has kept it for
+    _lr_used = (None, None)
+
+    def __setstate__(self, state):
+        super().__setstate__({**state, "_lr_used": (None, None)})
+
     @property
     def weight_decay(self) -> tuple:
         """Each parameter's weight decay; it is set as a number or a list of one for each."""
@@ -1011,6 +1017,10 @@ class AdamW(_Kept):
         parts[2::7] = [0 if w is None else w.data_ptr() for w in self.masters]
         stream = _raw_stream(dev)
         self._used_on(stream)
+        lr = self.lr
+        if isinstance(lr, T) and (self._lr_used[0] is not lr or self._lr_used[1] != stream):
+            lr.record_stream(_torch.cuda.current_stream(lr.device))
+            self._lr_used = lr, stream
         rc = _L.fbh_adamw_step(dev, self._packed(), _adamw_tensors(len(params)).pack(*parts),
                                len(params), stream)
         if rc:

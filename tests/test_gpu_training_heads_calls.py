@@ -99,3 +99,36 @@ def test_a_resumed_run_rounds_as_the_first_one_would(heads):
     other = heads.AdamW([q], bits=8, seed=5)
     other.load_state_dict(old)
     assert other.seed == 5
+
+
+def test_a_learning_rate_that_is_replaced_while_a_stream_still_reads_it(heads):
+    """Its memory is not given out again before the stream has passed the step."""
+    p = torch.randn(3000, device="cuda")
+    q, grad = p.clone(), torch.randn(3000, device="cuda")
+    heads.AdamW([q], lr=0.25).step([grad])
+    opt = heads.AdamW([p], lr=0.1)
+    a = torch.zeros(1 << 28, device="cuda")  # 1 GiB
+    b = torch.empty_like(a)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):  # (its state has been used there before)
+        opt.lr = 0.0
+        opt.step([torch.zeros_like(p)])
+    opt.load_state_dict({**opt.state_dict(), "step": 0, "decays": [1.0, 1.0]})
+    opt.mean.zero_()
+    opt.square.zero_()
+    opt.lr = torch.full((1,), 0.25, device="cuda")
+    at = opt.lr.data_ptr()
+    s.wait_stream(torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        for _ in range(200):  # some 80 ms
+            b.copy_(a)
+        opt.step([grad])
+        done = s.record_event()
+    opt.lr = 0.1
+    del opt
+    others = [torch.zeros(1, device="cuda") for _ in range(600)]
+    assert not done.query()  # (else the rest says nothing)
+    assert at not in {o.data_ptr() for o in others}
+    s.synchronize()
+    assert torch.equal(p, q)

@@ -196,3 +196,43 @@ def test_states_hold_their_seed():
         for bad in (-1, 1 << 64, "none"):
             with pytest.raises(ValueError, match="seed"):
                 _optimizer(bits=bits).load_state_dict({**state, "seed": bad})
+
+
+def test_learning_rates_on_the_device_are_kept_for_a_step_s_stream(monkeypatch):
+    """Each tensor that is set, on each stream that reads it: also one that is replaced while a
+    step of its stream is still to come."""
+    recorded = []
+
+    class Native:
+        @staticmethod
+        def fbh_adamw_step(*args):
+            return 0
+
+    opt = _optimizer()
+    now = [5]
+    monkeypatch.setattr(heads, "_raw_stream", lambda device: now[0])
+    monkeypatch.setattr(heads, "_L", Native)
+    monkeypatch.setattr(torch.Tensor, "record_stream",
+                        lambda self, stream: recorded.append((float(self), stream)))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: now[0])
+    monkeypatch.setattr(heads.AdamW, "_used_on", lambda self, stream: None)
+    monkeypatch.setattr(heads.AdamW, "_lr", lambda self: (0.0, 64))
+    grads = [torch.ones_like(p) for p in opt.params]
+
+    def step(o=opt):
+        o.step(grads)
+
+    step()
+    assert not recorded  # (a number)
+    opt.lr = torch.tensor([1.0])
+    step()
+    step()
+    assert recorded == [(1.0, 5)]
+    now[0] = 6
+    step()
+    opt.lr = torch.tensor([2.0])
+    step()
+    assert recorded == [(1.0, 5), (1.0, 6), (2.0, 6)]
+    for c in (copy.copy(opt), copy.deepcopy(opt)):
+        step(c)
+        assert recorded.pop() == (2.0, 6) and len(recorded) == 3
