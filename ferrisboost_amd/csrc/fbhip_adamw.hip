@@ -440,9 +440,9 @@ void check_adamw(const fbh_adamw *a) {
     head_input(a->n == 0 || a->bits == 32 || a->scales, "moments of 8 bits need scales");
 }
 
-// That no parameter shares memory with another one or with a gradient: steps of both would run
-// side by side.
-void check_overlaps(const fbh_adamw_tensor *tensors, uint64_t n_tensors) {
+// That no parameter shares memory with another one, a gradient or the learning rate: what a step
+// writes and what it reads would run side by side.
+void check_overlaps(const fbh_adamw_tensor *tensors, uint64_t n_tensors, const float *lr_at) {
     using Span = std::pair<uintptr_t, uintptr_t>;
     const auto span = [](const fbh_adamw_tensor &t, const void *p) {
         const auto at = reinterpret_cast<uintptr_t>(p);
@@ -455,13 +455,17 @@ void check_overlaps(const fbh_adamw_tensor *tensors, uint64_t n_tensors) {
     std::sort(params.begin(), params.end());
     for (size_t i = 1; i < params.size(); i++)
         head_input(params[i - 1].second <= params[i].first, "parameters overlap in memory");
-    for (uint64_t i = 0; i < n_tensors; i++) {
-        if (!tensors[i].n) continue;
-        const Span g = span(tensors[i], tensors[i].grad);
-        // the first parameter that begins behind the gradient; the one before ends last
-        const auto behind = std::lower_bound(params.begin(), params.end(), Span{g.second, 0});
-        head_input(behind == params.begin() || std::prev(behind)->second <= g.first,
+    const auto apart = [&](const Span &r) {
+        // the first parameter that begins behind what is read; the one before ends last
+        const auto behind = std::lower_bound(params.begin(), params.end(), Span{r.second, 0});
+        return behind == params.begin() || std::prev(behind)->second <= r.first;
+    };
+    for (uint64_t i = 0; i < n_tensors; i++)
+        head_input(!tensors[i].n || apart(span(tensors[i], tensors[i].grad)),
                    "a gradient overlaps a parameter in memory");
+    if (lr_at) {
+        const auto at = reinterpret_cast<uintptr_t>(lr_at);
+        head_input(apart({at, at + 4}), "the learning rate overlaps a parameter in memory");
     }
 }
 
@@ -487,7 +491,7 @@ int fbh_adamw_step(int device, const fbh_adamw *a, const fbh_adamw_tensor *tenso
             head_input(std::isfinite(t.weight_decay) && t.weight_decay >= 0.0f,
                        "weight_decay must be finite and not negative");
         }
-        check_overlaps(tensors, n_tensors);
+        check_overlaps(tensors, n_tensors, a->lr_at);
         const OnDevice on(device);
         const auto s = static_cast<hipStream_t>(stream);
         AdamLaunch<ADAM_TENSORS> L{};

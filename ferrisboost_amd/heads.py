@@ -848,8 +848,8 @@ class AdamW(_Kept):
     in float32. params are contiguous tensors of one device; one of 16 bits has a float32 copy
     in `masters`, which is what the steps move and round into it (call take_params() after
     writing into such a parameter). weight_decay is a number, or a list of one for each
-    parameter; lr a number, or a float32 tensor of one value on the device, which a step reads
-    when it runs. Both are attributes that may be set between steps. The steps are counted on
+    parameter; lr a number, or a float32 tensor of one value on the device, in memory that is no
+    parameter's, which a step reads when it runs. Both are attributes that may be set between steps. The steps are counted on
     the device too, so a captured step goes on at each replay. Steps of one optimizer follow
     one another: on another stream only when that has waited.
 

@@ -941,7 +941,7 @@ typedef struct {
  * as f32 and are then rounded to one of the two bytes around them, up with the
  * probability of what is cut off, to 2^-16: by the bits that fbh_dropout draws for seed
  * + t and the cell of the state, the low 16 for mean, the high 16 for square; a square
- * above 0 stays above 0. Parameters that overlap one another or a gradient are refused;
+ * above 0 stays above 0. Parameters that overlap one another, a gradient or *lr_at are refused;
  * no two tensors may overlap in the state or in their masters; steps of one state follow
  * one another. */
 int fbh_adamw_step(int device, const fbh_adamw *a, const fbh_adamw_tensor *tensors,

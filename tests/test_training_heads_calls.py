@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import copy
 import pickle
+import struct
 
 import numpy as np
 import pytest
@@ -236,3 +237,18 @@ def test_learning_rates_on_the_device_are_kept_for_a_step_s_stream(monkeypatch):
     for c in (copy.copy(opt), copy.deepcopy(opt)):
         step(c)
         assert recorded.pop() == (2.0, 6) and len(recorded) == 3
+
+
+def _step_arguments(params, lr_at, n=256):
+    """fbh_adamw and float32 tensors of n cells for the C entry."""
+    a = heads._ADAMW.pack(32, 1e-8, 0.9, 0.999, 0.0, lr_at, 0, 256 * len(params), 0x100000,
+                          0x200000, 0, 0x300000)
+    return a, b"".join(struct.pack("PPPQQfI", p, 0x400000, 0, n, 256 * i, 0.0, 0)
+                       for i, p in enumerate(params)), len(params)
+
+
+@pytest.mark.parametrize("lr_at", [0x1000, 0x13FC, 0x3004, 0x0FFD, 0x33FF])
+def test_a_learning_rate_in_a_parameter_s_memory_is_refused(lr_at):
+    """Some cells would be stepped by what it was and some by what it becomes."""
+    with pytest.raises(ValueError, match="learning rate overlaps a parameter"):
+        N.check_hip(N.hip().fbh_adamw_step(0, *_step_arguments([0x1000, 0x3000], lr_at), None))
