@@ -224,7 +224,7 @@ __device__ __forceinline__ void move_by(float (&m)[4], const float (&s)[4], cons
 // pair's number of this lane.
 template <class T, bool SMALL, bool WHOLE>
 __device__ __forceinline__ void adam_chunk(const Adam &A, const AdamStep &S, const AdamTensor &t,
-                                           float shrink, uint64_t at, uint64_t word) {
+                                           float decay, uint64_t at, uint64_t word) {
     const uint32_t lane = threadIdx.x & 63;
     const uint64_t flat = t.first + at;
     const uint32_t here = (uint32_t)min(t.n - at, (uint64_t)ADAM_CHUNK);
@@ -281,7 +281,10 @@ __device__ __forceinline__ void adam_chunk(const Adam &A, const AdamStep &S, con
     move_by(by, s, S);
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-        w[k] = fmaf(-S.size, by[k], w[k] * shrink);
+        // (what decays joins the step: 1 - lr decay in float32 would be off by up to 2^-25, a
+        // large part of a small decay. An infinite weight stays one: inf - decay * most)
+        const float most = __FLT_MAX__, part = __builtin_amdgcn_fmed3f(w[k], -most, most);
+        w[k] -= fmaf(decay, part, S.size * by[k]);
         // the 16-bit parameter is this float rounded, not the sum before
         if (MASTER) asm volatile("" : "+v"(w[k]));
     }
@@ -355,12 +358,12 @@ __global__ __launch_bounds__(ADAM_TPB) void adam_kernel(AdamLaunch<MOST> L) {
         const AdamTensor &t = L.t[lo];
         const uint64_t begin = (tile - t.tiles_before) * ADAM_TILE +
                                wave * (ADAM_CHUNKS * ADAM_CHUNK);
-        const float shrink = (float)(1.0 - S.lr * (double)t.decay);
+        const float decay = (float)(S.lr * (double)t.decay);
         const uint64_t word = ((t.first + begin) / 2 + (threadIdx.x & 63) * 2) * DROP_STEP;
         for (uint32_t c = 0; c < ADAM_CHUNKS; c++) {
             const uint64_t at = begin + c * ADAM_CHUNK, w = word + c * (ADAM_CHUNK / 2) * DROP_STEP;
-            if (at + ADAM_CHUNK <= t.n) adam_chunk<T, SMALL, true>(A, S, t, shrink, at, w);
-            else if (at < t.n) adam_chunk<T, SMALL, false>(A, S, t, shrink, at, w);
+            if (at + ADAM_CHUNK <= t.n) adam_chunk<T, SMALL, true>(A, S, t, decay, at, w);
+            else if (at < t.n) adam_chunk<T, SMALL, false>(A, S, t, decay, at, w);
         }
     }
     if (!A.ticks) return;

@@ -2,8 +2,11 @@
 
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
+
+import training_ref as ref
 
 pytestmark = pytest.mark.gpu
 
@@ -132,3 +135,32 @@ def test_a_learning_rate_that_is_replaced_while_a_stream_still_reads_it(heads):
     assert at not in {o.data_ptr() for o in others}
     s.synchronize()
     assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_small_weight_decay_is_not_rounded(heads, bits):
+    """Without a gradient a step is one product that is taken from the weight: the result is off
+    by half a step of the weight, and by what the product itself is, 3 half steps of it."""
+    rng = np.random.default_rng(3)
+    w = np.concatenate([rng.uniform(1, 2, 60_000), rng.normal(size=20_000)]).astype(np.float32)
+    for lr, decay in ((1e-5, 0.01), (1e-6, 0.3), (1e-3, 0.1), (0.5, 0.125)):
+        p = torch.from_numpy(w).cuda()
+        heads.AdamW([p], lr=lr, weight_decay=decay, bits=bits).step([torch.zeros_like(p)])
+        part = lr * float(np.float32(decay)) * w.astype(np.float64)
+        want = w - part
+        off = np.spacing(np.abs(want).astype(np.float32)).astype(np.float64) / 2
+        got = p.cpu().double().numpy()
+        assert (np.abs(got - want) <= off + 4 * ref.ULP * np.abs(part)).all(), (lr, decay)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_infinite_weights_decay_to_themselves(heads, bits, dtype):
+    """As those of masked classes may be."""
+    inf = float("inf")
+    for decay in (0.0, 0.25):
+        p = torch.tensor([inf, -inf, 1.0, float("nan"), -2.0], device="cuda").to(dtype)
+        opt = heads.AdamW([p], lr=0.5, weight_decay=decay, bits=bits)
+        opt.step([torch.zeros_like(p)])
+        keep = 1 - 0.5 * decay
+        assert p.tolist()[:3] == [inf, -inf, keep] and p[3].isnan() and float(p[4]) == -2 * keep
