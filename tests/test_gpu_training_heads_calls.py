@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+import norm_bounds
 import training_ref as ref
 
 pytestmark = pytest.mark.gpu
@@ -135,6 +136,25 @@ def test_a_learning_rate_that_is_replaced_while_a_stream_still_reads_it(heads):
     assert at not in {o.data_ptr() for o in others}
     s.synchronize()
     assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("n, dim", [(140_000, 16_386), (524_288, 4098), (1 << 27, 4)])
+def test_weights_sums_of_any_number_of_rows(heads, n, dim):
+    """Equal terms, whose float32 sum is off the same way at each addition, by a half step of the
+    sum at most, and the rounding of the result."""
+    c = float(np.float32(1.004119873046875))
+    g = torch.full((n, dim), c, device="cuda")
+    x = torch.ones((n, dim), device="cuda")
+    x[:, dim // 2:] = -1.0
+    stats = torch.zeros((n, 2), device="cuda")  # mean 0, deviation 1
+    stats[:, 1] = 1.0
+    w = torch.ones(dim, device="cuda")
+    _, dw, db = heads._layer_norm_grad(heads._norm_of(x, w, 1.0), g, x, stats, w,
+                                       (False, True, True))
+    sign = torch.where(torch.arange(dim, device="cuda") < dim // 2, 1.0, -1.0).double()
+    off = ref.ULP * (norm_bounds.weight_path(n, dim) + 1) * n * c
+    assert float((db.double() - n * c).abs().max()) <= off
+    assert float((dw.double() - sign * (n * c)).abs().max()) <= off
 
 
 @pytest.mark.parametrize("bits", [32, 8])
