@@ -138,6 +138,29 @@ def test_a_learning_rate_that_is_replaced_while_a_stream_still_reads_it(heads):
     assert torch.equal(p, q)
 
 
+def _off(got, want, off):
+    """Half a step of got's type more than `off`, in numpy's doubles."""
+    info = torch.finfo(got.dtype)
+    return np.abs(got.cpu().double().numpy() - want) <= (
+        off * (1 + info.eps) + np.abs(want) * info.eps / 2 + info.smallest_normal * info.eps / 2)
+
+
+# 1024 parts of a weight's sums, 781 and 512; 128 of some rows and of all
+@pytest.mark.parametrize("n, dim", [(200_000, 64), (300_001, 7), (100_000, 64), (30_000, 1000),
+                                    (6000, 130), (70_000, 260), (3001, 4100)])
+def test_layer_norm_gradients_of_many_rows(heads, n, dim):
+    rng = np.random.default_rng([n, dim])
+    x = torch.from_numpy(rng.normal(size=(n, dim)).astype(np.float32) +
+                         rng.normal(size=(n, 1)).astype(np.float32)).cuda()
+    g = torch.from_numpy(rng.normal(size=(n, dim)).astype(np.float32)).cuda()
+    w = torch.from_numpy((1 + rng.normal(size=dim) / 2).astype(np.float32)).cuda()
+    _, stats = heads.layer_norm(x, w, stats=True)
+    got = heads.layer_norm_grad(g, x, stats, w)
+    want = norm_bounds.layer_norm_grad(g.cpu().numpy(), x.cpu().numpy(), w.cpu().numpy(), 1e-5)
+    for a, (value, off), what in zip(got, want, ("dx", "dw", "db")):
+        assert _off(a, value, off).all(), what
+
+
 @pytest.mark.parametrize("n, dim", [(140_000, 16_386), (524_288, 4098), (1 << 27, 4)])
 def test_weights_sums_of_any_number_of_rows(heads, n, dim):
     """Equal terms, whose float32 sum is off the same way at each addition, by a half step of the
@@ -155,6 +178,28 @@ def test_weights_sums_of_any_number_of_rows(heads, n, dim):
     off = ref.ULP * (norm_bounds.weight_path(n, dim) + 1) * n * c
     assert float((db.double() - n * c).abs().max()) <= off
     assert float((dw.double() - sign * (n * c)).abs().max()) <= off
+
+
+def test_gradients_to_experts_rows_beyond_2_31_cells(heads):
+    n, k, dim = 600_001, 2, 2048
+    g = torch.Generator(device="cuda").manual_seed(4)
+    ids = torch.randint(-1, 64, (n, k), device="cuda", generator=g)
+    r = heads.Routes(ids, 64)
+    x = torch.randn(n, dim, device="cuda", dtype=torch.bfloat16, generator=g)
+    w = torch.rand(n, k, device="cuda", generator=g)
+    y = heads.to_experts(x, r)
+    dy, dw = heads.from_experts_grad(x, y, r, w)
+    end = int(r.starts[-1])
+    assert end * dim > (1 << 31) + 1000 * dim
+    at = torch.cat([torch.arange(0, 100), torch.arange((1 << 31) // dim - 50, (1 << 31) // dim + 50),
+                    torch.arange(end - 100, end)]).cuda()
+    position = r.order[at].long()
+    row = position // k
+    want = (w.view(-1)[position][:, None] * x[row].float()).bfloat16()
+    assert torch.equal(dy[at], want) and (dy[end:] == 0).all()
+    # (a lane's products in turn, a piece more, 6 levels of lanes)
+    dots = (x[row].double() * y[at].double()).sum(1)
+    assert ((dw.view(-1)[position] - dots).abs() <= dots * ref.ULP * (dim / 64 + 8 + 7)).all()
 
 
 @pytest.mark.parametrize("bits", [32, 8])
