@@ -55,6 +55,7 @@ _CELLS: dict = {}
 _IDS: dict = {}
 _raw_stream = None
 _forward_ad = None
+_Tensor = _strided = None
 # fbh_embed and fbh_sample_options (include/fbhip.h), packed in one call: a small
 # operation's time is its host time.
 _EMBED = struct.Struct("QIIIIIIPPdQfI")
@@ -67,7 +68,7 @@ _dtype_of, _shape_of = operator.attrgetter("dtype"), operator.attrgetter("shape"
 
 def _need_torch():
     """torch, once it is known to share this package's HIP runtime."""
-    global _torch, _L, _raw_stream, _forward_ad
+    global _torch, _L, _raw_stream, _forward_ad, _Tensor, _strided
     if _torch is not None:
         return _torch
     import torch
@@ -84,6 +85,7 @@ def _need_torch():
     # the current stream's handle, as torch.cuda.current_stream() wraps it
     _raw_stream = torch._C._cuda_getCurrentRawStream
     _forward_ad = torch.autograd.forward_ad
+    _Tensor, _strided = torch.Tensor, torch.strided
     _L = N.hip()
     _torch = torch
     return torch
@@ -95,18 +97,26 @@ def _no_tangent(x, what: str):
 
 
 def _dense(x, what: str):
-    if x.layout is not _torch.strided or x.is_nested:
+    if x.layout is not _strided or x.is_nested:
         raise ValueError(f"{what} must be dense, got "
                          f"{'a nested tensor' if x.is_nested else x.layout}")
 
 
-def _device_tensor(x, what: str):
-    if not isinstance(x, _torch.Tensor):
+def _device_tensor(x, what: str, on: int | None = None):
+    """x, contiguous, after checking that it is a dense tensor on a GPU, that of `on` where the
+    call has one already. (Each look at a tensor takes some 40 ns of a small call's 7 us.)"""
+    if not isinstance(x, _Tensor):
         raise ValueError(f"{what} must be a torch tensor, got {type(x).__name__}")
-    _no_tangent(x, what)
-    _dense(x, what)
-    if not x.is_cuda:
-        raise ValueError(f"{what} must be on a GPU, it is on {x.device}")
+    if _forward_ad._current_level >= 0:
+        _no_tangent(x, what)
+    if x.layout is not _strided or x.is_nested:
+        _dense(x, what)
+    dev = x.get_device()
+    if dev != on:
+        if dev < 0:
+            raise ValueError(f"{what} must be on a GPU, it is on {x.device}")
+        if on is not None:
+            raise ValueError(f"{what} is on {x.device}, the call's other tensors on cuda:{on}")
     return x if x.is_contiguous() else x.contiguous()
 
 
@@ -124,6 +134,8 @@ def _beside(x, other, what: str):
 
 
 def _whole(v, what: str) -> int:
+    if type(v) is int:
+        return v
     try:
         if _torch is not None and isinstance(v, _torch.Tensor) and v.numel() != 1:
             raise ValueError
@@ -136,6 +148,8 @@ def _whole(v, what: str) -> int:
 
 
 def _number(v, what: str) -> float:
+    if type(v) is float:
+        return v
     try:
         if _torch is not None and isinstance(v, _torch.Tensor) and v.numel() != 1:
             raise ValueError
@@ -375,7 +389,7 @@ def embed(table, ids, vocabulary: Vocabulary | None = None, *, scale: float = 1.
     if vocabulary is not None and vocabulary.n_tokens != table.shape[0]:
         raise ValueError(f"table has {table.shape[0]} rows, the vocabulary "
                          f"{vocabulary.n_tokens} tokens")
-    ids = _beside(_device_tensor(ids, "ids"), table, "ids")
+    ids = _device_tensor(ids, "ids", table.get_device())
     args = (table, ids, vocabulary, _scale(scale), bool(pooled), _drop(drop), _seed(seed))
     if table.requires_grad and torch.is_grad_enabled():
         return _functions()[0].apply(*args)
@@ -392,7 +406,7 @@ def embed_grad(grad, ids, tokens, *, scale: float = 1.0, pooled: bool = False,
     backward(); a captured training step can call it by itself.)"""
     _need_torch()
     grad = _device_tensor(grad, "grad")
-    ids = _beside(_device_tensor(ids, "ids"), grad, "ids")
+    ids = _device_tensor(ids, "ids", grad.get_device())
     vocabulary = tokens if isinstance(tokens, Vocabulary) else None
     n_tokens = vocabulary.n_tokens if vocabulary is not None else _whole(
         tokens, "tokens, other than a vocabulary,")
@@ -449,9 +463,9 @@ def dropout(x, drop: float, seed: int, first: int = 0):
 
 def _option(value, what: str, lead, like, dtype):
     """The tensor of one value a row that `value` is, or None."""
-    if not isinstance(value, _torch.Tensor) or value.dim() == 0:
+    if not isinstance(value, _Tensor) or value.dim() == 0:
         return None
-    v = _beside(_device_tensor(value, what), like, what)
+    v = _device_tensor(value, what, like.get_device())
     if tuple(v.shape) != lead:
         raise ValueError(f"{what} must have shape {lead}, got {tuple(v.shape)}")
     if v.dtype != dtype:
@@ -529,7 +543,7 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         raise ValueError(f"logits must be (..., 1 to 262144 classes), got shape "
                          f"{tuple(logits.shape)}")
     lead = tuple(logits.shape[:-1])
-    uniforms = _beside(_device_tensor(uniforms, "uniforms"), logits, "uniforms")
+    uniforms = _device_tensor(uniforms, "uniforms", logits.get_device())
     if uniforms.dtype != torch.float32 or tuple(uniforms.shape) != lead:
         raise ValueError(f"uniforms must be float32 of shape {lead}, got {uniforms.dtype} of "
                          f"{tuple(uniforms.shape)}")
@@ -572,7 +586,6 @@ def _norm_of(x, weight, eps: float) -> bytes:
         raise ValueError(f"x must be (..., 1 to 32768 cells), got shape {tuple(shape)}")
     kind = 0
     if weight is not None:
-        _beside(weight, x, "weight")
         if weight.shape != (dim,):
             raise ValueError(f"weight must have shape ({dim},), got {tuple(weight.shape)}")
         kind = _cells(weight, "weight")
@@ -598,13 +611,14 @@ def layer_norm(x, weight=None, bias=None, *, eps: float = 1e-5, stats: bool = Fa
     layer_norm_grad() takes: each row's mean and 1 / sqrt(variance + eps), (..., 2) float32."""
     torch = _need_torch()
     x = _device_tensor(x, "x")
+    dev = x.get_device()
     if weight is not None:
-        weight = _device_tensor(weight, "weight")
+        weight = _device_tensor(weight, "weight", dev)
     a = _norm_of(x, weight, _eps(eps))
     if bias is not None:
         if weight is None:
             raise ValueError("a bias needs a weight")
-        bias = _beside(_device_tensor(bias, "bias"), x, "bias")
+        bias = _device_tensor(bias, "bias", dev)
         if bias.dtype != weight.dtype or bias.shape != weight.shape:
             raise ValueError(f"bias is {bias.dtype} of {tuple(bias.shape)}, weight "
                              f"{weight.dtype} of {tuple(weight.shape)}")
@@ -642,10 +656,11 @@ def layer_norm_grad(grad, x, stats, weight=None):
     (layer_norm() does this in backward(); a captured training step can call it by itself.)"""
     torch = _need_torch()
     x = _device_tensor(x, "x")
-    grad = _beside(_device_tensor(grad, "grad"), x, "grad")
-    stats = _beside(_device_tensor(stats, "stats"), x, "stats")
+    dev = x.get_device()
+    grad = _device_tensor(grad, "grad", dev)
+    stats = _device_tensor(stats, "stats", dev)
     if weight is not None:
-        weight = _device_tensor(weight, "weight")
+        weight = _device_tensor(weight, "weight", dev)
     a = _norm_of(x, weight, 1.0)
     if grad.shape != x.shape or grad.dtype != x.dtype:
         raise ValueError(f"grad is {grad.dtype} of {tuple(grad.shape)}, x {x.dtype} of "
@@ -771,7 +786,7 @@ def _from_experts(y, routes, place, weights, dim: int, cells: int):
 
 
 def _weights(weights, place):
-    weights = _beside(_device_tensor(weights, "weights"), place, "weights")
+    weights = _device_tensor(weights, "weights", place.get_device())
     if weights.dtype is not _torch.float32 or weights.shape != place.shape:
         raise ValueError(f"weights must be float32 of {tuple(place.shape)}, got {weights.dtype} of "
                          f"{tuple(weights.shape)}")
@@ -823,7 +838,7 @@ def from_experts_grad(grad, y, routes: Routes, weights=None):
     grad = _device_tensor(grad, "grad")
     place = _routes(routes, grad)
     dim, cells = _rows_of(grad, "grad", place.shape[:-1]), _cells(grad, "grad")
-    y = _beside(_device_tensor(y, "y"), grad, "y")
+    y = _device_tensor(y, "y", grad.get_device())
     if y.shape != (place.numel(), dim) or y.dtype is not grad.dtype:
         raise ValueError(f"y must be {grad.dtype} of {(place.numel(), dim)}, got {y.dtype} of "
                          f"{tuple(y.shape)}")
@@ -953,8 +968,8 @@ class AdamW(_Kept):
     def _lr(self):
         """The learning rate as a number, and the address of one on the device or 0."""
         lr = self.lr
-        if isinstance(lr, _torch.Tensor):
-            _beside(_device_tensor(lr, "lr"), self.params[0], "lr")
+        if isinstance(lr, _Tensor):
+            _device_tensor(lr, "lr", self.params[0].get_device())
             if lr.dtype != _torch.float32 or lr.numel() != 1:
                 raise ValueError(f"lr must be one float32, got {lr.dtype} of {tuple(lr.shape)}")
             return 0.0, lr.data_ptr()
