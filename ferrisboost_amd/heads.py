@@ -677,7 +677,8 @@ class Routes(_Kept):
     """The positions of an id matrix `ids` (..., columns) in the order of their ids, each id
     from 0 to n_experts - 1 an expert (at most 1024): a tree's leaves, say, or a router's
     choices. An id that is anything else (-1) has no expert; ids are int32, int64, or float32
-    as predict(pred_leaf=True) gives leaf ids.
+    as predict(pred_leaf=True) gives leaf ids. All columns have the same experts: for leaves of
+    several trees add each tree's first token, Vocabulary.first, to its column.
 
     order   positions (row * columns + column) by expert, equal ones in their order, those
             without an expert behind all others; int32

@@ -229,3 +229,18 @@ def test_infinite_weights_decay_to_themselves(heads, bits, dtype):
         opt.step([torch.zeros_like(p)])
         keep = 1 - 0.5 * decay
         assert p.tolist()[:3] == [inf, -inf, keep] and p[3].isnan() and float(p[4]) == -2 * keep
+
+
+def test_leaves_of_two_trees_have_experts_of_their_own(heads):
+    """As a program with an expert a leaf numbers them: by the vocabulary."""
+    rng = np.random.default_rng(11)
+    voc = heads.Vocabulary([15, 15, 7])
+    leaves = rng.integers(7, 15, (400, 2)).astype(np.float32)
+    ids = torch.from_numpy(leaves).cuda() + voc.first[:2]
+    routes = heads.Routes(ids, int(voc.sizes[:2].sum()))
+    starts = routes.starts.tolist()
+    assert starts[-1] == 800 and len(starts) == 31
+    order = routes.order.cpu().numpy()
+    for expert, (a, b) in enumerate(zip(starts, starts[1:])):
+        want = np.flatnonzero(leaves[:, expert // 15] == expert % 15) * 2 + expert // 15
+        assert np.array_equal(order[a:b], want)
