@@ -71,7 +71,8 @@ struct Adam {
     uint32_t ticks;  // whether this launch moves the clock on
 };
 
-// (room for few tensors or many: 3.7 KB of arguments take 0.9 us more of the host than 64 bytes)
+// (room for few tensors or many: a call with 16 tensors and 1 KB of arguments takes 3.4 to 4.3 us
+// of the host, one with 17 and 3.7 KB 0.1 to 0.4 us more)
 template <uint32_t MOST>
 struct AdamLaunch {
     Adam a;
