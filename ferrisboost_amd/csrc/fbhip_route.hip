@@ -8,7 +8,10 @@
 // positions, their sums over the chunks before, and places from both; up to 4096 positions take
 // one workgroup and launch. All orders are fixed. 2M positions of 511 ids take 20.8 us (5.6 +
 // 3.7 + 13.4 by themselves) where memory would take 5: each launch's workgroups are all on the
-// device at once, and its time is what one of them takes from its loads to its stores.
+// device at once, and its time is what one of them takes from its loads to its stores. Of the last
+// launch waves wait 64 % (LDS counters, round after round, and barriers), and vector instructions,
+// most of them the search for equal ids, take 40 %; `order` in runs of 8 positions costs 22.4 MB of
+// writes for 16.
 #include "fbhip_heads.h"
 
 #include <algorithm>
