@@ -866,9 +866,10 @@ class AdamW(_Kept):
     in `masters`, which is what the steps move and round into it (call take_params() after
     writing into such a parameter). weight_decay is a number, or a list of one for each
     parameter; lr a number, or a float32 tensor of one value on the device, in memory that is no
-    parameter's, which a step reads when it runs. Both are attributes that may be set between steps. The steps are counted on
-    the device too, so a captured step goes on at each replay. Steps of one optimizer follow
-    one another: on another stream only when that has waited.
+    parameter's, which a step reads when it runs. Both are attributes that may be set between
+    steps. The steps are counted on the device too, so a captured step goes on at each replay (and
+    the optimizer and that lr have to live as long as the graph). Steps of one optimizer follow one
+    another: on another stream only when that has waited.
 
     bits=32 keeps m and s in float32, bits=8 in a byte each and an exponent for 256 cells:
     small floats with 3 bits behind the point, rounded up or down at random (from `seed`, the
@@ -881,8 +882,7 @@ class AdamW(_Kept):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay=0.01, *, bits: int = 32, seed: int = 0):
         torch = _need_torch()
-        self.params = [params] if isinstance(params, torch.Tensor) else _list(
-            params, "params")
+        self.params = [params] if isinstance(params, torch.Tensor) else _list(params, "params")
         if not self.params:
             raise ValueError("no parameters")
         betas = tuple(_number(b, "betas must be two numbers in [0, 1): each")
@@ -1002,8 +1002,7 @@ class AdamW(_Kept):
         each parameter, of its shape and type. Every parameter needs one, in memory that is no
         parameter's."""
         params = self.params
-        grads = [p.grad for p in params] if grads is None else _list(
-            grads, "grads")
+        grads = [p.grad for p in params] if grads is None else _list(grads, "grads")
         if len(grads) != len(params):
             raise ValueError(f"{len(grads)} gradients for {len(params)} parameters")
         # (a small step's time is what the host takes for these)

@@ -856,7 +856,8 @@ uint64_t fbh_layer_norm_grad_bytes(const fbh_norm *a);
  * wide rows are read again), dweight and dbias [dim], summed over all rows (each may be
  * NULL: not wanted); stats as fbh_layer_norm gave them. At most 256 rows are added up in
  * f32 one after the other, then the sums of up to 64 such chains; those of workgroups are
- * added in f64. Orders of sums depend on n_rows and dim alone. work may be NULL where neither dweight nor dbias is wanted. */
+ * added in f64. Orders of sums depend on n_rows and dim alone. work may be NULL where
+ * neither dweight nor dbias is wanted. */
 int fbh_layer_norm_grad(int device, const fbh_norm *a, const void *grad, const void *x,
                         const float *stats, const void *weight, void *dx, void *dweight,
                         void *dbias, void *work, uint64_t work_bytes, void *stream);
