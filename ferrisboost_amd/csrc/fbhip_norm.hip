@@ -282,8 +282,10 @@ void with_type(uint32_t dtype, F &&f) {
 // writes its part, and the parts are added in order.
 constexpr uint32_t SPLIT_DIM = 16384;  // wider rows' sums have no room in registers
 // Rows that are added up in f32, one after the other: of more the parts' sums are taken in
-// several batches of rows (65536 of 16384 cells, say), so that what rounding leaves has a bound.
-constexpr uint64_t CHAIN = 256;
+// several batches of rows (65024 of 32768 cells, say), so that what rounding leaves has a bound.
+// (With 256 a launch's end comes often enough to be seen: 20,000 x 20,000 in 780 us, in one batch
+// 761; 2^25 x 8 in 676 and 650.)
+constexpr uint64_t CHAIN = 1024;
 
 struct NormGrad {
     uint64_t n_rows;

@@ -651,7 +651,7 @@ def layer_norm_grad(grad, x, stats, weight=None):
     """The gradients of layer_norm()'s x, weight and bias for `grad`, that of its output:
     (dx, dweight, dbias), the last two in weight's type and None without one. x, weight and
     `stats` are those of the call layer_norm(..., stats=True). Sums over rows are taken in a
-    fixed order, a workgroup's in float32 (at most 256 rows one after the other) and theirs in
+    fixed order, a workgroup's in float32 (at most 1024 rows one after the other) and theirs in
     float64, and rounded once.
     (layer_norm() does this in backward(); a captured training step can call it by itself.)"""
     torch = _need_torch()

@@ -854,7 +854,7 @@ int fbh_layer_norm(int device, const fbh_norm *a, const void *x, const void *wei
 uint64_t fbh_layer_norm_grad_bytes(const fbh_norm *a);
 /* The gradients for the output's gradient grad: dx [n_rows][dim] (apart from the inputs:
  * wide rows are read again), dweight and dbias [dim], summed over all rows (each may be
- * NULL: not wanted); stats as fbh_layer_norm gave them. At most 256 rows are added up in
+ * NULL: not wanted); stats as fbh_layer_norm gave them. At most 1024 rows are added up in
  * f32 one after the other, then the sums of up to 64 such chains; those of workgroups are
  * added in f64. Orders of sums depend on n_rows and dim alone. work may be NULL where
  * neither dweight nor dbias is wanted. */

@@ -12,7 +12,7 @@ import training_ref as ref
 # widths up to these have so many lanes a row, of so many cells each
 SHAPES = [(32, 4, 8), (64, 8, 8), (128, 16, 8), (256, 16, 16), (512, 64, 8), (1024, 64, 16),
           (2048, 256, 8), (4096, 256, 16), (8192, 512, 16), (16_384, 512, 32), (32_768, 512, 64)]
-CHAIN = 256  # rows that a lane adds up in float32 at most
+CHAIN = 1024  # rows that a lane adds up in float32 at most
 
 
 def _shape(dim):

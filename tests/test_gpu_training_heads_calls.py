@@ -161,23 +161,25 @@ def test_layer_norm_gradients_of_many_rows(heads, n, dim):
         assert _off(a, value, off).all(), what
 
 
-@pytest.mark.parametrize("n, dim", [(140_000, 16_386), (524_288, 4098), (1 << 27, 4)])
+@pytest.mark.parametrize("n, dim", [(1 << 19, 16_386), (1 << 21, 4098), (1 << 29, 4)])
 def test_weights_sums_of_any_number_of_rows(heads, n, dim):
     """Equal terms, whose float32 sum is off the same way at each addition, by a half step of the
-    sum at most, and the rounding of the result."""
-    c = float(np.float32(1.004119873046875))
-    g = torch.full((n, dim), c, device="cuda")
-    x = torch.ones((n, dim), device="cuda")
-    x[:, dim // 2:] = -1.0
+    sum at most, and the rounding of the result. (In a chain of 8192 rows, as there would be, sums
+    of this number are off by 1.2e-4.)"""
+    c = float(np.float32(1.9545904397964478))
+    x = torch.full((n, dim), c, device="cuda")  # up to 34 GB
+    x[:, dim // 2:] = -c
     stats = torch.zeros((n, 2), device="cuda")  # mean 0, deviation 1
     stats[:, 1] = 1.0
     w = torch.ones(dim, device="cuda")
-    _, dw, db = heads._layer_norm_grad(heads._norm_of(x, w, 1.0), g, x, stats, w,
+    _, dw, db = heads._layer_norm_grad(heads._norm_of(x, w, 1.0), x, x, stats, w,
                                        (False, True, True))
+    del x
     sign = torch.where(torch.arange(dim, device="cuda") < dim // 2, 1.0, -1.0).double()
-    off = ref.ULP * (norm_bounds.weight_path(n, dim) + 1) * n * c
-    assert float((db.double() - n * c).abs().max()) <= off
-    assert float((dw.double() - sign * (n * c)).abs().max()) <= off
+    off = ref.ULP * (norm_bounds.weight_path(n, dim) + 1) * n
+    assert float((db.double() - sign * (n * c)).abs().max()) <= off * c
+    assert float((dw.double() - n * c * c).abs().max()) <= off * c * c
+    torch.cuda.empty_cache()
 
 
 def test_gradients_to_experts_rows_beyond_2_31_cells(heads):
@@ -191,7 +193,8 @@ def test_gradients_to_experts_rows_beyond_2_31_cells(heads):
     dy, dw = heads.from_experts_grad(x, y, r, w)
     end = int(r.starts[-1])
     assert end * dim > (1 << 31) + 1000 * dim
-    at = torch.cat([torch.arange(0, 100), torch.arange((1 << 31) // dim - 50, (1 << 31) // dim + 50),
+    far = (1 << 31) // dim
+    at = torch.cat([torch.arange(0, 100), torch.arange(far - 50, far + 50),
                     torch.arange(end - 100, end)]).cuda()
     position = r.order[at].long()
     row = position // k
