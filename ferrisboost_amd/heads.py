@@ -1065,6 +1065,9 @@ class AdamW(_Kept):
 
     def split(self, flat):
         """A flat tensor's parts as views in the parameters' shapes."""
+        if not isinstance(flat, _Tensor) or flat.shape != self.mean.shape:
+            raise ValueError(f"flat must be a tensor of {tuple(self.mean.shape)}, as moments() "
+                             f"gives")
         return [flat[a:a + n].view(p.shape)
                 for a, n, p in zip(self.first, self._sizes, self.params)]
 

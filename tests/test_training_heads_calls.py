@@ -252,3 +252,11 @@ def test_a_learning_rate_in_a_parameter_s_memory_is_refused(lr_at):
     """Some cells would be stepped by what it was and some by what it becomes."""
     with pytest.raises(ValueError, match="learning rate overlaps a parameter"):
         N.check_hip(N.hip().fbh_adamw_step(0, *_step_arguments([0x1000, 0x3000], lr_at), None))
+
+
+def test_split_takes_a_flat_tensor_of_the_state_s_size():
+    opt = _optimizer()
+    assert [v.shape for v in opt.split(opt.mean)] == [p.shape for p in opt.params]
+    for bad in (torch.zeros(5), torch.zeros(opt.mean.numel() + 1), opt.mean[None], None, [0.0]):
+        with pytest.raises(ValueError, match="flat must be a tensor"):
+            opt.split(bad)
